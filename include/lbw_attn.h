@@ -243,6 +243,121 @@ int lbw_kv_quant_fp8(const void* x, int32_t batch, int64_t len, int32_t heads,
                      int32_t head_dim, int64_t s_b, int64_t s_l, int64_t s_h,
                      uint8_t* codes, float* scales, int32_t block, void* stream);
 
+/* ---- Operators on packed sequences: training and token-by-token serving beside the chunk path.
+ * All bf16 with fp32 sums; token rows [tokens, heads, head_dim] with a stride per token and per
+ * head (elements, multiples of 8; the head dim contiguous, 16-byte aligned). k_heads divides
+ * q_heads: query head h uses key/value head h / (q_heads / k_heads).
+ *
+ * Per-head RMSNorm of q and k and the rotation of their pairs:
+ *   y = x * rsqrt(mean_d x^2 + eps) * w; the first 2 * rope_pairs values of y turn by pairs,
+ *   interleaved (2i, 2i + 1) or split halves (i, i + rope_pairs), pair i of a token by the angle
+ *   at row pos[token][axis of i] of the table; times q_out_scale / k_out_scale; one rounding.
+ * `rope` holds (cos, sin) float pairs, [rope_rows][rope_pairs]. The pairs of axis a follow those of
+ * axis a - 1, axis_pairs[a] of them; they add up to rope_pairs. A position outside the table turns
+ * the axis's pairs into NaN. head_dim 32, 64, 128 or 256; split halves need rope_pairs % 8 == 0.
+ * Optional: v copied to v_out. With `rows` (int32 [tokens], device), token t is the new token of
+ * sequence t and its k and v go to row rows[t] (0 <= rows[t] < row_count, else not written) of
+ * k_out / v_out [tokens][row_count][k_heads][head_dim], whose sequences are *_stride_b apart.
+ * Outputs may be the inputs themselves, and must not overlap them otherwise. */
+#define LBW_MAX_AXES 4
+#define LBW_W_BF16 0
+#define LBW_W_FP32 1
+typedef struct lbw_head_norm_rope_params {
+  int32_t tokens, q_heads, k_heads, head_dim;
+  const void* q; int64_t q_stride_l, q_stride_h;
+  const void* k; int64_t k_stride_l, k_stride_h;
+  const void* wq; const void* wk;  /* [head_dim] or NULL (1) */
+  int32_t w_dtype;                 /* LBW_W_BF16 or LBW_W_FP32 */
+  float eps;
+  const float* rope; int64_t rope_rows;
+  int32_t rope_pairs, n_axes;
+  int32_t axis_pairs[LBW_MAX_AXES];
+  int32_t interleaved;
+  const int32_t* pos; int64_t pos_stride; /* int32 [tokens][n_axes], row stride in elements */
+  void* q_out; int64_t q_out_stride_l, q_out_stride_h;
+  void* k_out; int64_t k_out_stride_l, k_out_stride_h;
+  const void* v; int64_t v_stride_l, v_stride_h; /* NULL: no copy */
+  void* v_out; int64_t v_out_stride_l, v_out_stride_h;
+  const int32_t* rows;             /* NULL: token t goes to row t of k_out and v_out */
+  int32_t row_count;
+  int64_t k_out_stride_b, v_out_stride_b;
+  float q_out_scale, k_out_scale;
+} lbw_head_norm_rope_params;
+int lbw_head_norm_rope(const lbw_head_norm_rope_params* p, void* stream);
+
+/* Its gradient: from the outputs' gradients to dq, dk (rows as above) and the weights' dwq, dwk
+ * ([head_dim], of w_dtype; NULL: not wanted). Reads q, k, the weights, the table and the positions of
+ * `p`; its outputs, v and rows are ignored. The same result on every run. */
+typedef struct lbw_head_norm_rope_grads {
+  const void* dq_out; int64_t dq_out_stride_l, dq_out_stride_h;
+  const void* dk_out; int64_t dk_out_stride_l, dk_out_stride_h;
+  void* dq; int64_t dq_stride_l, dq_stride_h;
+  void* dk; int64_t dk_stride_l, dk_stride_h;
+  void* dwq; void* dwk;
+} lbw_head_norm_rope_grads;
+size_t lbw_head_norm_rope_bwd_workspace_size(const lbw_head_norm_rope_params* p);
+int lbw_head_norm_rope_bwd(const lbw_head_norm_rope_params* p, const lbw_head_norm_rope_grads* g,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention over sequences packed one after another (no padding): sequence s has q_lens[s] query
+ * rows and k_lens[s] key rows. Causal: query i sees key j when j <= i + k_len - q_len (the last
+ * query sees every key); otherwise every key of its own sequence. A query that sees no key
+ * gives 0 and lse -inf. head_dim 128.
+ *
+ * lbw_attention_packed_plan (host only, no GPU call) cuts the sequences into the work items of
+ * the kernels, int32 [LBW_PACKED_ITEM] each, the costliest first; copy both tables to the device.
+ * With q_items == NULL and k_items == NULL it only counts. A table belongs to its lengths and serves any
+ * number of heads and layers. A table of other lengths gives wrong results, but its items never lead a
+ * kernel outside the q_tokens / k_tokens rows given. */
+#define LBW_PACKED_ITEM 8
+int lbw_attention_packed_plan(int32_t n_seqs, const int32_t* q_lens, const int32_t* k_lens,
+                              int32_t causal, int32_t* q_items, int64_t q_items_cap,
+                              int64_t* n_q_items, int32_t* k_items, int64_t k_items_cap,
+                              int64_t* n_k_items);
+typedef struct lbw_packed_params {
+  int32_t q_heads, k_heads, head_dim;
+  int64_t q_tokens, k_tokens;      /* packed rows of q, out and of k, v */
+  const void* q; int64_t q_stride_l, q_stride_h;
+  const void* k; int64_t k_stride_l, k_stride_h;
+  const void* v; int64_t v_stride_l, v_stride_h;
+  void* out; int64_t out_stride_l, out_stride_h;
+  float* lse;                      /* fp32 [q_heads][q_tokens], natural log; NULL: not wanted */
+  float softmax_scale;             /* > 0; 0: 1 / sqrt(head_dim) */
+  const int32_t* q_items; int32_t n_q_items;
+  const int32_t* k_items; int32_t n_k_items; /* gradient only */
+} lbw_packed_params;
+int lbw_attention_packed_fwd(const lbw_packed_params* p, void* stream);
+
+/* Its gradient, from q, k, v, out and lse of the forward call: the same result on every run (no
+ * atomics). dq, dk, dv have no overlap with anything. */
+typedef struct lbw_packed_grads {
+  const void* dout; int64_t dout_stride_l, dout_stride_h;
+  void* dq; int64_t dq_stride_l, dq_stride_h;
+  void* dk; int64_t dk_stride_l, dk_stride_h;
+  void* dv; int64_t dv_stride_l, dv_stride_h;
+} lbw_packed_grads;
+size_t lbw_attention_packed_bwd_workspace_size(const lbw_packed_params* p);
+int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads* g,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* One query token per sequence over its cache: q [batch, q_heads, D], k / v [batch, capacity,
+ * k_heads, D], lens int32 [batch] on the device (read there, limited to [0, capacity]); a
+ * sequence of no keys gives 0. head_dim 128. */
+typedef struct lbw_decode_params {
+  int32_t batch, q_heads, k_heads, head_dim;
+  int64_t capacity;
+  const void* q; int64_t q_stride_b, q_stride_h;
+  const void* k; int64_t k_stride_b, k_stride_l, k_stride_h;
+  const void* v; int64_t v_stride_b, v_stride_l, v_stride_h;
+  const int32_t* lens;
+  void* out; int64_t out_stride_b, out_stride_h;
+  float softmax_scale;             /* > 0; 0: 1 / sqrt(head_dim) */
+  int32_t num_splits;              /* pieces of a sequence's keys; 0: chosen by the library */
+} lbw_decode_params;
+size_t lbw_attention_decode_workspace_size(const lbw_decode_params* p);
+int lbw_attention_decode(const lbw_decode_params* p, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 const char* lbw_last_error(void);
 int lbw_abi_version(void);
 

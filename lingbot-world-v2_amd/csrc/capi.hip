@@ -15,14 +15,14 @@
 
 #include "lbw_attn.h"
 #include "attn_fwd.h"
+#include "capi_util.h"
 
 using namespace lbw;
 
-namespace {
+namespace lbw {
 
-thread_local std::string g_err;
+static thread_local std::string g_err;
 
-int fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 int fail(int code, const char* fmt, ...) {
   char buf[512];
   va_list ap;
@@ -36,9 +36,6 @@ int fail(int code, const char* fmt, ...) {
 int hip_fail(hipError_t e, const char* what) {
   return fail(LBW_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-bool mult8(int64_t s) { return (s & 7) == 0; }
 
 int num_cus() {
   static std::mutex mu;
@@ -54,6 +51,10 @@ int num_cus() {
   }
   return cache[dev];
 }
+
+}  // namespace lbw
+
+namespace {
 
 // Estimated run time, in tile steps (1.5 us), of a launch with s KV splits: greedy list
 // scheduling of the workgroups in dispatch order (q-tile fastest, then split, then batch x head)

@@ -1,0 +1,378 @@
+// extern "C" entry points of the operators on packed sequences: argument checks, the work items of
+// packed attention, launches. No allocation on the device and no synchronisation.
+
+#include <math.h>
+#include <string.h>
+
+#include <algorithm>
+#include <array>
+#include <new>
+#include <vector>
+
+#include "capi_util.h"
+#include "lbw_attn.h"
+#include "packed.h"
+
+using namespace lbw;
+
+namespace {
+
+// hipLaunchKernel's limit: fewer than 2^32 threads in a grid
+constexpr int64_t kMaxWorkgroups = (int64_t(1) << 32) / 256 - 1;
+
+// bf16 rows [n, heads, D]; n == 0: no pointer needed. `tile`: rows are copied in tiles of 64 with
+// 32-bit byte offsets.
+int check_rows(const char* name, const void* p, int64_t n, int64_t sl, int64_t sh, bool tile = false) {
+  if (n > 0 && (p == nullptr || !aligned16(p)))
+    return fail(LBW_ERR_INVALID, "%s must be a 16-byte aligned device pointer", name);
+  if (!mult8(sl) || !mult8(sh))
+    return fail(LBW_ERR_INVALID, "%s strides must be multiples of 8 elements", name);
+  if (sl < 0 || sh < 0) return fail(LBW_ERR_INVALID, "%s has a negative stride", name);
+  if (tile && sl >= (int64_t(1) << 31) / (64 * 2))
+    return fail(LBW_ERR_UNSUPPORTED, "%s: token stride %lld exceeds %lld", name, (long long)sl,
+                (long long)((int64_t(1) << 31) / (64 * 2) - 1));
+  return LBW_OK;
+}
+
+int check_heads(int32_t hq, int32_t hk) {
+  if (hq < 1 || hk < 1 || hq % hk != 0)
+    return fail(LBW_ERR_INVALID, "k_heads %d must divide q_heads %d", hk, hq);
+  return LBW_OK;
+}
+
+int check_scale(float s, int head_dim, float* scale) {
+  if (!(s >= 0.0f) || isinf(s))
+    return fail(LBW_ERR_INVALID, "softmax_scale must be positive and finite (0: 1/sqrt(head_dim))");
+  *scale = s > 0.0f ? s : 1.0f / sqrtf((float)head_dim);
+  return LBW_OK;
+}
+
+constexpr double kLog2e = 1.4426950408889634;
+
+#define LBW_TRY(x)                  \
+  do {                              \
+    const int rc_ = (x);            \
+    if (rc_ != LBW_OK) return rc_;  \
+  } while (0)
+
+int fill_head_norm(const lbw_head_norm_rope_params* p, HeadNormArgs* a) {
+  if (p == nullptr) return fail(LBW_ERR_INVALID, "params is NULL");
+  memset(a, 0, sizeof(*a));
+  if (p->tokens < 0) return fail(LBW_ERR_INVALID, "tokens %d", p->tokens);
+  LBW_TRY(check_heads(p->q_heads, p->k_heads));
+  const int D = p->head_dim;
+  if (D != 32 && D != 64 && D != 128 && D != 256)
+    return fail(LBW_ERR_UNSUPPORTED, "head_dim %d: 32, 64, 128 or 256", D);
+  if (p->q_heads > 32768) return fail(LBW_ERR_UNSUPPORTED, "q_heads %d above 32768", p->q_heads);
+  if (!(p->eps >= 0.0f)) return fail(LBW_ERR_INVALID, "eps must not be negative");
+  if (p->n_axes < 1 || p->n_axes > LBW_MAX_AXES)
+    return fail(LBW_ERR_INVALID, "n_axes %d not in [1, %d]", p->n_axes, LBW_MAX_AXES);
+  if (p->rope_pairs < 0 || 2 * (int64_t)p->rope_pairs > D)
+    return fail(LBW_ERR_INVALID, "rope_pairs %d of head_dim %d", p->rope_pairs, D);
+  int64_t sum = 0;
+  for (int i = 0; i < LBW_MAX_AXES; ++i) {
+    if (i < p->n_axes) {
+      if (p->axis_pairs[i] < 0) return fail(LBW_ERR_INVALID, "axis_pairs[%d] is negative", i);
+      sum += p->axis_pairs[i];
+    }
+    a->ax_end[i] = i + 1 < p->n_axes ? (int)sum : p->rope_pairs;
+  }
+  if (sum != p->rope_pairs)
+    return fail(LBW_ERR_INVALID, "axis_pairs add up to %lld, rope_pairs is %d", (long long)sum,
+                p->rope_pairs);
+  if (!p->interleaved && p->rope_pairs % 8 != 0)
+    return fail(LBW_ERR_UNSUPPORTED, "split halves need rope_pairs %d a multiple of 8", p->rope_pairs);
+  if (p->rope_rows < 0 || p->rope_rows > 0x7fffffff)
+    return fail(LBW_ERR_INVALID, "rope_rows %lld", (long long)p->rope_rows);
+  if (p->rope_pairs > 0 && p->rope_rows > 0 &&
+      (p->rope == nullptr || (reinterpret_cast<uintptr_t>(p->rope) & 7u)))
+    return fail(LBW_ERR_INVALID, "the rotation table must be 8-byte aligned");
+  if (p->tokens > 0 && p->pos == nullptr) return fail(LBW_ERR_INVALID, "pos missing");
+  if (p->w_dtype != LBW_W_BF16 && p->w_dtype != LBW_W_FP32)
+    return fail(LBW_ERR_INVALID, "w_dtype %d: LBW_W_BF16 or LBW_W_FP32", p->w_dtype);
+  if ((p->wq && !aligned16(p->wq)) || (p->wk && !aligned16(p->wk)))
+    return fail(LBW_ERR_INVALID, "weights must be 16-byte aligned");
+  LBW_TRY(check_rows("q", p->q, p->tokens, p->q_stride_l, p->q_stride_h));
+  LBW_TRY(check_rows("k", p->k, p->tokens, p->k_stride_l, p->k_stride_h));
+  if ((int64_t)p->tokens * 32 / 4 >= kMaxWorkgroups)
+    return fail(LBW_ERR_UNSUPPORTED, "tokens %d", p->tokens);
+  a->T = p->tokens; a->Hq = p->q_heads; a->Hk = p->k_heads;
+  a->q = {static_cast<const uint16_t*>(p->q), p->q_stride_l, p->q_stride_h};
+  a->k = {static_cast<const uint16_t*>(p->k), p->k_stride_l, p->k_stride_h};
+  a->wq = p->wq; a->wk = p->wk; a->w32 = p->w_dtype == LBW_W_FP32;
+  a->eps = p->eps;
+  a->inv_d = 1.0f / (float)D;
+  a->table = reinterpret_cast<const float2*>(p->rope);
+  a->P = (int)p->rope_rows; a->npairs = p->rope_pairs;
+  a->naxes = p->n_axes; a->inter = p->interleaved != 0;
+  a->pos = p->pos; a->pos_sl = p->pos_stride;
+  a->q_scale = p->q_out_scale; a->k_scale = p->k_out_scale;
+  return LBW_OK;
+}
+
+int fill_packed(const lbw_packed_params* p, PackedArgs* a) {
+  if (p == nullptr) return fail(LBW_ERR_INVALID, "params is NULL");
+  memset(a, 0, sizeof(*a));
+  if (p->head_dim != 128) return fail(LBW_ERR_UNSUPPORTED, "head_dim %d: only 128", p->head_dim);
+  LBW_TRY(check_heads(p->q_heads, p->k_heads));
+  if (p->q_tokens < 0 || p->k_tokens < 0 || p->q_tokens > 0x7fffffff || p->k_tokens > 0x7fffffff)
+    return fail(LBW_ERR_INVALID, "q_tokens %lld, k_tokens %lld", (long long)p->q_tokens,
+                (long long)p->k_tokens);
+  LBW_TRY(check_rows("q", p->q, p->q_tokens, p->q_stride_l, p->q_stride_h, true));
+  LBW_TRY(check_rows("k", p->k, p->k_tokens, p->k_stride_l, p->k_stride_h, true));
+  LBW_TRY(check_rows("v", p->v, p->k_tokens, p->v_stride_l, p->v_stride_h, true));
+  LBW_TRY(check_rows("out", p->out, p->q_tokens, p->out_stride_l, p->out_stride_h));
+  float scale = 0.0f;
+  LBW_TRY(check_scale(p->softmax_scale, p->head_dim, &scale));
+  if (p->n_q_items < 0 || (p->n_q_items > 0 && p->q_items == nullptr))
+    return fail(LBW_ERR_INVALID, "q_items missing");
+  if ((int64_t)p->n_q_items * p->q_heads > kMaxWorkgroups)
+    return fail(LBW_ERR_UNSUPPORTED, "%d query items x %d heads", p->n_q_items, p->q_heads);
+  a->q = {static_cast<const uint16_t*>(p->q), p->q_stride_l, p->q_stride_h};
+  a->k = {static_cast<const uint16_t*>(p->k), p->k_stride_l, p->k_stride_h};
+  a->v = {static_cast<const uint16_t*>(p->v), p->v_stride_l, p->v_stride_h};
+  a->out = {static_cast<uint16_t*>(p->out), p->out_stride_l, p->out_stride_h};
+  a->lse = p->lse;
+  a->Tq = p->q_tokens; a->Tk = p->k_tokens; a->Hq = p->q_heads; a->Hk = p->k_heads;
+  a->scale = scale;
+  a->scale_log2 = (float)((double)scale * kLog2e);
+  a->q_items = p->q_items; a->n_q_items = p->n_q_items;
+  a->k_items = p->k_items; a->n_k_items = p->n_k_items;
+  return LBW_OK;
+}
+
+int decode_pieces(const lbw_decode_params* p) {
+  return p->num_splits > 0 ? p->num_splits
+                           : decode_splits(p->batch, p->q_heads, p->k_heads, p->capacity, num_cus());
+}
+
+int check_decode(const lbw_decode_params* p) {
+  if (p == nullptr) return fail(LBW_ERR_INVALID, "params is NULL");
+  if (p->batch < 0 || p->capacity < 0 || p->capacity > 0x7fffff00)
+    return fail(LBW_ERR_INVALID, "batch %d, capacity %lld", p->batch, (long long)p->capacity);
+  if (p->head_dim != 128) return fail(LBW_ERR_UNSUPPORTED, "head_dim %d: only 128", p->head_dim);
+  LBW_TRY(check_heads(p->q_heads, p->k_heads));
+  if (p->num_splits < 0 || p->num_splits > 128)
+    return fail(LBW_ERR_INVALID, "num_splits %d not in [0, 128]", p->num_splits);
+  const int64_t blocks = (p->q_heads / p->k_heads + 31) / 32;
+  if ((int64_t)p->batch * p->k_heads * blocks * 128 > kMaxWorkgroups)
+    return fail(LBW_ERR_UNSUPPORTED, "batch %d x %d heads", p->batch, p->q_heads);
+  return LBW_OK;
+}
+
+using Item = std::array<int32_t, LBW_PACKED_ITEM>;
+static_assert(LBW_PACKED_ITEM == PK_ITEM, "the kernels' item size");
+
+}  // namespace
+
+extern "C" {
+
+int lbw_head_norm_rope(const lbw_head_norm_rope_params* p, void* stream) {
+  HeadNormArgs a;
+  LBW_TRY(fill_head_norm(p, &a));
+  LBW_TRY(check_rows("q_out", p->q_out, p->tokens, p->q_out_stride_l, p->q_out_stride_h));
+  LBW_TRY(check_rows("k_out", p->k_out, p->tokens, p->k_out_stride_l, p->k_out_stride_h));
+  a.qo = {static_cast<uint16_t*>(p->q_out), p->q_out_stride_l, p->q_out_stride_h};
+  a.ko = {static_cast<uint16_t*>(p->k_out), p->k_out_stride_l, p->k_out_stride_h};
+  if (p->v != nullptr) {
+    LBW_TRY(check_rows("v", p->v, p->tokens, p->v_stride_l, p->v_stride_h));
+    LBW_TRY(check_rows("v_out", p->v_out, p->tokens, p->v_out_stride_l, p->v_out_stride_h));
+    a.v = {static_cast<const uint16_t*>(p->v), p->v_stride_l, p->v_stride_h};
+    a.vo = {static_cast<uint16_t*>(p->v_out), p->v_out_stride_l, p->v_out_stride_h};
+  }
+  if (p->rows != nullptr) {
+    if (p->row_count < 0 || !mult8(p->k_out_stride_b) || p->k_out_stride_b < 0 ||
+        (p->v != nullptr && (!mult8(p->v_out_stride_b) || p->v_out_stride_b < 0)))
+      return fail(LBW_ERR_INVALID, "rows: row_count %d, sequence strides must be multiples of 8",
+                  p->row_count);
+    a.rows = p->rows;
+    a.cap = p->row_count;
+    a.kosb = p->k_out_stride_b;
+    a.vosb = p->v_out_stride_b;
+  }
+  if (p->tokens == 0) return LBW_OK;
+  const hipError_t e = launch_head_norm(a, p->head_dim, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? LBW_OK : hip_fail(e, "head_norm_rope launch");
+}
+
+size_t lbw_head_norm_rope_bwd_workspace_size(const lbw_head_norm_rope_params* p) {
+  if (p == nullptr || p->tokens <= 0 || p->head_dim <= 0) return 0;
+  return (size_t)head_norm_bwd_workgroups(p->tokens, num_cus()) * 2 * p->head_dim * sizeof(float);
+}
+
+int lbw_head_norm_rope_bwd(const lbw_head_norm_rope_params* p, const lbw_head_norm_rope_grads* g,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  HeadNormArgs a;
+  LBW_TRY(fill_head_norm(p, &a));
+  if (g == nullptr) return fail(LBW_ERR_INVALID, "grads is NULL");
+  LBW_TRY(check_rows("dq_out", g->dq_out, p->tokens, g->dq_out_stride_l, g->dq_out_stride_h));
+  LBW_TRY(check_rows("dk_out", g->dk_out, p->tokens, g->dk_out_stride_l, g->dk_out_stride_h));
+  LBW_TRY(check_rows("dq", g->dq, p->tokens, g->dq_stride_l, g->dq_stride_h));
+  LBW_TRY(check_rows("dk", g->dk, p->tokens, g->dk_stride_l, g->dk_stride_h));
+  const size_t need = lbw_head_norm_rope_bwd_workspace_size(p);
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
+    return fail(LBW_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need,
+                workspace_bytes);
+  a.dqo = {static_cast<const uint16_t*>(g->dq_out), g->dq_out_stride_l, g->dq_out_stride_h};
+  a.dko = {static_cast<const uint16_t*>(g->dk_out), g->dk_out_stride_l, g->dk_out_stride_h};
+  a.qo = {static_cast<uint16_t*>(g->dq), g->dq_stride_l, g->dq_stride_h};
+  a.ko = {static_cast<uint16_t*>(g->dk), g->dk_stride_l, g->dk_stride_h};
+  a.dwq = g->dwq;
+  a.dwk = g->dwk;
+  a.part = static_cast<float*>(workspace);
+  a.nwg = head_norm_bwd_workgroups(p->tokens, num_cus());
+  // (no tokens: the sum over no partial rows gives zero weight gradients)
+  const hipError_t e = launch_head_norm_bwd(a, p->head_dim, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? LBW_OK : hip_fail(e, "head_norm_rope_bwd launch");
+}
+
+int lbw_attention_packed_plan(int32_t n_seqs, const int32_t* q_lens, const int32_t* k_lens,
+                              int32_t causal, int32_t* q_items, int64_t q_items_cap,
+                              int64_t* n_q_items, int32_t* k_items, int64_t k_items_cap,
+                              int64_t* n_k_items) {
+  if (n_seqs < 0 || (n_seqs > 0 && (q_lens == nullptr || k_lens == nullptr)))
+    return fail(LBW_ERR_INVALID, "n_seqs %d needs q_lens and k_lens", n_seqs);
+  if (n_q_items == nullptr || n_k_items == nullptr)
+    return fail(LBW_ERR_INVALID, "n_q_items and n_k_items must not be NULL");
+  int64_t tq = 0, tk = 0, nq = 0, nk = 0;
+  for (int32_t s = 0; s < n_seqs; ++s) {
+    if (q_lens[s] < 0 || k_lens[s] < 0)
+      return fail(LBW_ERR_INVALID, "sequence %d: negative length", s);
+    tq += q_lens[s];
+    tk += k_lens[s];
+    nq += (q_lens[s] + (int64_t)PK_BLOCK - 1) / PK_BLOCK;
+    nk += (k_lens[s] + (int64_t)PK_BLOCK - 1) / PK_BLOCK;
+  }
+  if (tq > 0x7fffffff || tk > 0x7fffffff)
+    return fail(LBW_ERR_UNSUPPORTED, "%lld query and %lld key rows: below 2^31", (long long)tq,
+                (long long)tk);
+  *n_q_items = nq;
+  *n_k_items = nk;
+  if (q_items == nullptr && k_items == nullptr) return LBW_OK;
+  if ((nq > 0 && q_items == nullptr) || (nk > 0 && k_items == nullptr) || q_items_cap < nq ||
+      k_items_cap < nk)
+    return fail(LBW_ERR_INVALID, "room for %lld and %lld items needed", (long long)nq, (long long)nk);
+  try {
+    std::vector<Item> qi, ki;
+    qi.reserve(nq);
+    ki.reserve(nk);
+    int32_t q0 = 0, k0 = 0;
+    for (int32_t s = 0; s < n_seqs; ++s) {
+      const int32_t lq = q_lens[s], lk = k_lens[s];
+      // full attention: a shift past every key
+      const int32_t shift = causal ? lk - lq : lk;
+      for (int64_t i = 0; i < lq; i += PK_BLOCK) {
+        const int64_t rows = std::min<int64_t>(PK_BLOCK, lq - i);
+        const int64_t seen = std::clamp<int64_t>(i + rows + shift, 0, lk);
+        qi.push_back({q0 + (int32_t)i, (int32_t)rows, (int32_t)i, k0, lk, (int32_t)seen, shift, 0});
+      }
+      for (int64_t j = 0; j < lk; j += PK_BLOCK) {
+        const int64_t rows = std::min<int64_t>(PK_BLOCK, lk - j);
+        const int64_t first = std::clamp<int64_t>(j - shift, 0, lq);
+        ki.push_back({k0 + (int32_t)j, (int32_t)rows, (int32_t)j, q0, lq, (int32_t)first, shift, 0});
+      }
+      q0 += lq;
+      k0 += lk;
+    }
+    std::stable_sort(qi.begin(), qi.end(), [](const Item& x, const Item& y) { return x[5] > y[5]; });
+    std::stable_sort(ki.begin(), ki.end(), [](const Item& x, const Item& y) {
+      return (int64_t)x[4] - x[5] > (int64_t)y[4] - y[5];
+    });
+    if (nq > 0) memcpy(q_items, qi.data(), qi.size() * sizeof(Item));
+    if (nk > 0) memcpy(k_items, ki.data(), ki.size() * sizeof(Item));
+  } catch (const std::bad_alloc&) {
+    return fail(LBW_ERR_INVALID, "no memory for %lld items", (long long)(nq + nk));
+  }
+  return LBW_OK;
+}
+
+int lbw_attention_packed_fwd(const lbw_packed_params* p, void* stream) {
+  PackedArgs a;
+  LBW_TRY(fill_packed(p, &a));
+  if (a.n_q_items == 0) return LBW_OK;
+  const hipError_t e = launch_packed_fwd(a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? LBW_OK : hip_fail(e, "packed attention launch");
+}
+
+size_t lbw_attention_packed_bwd_workspace_size(const lbw_packed_params* p) {
+  if (p == nullptr || p->q_tokens <= 0 || p->q_heads <= 0) return 0;
+  return (size_t)p->q_heads * (size_t)p->q_tokens * sizeof(float);
+}
+
+int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads* g,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  PackedArgs a;
+  LBW_TRY(fill_packed(p, &a));
+  if (g == nullptr) return fail(LBW_ERR_INVALID, "grads is NULL");
+  if (p->n_k_items < 0 || (p->n_k_items > 0 && p->k_items == nullptr))
+    return fail(LBW_ERR_INVALID, "k_items missing");
+  if ((int64_t)p->n_k_items * p->k_heads > kMaxWorkgroups)
+    return fail(LBW_ERR_UNSUPPORTED, "%d key items x %d heads", p->n_k_items, p->k_heads);
+  if (p->q_tokens > 0 && p->lse == nullptr) return fail(LBW_ERR_INVALID, "lse missing");
+  LBW_TRY(check_rows("dout", g->dout, p->q_tokens, g->dout_stride_l, g->dout_stride_h, true));
+  LBW_TRY(check_rows("dq", g->dq, p->q_tokens, g->dq_stride_l, g->dq_stride_h));
+  LBW_TRY(check_rows("dk", g->dk, p->k_tokens, g->dk_stride_l, g->dk_stride_h));
+  LBW_TRY(check_rows("dv", g->dv, p->k_tokens, g->dv_stride_l, g->dv_stride_h));
+  const size_t need = lbw_attention_packed_bwd_workspace_size(p);
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
+    return fail(LBW_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need,
+                workspace_bytes);
+  a.o = {static_cast<const uint16_t*>(p->out), p->out_stride_l, p->out_stride_h};
+  a.dout = {static_cast<const uint16_t*>(g->dout), g->dout_stride_l, g->dout_stride_h};
+  a.delta = static_cast<float*>(workspace);
+  a.dq = {static_cast<uint16_t*>(g->dq), g->dq_stride_l, g->dq_stride_h};
+  a.dk = {static_cast<uint16_t*>(g->dk), g->dk_stride_l, g->dk_stride_h};
+  a.dv = {static_cast<uint16_t*>(g->dv), g->dv_stride_l, g->dv_stride_h};
+  if (a.n_q_items > 0) {
+    const hipError_t e = launch_packed_dq(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "packed attention dQ launch");
+  }
+  if (a.n_k_items > 0) {
+    const hipError_t e = launch_packed_dkv(a, static_cast<hipStream_t>(stream));
+    if (e != hipSuccess) return hip_fail(e, "packed attention dK/dV launch");
+  }
+  return LBW_OK;
+}
+
+size_t lbw_attention_decode_workspace_size(const lbw_decode_params* p) {
+  if (check_decode(p) != LBW_OK || p->batch == 0) return 0;
+  const int s = decode_pieces(p);
+  if (s <= 1) return 0;
+  return (size_t)s * p->batch * p->q_heads * (p->head_dim + 2) * sizeof(float);
+}
+
+int lbw_attention_decode(const lbw_decode_params* p, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  LBW_TRY(check_decode(p));
+  const int64_t B = p->batch;
+  LBW_TRY(check_rows("q", p->q, B, p->q_stride_b, p->q_stride_h));
+  LBW_TRY(check_rows("out", p->out, B, p->out_stride_b, p->out_stride_h));
+  LBW_TRY(check_rows("k", p->k, B * p->capacity, p->k_stride_l, p->k_stride_h, true));
+  LBW_TRY(check_rows("v", p->v, B * p->capacity, p->v_stride_l, p->v_stride_h, true));
+  if (!mult8(p->k_stride_b) || !mult8(p->v_stride_b) || p->k_stride_b < 0 || p->v_stride_b < 0)
+    return fail(LBW_ERR_INVALID, "cache batch strides must be multiples of 8 elements");
+  if (B > 0 && p->lens == nullptr) return fail(LBW_ERR_INVALID, "lens missing");
+  DecodeArgs a;
+  memset(&a, 0, sizeof(a));
+  LBW_TRY(check_scale(p->softmax_scale, p->head_dim, &a.scale));
+  if (B == 0) return LBW_OK;
+  a.splits = decode_pieces(p);
+  const size_t need = lbw_attention_decode_workspace_size(p);
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
+    return fail(LBW_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need,
+                workspace_bytes);
+  a.q = {static_cast<const uint16_t*>(p->q), p->q_stride_b, p->q_stride_h};
+  a.k = static_cast<const uint16_t*>(p->k);
+  a.v = static_cast<const uint16_t*>(p->v);
+  a.ksb = p->k_stride_b; a.ksl = p->k_stride_l; a.ksh = p->k_stride_h;
+  a.vsb = p->v_stride_b; a.vsl = p->v_stride_l; a.vsh = p->v_stride_h;
+  a.lens = p->lens;
+  a.out = {static_cast<uint16_t*>(p->out), p->out_stride_b, p->out_stride_h};
+  a.B = p->batch; a.Hq = p->q_heads; a.Hk = p->k_heads; a.S = (int)p->capacity;
+  a.scale_log2 = (float)((double)a.scale * kLog2e);
+  a.part = static_cast<float*>(workspace);
+  const hipError_t e = launch_decode(a, static_cast<hipStream_t>(stream));
+  return e == hipSuccess ? LBW_OK : hip_fail(e, "single-token attention launch");
+}
+
+}  // extern "C"

@@ -1,0 +1,290 @@
+// Gradient of attention over packed sequences (gfx950), from q, k, v, out, dout and lse.
+//
+//   P = exp(scale Q K^T - lse);  delta_i = sum_d dO O;  dS = P (dO V^T - delta)
+//   dQ = scale dS K;  dK = scale dS^T Q;  dV = P^T dO
+//
+// Two kernels, each with its sums in its own registers: no atomics, so the result does not depend
+// on the order of workgroups. The first has 128 queries of a head per workgroup and walks their keys: it
+// makes delta and dQ (three products a tile). The second has 128 keys of a key/value head and
+// walks the queries of all heads of its group: dK and dV (four products a tile).
+// Both recompute S; P and dS go to bf16 as operands, one rounding each.
+
+#include "packed_tiles.h"
+
+namespace lbw {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int V_AT = 2 * PK_TILE_B;
+constexpr int BWD_LDS = 4 * PK_TILE_B;
+constexpr int STAT_AT = 4 * PK_TILE_B;             // lse and delta of the query tiles, two stages
+constexpr int DKV_LDS = STAT_AT + 2 * 2 * BN * 4;
+
+// ---- dQ: a lane holds one query's column of S^T = K Q^T and dP^T = V dO^T
+__global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const PackedArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hl = lane >> 5, l32 = lane & 31;
+  int h, kv;
+  pick_head(blockIdx.x % (uint32_t)a.Hq, a.Hk, a.Hq / a.Hk, h, kv);
+  const PackedItem it = load_item(a.q_items, blockIdx.x / (uint32_t)a.Hq);
+  if (!item_fits(it, a.Tq, a.Tk)) return;
+  const int r0 = 32 * wave, rows = it.rows - r0;
+  const bool active = rows > 0;
+
+  u32x4 qf[8], gf[8];
+  float lse2 = INFINITY, delta = 0.0f;  // (lse = -inf, no key seen: every p becomes 0)
+  if (active) {
+    const int64_t row = it.row0 + r0;
+    load_rows(a.q.p + row * a.q.sl + h * a.q.sh, a.q.sl, rows, l32, hl, qf);
+    load_rows(a.dout.p + row * a.dout.sl + h * a.dout.sh, a.dout.sl, rows, l32, hl, gf);
+    u32x4 of[8];
+    load_rows(a.o.p + row * a.o.sl + h * a.o.sh, a.o.sl, rows, l32, hl, of);
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+        delta += bf16_lo(gf[s][w]) * bf16_lo(of[s][w]) + bf16_hi(gf[s][w]) * bf16_hi(of[s][w]);
+    delta = wave_sum_xor32(delta);
+    if (l32 < rows) {
+      const int64_t at = (int64_t)h * a.Tq + row + l32;
+      const float x = a.lse[at];
+      lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
+      if (hl == 0) a.delta[at] = delta;
+    }
+  }
+  const unsigned char* kb = reinterpret_cast<const unsigned char*>(
+      a.k.p + (int64_t)it.other0 * a.k.sl + kv * a.k.sh);
+  const unsigned char* vb = reinterpret_cast<const unsigned char*>(
+      a.v.p + (int64_t)it.other0 * a.v.sl + kv * a.v.sh);
+  const int64_t ks = a.k.sl * 2, vs = a.v.sl * 2;
+  const int i0 = it.pos0 + r0;
+  auto limit = [&](int i) {
+    const int64_t x = (int64_t)i + it.shift + 1;
+    return (int)(x < 0 ? 0 : (x < it.other_len ? x : it.other_len));
+  };
+  const int lim = limit(i0 + l32);
+  const int lim_lo = limit(i0), lim_hi = limit(i0 + (rows < 32 ? rows : 32) - 1);
+
+  const int lds0 = (int)lds_addr(lds);
+  int off[8], toff[4][2];
+  row_offsets(lds0, l32, hl, off);
+  tr_offsets(lds0, lane, hl, toff);
+  TileCopy copy;
+  copy.init(wave, lane);
+  const uint32_t dst = (uint32_t)lds0 + 1024 * PK_NDMA * wave;
+  floatx16 acc[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db) zero(acc[db]);
+  const float c = a.scale_log2;
+  const int T = (it.bound + BN - 1) / BN;
+  if (T > 0) {
+    copy.issue(kb, ks, 0, it.other_len, dst);
+    copy.issue(vb, vs, 0, it.other_len, dst + V_AT);
+  }
+#pragma unroll 1
+  for (int u = 0; u < T; ++u) {
+    const int st = (u & 1) * PK_TILE_B;
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    barrier_nofence();
+    if (u + 1 < T) {
+      copy.issue(kb, ks, (u + 1) * BN, it.other_len, dst + (PK_TILE_B - st));
+      copy.issue(vb, vs, (u + 1) * BN, it.other_len, dst + V_AT + (PK_TILE_B - st));
+    }
+    if (!active || u * BN >= lim_hi) continue;
+#pragma unroll
+    for (int kb32 = 0; kb32 < 2; ++kb32) {
+      const int at = st + kb32 * 32 * PK_ROWB;
+      floatx16 s, dp;
+      zero(s);
+      zero(dp);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        s = mfma32x32x16(lds_read_b128(off[d] + at), qf[d], s);
+        dp = mfma32x32x16(lds_read_b128(off[d] + at + V_AT), gf[d], dp);
+      }
+      const int key0 = u * BN + 32 * kb32;
+      floatx16 ds;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        ds[r] = fast_exp2(__builtin_fmaf(s[r], c, -lse2)) * (dp[r] - delta);
+      if (key0 + 32 > lim_lo) {
+        const int left = lim - (key0 + 4 * hl);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ds[r] = acc_row(r) < left ? ds[r] : 0.0f;
+      }
+      const u32x4 pf[2] = {pack_half(ds, 0), pack_half(ds, 1)};
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int mm = 0; mm < 2; ++mm)
+          acc[db] = mfma32x32x16(read_tr(toff, db, mm, at), pf[mm], acc[db]);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  barrier_nofence();
+  if (!active) return;
+  store_rows(lds + 8192 * wave, acc, a.scale, lane, rows, [&](int r) {
+    return a.dq.p + (int64_t)(it.row0 + r0 + r) * a.dq.sl + h * a.dq.sh;
+  });
+}
+
+// ---- dK, dV: a lane holds one key's column of S = Q K^T and dP = dO V^T
+__global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const PackedArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hl = lane >> 5, l32 = lane & 31;
+  const int kv = blockIdx.x % (uint32_t)a.Hk, group = a.Hq / a.Hk;
+  const PackedItem it = load_item(a.k_items, blockIdx.x / (uint32_t)a.Hk);
+  if (!item_fits(it, a.Tk, a.Tq)) return;
+  const int r0 = 32 * wave, rows = it.rows - r0;
+  const bool active = rows > 0;
+
+  u32x4 kf[8], vf[8];
+  if (active) {
+    const int64_t row = it.row0 + r0;
+    load_rows(a.k.p + row * a.k.sl + kv * a.k.sh, a.k.sl, rows, l32, hl, kf);
+    load_rows(a.v.p + row * a.v.sl + kv * a.v.sh, a.v.sl, rows, l32, hl, vf);
+  }
+  // first query that sees this lane's key, and the wave's smallest and largest such
+  const int j0 = it.pos0 + r0;
+  auto first = [&](int j) {
+    const int64_t x = (int64_t)j - it.shift;
+    return (int)(x < 0 ? 0 : (x < it.other_len ? x : it.other_len));
+  };
+  const int lo = first(j0 + l32);
+  const int lo_min = first(j0), lo_max = first(j0 + 31);
+
+  const int lds0 = (int)lds_addr(lds);
+  int off[8], toff[4][2];
+  row_offsets(lds0, l32, hl, off);
+  tr_offsets(lds0, lane, hl, toff);
+  TileCopy copy;
+  copy.init(wave, lane);
+  const uint32_t dst = (uint32_t)lds0 + 1024 * PK_NDMA * wave;
+  floatx16 dk[4], dv[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db) {
+    zero(dk[db]);
+    zero(dv[db]);
+  }
+  const float c = a.scale_log2;
+  const int t_first = it.bound / BN, t_end = (it.other_len + BN - 1) / BN;
+  const int per = it.bound < it.other_len ? t_end - t_first : 0;  // query tiles of a head
+  const int T = per * group;
+  const int64_t qs = a.q.sl * 2, gs = a.dout.sl * 2;
+  float* const stat = reinterpret_cast<float*>(lds + STAT_AT);
+  // query tile n (head n / per of the group) into stage n % 2; wave 0 fetches the rows' lse and delta
+  float st_l = 0.0f, st_d = 0.0f;
+  auto issue = [&](int n) {
+    const int h = kv * group + n / per, first_row = (t_first + n % per) * BN;
+    const uint32_t to = dst + (n & 1) * PK_TILE_B;
+    if (wave == 0) {
+      const bool in = first_row + lane < it.other_len;
+      const int64_t at = (int64_t)h * a.Tq + it.other0 + first_row + lane;
+      st_l = in ? a.lse[at] : -INFINITY;
+      st_d = in ? a.delta[at] : 0.0f;
+    }
+    copy.issue(reinterpret_cast<const unsigned char*>(a.q.p + (int64_t)it.other0 * a.q.sl + h * a.q.sh),
+               qs, first_row, it.other_len, to);
+    copy.issue(reinterpret_cast<const unsigned char*>(a.dout.p + (int64_t)it.other0 * a.dout.sl +
+                                                      h * a.dout.sh),
+               gs, first_row, it.other_len, to + V_AT);
+  };
+  // rows past the sequence's end, and rows that see no key: p = exp2(s - inf) = 0
+  auto put_stat = [&](int n) {
+    if (wave == 0) {
+      stat[(n & 1) * 2 * BN + lane] = st_l == -INFINITY ? INFINITY : st_l * LOG2E;
+      stat[(n & 1) * 2 * BN + BN + lane] = st_d;
+    }
+  };
+  if (T > 0) issue(0);
+#pragma unroll 1
+  for (int n = 0; n < T; ++n) {
+    const int st = (n & 1) * PK_TILE_B;
+    put_stat(n);
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): the tile and its statistics
+    barrier_nofence();
+    if (n + 1 < T) issue(n + 1);
+    const int row0 = (t_first + n % per) * BN;
+    if (!active || row0 + BN <= lo_min) continue;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      const int at = st + qb * 32 * PK_ROWB;
+      const int sa = lds0 + STAT_AT + (n & 1) * 2 * BN * 4 + (32 * qb + 4 * hl) * 4;
+      floatx16 s, dp;
+      zero(s);
+      zero(dp);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) {
+        s = mfma32x32x16(lds_read_b128(off[d] + at), kf[d], s);
+        dp = mfma32x32x16(lds_read_b128(off[d] + at + V_AT), vf[d], dp);
+      }
+      floatx16 p, ds;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const u32x4 l4 = lds_read_b128(sa + 32 * g), d4 = lds_read_b128(sa + 32 * g + BN * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * g + e;
+          p[r] = fast_exp2(__builtin_fmaf(s[r], c, -__uint_as_float(l4[e])));
+          ds[r] = dp[r] - __uint_as_float(d4[e]);
+        }
+      }
+      const int i0 = row0 + 32 * qb;
+      if (i0 < lo_max) {  // (register r is query i0 + 4 hl + acc_row(r))
+        const int skip = lo - (i0 + 4 * hl);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          p[r] = acc_row(r) >= skip ? p[r] : 0.0f;
+          ds[r] = acc_row(r) >= skip ? ds[r] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] *= p[r];
+      const u32x4 pf[2] = {pack_half(p, 0), pack_half(p, 1)};
+      const u32x4 df[2] = {pack_half(ds, 0), pack_half(ds, 1)};
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int mm = 0; mm < 2; ++mm) {
+          dv[db] = mfma32x32x16(read_tr(toff, db, mm, at + V_AT), pf[mm], dv[db]);
+          dk[db] = mfma32x32x16(read_tr(toff, db, mm, at), df[mm], dk[db]);
+        }
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  barrier_nofence();
+  if (!active) return;
+  store_rows(lds + 8192 * wave, dk, a.scale, lane, rows, [&](int r) {
+    return a.dk.p + (int64_t)(it.row0 + r0 + r) * a.dk.sl + kv * a.dk.sh;
+  });
+  wave_lds_fence();
+  store_rows(lds + 8192 * wave, dv, 1.0f, lane, rows, [&](int r) {
+    return a.dv.p + (int64_t)(it.row0 + r0 + r) * a.dv.sl + kv * a.dv.sh;
+  });
+}
+
+}  // namespace
+
+hipError_t launch_packed_dq(const PackedArgs& a, hipStream_t stream) {
+  static hipError_t attr = hipFuncSetAttribute((const void*)packed_dq_kernel,
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, BWD_LDS);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL(packed_dq_kernel, dim3((uint32_t)a.n_q_items * a.Hq), dim3(PK_WAVES * 64),
+                     BWD_LDS, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream) {
+  static hipError_t attr = hipFuncSetAttribute((const void*)packed_dkv_kernel,
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, DKV_LDS);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL(packed_dkv_kernel, dim3((uint32_t)a.n_k_items * a.Hk), dim3(PK_WAVES * 64),
+                     DKV_LDS, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace lbw

@@ -1,0 +1,151 @@
+// What the packed attention kernels share: work items, tile staging and masks.
+//
+// A 64-row tile of a bf16 operand lies in LDS as 64 rows of 256 bytes, 16-byte chunk c of row r at
+// chunk c ^ swz(r) (attn_tiles.h), so that both the row reads (A operand, ds_read_b128) and the
+// transpose reads (ds_read_b64_tr_b16) are free of bank conflicts.
+#pragma once
+
+#include "attn_tiles.h"
+#include "packed.h"
+
+namespace lbw {
+
+constexpr int PK_WAVES = PK_BLOCK / 32;         // waves per workgroup, 32 rows each
+constexpr int PK_ROWB = D * 2;                  // bytes per row in LDS
+constexpr int PK_TILE_B = BN * PK_ROWB;         // 16 KB
+constexpr int PK_NDMA = PK_TILE_B / (PK_WAVES * 64 * 16);  // 16-byte copies per lane and tile
+
+// A work item's fields, in scalar registers.
+struct PackedItem {
+  int row0, rows, pos0, other0, other_len, bound, shift;
+};
+__device__ __forceinline__ PackedItem load_item(const int32_t* items, int i) {
+  const int32_t* p = items + (int64_t)i * PK_ITEM;
+  PackedItem t;
+  t.row0 = __builtin_amdgcn_readfirstlane(p[0]);
+  t.rows = __builtin_amdgcn_readfirstlane(p[1]);
+  t.pos0 = __builtin_amdgcn_readfirstlane(p[2]);
+  t.other0 = __builtin_amdgcn_readfirstlane(p[3]);
+  t.other_len = __builtin_amdgcn_readfirstlane(p[4]);
+  t.bound = __builtin_amdgcn_readfirstlane(p[5]);
+  t.shift = __builtin_amdgcn_readfirstlane(p[6]);
+  return t;
+}
+// Whether the item stays inside the packed rows it names (tables come from lbw_attention_packed_plan;
+// one made for other tensors is skipped rather than followed out of them).
+__device__ __forceinline__ bool item_fits(const PackedItem& t, int64_t own, int64_t other) {
+  return t.row0 >= 0 && t.rows > 0 && t.rows <= PK_BLOCK && (int64_t)t.row0 + t.rows <= own &&
+         t.pos0 >= 0 && t.other0 >= 0 && t.other_len >= 0 &&
+         (int64_t)t.other0 + t.other_len <= other && t.bound >= 0 && t.bound <= t.other_len;
+}
+
+// Workgroup i works on item i / Hq (the costliest first) for head i % Hq, counted with the
+// key/value head fastest: with a multiple of 8 of them, every XCD keeps its own key/value heads in L2.
+__device__ __forceinline__ void pick_head(uint32_t c, int Hk, int group, int& h, int& kv) {
+  kv = c % (uint32_t)Hk;
+  h = kv * group + c / (uint32_t)Hk;
+}
+
+// This wave's share of a tile copied HBM -> LDS: rows first .. first + 63 of a sequence of `len`
+// rows at `base` (its row 0), row stride `stride_b` bytes; rows past the end copy the last row, so
+// a tile never touches another sequence.
+struct TileCopy {
+  int row[PK_NDMA], col[PK_NDMA];
+  __device__ __forceinline__ void init(int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < PK_NDMA; ++i) {
+      row[i] = 4 * (PK_NDMA * wave + i) + (lane >> 4);
+      col[i] = ((lane & 15) ^ swz(row[i])) * 16;
+    }
+  }
+  __device__ __forceinline__ void issue(const unsigned char* base, int64_t stride_b, int first,
+                                        int len, uint32_t dst) const {
+    const unsigned char* b = base + (int64_t)first * stride_b;
+    const int last = len - 1 - first;
+#pragma unroll
+    for (int i = 0; i < PK_NDMA; ++i) {
+      const int r = row[i] < last ? row[i] : last;
+      dma16_guarded(b, (uint32_t)r * (uint32_t)stride_b + col[i], dst + 1024 * i);
+    }
+  }
+};
+
+// Per-lane LDS byte offsets of a tile's fragments, 32-row block 0.
+// Row reads (A operand, d-slice s): row l32, logical chunk 2s + hl.
+__device__ __forceinline__ void row_offsets(int base, int l32, int hl, int (&off)[8]) {
+#pragma unroll
+  for (int s = 0; s < 8; ++s) off[s] = base + l32 * PK_ROWB + (((2 * s + hl) ^ swz(l32)) << 4);
+}
+// Transpose reads for d-block db and row half j: source row 4hl + 8j + s / 4, columns
+// 32 db + 16 g + 4 (s % 4) .. +3 (s = lane % 16, g = (lane / 16) % 2); rows 16m further along
+// give the lane values k = 16m + 4hl + 8 (e / 4) + e % 4 of the operand's k-group, the order of
+// the accumulator registers 8m + e.
+__device__ __forceinline__ void tr_offsets(int base, int lane, int hl, int (&off)[4][2]) {
+  const int s16 = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = 4 * hl + 8 * j + (s16 >> 2);
+      const int lc = 4 * db + 2 * g + ((s16 & 3) >> 1);
+      off[db][j] = base + r * PK_ROWB + ((lc ^ swz(r)) << 4) + 8 * (s16 & 1);
+    }
+}
+__device__ __forceinline__ u32x4 read_tr(const int (&off)[4][2], int db, int m, int at) {
+  const u32x2 v0 = lds_read_tr16(off[db][0] + at + 16 * m * PK_ROWB);
+  const u32x2 v1 = lds_read_tr16(off[db][1] + at + 16 * m * PK_ROWB);
+  return u32x4{v0[0], v0[1], v1[0], v1[1]};
+}
+
+// Index within its 32-block of accumulator register r (rows of the product).
+__device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+__device__ __forceinline__ void zero(floatx16& x) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+}
+
+// Registers 8m .. 8m + 7 as a bf16 operand of 8 k-values.
+__device__ __forceinline__ u32x4 pack_half(const floatx16& p, int m) {
+  u32x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = pack_bf16x2(p[8 * m + 2 * e], p[8 * m + 2 * e + 1]);
+  return w;
+}
+
+// A wave's [32 rows x 128] result from the transposed accumulators (lane: row l32, d = 32 db +
+// 8 g + 4 hl ..) times f, to bf16 rows: through 8 KB of LDS, so that whole rows leave.
+template <typename RowPtr>
+__device__ __forceinline__ void store_rows(unsigned char* stg, const floatx16 (&acc)[4], float f,
+                                           int lane, int rows, RowPtr row_ptr) {
+  const int l32 = lane & 31, hl = lane >> 5;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      u32x2 w;
+      w[0] = pack_bf16x2(acc[db][4 * g + 0] * f, acc[db][4 * g + 1] * f);
+      w[1] = pack_bf16x2(acc[db][4 * g + 2] * f, acc[db][4 * g + 3] * f);
+      *reinterpret_cast<u32x2*>(stg + l32 * 256 + (((4 * db + g) ^ (l32 & 15)) << 4) + 8 * hl) = w;
+    }
+  wave_lds_fence();
+  const int rrow = lane >> 4, rch = lane & 15;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const int r = 4 * k + rrow;
+    const u32x4 v = *reinterpret_cast<const u32x4*>(stg + r * 256 + ((rch ^ (r & 15)) << 4));
+    if (r < rows) *reinterpret_cast<u32x4*>(row_ptr(r) + 8 * rch) = v;
+  }
+}
+
+// 32 rows x 128 as a B operand in registers: lane column l32 holds row min(l32, rows - 1),
+// d = 16 s + 8 hl .. +7.
+__device__ __forceinline__ void load_rows(const uint16_t* base, int64_t stride, int rows, int l32,
+                                          int hl, u32x4 (&f)[8]) {
+  const int r = l32 < rows ? l32 : rows - 1;
+  const uint16_t* p = base + (int64_t)r * stride + 8 * hl;
+#pragma unroll
+  for (int s = 0; s < 8; ++s) f[s] = *reinterpret_cast<const u32x4*>(p + 16 * s);
+}
+
+}  // namespace lbw

@@ -12,7 +12,10 @@ from .attention import (PRESCALED_SOFTMAX_SCALE, attention, attention_chain, att
 from .chunked_kv_cache import (FlatKVCache, allocate_self_kv_chunks, allocate_self_kv_chunks_fp8,
                                chunk_routing, num_chunks)
 from .fp8 import Fp8KV, attention_fp8kv, quantize_kv_fp8
+from .head_norm import AxisRope, axis_rope, qk_head_norm_rope, qk_head_norm_rope_
 from .layer import WanCrossAttention, WanSelfAttention
+from .packed import (PackedPlan, attention_decode, attention_packed, attention_packed_backward,
+                     packed_plan)
 from .qk_post import (qk_norm_rope, qk_norm_rope3, qk_norm_rope_, qk_norm_rope_t, qk_norm_rope_t3,
                       x_norm_rope, x_norm_rope_t3)
 from .rope import RopeTables, causal_rope_tables, rope_params, wan_rope_freqs
@@ -27,4 +30,6 @@ __all__ = [
     "wan_rope_freqs", "Fp8KV", "quantize_kv_fp8", "attention_fp8kv", "FlatKVCache",
     "allocate_self_kv_chunks", "allocate_self_kv_chunks_fp8", "chunk_routing", "num_chunks", "WanSelfAttention",
     "WanCrossAttention",
+    "AxisRope", "axis_rope", "qk_head_norm_rope", "qk_head_norm_rope_",
+    "PackedPlan", "packed_plan", "attention_packed", "attention_packed_backward", "attention_decode",
 ]

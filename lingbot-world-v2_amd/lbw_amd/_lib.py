@@ -77,6 +77,76 @@ class QkNormRopeParams(ctypes.Structure):
     ]
 
 
+class HeadNormRopeParams(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("q_stride_l", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_stride_l", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p), ("w_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("rope", ctypes.c_void_p), ("rope_rows", ctypes.c_int64),
+        ("rope_pairs", ctypes.c_int32), ("n_axes", ctypes.c_int32),
+        ("axis_pairs", ctypes.c_int32 * 4), ("interleaved", ctypes.c_int32),
+        ("pos", ctypes.c_void_p), ("pos_stride", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p), ("q_out_stride_l", ctypes.c_int64), ("q_out_stride_h", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p), ("k_out_stride_l", ctypes.c_int64), ("k_out_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride_l", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+        ("v_out", ctypes.c_void_p), ("v_out_stride_l", ctypes.c_int64), ("v_out_stride_h", ctypes.c_int64),
+        ("rows", ctypes.c_void_p), ("row_count", ctypes.c_int32),
+        ("k_out_stride_b", ctypes.c_int64), ("v_out_stride_b", ctypes.c_int64),
+        ("q_out_scale", ctypes.c_float), ("k_out_scale", ctypes.c_float),
+    ]
+
+
+class HeadNormRopeGrads(ctypes.Structure):
+    _fields_ = [
+        ("dq_out", ctypes.c_void_p), ("dq_out_stride_l", ctypes.c_int64), ("dq_out_stride_h", ctypes.c_int64),
+        ("dk_out", ctypes.c_void_p), ("dk_out_stride_l", ctypes.c_int64), ("dk_out_stride_h", ctypes.c_int64),
+        ("dq", ctypes.c_void_p), ("dq_stride_l", ctypes.c_int64), ("dq_stride_h", ctypes.c_int64),
+        ("dk", ctypes.c_void_p), ("dk_stride_l", ctypes.c_int64), ("dk_stride_h", ctypes.c_int64),
+        ("dwq", ctypes.c_void_p), ("dwk", ctypes.c_void_p),
+    ]
+
+
+class PackedParams(ctypes.Structure):
+    _fields_ = [
+        ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("q_tokens", ctypes.c_int64), ("k_tokens", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("q_stride_l", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_stride_l", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride_l", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_stride_l", ctypes.c_int64), ("out_stride_h", ctypes.c_int64),
+        ("lse", ctypes.c_void_p), ("softmax_scale", ctypes.c_float),
+        ("q_items", ctypes.c_void_p), ("n_q_items", ctypes.c_int32),
+        ("k_items", ctypes.c_void_p), ("n_k_items", ctypes.c_int32),
+    ]
+
+
+class PackedGrads(ctypes.Structure):
+    _fields_ = [
+        ("dout", ctypes.c_void_p), ("dout_stride_l", ctypes.c_int64), ("dout_stride_h", ctypes.c_int64),
+        ("dq", ctypes.c_void_p), ("dq_stride_l", ctypes.c_int64), ("dq_stride_h", ctypes.c_int64),
+        ("dk", ctypes.c_void_p), ("dk_stride_l", ctypes.c_int64), ("dk_stride_h", ctypes.c_int64),
+        ("dv", ctypes.c_void_p), ("dv_stride_l", ctypes.c_int64), ("dv_stride_h", ctypes.c_int64),
+    ]
+
+
+class DecodeParams(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("capacity", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("q_stride_b", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_stride_b", ctypes.c_int64), ("k_stride_l", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride_b", ctypes.c_int64), ("v_stride_l", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64),
+        ("lens", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("out_stride_b", ctypes.c_int64), ("out_stride_h", ctypes.c_int64),
+        ("softmax_scale", ctypes.c_float), ("num_splits", ctypes.c_int32),
+    ]
+
+
 EXPORTS = (
     "lbw_attention_workspace_size", "lbw_attention_fp8kv_workspace_size", "lbw_attention_fwd",
     "lbw_cross_attention_fwd",
@@ -85,6 +155,10 @@ EXPORTS = (
     "lbw_attn_merge_partials", "lbw_attention_chain_workspace_size", "lbw_attention_chain",
     "lbw_qk_norm_rope",
     "lbw_kv_quant_fp8",
+    "lbw_head_norm_rope", "lbw_head_norm_rope_bwd_workspace_size", "lbw_head_norm_rope_bwd",
+    "lbw_attention_packed_plan", "lbw_attention_packed_fwd",
+    "lbw_attention_packed_bwd_workspace_size", "lbw_attention_packed_bwd",
+    "lbw_attention_decode_workspace_size", "lbw_attention_decode",
     "lbw_last_error", "lbw_abi_version",
 )
 
@@ -123,6 +197,27 @@ def _declare(lib):
     lib.lbw_qk_norm_rope.restype = ctypes.c_int
     lib.lbw_kv_quant_fp8.argtypes = [vp, i32, i64, i32, i32, i64, i64, i64, vp, vp, i32, vp]
     lib.lbw_kv_quant_fp8.restype = ctypes.c_int
+    lib.lbw_head_norm_rope.argtypes = [P(HeadNormRopeParams), vp]
+    lib.lbw_head_norm_rope.restype = ctypes.c_int
+    lib.lbw_head_norm_rope_bwd_workspace_size.argtypes = [P(HeadNormRopeParams)]
+    lib.lbw_head_norm_rope_bwd_workspace_size.restype = ctypes.c_size_t
+    lib.lbw_head_norm_rope_bwd.argtypes = [P(HeadNormRopeParams), P(HeadNormRopeGrads), vp,
+                                           ctypes.c_size_t, vp]
+    lib.lbw_head_norm_rope_bwd.restype = ctypes.c_int
+    lib.lbw_attention_packed_plan.argtypes = [i32, P(i32), P(i32), i32, P(i32), i64, P(i64),
+                                              P(i32), i64, P(i64)]
+    lib.lbw_attention_packed_plan.restype = ctypes.c_int
+    lib.lbw_attention_packed_fwd.argtypes = [P(PackedParams), vp]
+    lib.lbw_attention_packed_fwd.restype = ctypes.c_int
+    lib.lbw_attention_packed_bwd_workspace_size.argtypes = [P(PackedParams)]
+    lib.lbw_attention_packed_bwd_workspace_size.restype = ctypes.c_size_t
+    lib.lbw_attention_packed_bwd.argtypes = [P(PackedParams), P(PackedGrads), vp, ctypes.c_size_t,
+                                             vp]
+    lib.lbw_attention_packed_bwd.restype = ctypes.c_int
+    lib.lbw_attention_decode_workspace_size.argtypes = [P(DecodeParams)]
+    lib.lbw_attention_decode_workspace_size.restype = ctypes.c_size_t
+    lib.lbw_attention_decode.argtypes = [P(DecodeParams), vp, ctypes.c_size_t, vp]
+    lib.lbw_attention_decode.restype = ctypes.c_int
     lib.lbw_last_error.argtypes = []
     lib.lbw_last_error.restype = ctypes.c_char_p
     lib.lbw_abi_version.argtypes = []

@@ -1,0 +1,182 @@
+"""qk_head_norm_rope and its gradient against the 64-bit definition."""
+import pytest
+import torch
+
+import packed_ref as R
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def _data(T, hq, hk, d, seed, w_dtype=BF, gain=2.0):
+    g = torch.Generator().manual_seed(seed)
+    qkv = (torch.randn(T, (hq + 2 * hk) * d, generator=g) * gain).to(BF).cuda()
+    q = qkv[:, :hq * d].unflatten(1, (hq, d))
+    k = qkv[:, hq * d:(hq + hk) * d].unflatten(1, (hk, d))
+    v = qkv[:, (hq + hk) * d:].unflatten(1, (hk, d))
+    w = [(1 + 0.2 * torch.randn(d, generator=g)).to(w_dtype).cuda() for _ in range(2)]
+    return q, k, v, w
+
+
+def _rope(axes, rows, inter, seed=0):
+    import lbw_amd
+    g = torch.Generator().manual_seed(100 + seed)
+    ang = (torch.rand(rows, sum(axes), generator=g) * 50 - 25).cuda()
+    return ang, lbw_amd.axis_rope(ang, axes, interleaved=inter)
+
+
+def _pos(T, axes, rows, seed=0):
+    g = torch.Generator().manual_seed(200 + seed)
+    return torch.randint(0, rows, (T, len(axes)), generator=g, dtype=torch.int32).cuda()
+
+
+CASES = [  # T, hq, hk, d, axes, interleaved, weights
+    (1, 1, 1, 32, (16,), True, BF), (3, 5, 1, 64, (8,), False, BF), (67, 40, 8, 128, (22, 21, 21), True, BF),
+    (130, 12, 12, 128, (64,), False, torch.float32), (257, 6, 3, 256, (40, 24), False, BF),
+    (9, 3, 3, 128, (5, 1, 4, 3), True, torch.float32), (33, 7, 7, 64, (0, 32), True, None),
+    (5000, 2, 1, 128, (30, 10), True, BF), (4, 33, 11, 32, (0,), True, BF),
+]
+
+
+@pytest.mark.parametrize("T,hq,hk,d,axes,inter,wd", CASES)
+def test_forward_and_gradient(T, hq, hk, d, axes, inter, wd):
+    import lbw_amd
+    q, k, _, w = _data(T, hq, hk, d, T + d, wd or BF)
+    w = w if wd is not None else [None, None]
+    ang, rope = _rope(axes, 50, inter)
+    pos = _pos(T, axes, 50)
+    qs, ks, eps = 0.7, 1.0, 1e-5
+    q, k = q.detach().requires_grad_(), k.detach().requires_grad_()
+    for x in w:
+        if x is not None:
+            x.requires_grad_()
+    q2, k2 = lbw_amd.qk_head_norm_rope(q, k, w[0], w[1], rope, pos, eps, q_scale=qs, k_scale=ks)
+    g = torch.Generator().manual_seed(7)
+    # gradients as a network hands them back: another layout, and one broadcast over the heads
+    dq2 = torch.randn(hq, T, d, generator=g).to(BF).cuda().transpose(0, 1)
+    dk2 = torch.randn(T, 1, d, generator=g).to(BF).cuda().expand(T, hk, d)
+    leaves = [x for x in (q, k, *w) if x is not None]
+    grads = torch.autograd.grad((q2, k2), leaves, (dq2, dk2))
+    a = R.token_angles(ang, axes, pos)
+    for n, (x, y, dy, ww, s) in enumerate(((q, q2, dq2, w[0], qs), (k, k2, dk2, w[1], ks))):
+        X = x.detach().double().requires_grad_()
+        W = ww.detach().double().requires_grad_() if ww is not None else None
+        Y = R.head_norm(X, W, a, inter, eps, s)
+        R.assert_within("qk"[n] + "'", y, Y.detach(), R.head_norm_allow(Y.detach()))
+        G = torch.autograd.grad(Y, [X] if W is None else [X, W], dy.double())
+        # r (g w - x r mean(g w x r)): before the one rounding an fp32 sum over the head (d <= 256 terms)
+        # of products; 2^10 E of the sizes of the two terms
+        r = torch.rsqrt(X.detach().square().mean(-1, keepdim=True) + eps)
+        gw = R.rotate(dy.double(), a.cos(), -a.sin(), inter).abs() * s
+        gw = gw * (W.detach().abs() if W is not None else 1)
+        size = r * (gw.amax(-1, keepdim=True) +
+                    (X.detach().abs() * r).amax(-1, keepdim=True) *
+                    (gw * X.detach().abs() * r).mean(-1, keepdim=True))
+        R.assert_within("d" + "qk"[n], grads[n], G[0], R.H * G[0].abs() + 2 ** 10 * R.E * size)
+        if W is not None:
+            terms = (R.rotate(dy.double(), a.cos(), -a.sin(), inter) * s * X.detach() * r).abs().sum((0, 1))
+            half = R.H if ww.dtype == BF else R.E
+            # each lane adds its tokens in turn, then lanes, waves and workgroups: no term passes
+            # through more than T + 200 additions
+            R.assert_within("dw" + "qk"[n], grads[2 + n], G[1],
+                            half * G[1].abs() + (T + 200) * R.E * terms)
+
+
+def test_same_bits_every_run():
+    import lbw_amd
+    q, k, _, w = _data(3001, 12, 4, 128, 5)
+    _, rope = _rope((64,), 3001, False)
+    pos = torch.arange(3001, dtype=torch.int32, device="cuda")
+    leaves = [x.detach().requires_grad_() for x in (q, k, *w)]
+    out = []
+    for _ in range(3):
+        y = lbw_amd.qk_head_norm_rope(*leaves, rope, pos)
+        out.append(y + torch.autograd.grad(y, leaves, (y[0].detach(), y[1].detach())))
+    for o in out[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(out[0], o))
+
+
+def test_only_one_output_used_and_int_edges():
+    import lbw_amd
+    q, k, _, w = _data(8, 4, 2, 64, 6)
+    _, rope = _rope((32,), 8, True)
+    pos = torch.arange(8, dtype=torch.int32, device="cuda")
+    leaves = [x.detach().requires_grad_() for x in (q, k, *w)]
+    y = lbw_amd.qk_head_norm_rope(*leaves, rope, pos)
+    g = torch.autograd.grad(y[0], leaves, torch.ones_like(y[0]))
+    assert torch.all(g[1] == 0) and torch.all(g[3] == 0) and g[0].abs().max() > 0
+    # no tokens
+    y = lbw_amd.qk_head_norm_rope(leaves[0][:0], leaves[1][:0], leaves[2], leaves[3], rope, pos[:0])
+    assert y[0].shape == (0, 4, 64)
+    g = torch.autograd.grad(y[0].sum() + y[1].sum(), leaves[2:])
+    assert all(torch.all(x == 0) for x in g)
+
+
+def test_position_outside_the_table_is_nan_only_there():
+    import lbw_amd
+    q, k, _, w = _data(4, 2, 2, 128, 8)
+    _, rope = _rope((20, 12), 10, True)
+    pos = torch.tensor([[3, 3], [10, 3], [3, -1], [9, 0]], dtype=torch.int32, device="cuda")
+    y, _ = lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos)
+    nan = torch.isnan(y)
+    assert not nan[0].any() and not nan[3].any()
+    assert nan[1, :, :40].all() and not nan[1, :, 40:].any()
+    assert nan[2, :, 40:64].all() and not nan[2, :, :40].any() and not nan[2, :, 64:].any()
+
+
+@pytest.mark.parametrize("T,hq,hk,d", [(1, 40, 8, 128), (64, 12, 4, 128), (7, 3, 3, 64), (5, 6, 2, 256)])
+def test_write_form_into_cache_rows(T, hq, hk, d):
+    import lbw_amd
+    q, k, v, w = _data(T, hq, hk, d, 9)
+    ang, rope = _rope((d // 4,), 40, False)
+    cap = 33
+    buf = torch.full((2, T, cap + 1, hk, d), 7.0, dtype=BF, device="cuda")
+    kc, vc = buf[0][:, :cap], buf[1][:, :cap]      # (strided: the caches end before their buffers)
+    rows = torch.arange(T, dtype=torch.int32, device="cuda") * 5 % cap
+    if T > 3:
+        rows[1], rows[2] = -1, cap               # not written
+    pos = torch.arange(T, dtype=torch.int32, device="cuda") % 40
+    qo = torch.empty(T, hq, d, dtype=BF, device="cuda")
+    lbw_amd.qk_head_norm_rope_(q, k, *w, rope, pos, q_out=qo, k_out=kc, v=v, v_out=vc, rows=rows)
+    q2, k2 = lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos)
+    assert torch.equal(qo, q2)
+    want = torch.full_like(buf, 7.0)
+    for t, r in enumerate(rows.tolist()):
+        if 0 <= r < cap:
+            want[0, t, r], want[1, t, r] = k2[t], v[t]
+    assert torch.equal(buf, want)
+
+
+def test_write_form_in_place_and_strided():
+    import lbw_amd
+    q, k, v, w = _data(50, 10, 5, 128, 10)
+    _, rope = _rope((64,), 50, False)
+    pos = torch.arange(50, dtype=torch.int32, device="cuda")
+    want = lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos)
+    v0 = v.clone()
+    lbw_amd.qk_head_norm_rope_(q, k, *w, rope, pos, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, v0)
+
+
+def test_refusals_on_the_device():
+    import lbw_amd
+    q, k, v, w = _data(8, 4, 2, 128, 11)
+    _, rope = _rope((64,), 8, True)
+    pos = torch.zeros(8, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="overlaps"):
+        buf = torch.zeros(9, 4, 128, dtype=BF, device="cuda")
+        lbw_amd.qk_head_norm_rope_(buf[:8], k, *w, rope, pos, q_out=buf[1:], k_out=k.clone())
+    with pytest.raises(RuntimeError, match="one place"):
+        lbw_amd.qk_head_norm_rope_(q, k, *w, rope, pos, q_out=q[:1].expand(8, 4, 128), k_out=k.clone())
+    with pytest.raises(RuntimeError, match="multiples of 8"):
+        lbw_amd.qk_head_norm_rope(torch.zeros(8, 4 * 129, dtype=BF, device="cuda").unflatten(1, (4, 129))[..., :128],
+                                  k, *w, rope, pos)
+    with pytest.raises(ValueError, match="another device"):
+        lbw_amd.qk_head_norm_rope(q, k, *w, lbw_amd.axis_rope(torch.zeros(8, 64)), pos)
+    with pytest.raises(RuntimeError, match="pos"):
+        lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos.cpu())
+    x = q.detach().requires_grad_()
+    y = lbw_amd.qk_head_norm_rope(x, k, *w, rope, pos)[0]
+    g, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()  # no second derivatives

@@ -1,0 +1,251 @@
+"""CPU checks of the operators on packed sequences: the plan covers every row and pair once, the
+oracle's gradients against differences, refusals of arguments, struct layouts."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+import packed_ref as R
+from test_capi import HEADER, _header_struct, _header_struct_fields, _layout  # noqa: F401
+
+
+def lbw():
+    import lbw_amd
+    return lbw_amd
+
+
+LENS = [([300, 1, 0, 129], [300, 5, 3, 20], True), ([128, 256, 127], [128, 256, 127], True),
+        ([5], [5], False), ([0, 0], [0, 7], True), ([7, 3], [0, 0], False), ([], [], True),
+        ([64, 200], [1000, 30], True), ([64, 200], [1000, 30], False)]
+
+
+@pytest.mark.parametrize("ql,kl,causal", LENS)
+def test_plan_covers_every_row_once_and_bounds_what_is_seen(ql, kl, causal):
+    p = lbw().packed_plan(ql, kl, causal=causal, device="cpu")
+    assert (p.q_tokens, p.k_tokens) == (sum(ql), sum(kl))
+    q_at = [sum(ql[:s]) for s in range(len(ql))]
+    k_at = [sum(kl[:s]) for s in range(len(kl))]
+    rows = []
+    for row0, n, pos, other0, other, bound, shift, _ in p.q_items.tolist():
+        assert 0 < n <= 128
+        s = max(x for x in range(len(ql)) if q_at[x] == row0 - pos and ql[x] > 0 and pos < ql[x])
+        assert (other0, other) == (k_at[s], kl[s]) and pos + n <= ql[s]
+        for i in range(pos, pos + n):
+            seen = [j for j in range(kl[s]) if not causal or j <= i + kl[s] - ql[s]]
+            assert seen == [j for j in range(kl[s]) if j <= i + shift]
+            assert not seen or seen[-1] < bound
+        assert bound == (seen[-1] + 1 if seen else 0)
+        rows += range(row0, row0 + n)
+    assert sorted(rows) == list(range(sum(ql)))
+    keys = []
+    for row0, n, pos, other0, other, bound, shift, _ in p.k_items.tolist():
+        assert 0 < n <= 128
+        s = max(x for x in range(len(kl)) if k_at[x] == row0 - pos and kl[x] > 0 and pos < kl[x])
+        assert (other0, other) == (q_at[s], ql[s]) and pos + n <= kl[s]
+        sees = [i for i in range(ql[s]) if pos <= i + shift]
+        assert bound == (sees[0] if sees else ql[s])
+        keys += range(row0, row0 + n)
+    assert sorted(keys) == list(range(sum(kl)))
+    cost = [x[5] for x in p.q_items.tolist()]
+    assert cost == sorted(cost, reverse=True)
+
+
+def test_plan_refusals():
+    with pytest.raises(ValueError, match="negative"):
+        lbw().packed_plan([3, -1], device="cpu")
+    with pytest.raises(ValueError, match="lengths"):
+        lbw().packed_plan([3], [3, 4], device="cpu")
+    with pytest.raises(ValueError, match="2\\^31"):
+        lbw().packed_plan([2 ** 30, 2 ** 30], device="cpu")
+    from lbw_amd import _lib
+    lib = _lib.load()
+    n = ctypes.c_int64()
+    lens = (ctypes.c_int32 * 1)(300)
+    items = (ctypes.c_int32 * 8)()
+    assert lib.lbw_attention_packed_plan(1, lens, lens, 1, items, 1, ctypes.byref(n), items, 1,
+                                         ctypes.byref(n)) == 1
+    assert b"room for 3" in lib.lbw_last_error()
+    assert lib.lbw_attention_packed_plan(1, None, lens, 1, None, 0, ctypes.byref(n), None, 0,
+                                         ctypes.byref(n)) == 1
+    assert lib.lbw_attention_packed_plan(1, lens, lens, 1, None, 0, None, None, 0, None) == 1
+
+
+@pytest.mark.parametrize("cname,pyname", [("lbw_head_norm_rope_params", "HeadNormRopeParams"),
+                                          ("lbw_head_norm_rope_grads", "HeadNormRopeGrads"),
+                                          ("lbw_packed_params", "PackedParams"),
+                                          ("lbw_packed_grads", "PackedGrads"),
+                                          ("lbw_decode_params", "DecodeParams")])
+def test_struct_layouts_match_the_header(cname, pyname):
+    from lbw_amd import _lib
+    py = getattr(_lib, pyname)
+    assert [f[0] for f in py._fields_] == _header_struct_fields(cname)
+    text = open(HEADER).read()
+    assert "#define LBW_MAX_AXES 4" in text
+    assert _layout(py) == _layout(_header_struct(cname, {}))
+
+
+# ---- the oracle
+
+def _differences(f, xs, grads, seed, steps=3):
+    """Directional differences of scalar f against the gradients, in 64 bits."""
+    gen = torch.Generator().manual_seed(seed)
+    for _ in range(steps):
+        ds = [torch.randn(x.shape, generator=gen, dtype=torch.float64) for x in xs]
+        h = 1e-5
+        num = (f([x + h * d for x, d in zip(xs, ds)]) - f([x - h * d for x, d in zip(xs, ds)])) / (2 * h)
+        ana = sum((g * d).sum() for g, d in zip(grads, ds))
+        # the third derivative's h^2 and the differences' rounding 1e-16 / h, both near 1e-10 of sums of
+        # order 1 to 100
+        assert abs(num - ana) <= 1e-6 * (1 + abs(ana)), (num, ana)
+
+
+@pytest.mark.parametrize("ql,kl,causal", [([5, 0, 9], [5, 3, 4], True), ([4, 6], [9, 6], True),
+                                          ([3, 8], [8, 2], False)])
+def test_oracle_attention_gradient_against_differences(ql, kl, causal):
+    gen = torch.Generator().manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, generator=gen, dtype=torch.float64)  # noqa: E731
+    q, k, v, do = rnd(sum(ql), 4, 16), rnd(sum(kl), 2, 16), rnd(sum(kl), 2, 16), rnd(sum(ql), 4, 16)
+    r = R.attention(q, k, v, ql, kl, causal, 0.3, do)
+    f = lambda xs: (R.attention(*xs, ql, kl, causal, 0.3)["out"] * do).sum()  # noqa: E731
+    _differences(f, [q, k, v], [r["dq"], r["dk"], r["dv"]], 2)
+
+
+@pytest.mark.parametrize("inter", [True, False])
+def test_oracle_norm_is_a_rotation_of_the_normed_head(inter):
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(7, 3, 32, generator=gen, dtype=torch.float64)
+    ang = torch.rand(7, 8, generator=gen, dtype=torch.float64) * 6
+    y = R.head_norm(x, None, ang, inter, 0.0, 1.0)
+    assert torch.allclose(y.square().mean(-1), torch.ones(7, 3, dtype=torch.float64))
+    back = R.rotate(y, ang.cos(), -ang.sin(), inter)
+    assert torch.allclose(back, x / x.square().mean(-1, keepdim=True).sqrt())
+
+
+# ---- refusals (no kernel runs: the wrappers' ValueError, or the C entry's status)
+
+def _rope(pairs=64, **kw):
+    return lbw().axis_rope(torch.zeros(10, pairs), **kw)
+
+
+def test_axis_rope_refusals():
+    with pytest.raises(ValueError, match="add up"):
+        _rope(axes=(10, 20))
+    with pytest.raises(ValueError, match="1 to 4"):
+        _rope(axes=(60, 1, 1, 1, 1))
+    with pytest.raises(ValueError, match="multiple of 8"):
+        _rope(12, interleaved=False)
+    with pytest.raises(ValueError, match="floating"):
+        lbw().axis_rope(torch.zeros(10, dtype=torch.int64))
+
+
+BF = torch.bfloat16
+
+
+def _qk(T=5, hq=4, hk=2, d=128):
+    return torch.zeros(T, hq, d, dtype=BF), torch.zeros(T, hk, d, dtype=BF)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(q=torch.zeros(5, 4, 128)), "bf16"),
+    (dict(q=torch.zeros(5, 128, 4, dtype=BF).transpose(1, 2)), "contiguous head dim"),
+    (dict(k=torch.zeros(4, 2, 128, dtype=BF)), "does not fit"),
+    (dict(k=torch.zeros(5, 3, 128, dtype=BF)), "divides"),
+    (dict(pos=torch.zeros(5, dtype=torch.int64)), "int32"),
+    (dict(pos=torch.zeros(5, 2, dtype=torch.int32)), "pos must"),
+    (dict(wk=None), "both or neither"),
+    (dict(q=torch.zeros(5, 4, 64, dtype=BF), k=torch.zeros(5, 2, 64, dtype=BF)), "pairs do not fit"),
+])
+def test_head_norm_refusals(change, match):
+    q, k = _qk()
+    a = dict(q=q, k=k, wq=torch.ones(128, dtype=BF), wk=torch.ones(128, dtype=BF), rope=_rope(),
+             pos=torch.zeros(5, dtype=torch.int32))
+    a.update(change)
+    with pytest.raises(ValueError, match=match):
+        lbw().qk_head_norm_rope(a["q"], a["k"], a["wq"], a["wk"], a["rope"], a["pos"])
+
+
+def test_head_norm_write_form_refusals():
+    q, k = _qk()
+    call = lambda **kw: lbw().qk_head_norm_rope_(  # noqa: E731
+        q, k, None, None, _rope(), torch.zeros(5, dtype=torch.int32),
+        **{"q_out": q.clone(), "k_out": k.clone(), **kw})
+    with pytest.raises(ValueError, match="q_out"):
+        call(q_out=k)
+    with pytest.raises(ValueError, match="v and v_out"):
+        call(v=k)
+    with pytest.raises(ValueError, match="cache"):
+        call(rows=torch.zeros(5, dtype=torch.int32))
+    with pytest.raises(ValueError, match="cache"):
+        call(rows=torch.zeros(5, dtype=torch.int32), k_out=torch.zeros(4, 8, 2, 128, dtype=BF))
+    with pytest.raises(ValueError, match="rows must"):
+        call(rows=torch.zeros(5, dtype=torch.int64), k_out=torch.zeros(5, 8, 2, 128, dtype=BF))
+
+
+def test_packed_refusals():
+    plan = lbw().packed_plan([5, 3], device="cpu")
+    z = lambda *s: torch.zeros(*s, dtype=BF)  # noqa: E731
+    call = lambda q, k, v, **kw: lbw().attention_packed(q, k, v, plan, **kw)  # noqa: E731
+    with pytest.raises(ValueError, match="the plan 8"):
+        call(z(9, 4, 128), z(8, 2, 128), z(8, 2, 128))
+    with pytest.raises(ValueError, match="bf16"):
+        call(z(8, 4, 64), z(8, 2, 64), z(8, 2, 64))
+    with pytest.raises(ValueError, match="bf16"):
+        call(z(8, 4, 128).half(), z(8, 2, 128), z(8, 2, 128))
+    with pytest.raises(ValueError, match="divides"):
+        call(z(8, 4, 128), z(8, 3, 128), z(8, 3, 128))
+    for bad in (-1.0, 0.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="softmax_scale"):
+            call(z(8, 4, 128), z(8, 2, 128), z(8, 2, 128), softmax_scale=bad)
+    with pytest.raises(ValueError, match="lse"):
+        lbw().attention_packed_backward(z(8, 4, 128), z(8, 4, 128), z(8, 2, 128), z(8, 2, 128),
+                                        z(8, 4, 128), torch.zeros(8, 4), plan)
+
+
+def test_decode_refusals():
+    z = lambda *s: torch.zeros(*s, dtype=BF)  # noqa: E731
+    lens = torch.zeros(2, dtype=torch.int32)
+    call = lbw().attention_decode
+    with pytest.raises(ValueError, match="q must"):
+        call(z(2, 4, 64), z(2, 8, 2, 64), z(2, 8, 2, 64), lens)
+    with pytest.raises(ValueError, match="k_cache"):
+        call(z(2, 4, 128), z(3, 8, 2, 128), z(3, 8, 2, 128), lens)
+    with pytest.raises(ValueError, match="v_cache"):
+        call(z(2, 4, 128), z(2, 8, 2, 128), z(2, 9, 2, 128), lens)
+    with pytest.raises(ValueError, match="divide"):
+        call(z(2, 4, 128), z(2, 8, 3, 128), z(2, 8, 3, 128), lens)
+    with pytest.raises(ValueError, match="lens"):
+        call(z(2, 4, 128), z(2, 8, 2, 128), z(2, 8, 2, 128), lens.long())
+    with pytest.raises(ValueError, match="num_splits"):
+        call(z(2, 4, 128), z(2, 8, 2, 128), z(2, 8, 2, 128), lens, num_splits=129)
+    with pytest.raises(ValueError, match="out must"):
+        call(z(2, 4, 128), z(2, 8, 2, 128), z(2, 8, 2, 128), lens, out=z(2, 5, 128))
+
+
+def test_c_entries_refuse_before_any_gpu_call():
+    from lbw_amd import _lib
+    lib = _lib.load()
+    d = _lib.DecodeParams(batch=1, q_heads=4, k_heads=2, head_dim=64, capacity=8)
+    assert lib.lbw_attention_decode(ctypes.byref(d), None, 0, None) == 2
+    p = _lib.PackedParams(q_heads=4, k_heads=3, head_dim=128, q_tokens=1, k_tokens=1)
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 1
+    p = _lib.PackedParams(q_heads=4, k_heads=2, head_dim=128, q_tokens=1, k_tokens=1, q=8)
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 1
+    assert b"16-byte" in lib.lbw_last_error()
+    p = _lib.PackedParams(q_heads=4, k_heads=2, head_dim=128, q_tokens=1, k_tokens=1, q=16, k=16, v=16,
+                          out=16, q_stride_l=12)
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 1
+    assert b"multiples of 8" in lib.lbw_last_error()
+    p.q_stride_l = 1 << 26
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 2
+    p.q_stride_l = 512
+    p.softmax_scale = -1.0
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 1
+    n = _lib.HeadNormRopeParams(tokens=1, q_heads=4, k_heads=2, head_dim=48)
+    assert lib.lbw_head_norm_rope(ctypes.byref(n), None) == 2
+    n = _lib.HeadNormRopeParams(tokens=1, q_heads=4, k_heads=2, head_dim=128, n_axes=2, rope_pairs=64)
+    n.axis_pairs[0] = 60
+    assert lib.lbw_head_norm_rope(ctypes.byref(n), None) == 1
+    assert b"add up" in lib.lbw_last_error()
+    for f in (lib.lbw_attention_packed_fwd, lib.lbw_head_norm_rope):
+        assert f(None, None) == 1
