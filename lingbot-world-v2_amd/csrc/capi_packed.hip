@@ -296,7 +296,7 @@ int lbw_attention_packed_fwd(const lbw_packed_params* p, void* stream) {
 
 size_t lbw_attention_packed_bwd_workspace_size(const lbw_packed_params* p) {
   if (p == nullptr || p->q_tokens <= 0 || p->q_heads <= 0) return 0;
-  return (size_t)p->q_heads * (size_t)p->q_tokens * sizeof(float);
+  return 2 * (size_t)p->q_heads * (size_t)p->q_tokens * sizeof(float);  // delta and -lse
 }
 
 int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads* g,
@@ -320,6 +320,7 @@ int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads*
   a.o = {static_cast<const uint16_t*>(p->out), p->out_stride_l, p->out_stride_h};
   a.dout = {static_cast<const uint16_t*>(g->dout), g->dout_stride_l, g->dout_stride_h};
   a.delta = static_cast<float*>(workspace);
+  a.nlse2 = a.delta + (size_t)p->q_heads * (size_t)p->q_tokens;
   a.dq = {static_cast<uint16_t*>(g->dq), g->dq_stride_l, g->dq_stride_h};
   a.dk = {static_cast<uint16_t*>(g->dk), g->dk_stride_l, g->dk_stride_h};
   a.dv = {static_cast<uint16_t*>(g->dv), g->dv_stride_l, g->dv_stride_h};

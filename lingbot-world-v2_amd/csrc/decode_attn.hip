@@ -52,9 +52,7 @@ __global__ void __launch_bounds__(DW * 64, 1) decode_kernel(const DecodeArgs a) 
   const unsigned char* vb = reinterpret_cast<const unsigned char*>(a.v + b * a.vsb + kv * a.vsh);
 
   const int ring = (int)lds_addr(lds) + RING_B * wave;
-  int koff[8], voff[4][2];
-  row_offsets(ring, l32, hl, koff);
-  tr_offsets(ring + DT_B, lane, hl, voff);
+  const int ka = row_address(ring, l32, hl), va = tr_address(ring + DT_B, lane, hl);
   int crow[NCOPY], ccol[NCOPY];
 #pragma unroll
   for (int i = 0; i < NCOPY; ++i) {
@@ -96,7 +94,7 @@ __global__ void __launch_bounds__(DW * 64, 1) decode_kernel(const DecodeArgs a) 
     floatx16 s;
     zero(s);
 #pragma unroll
-    for (int d = 0; d < 8; ++d) s = mfma32x32x16(lds_read_b128(koff[d] + at), qf[d], s);
+    for (int d = 0; d < 8; ++d) s = mfma32x32x16(read_row(ka, d, at), qf[d], s);
     const int left = len - (t * DT + 4 * hl);
     if (t * DT + DT > len) {
 #pragma unroll
@@ -126,7 +124,7 @@ __global__ void __launch_bounds__(DW * 64, 1) decode_kernel(const DecodeArgs a) 
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
-      for (int mm = 0; mm < 2; ++mm) o[db] = mfma32x32x16(read_tr(voff, db, mm, at), pf[mm], o[db]);
+      for (int mm = 0; mm < 2; ++mm) o[db] = mfma32x32x16(read_tr(va, db, mm, at), pf[mm], o[db]);
     // its reads of this stage are over before the next turn's copies into it
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }

@@ -71,6 +71,7 @@ struct PackedArgs {
   // gradient
   Rows o, dout;
   float* delta;                // [Hq][Tq]: sum_d dout out
+  float* nlse2;                // [Hq][Tq]: -lse log2(e), -inf for a query that sees no key
   RowsOut dq, dk, dv;
 };
 hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t stream);

@@ -17,7 +17,7 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int V_AT = 2 * PK_TILE_B;
 constexpr int BWD_LDS = 4 * PK_TILE_B;
-constexpr int STAT_AT = 4 * PK_TILE_B;             // lse and delta of the query tiles, two stages
+constexpr int STAT_AT = 4 * PK_TILE_B;             // -lse and delta of the query tiles, two stages
 constexpr int DKV_LDS = STAT_AT + 2 * 2 * BN * 4;
 
 // ---- dQ: a lane holds one query's column of S^T = K Q^T and dP^T = V dO^T
@@ -34,7 +34,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
   const bool active = rows > 0;
 
   u32x4 qf[8], gf[8];
-  float lse2 = INFINITY, delta = 0.0f;  // (lse = -inf, no key seen: every p becomes 0)
+  float nlse2 = -INFINITY, delta = 0.0f;  // -lse log2(e); no key seen (lse = -inf): every p becomes 0
   if (active) {
     const int64_t row = it.row0 + r0;
     load_rows(a.q.p + row * a.q.sl + h * a.q.sh, a.q.sl, rows, l32, hl, qf);
@@ -50,8 +50,11 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
     if (l32 < rows) {
       const int64_t at = (int64_t)h * a.Tq + row + l32;
       const float x = a.lse[at];
-      lse2 = x == -INFINITY ? INFINITY : x * LOG2E;
-      if (hl == 0) a.delta[at] = delta;
+      nlse2 = x == -INFINITY ? -INFINITY : -x * LOG2E;
+      if (hl == 0) {
+        a.delta[at] = delta;
+        a.nlse2[at] = nlse2;
+      }
     }
   }
   const unsigned char* kb = reinterpret_cast<const unsigned char*>(
@@ -68,9 +71,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
   const int lim_lo = limit(i0), lim_hi = limit(i0 + (rows < 32 ? rows : 32) - 1);
 
   const int lds0 = (int)lds_addr(lds);
-  int off[8], toff[4][2];
-  row_offsets(lds0, l32, hl, off);
-  tr_offsets(lds0, lane, hl, toff);
+  int ra = row_address(lds0, l32, hl), ta = tr_address(lds0, lane, hl);
   TileCopy copy;
   copy.init(wave, lane);
   const uint32_t dst = (uint32_t)lds0 + 1024 * PK_NDMA * wave;
@@ -101,14 +102,14 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
       zero(dp);
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
-        s = mfma32x32x16(lds_read_b128(off[d] + at), qf[d], s);
-        dp = mfma32x32x16(lds_read_b128(off[d] + at + V_AT), gf[d], dp);
+        s = mfma32x32x16(read_row(ra, d, at), qf[d], s);
+        dp = mfma32x32x16(read_row(ra, d, at + V_AT), gf[d], dp);
       }
       const int key0 = u * BN + 32 * kb32;
       floatx16 ds;
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        ds[r] = fast_exp2(__builtin_fmaf(s[r], c, -lse2)) * (dp[r] - delta);
+        ds[r] = fast_exp2(__builtin_fmaf(s[r], c, nlse2)) * (dp[r] - delta);
       if (key0 + 32 > lim_lo) {
         const int left = lim - (key0 + 4 * hl);
 #pragma unroll
@@ -119,7 +120,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int mm = 0; mm < 2; ++mm)
-          acc[db] = mfma32x32x16(read_tr(toff, db, mm, at), pf[mm], acc[db]);
+          acc[db] = mfma32x32x16(read_tr(ta, db, mm, at), pf[mm], acc[db]);
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0070);
@@ -158,9 +159,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const Pack
   const int lo_min = first(j0), lo_max = first(j0 + 31);
 
   const int lds0 = (int)lds_addr(lds);
-  int off[8], toff[4][2];
-  row_offsets(lds0, l32, hl, off);
-  tr_offsets(lds0, lane, hl, toff);
+  const int ra0 = row_address(lds0, l32, hl), ta0 = tr_address(lds0, lane, hl);
   TileCopy copy;
   copy.init(wave, lane);
   const uint32_t dst = (uint32_t)lds0 + 1024 * PK_NDMA * wave;
@@ -175,17 +174,15 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const Pack
   const int per = it.bound < it.other_len ? t_end - t_first : 0;  // query tiles of a head
   const int T = per * group;
   const int64_t qs = a.q.sl * 2, gs = a.dout.sl * 2;
-  float* const stat = reinterpret_cast<float*>(lds + STAT_AT);
-  // query tile n (head n / per of the group) into stage n % 2; wave 0 fetches the rows' lse and delta
-  float st_l = 0.0f, st_d = 0.0f;
+  // query tile n (head n / per of the group) into stage n % 2; waves 0 and 1 fetch its rows' -lse and
+  // delta (rows past the sequence's end: the last one's)
   auto issue = [&](int n) {
     const int h = kv * group + n / per, first_row = (t_first + n % per) * BN;
     const uint32_t to = dst + (n & 1) * PK_TILE_B;
-    if (wave == 0) {
-      const bool in = first_row + lane < it.other_len;
-      const int64_t at = (int64_t)h * a.Tq + it.other0 + first_row + lane;
-      st_l = in ? a.lse[at] : -INFINITY;
-      st_d = in ? a.delta[at] : 0.0f;
+    if (wave < 2) {
+      const int r = min(first_row + lane, it.other_len - 1);
+      const float* x = (wave == 0 ? a.nlse2 : a.delta) + (int64_t)h * a.Tq + it.other0 + r;
+      dma4((uint64_t)(uintptr_t)x, (uint32_t)lds0 + STAT_AT + ((n & 1) * 2 + wave) * BN * 4);
     }
     copy.issue(reinterpret_cast<const unsigned char*>(a.q.p + (int64_t)it.other0 * a.q.sl + h * a.q.sh),
                qs, first_row, it.other_len, to);
@@ -193,34 +190,34 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const Pack
                                                       h * a.dout.sh),
                gs, first_row, it.other_len, to + V_AT);
   };
-  // rows past the sequence's end, and rows that see no key: p = exp2(s - inf) = 0
-  auto put_stat = [&](int n) {
-    if (wave == 0) {
-      stat[(n & 1) * 2 * BN + lane] = st_l == -INFINITY ? INFINITY : st_l * LOG2E;
-      stat[(n & 1) * 2 * BN + BN + lane] = st_d;
-    }
-  };
   if (T > 0) issue(0);
 #pragma unroll 1
   for (int n = 0; n < T; ++n) {
     const int st = (n & 1) * PK_TILE_B;
-    put_stat(n);
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0): the tile and its statistics
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     barrier_nofence();
     if (n + 1 < T) issue(n + 1);
     const int row0 = (t_first + n % per) * BN;
     if (!active || row0 + BN <= lo_min) continue;
-#pragma unroll
+#pragma unroll 1
     for (int qb = 0; qb < 2; ++qb) {
-      const int at = st + qb * 32 * PK_ROWB;
+      const int at = 0;
+      const int ra = opaque(ra0 + st + qb * 32 * PK_ROWB), ta = opaque(ta0 + st + qb * 32 * PK_ROWB);
       const int sa = lds0 + STAT_AT + (n & 1) * 2 * BN * 4 + (32 * qb + 4 * hl) * 4;
       floatx16 s, dp;
       zero(s);
       zero(dp);
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
-        s = mfma32x32x16(lds_read_b128(off[d] + at), kf[d], s);
-        dp = mfma32x32x16(lds_read_b128(off[d] + at + V_AT), vf[d], dp);
+        s = mfma32x32x16(read_row(ra, d, at), kf[d], s);
+        dp = mfma32x32x16(read_row(ra, d, at + V_AT), vf[d], dp);
+      }
+      const int i0 = row0 + 32 * qb;
+      if (i0 < lo_max || i0 + 32 > it.other_len) {  // (register r is query i0 + 4 hl + acc_row(r))
+        const int skip = lo - (i0 + 4 * hl), end = it.other_len - (i0 + 4 * hl);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = acc_row(r) >= skip && acc_row(r) < end ? s[r] : -INFINITY;
       }
       floatx16 p, ds;
 #pragma unroll
@@ -229,40 +226,31 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const Pack
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g + e;
-          p[r] = fast_exp2(__builtin_fmaf(s[r], c, -__uint_as_float(l4[e])));
-          ds[r] = dp[r] - __uint_as_float(d4[e]);
+          p[r] = fast_exp2(__builtin_fmaf(s[r], c, __uint_as_float(l4[e])));
+          ds[r] = p[r] * (dp[r] - __uint_as_float(d4[e]));
         }
       }
-      const int i0 = row0 + 32 * qb;
-      if (i0 < lo_max) {  // (register r is query i0 + 4 hl + acc_row(r))
-        const int skip = lo - (i0 + 4 * hl);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          p[r] = acc_row(r) >= skip ? p[r] : 0.0f;
-          ds[r] = acc_row(r) >= skip ? ds[r] : 0.0f;
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) ds[r] *= p[r];
       const u32x4 pf[2] = {pack_half(p, 0), pack_half(p, 1)};
       const u32x4 df[2] = {pack_half(ds, 0), pack_half(ds, 1)};
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int mm = 0; mm < 2; ++mm) {
-          dv[db] = mfma32x32x16(read_tr(toff, db, mm, at + V_AT), pf[mm], dv[db]);
-          dk[db] = mfma32x32x16(read_tr(toff, db, mm, at), df[mm], dk[db]);
+          dv[db] = mfma32x32x16(read_tr(ta, db, mm, at + V_AT), pf[mm], dv[db]);
+          dk[db] = mfma32x32x16(read_tr(ta, db, mm, at), df[mm], dk[db]);
         }
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0070);
   barrier_nofence();
   if (!active) return;
-  store_rows(lds + 8192 * wave, dk, a.scale, lane, rows, [&](int r) {
+  // (the lane index taken anew rather than kept, or spilled, across the loop)
+  const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  store_rows(lds + 8192 * wave, dk, a.scale, ln, rows, [&](int r) {
     return a.dk.p + (int64_t)(it.row0 + r0 + r) * a.dk.sl + kv * a.dk.sh;
   });
   wave_lds_fence();
-  store_rows(lds + 8192 * wave, dv, 1.0f, lane, rows, [&](int r) {
+  store_rows(lds + 8192 * wave, dv, 1.0f, ln, rows, [&](int r) {
     return a.dv.p + (int64_t)(it.row0 + r0 + r) * a.dv.sl + kv * a.dv.sh;
   });
 }

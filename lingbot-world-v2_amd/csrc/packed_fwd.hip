@@ -50,9 +50,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
   const int lim_lo = limit(i0), lim_hi = limit(i0 + (rows < 32 ? rows : 32) - 1);
 
   const int lds0 = (int)lds_addr(lds);
-  int koff[8], voff[4][2];
-  row_offsets(lds0, l32, hl, koff);
-  tr_offsets(lds0 + V_AT, lane, hl, voff);
+  const int ka = row_address(lds0, l32, hl), va = tr_address(lds0 + V_AT, lane, hl);
   TileCopy copy;
   copy.init(wave, lane);
   const uint32_t dst = (uint32_t)lds0 + 1024 * PK_NDMA * wave;
@@ -83,7 +81,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
       floatx16 s;
       zero(s);
 #pragma unroll
-      for (int d = 0; d < 8; ++d) s = mfma32x32x16(lds_read_b128(koff[d] + at), qf[d], s);
+      for (int d = 0; d < 8; ++d) s = mfma32x32x16(read_row(ka, d, at), qf[d], s);
       const int key0 = u * BN + 32 * kb32;
       if (key0 + 32 > lim_lo) {
         const int left = lim - (key0 + 4 * hl);  // keys of this lane from register 0 on
@@ -114,7 +112,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
-        for (int mm = 0; mm < 2; ++mm) o[db] = mfma32x32x16(read_tr(voff, db, mm, at), pf[mm], o[db]);
+        for (int mm = 0; mm < 2; ++mm) o[db] = mfma32x32x16(read_tr(va, db, mm, at), pf[mm], o[db]);
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0070);

@@ -50,13 +50,13 @@ __device__ __forceinline__ void pick_head(uint32_t c, int Hk, int group, int& h,
 // rows at `base` (its row 0), row stride `stride_b` bytes; rows past the end copy the last row, so
 // a tile never touches another sequence.
 struct TileCopy {
-  int row[PK_NDMA], col[PK_NDMA];
+  int row0, col0;
   __device__ __forceinline__ void init(int wave, int lane) {
-#pragma unroll
-    for (int i = 0; i < PK_NDMA; ++i) {
-      row[i] = 4 * (PK_NDMA * wave + i) + (lane >> 4);
-      col[i] = ((lane & 15) ^ swz(row[i])) * 16;
-    }
+    // copy i fills the wave's 1 KB block i: row row0 + 4 i, chunk (lane % 16) ^ swz(row), whose
+    // (row / 4) % 4 part is i, as a wave's four blocks are rows 16 wave ..
+    static_assert(PK_NDMA == 4, "four blocks of four rows per wave");
+    row0 = 16 * wave + (lane >> 4);
+    col0 = ((lane & 15) ^ swz(lane >> 4)) * 16;
   }
   __device__ __forceinline__ void issue(const unsigned char* base, int64_t stride_b, int first,
                                         int len, uint32_t dst) const {
@@ -64,36 +64,35 @@ struct TileCopy {
     const int last = len - 1 - first;
 #pragma unroll
     for (int i = 0; i < PK_NDMA; ++i) {
-      const int r = row[i] < last ? row[i] : last;
-      dma16_guarded(b, (uint32_t)r * (uint32_t)stride_b + col[i], dst + 1024 * i);
+      const int r = row0 + 4 * i < last ? row0 + 4 * i : last;
+      dma16_guarded(b, (uint32_t)r * (uint32_t)stride_b + (col0 ^ (i << 4)), dst + 1024 * i);
     }
   }
 };
 
-// Per-lane LDS byte offsets of a tile's fragments, 32-row block 0.
+// Per-lane LDS byte addresses of a tile's fragments (32-row block 0 at `base`, a multiple of 1 KB).
+// The swizzle only exchanges bits 4 to 7 of an address, so the fragments of a tile differ from one
+// of them by an exclusive or and a constant: one register each instead of eight.
 // Row reads (A operand, d-slice s): row l32, logical chunk 2s + hl.
-__device__ __forceinline__ void row_offsets(int base, int l32, int hl, int (&off)[8]) {
-#pragma unroll
-  for (int s = 0; s < 8; ++s) off[s] = base + l32 * PK_ROWB + (((2 * s + hl) ^ swz(l32)) << 4);
+__device__ __forceinline__ int row_address(int base, int l32, int hl) {
+  return base + l32 * PK_ROWB + ((hl ^ swz(l32)) << 4);
+}
+__device__ __forceinline__ u32x4 read_row(int addr, int s, int at) {
+  return lds_read_b128((addr ^ (s << 5)) + at);
 }
 // Transpose reads for d-block db and row half j: source row 4hl + 8j + s / 4, columns
 // 32 db + 16 g + 4 (s % 4) .. +3 (s = lane % 16, g = (lane / 16) % 2); rows 16m further along
 // give the lane values k = 16m + 4hl + 8 (e / 4) + e % 4 of the operand's k-group, the order of
 // the accumulator registers 8m + e.
-__device__ __forceinline__ void tr_offsets(int base, int lane, int hl, int (&off)[4][2]) {
+__device__ __forceinline__ int tr_address(int base, int lane, int hl) {
   const int s16 = lane & 15, g = (lane >> 4) & 1;
-#pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = 4 * hl + 8 * j + (s16 >> 2);
-      const int lc = 4 * db + 2 * g + ((s16 & 3) >> 1);
-      off[db][j] = base + r * PK_ROWB + ((lc ^ swz(r)) << 4) + 8 * (s16 & 1);
-    }
+  const int r = 4 * hl + (s16 >> 2), lc = 2 * g + ((s16 & 3) >> 1);
+  return base + r * PK_ROWB + ((lc ^ swz(r)) << 4) + 8 * (s16 & 1);
 }
-__device__ __forceinline__ u32x4 read_tr(const int (&off)[4][2], int db, int m, int at) {
-  const u32x2 v0 = lds_read_tr16(off[db][0] + at + 16 * m * PK_ROWB);
-  const u32x2 v1 = lds_read_tr16(off[db][1] + at + 16 * m * PK_ROWB);
+__device__ __forceinline__ u32x4 read_tr(int addr, int db, int m, int at) {
+  const int x = addr ^ (db << 6);  // (chunk 4 db; rows 8 further: swz's low part changes by 2)
+  const u32x2 v0 = lds_read_tr16(x + at + 16 * m * PK_ROWB);
+  const u32x2 v1 = lds_read_tr16((x ^ 32) + at + (16 * m + 8) * PK_ROWB);
   return u32x4{v0[0], v0[1], v1[0], v1[1]};
 }
 
