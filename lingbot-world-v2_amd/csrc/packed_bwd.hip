@@ -9,6 +9,7 @@
 // walks the queries of all heads of its group: dK and dV (four products a tile).
 // Both recompute S; P and dS go to bf16 as operands, one rounding each.
 
+#include <stdlib.h>
 #include "packed_tiles.h"
 
 namespace lbw {
@@ -18,7 +19,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int V_AT = 2 * PK_TILE_B;
 constexpr int BWD_LDS = 4 * PK_TILE_B;
 constexpr int STAT_AT = 4 * PK_TILE_B;             // -lse and delta of the query tiles, two stages
-constexpr int DKV_LDS = STAT_AT + 2 * 2 * BN * 4;
+constexpr int DKV_GROUP_B = STAT_AT + 2 * 2 * BN * 4;  // LDS of a group of 4 waves
 
 // ---- dQ: a lane holds one query's column of S^T = K Q^T and dP^T = V dO^T
 __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const PackedArgs a) {
@@ -132,10 +133,13 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
 }
 
 // ---- dK, dV: a lane holds one key's column of S = Q K^T and dP = dO V^T
-__global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const PackedArgs a) {
+template <int GROUPS>
+__global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, GROUPS == 1 ? 2 : 1)
+packed_dkv_kernel(const PackedArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = wave_id % PK_WAVES, grp = wave_id / PK_WAVES;
   const int hl = lane >> 5, l32 = lane & 31;
   const int kv = blockIdx.x % (uint32_t)a.Hk, group = a.Hq / a.Hk;
   const PackedItem it = load_item(a.k_items, blockIdx.x / (uint32_t)a.Hk);
@@ -158,7 +162,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const Pack
   const int lo = first(j0 + l32);
   const int lo_min = first(j0), lo_max = first(j0 + 31);
 
-  const int lds0 = (int)lds_addr(lds);
+  const int lds0 = (int)lds_addr(lds) + DKV_GROUP_B * grp;
   const int ra0 = row_address(lds0, l32, hl), ta0 = tr_address(lds0, lane, hl);
   TileCopy copy;
   copy.init(wave, lane);
@@ -172,7 +176,9 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const Pack
   const float c = a.scale_log2;
   const int t_first = it.bound / BN, t_end = (it.other_len + BN - 1) / BN;
   const int per = it.bound < it.other_len ? t_end - t_first : 0;  // query tiles of a head
-  const int T = per * group;
+  const int all = per * group;
+  const int n0 = all * grp / GROUPS, T = all * (grp + 1) / GROUPS;  // this group's share
+  const int Tmax = n0 + (all + GROUPS - 1) / GROUPS;
   const int64_t qs = a.q.sl * 2, gs = a.dout.sl * 2;
   // query tile n (head n / per of the group) into stage n % 2; waves 0 and 1 fetch its rows' -lse and
   // delta (rows past the sequence's end: the last one's)
@@ -190,15 +196,15 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const Pack
                                                       h * a.dout.sh),
                gs, first_row, it.other_len, to + V_AT);
   };
-  if (T > 0) issue(0);
+  if (n0 < T) issue(n0);
 #pragma unroll 1
-  for (int n = 0; n < T; ++n) {
+  for (int n = n0; n < Tmax; ++n) {
     const int st = (n & 1) * PK_TILE_B;
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     barrier_nofence();
     if (n + 1 < T) issue(n + 1);
     const int row0 = (t_first + n % per) * BN;
-    if (!active || row0 + BN <= lo_min) continue;
+    if (!active || n >= T || row0 + BN <= lo_min) continue;
 #pragma unroll 1
     for (int qb = 0; qb < 2; ++qb) {
       const int at = 0;
@@ -243,6 +249,37 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dkv_kernel(const Pack
   }
   __builtin_amdgcn_s_waitcnt(0x0070);
   barrier_nofence();
+  if constexpr (GROUPS == 2) {
+    // group 1 hands its sums over in register order, 16 bytes per lane: dK through its own LDS, dV
+    // through group 0's
+    unsigned char* g1 = lds + DKV_GROUP_B + 16384 * wave;
+    unsigned char* g0 = lds + 16384 * wave;
+    const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    if (grp == 1) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const floatx16 &y = dk[x >> 2], &z = dv[x >> 2];
+        const int e = 4 * (x & 3);
+        *reinterpret_cast<floatx4*>(g1 + 1024 * x + 16 * ln) = floatx4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        *reinterpret_cast<floatx4*>(g0 + 1024 * x + 16 * ln) = floatx4{z[e], z[e + 1], z[e + 2], z[e + 3]};
+      }
+    }
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const floatx4 y = *reinterpret_cast<const floatx4*>(g1 + 1024 * x + 16 * ln);
+        const floatx4 z = *reinterpret_cast<const floatx4*>(g0 + 1024 * x + 16 * ln);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dk[x >> 2][4 * (x & 3) + e] += y[e];
+          dv[x >> 2][4 * (x & 3) + e] += z[e];
+        }
+      }
+    }
+    __syncthreads();  // the sums are read: the LDS is free for staging
+    if (grp == 1) return;
+  }
   if (!active) return;
   // (the lane index taken anew rather than kept, or spilled, across the loop)
   const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
@@ -266,13 +303,19 @@ hipError_t launch_packed_dq(const PackedArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream) {
-  static hipError_t attr = hipFuncSetAttribute((const void*)packed_dkv_kernel,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, DKV_LDS);
+template <int GROUPS>
+static hipError_t run_dkv(const PackedArgs& a, hipStream_t stream) {
+  constexpr int bytes = GROUPS * DKV_GROUP_B;
+  static hipError_t attr = hipFuncSetAttribute((const void*)packed_dkv_kernel<GROUPS>,
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL(packed_dkv_kernel, dim3((uint32_t)a.n_k_items * a.Hk), dim3(PK_WAVES * 64),
-                     DKV_LDS, stream, a);
+  hipLaunchKernelGGL(packed_dkv_kernel<GROUPS>, dim3((uint32_t)a.n_k_items * a.Hk),
+                     dim3(GROUPS * PK_WAVES * 64), bytes, stream, a);
   return hipGetLastError();
+}
+hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream) {
+  const char* e = getenv("LBW_G");
+  return e && e[0] == '1' ? run_dkv<1>(a, stream) : run_dkv<2>(a, stream);
 }
 
 }  // namespace lbw

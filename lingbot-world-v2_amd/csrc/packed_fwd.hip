@@ -270,7 +270,7 @@ hipError_t run(const PackedArgs& a, hipStream_t stream) {
 
 hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t stream) {
   const char* e = getenv("LBW_G");
-  return e && e[0] == '2' ? run<2>(a, stream) : run<1>(a, stream);
+  return e && e[0] == '3' ? run<2>(a, stream) : run<1>(a, stream);
 }
 
 }  // namespace lbw
