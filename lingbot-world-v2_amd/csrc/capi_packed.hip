@@ -34,6 +34,14 @@ int check_rows(const char* name, const void* p, int64_t n, int64_t sl, int64_t s
   return LBW_OK;
 }
 
+// per-head norm: a lane's offset among the heads of one wave step is 32-bit
+int check_head_strides(const char* name, int64_t sh) {
+  if (sh >= (int64_t(1) << 26))
+    return fail(LBW_ERR_UNSUPPORTED, "%s: head stride %lld exceeds %lld", name, (long long)sh,
+                (long long)((int64_t(1) << 26) - 1));
+  return LBW_OK;
+}
+
 int check_heads(int32_t hq, int32_t hk) {
   if (hq < 1 || hk < 1 || hq % hk != 0)
     return fail(LBW_ERR_INVALID, "k_heads %d must divide q_heads %d", hk, hq);
@@ -94,6 +102,8 @@ int fill_head_norm(const lbw_head_norm_rope_params* p, HeadNormArgs* a) {
     return fail(LBW_ERR_INVALID, "weights must be 16-byte aligned");
   LBW_TRY(check_rows("q", p->q, p->tokens, p->q_stride_l, p->q_stride_h));
   LBW_TRY(check_rows("k", p->k, p->tokens, p->k_stride_l, p->k_stride_h));
+  LBW_TRY(check_head_strides("q", p->q_stride_h));
+  LBW_TRY(check_head_strides("k", p->k_stride_h));
   if ((int64_t)p->tokens * 32 / 4 >= kMaxWorkgroups)
     return fail(LBW_ERR_UNSUPPORTED, "tokens %d", p->tokens);
   a->T = p->tokens; a->Hq = p->q_heads; a->Hk = p->k_heads;
@@ -172,11 +182,15 @@ int lbw_head_norm_rope(const lbw_head_norm_rope_params* p, void* stream) {
   LBW_TRY(fill_head_norm(p, &a));
   LBW_TRY(check_rows("q_out", p->q_out, p->tokens, p->q_out_stride_l, p->q_out_stride_h));
   LBW_TRY(check_rows("k_out", p->k_out, p->tokens, p->k_out_stride_l, p->k_out_stride_h));
+  LBW_TRY(check_head_strides("q_out", p->q_out_stride_h));
+  LBW_TRY(check_head_strides("k_out", p->k_out_stride_h));
   a.qo = {static_cast<uint16_t*>(p->q_out), p->q_out_stride_l, p->q_out_stride_h};
   a.ko = {static_cast<uint16_t*>(p->k_out), p->k_out_stride_l, p->k_out_stride_h};
   if (p->v != nullptr) {
     LBW_TRY(check_rows("v", p->v, p->tokens, p->v_stride_l, p->v_stride_h));
     LBW_TRY(check_rows("v_out", p->v_out, p->tokens, p->v_out_stride_l, p->v_out_stride_h));
+    LBW_TRY(check_head_strides("v", p->v_stride_h));
+    LBW_TRY(check_head_strides("v_out", p->v_out_stride_h));
     a.v = {static_cast<const uint16_t*>(p->v), p->v_stride_l, p->v_stride_h};
     a.vo = {static_cast<uint16_t*>(p->v_out), p->v_out_stride_l, p->v_out_stride_h};
   }
@@ -197,7 +211,7 @@ int lbw_head_norm_rope(const lbw_head_norm_rope_params* p, void* stream) {
 
 size_t lbw_head_norm_rope_bwd_workspace_size(const lbw_head_norm_rope_params* p) {
   if (p == nullptr || p->tokens <= 0 || p->head_dim <= 0) return 0;
-  return (size_t)head_norm_bwd_workgroups(p->tokens, num_cus()) * 2 * p->head_dim * sizeof(float);
+  return (size_t)head_norm_bwd_workgroups(p->tokens, num_cus()) * p->head_dim * sizeof(float);
 }
 
 int lbw_head_norm_rope_bwd(const lbw_head_norm_rope_params* p, const lbw_head_norm_rope_grads* g,
@@ -209,6 +223,10 @@ int lbw_head_norm_rope_bwd(const lbw_head_norm_rope_params* p, const lbw_head_no
   LBW_TRY(check_rows("dk_out", g->dk_out, p->tokens, g->dk_out_stride_l, g->dk_out_stride_h));
   LBW_TRY(check_rows("dq", g->dq, p->tokens, g->dq_stride_l, g->dq_stride_h));
   LBW_TRY(check_rows("dk", g->dk, p->tokens, g->dk_stride_l, g->dk_stride_h));
+  LBW_TRY(check_head_strides("dq_out", g->dq_out_stride_h));
+  LBW_TRY(check_head_strides("dk_out", g->dk_out_stride_h));
+  LBW_TRY(check_head_strides("dq", g->dq_stride_h));
+  LBW_TRY(check_head_strides("dk", g->dk_stride_h));
   const size_t need = lbw_head_norm_rope_bwd_workspace_size(p);
   if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
     return fail(LBW_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need,

@@ -62,158 +62,187 @@ struct Turn {
   int lane;  // split halves: the lane that holds the partners (the own one: not rotated)
 };
 
+template <bool INTER>
 __device__ __forceinline__ void load_turn(const HeadNormArgs& a, int t, int e0, int lane, Turn& r) {
   const int h = a.npairs;
-  // the axes' table rows; a position outside the table turns by NaN
-  int64_t row[kMaxAxes];
-#pragma unroll
-  for (int x = 0; x < kMaxAxes; ++x) {
-    const int p = x < a.naxes ? a.pos[t * a.pos_sl + x] : 0;
-    row[x] = (p < 0 || p >= a.P) ? -1 : (int64_t)p * h;
-  }
-  const bool second = !a.inter && e0 >= h;
-  const bool halves_rot = !a.inter && e0 < 2 * h;
-  r.lane = halves_rot ? (second ? lane - h / 8 : lane + h / 8) : lane;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int i = a.inter ? (e0 + j) >> 1 : (second ? e0 + j - h : e0 + j);
-    float c = 1.0f, s = 0.0f;
-    if (i < h) {
-      int64_t base = row[0];
-      if (i >= a.ax_end[0]) base = row[1];
-      if (i >= a.ax_end[1]) base = row[2];
-      if (i >= a.ax_end[2]) base = row[3];
-      float2 cs = {__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u)};
-      if (base >= 0) cs = a.table[base + i];
-      c = cs.x;
-      s = (a.inter ? (j & 1) == 0 : !second) ? -cs.y : cs.y;
+  // the token's positions (selected by comparisons: an array would be put into LDS)
+  const int32_t* pos = a.pos + (int64_t)t * a.pos_sl;
+  const int p0 = pos[0], p1 = a.naxes > 1 ? pos[1] : 0, p2 = a.naxes > 2 ? pos[2] : 0,
+            p3 = a.naxes > 3 ? pos[3] : 0;
+  auto angle = [&](int i) {
+    const int lo = i >= a.ax_end[0] ? p1 : p0, hi = i >= a.ax_end[2] ? p3 : p2;
+    const int p = i >= a.ax_end[1] ? hi : lo;
+    float2 cs = {1.0f, 0.0f};
+    if (i < h) {  // a position outside the table turns by NaN
+      cs = {__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u)};
+      if (p >= 0 && p < a.P) cs = a.table[(int64_t)p * h + i];
     }
-    r.c[j] = c;
-    r.s[j] = s;
+    return cs;
+  };
+  r.lane = lane;
+  if constexpr (INTER) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 cs = angle((e0 >> 1) + j);
+      r.c[2 * j] = r.c[2 * j + 1] = cs.x;
+      r.s[2 * j] = -cs.y;
+      r.s[2 * j + 1] = cs.y;
+    }
+  } else {
+    const bool second = e0 >= h;
+    if (e0 < 2 * h) r.lane = second ? lane - h / 8 : lane + h / 8;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 cs = angle(second ? e0 + j - h : e0 + j);
+      r.c[j] = cs.x;
+      r.s[j] = second ? cs.y : -cs.y;
+    }
   }
 }
 
 // y turned; back: by the negative angle.
-template <bool BACK>
-__device__ __forceinline__ void turn(const Turn& r, bool inter, const float (&y)[8], float (&o)[8]) {
+template <bool INTER, bool BACK>
+__device__ __forceinline__ void turn(const Turn& r, const float (&y)[8], float (&o)[8]) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float p = inter ? y[j ^ 1] : __shfl(y[j], r.lane);
+    const float p = INTER ? y[j ^ 1] : __shfl(y[j], r.lane);
     o[j] = y[j] * r.c[j] + p * (BACK ? -r.s[j] : r.s[j]);
   }
 }
 
-template <int LPH>
-__global__ void __launch_bounds__(HN_WAVES * 64) head_norm_kernel(const HeadNormArgs a) {
-  constexpr int HPW = 64 / LPH;  // heads of one wave step
-  constexpr int U = 4;           // steps in flight
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * HN_WAVES + (threadIdx.x >> 6);
-  const int64_t tt = id / a.parts;
-  if (tt >= a.T) return;
-  const int t = (int)tt, part = (int)(id % a.parts);
-  const int e0 = 8 * (lane % LPH), hsub = lane / LPH;
-  Turn rot;
-  load_turn(a, t, e0, lane, rot);
-  float wq[8], wk[8];
-  load_weights(a.wq, a.w32, e0, wq);
-  load_weights(a.wk, a.w32, e0, wk);
-  int64_t krow = (int64_t)t * a.ko.sl, vrow = (int64_t)t * a.vo.sl;
-  bool kput = true;
-  if (a.rows != nullptr) {
-    const int row = a.rows[t];
-    kput = row >= 0 && row < a.cap;
-    krow = (int64_t)t * a.kosb + (int64_t)row * a.ko.sl;
-    vrow = (int64_t)t * a.vosb + (int64_t)row * a.vo.sl;
-  }
-  const int nh = a.Hq + a.Hk, nall = nh + (a.v.p != nullptr ? a.Hk : 0);
-  const int nch = (nall + HPW - 1) / HPW;
-  for (int it = part; it < nch; it += U * a.parts) {
+// One tensor of a token: chunk i holds heads i HPW .. (lane / LPH counts them). Element offsets of a lane
+// within a chunk fit 32 bits (the host checks); the chunk's base is scalar.
+struct Lane {
+  int e0, hsub;
+};
+
+// Chunks first, first + step, .. of `heads` heads: normed and turned (w, scale), or copied.
+template <int LPH, bool INTER, bool COPY>
+__device__ __forceinline__ void norm_rows(const uint16_t* src, int64_t ssh, uint16_t* dst, int64_t dsh,
+                                          int heads, int first, int step, Lane ln, const void* w,
+                                          int w32, float scale, const Turn& rot, float inv_d, float eps) {
+  constexpr int HPW = 64 / LPH, U = 4;
+  const int nch = (heads + HPW - 1) / HPW;
+  if (first >= nch) return;
+  const uint32_t so = (uint32_t)(ln.hsub * (int)ssh + ln.e0), dof = (uint32_t)(ln.hsub * (int)dsh + ln.e0);
+  float wt[8];
+  if constexpr (!COPY) load_weights(w, w32, ln.e0, wt);
+  for (int it = first; it < nch; it += U * step) {
     u32x4 x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int hh = (it + u * a.parts) * HPW + hsub;
-      const uint16_t* src = nullptr;
-      if (hh < a.Hq) src = a.q.p + t * a.q.sl + hh * a.q.sh;
-      else if (hh < nh) src = a.k.p + t * a.k.sl + (hh - a.Hq) * a.k.sh;
-      else if (hh < nall) src = a.v.p + t * a.v.sl + (hh - nh) * a.v.sh;
+      const int ch = it + u * step;
       x[u] = u32x4{0u, 0u, 0u, 0u};
-      if (src != nullptr) x[u] = load16(src + e0);
+      if (ch * HPW + ln.hsub < heads) x[u] = load16(src + (int64_t)ch * HPW * ssh + so);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      if ((it + u * a.parts) >= nch) break;
-      const int hh = (it + u * a.parts) * HPW + hsub;
-      const bool is_q = hh < a.Hq;
-      float f[8], y[8], o[8];
-      unpack8(x[u], f);
-      float ss = 0.0f;
+      const int ch = it + u * step;
+      if (ch >= nch) break;
+      u32x4 out = x[u];
+      if constexpr (!COPY) {
+        float f[8], o[8];
+        unpack8(x[u], f);
+        float ss = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
-      ss = head_sum<LPH>(ss);
-      const float r = rsqrtf(ss * a.inv_d + a.eps) * (is_q ? a.q_scale : a.k_scale);
+        for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+        const float r = rsqrtf(head_sum<LPH>(ss) * inv_d + eps) * scale;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = f[j] * r * (is_q ? wq[j] : wk[j]);
-      turn<false>(rot, a.inter, y, o);
-      const u32x4 w = pack8(o);
-      if (is_q)
-        *reinterpret_cast<u32x4*>(a.qo.p + t * a.qo.sl + hh * a.qo.sh + e0) = w;
-      else if (hh < nh && kput)
-        *reinterpret_cast<u32x4*>(a.ko.p + krow + (hh - a.Hq) * a.ko.sh + e0) = w;
-      else if (hh >= nh && hh < nall && kput)
-        *reinterpret_cast<u32x4*>(a.vo.p + vrow + (hh - nh) * a.vo.sh + e0) = x[u];
+        for (int j = 0; j < 8; ++j) f[j] *= r * wt[j];
+        turn<INTER, false>(rot, f, o);
+        out = pack8(o);
+      }
+      if (dst != nullptr && ch * HPW + ln.hsub < heads)
+        *reinterpret_cast<u32x4*>(dst + (int64_t)ch * HPW * dsh + dof) = out;
     }
   }
 }
 
-// A workgroup's waves take tokens in turn (wave w of workgroup i: tokens 4 i + w, then every
-// 4 nwg-th) and keep the weights' gradient of their lanes' values in registers; each workgroup
-// writes one partial row, which the second kernel adds in a fixed order: no atomics.
-template <int LPH>
+template <int LPH, bool INTER>
+__global__ void __launch_bounds__(HN_WAVES * 64) head_norm_kernel(const HeadNormArgs a) {
+  constexpr int HPW = 64 / LPH;
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * HN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t tt = id / a.parts;
+  if (tt >= a.T) return;
+  const int t = (int)tt, part = (int)(id % a.parts);
+  const Lane ln = {8 * (lane % LPH), lane / LPH};
+  Turn rot;
+  load_turn<INTER>(a, t, ln.e0, lane, rot);
+  uint16_t *ko = a.ko.p + (int64_t)t * a.ko.sl, *vo = a.vo.p + (int64_t)t * a.vo.sl;
+  if (a.rows != nullptr) {
+    const int row = __builtin_amdgcn_readfirstlane(a.rows[t]);
+    const bool put = row >= 0 && row < a.cap;
+    ko = put ? a.ko.p + (int64_t)t * a.kosb + (int64_t)row * a.ko.sl : nullptr;
+    vo = put ? a.vo.p + (int64_t)t * a.vosb + (int64_t)row * a.vo.sl : nullptr;
+  }
+  // the token's chunks, q's, k's, v's, in turn to the waves that share it
+  const int cq = (a.Hq + HPW - 1) / HPW, ck = (a.Hk + HPW - 1) / HPW;
+  auto first = [&](int before) {
+    const int x = (part - before) % a.parts;
+    return x < 0 ? x + a.parts : x;
+  };
+  norm_rows<LPH, INTER, false>(a.q.p + t * a.q.sl, a.q.sh, a.qo.p + t * a.qo.sl, a.qo.sh, a.Hq, part, a.parts,
+                               ln, a.wq, a.w32, a.q_scale, rot, a.inv_d, a.eps);
+  norm_rows<LPH, INTER, false>(a.k.p + t * a.k.sl, a.k.sh, ko, a.ko.sh, a.Hk, first(cq), a.parts, ln, a.wk,
+                               a.w32, a.k_scale, rot, a.inv_d, a.eps);
+  if (a.v.p != nullptr)
+    norm_rows<LPH, INTER, true>(a.v.p + t * a.v.sl, a.v.sh, vo, a.vo.sh, a.Hk, first(cq + ck), a.parts, ln,
+                                nullptr, 0, 1.0f, rot, a.inv_d, a.eps);
+}
+
+// Workgroups 0 .. nwg_q - 1 take q, the others k, in proportion to their heads. A workgroup's waves take
+// tokens in turn and keep the weights' gradient of their lanes' values in registers; each workgroup writes
+// one partial row, which the second kernel adds in a fixed order: no atomics.
+template <int LPH, bool INTER>
 __global__ void __launch_bounds__(HN_WAVES * 64) head_norm_bwd_kernel(const HeadNormArgs a) {
-  constexpr int HPW = 64 / LPH, D = 8 * LPH;
-  constexpr int U = 2;
-  __shared__ float red[HN_WAVES][2][D];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int HPW = 64 / LPH, D = 8 * LPH, U = 2;
+  __shared__ float red[HN_WAVES][D];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int e0 = 8 * (lane % LPH), hsub = lane / LPH;
-  float wq[8], wk[8], gq[8], gk[8];
-  load_weights(a.wq, a.w32, e0, wq);
-  load_weights(a.wk, a.w32, e0, wk);
+  const bool is_q = (int)blockIdx.x < a.nwg_q;
+  const int wg = is_q ? blockIdx.x : blockIdx.x - a.nwg_q, nwg = is_q ? a.nwg_q : a.nwg - a.nwg_q;
+  const Rows src = is_q ? a.q : a.k, grad = is_q ? a.dqo : a.dko;
+  const RowsOut dst = is_q ? a.qo : a.ko;
+  const int heads = is_q ? a.Hq : a.Hk, nch = (heads + HPW - 1) / HPW;
+  const float scale = is_q ? a.q_scale : a.k_scale;
+  const uint32_t so = (uint32_t)(hsub * (int)src.sh + e0), go = (uint32_t)(hsub * (int)grad.sh + e0),
+                 dof = (uint32_t)(hsub * (int)dst.sh + e0);
+  float wt[8], gw[8];
+  load_weights(is_q ? a.wq : a.wk, a.w32, e0, wt);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) gq[j] = gk[j] = 0.0f;
-  const int nh = a.Hq + a.Hk, nch = (nh + HPW - 1) / HPW;
-  for (int64_t t = (int64_t)blockIdx.x * HN_WAVES + wave; t < a.T; t += (int64_t)a.nwg * HN_WAVES) {
-    Turn rot;
-    load_turn(a, (int)t, e0, lane, rot);
-    for (int it = 0; it < nch; it += U) {
-      u32x4 x[U], dy[U];
+  for (int j = 0; j < 8; ++j) gw[j] = 0.0f;
+  for (int64_t t = (int64_t)wg * HN_WAVES + wave; t < a.T; t += (int64_t)nwg * HN_WAVES) {
+    const uint16_t *xs = src.p + t * src.sl, *gs = grad.p + t * grad.sl;
+    uint16_t* ds = dst.p + t * dst.sl;
+    u32x4 x[U], dy[U];
+    auto load = [&](int it) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int hh = (it + u) * HPW + hsub;
         x[u] = dy[u] = u32x4{0u, 0u, 0u, 0u};
-        if (hh < a.Hq) {
-          x[u] = load16(a.q.p + t * a.q.sl + hh * a.q.sh + e0);
-          dy[u] = load16(a.dqo.p + t * a.dqo.sl + hh * a.dqo.sh + e0);
-        } else if (hh < nh) {
-          x[u] = load16(a.k.p + t * a.k.sl + (hh - a.Hq) * a.k.sh + e0);
-          dy[u] = load16(a.dko.p + t * a.dko.sl + (hh - a.Hq) * a.dko.sh + e0);
+        if ((it + u) * HPW + hsub < heads) {
+          x[u] = load16(xs + (int64_t)(it + u) * HPW * src.sh + so);
+          dy[u] = load16(gs + (int64_t)(it + u) * HPW * grad.sh + go);
         }
       }
+    };
+    load(0);  // ahead of the table, whose rows depend on the positions
+    Turn rot;
+    load_turn<INTER>(a, (int)t, e0, lane, rot);
+    for (int it = 0; it < nch; it += U) {
+      if (it != 0) load(it);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int hh = (it + u) * HPW + hsub;
-        const bool is_q = hh < a.Hq;
-        float f[8], d[8], g[8], o[8];
+        float f[8], g[8], o[8];
+        unpack8(dy[u], f);
+        turn<INTER, true>(rot, f, g);
         unpack8(x[u], f);
-        unpack8(dy[u], d);
-        turn<true>(rot, a.inter, d, g);
-        const float sc = is_q ? a.q_scale : a.k_scale;
         float ss = 0.0f, dot = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          g[j] *= sc;
+          g[j] *= scale;
           ss += f[j] * f[j];
-          dot += g[j] * (is_q ? wq[j] : wk[j]) * f[j];
+          dot += g[j] * wt[j] * f[j];
         }
         ss = head_sum<LPH>(ss);
         dot = head_sum<LPH>(dot);
@@ -221,16 +250,11 @@ __global__ void __launch_bounds__(HN_WAVES * 64) head_norm_bwd_kernel(const Head
         const float m = r * r * dot * a.inv_d;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float gx = g[j] * f[j] * r;
-          if (is_q) gq[j] += gx;
-          else if (hh < nh) gk[j] += gx;
-          o[j] = r * (g[j] * (is_q ? wq[j] : wk[j]) - f[j] * m);
+          gw[j] += g[j] * f[j] * r;  // (a lane past the last head holds zeros)
+          o[j] = r * (g[j] * wt[j] - f[j] * m);
         }
-        const u32x4 w = pack8(o);
-        if (is_q)
-          *reinterpret_cast<u32x4*>(a.qo.p + t * a.qo.sl + hh * a.qo.sh + e0) = w;
-        else if (hh < nh)
-          *reinterpret_cast<u32x4*>(a.ko.p + t * a.ko.sl + (hh - a.Hq) * a.ko.sh + e0) = w;
+        if ((it + u) * HPW + hsub < heads)
+          *reinterpret_cast<u32x4*>(ds + (int64_t)(it + u) * HPW * dst.sh + dof) = pack8(o);
       }
     }
   }
@@ -238,38 +262,38 @@ __global__ void __launch_bounds__(HN_WAVES * 64) head_norm_bwd_kernel(const Head
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
 #pragma unroll
-    for (int o = 32; o >= LPH; o >>= 1) {
-      gq[j] += __shfl_xor(gq[j], o);
-      gk[j] += __shfl_xor(gk[j], o);
-    }
+    for (int o = 32; o >= LPH; o >>= 1) gw[j] += __shfl_xor(gw[j], o);
   }
   if (lane < LPH) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      red[wave][0][e0 + j] = gq[j];
-      red[wave][1][e0 + j] = gk[j];
-    }
+    for (int j = 0; j < 8; ++j) red[wave][e0 + j] = gw[j];
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * D; i += HN_WAVES * 64) {
+  for (int i = threadIdx.x; i < D; i += HN_WAVES * 64) {
     float s = 0.0f;
 #pragma unroll
-    for (int w = 0; w < HN_WAVES; ++w) s += red[w][i / D][i % D];
-    a.part[(int64_t)blockIdx.x * 2 * D + i] = s;
+    for (int w = 0; w < HN_WAVES; ++w) s += red[w][i];
+    a.part[(int64_t)blockIdx.x * D + i] = s;
   }
 }
 
-// The weights' gradient: the workgroups' partial rows added up, 32 columns per workgroup.
-__global__ void __launch_bounds__(256) head_norm_dw_kernel(const HeadNormArgs a, int D) {
-  __shared__ float red[8][32];
-  const int col = blockIdx.x * 32 + (threadIdx.x & 31), strip = threadIdx.x >> 5;
+// The weights' gradient: the workgroups' partial rows added up in a fixed order, 16 columns per
+// workgroup, 64 strips of rows.
+__global__ void __launch_bounds__(1024) head_norm_dw_kernel(const HeadNormArgs a, int D) {
+  __shared__ float red[64][17];
+  const int c = threadIdx.x & 15, strip = threadIdx.x >> 4, col = blockIdx.x * 16 + c;
+  const int w0 = col < D ? 0 : a.nwg_q, w1 = col < D ? a.nwg_q : a.nwg;
   float s = 0.0f;
-  for (int w = strip; w < a.nwg; w += 8) s += a.part[(int64_t)w * 2 * D + col];
-  red[strip][threadIdx.x & 31] = s;
-  __syncthreads();
-  if (strip != 0) return;
+#pragma unroll 8
+  for (int w = w0 + strip; w < w1; w += 64) s += a.part[(int64_t)w * D + col % D];
+  red[strip][c] = s;
 #pragma unroll
-  for (int i = 1; i < 8; ++i) s += red[i][threadIdx.x];
+  for (int o = 32; o >= 1; o >>= 1) {
+    __syncthreads();
+    if (strip < o) red[strip][c] += red[strip + o][c];
+  }
+  if (strip != 0) return;
+  s = red[0][c];
   void* dst = col < D ? a.dwq : a.dwk;
   if (dst == nullptr) return;
   if (a.w32) static_cast<float*>(dst)[col % D] = s;
@@ -279,25 +303,29 @@ __global__ void __launch_bounds__(256) head_norm_dw_kernel(const HeadNormArgs a,
 template <int LPH>
 hipError_t run_fwd(const HeadNormArgs& a, hipStream_t stream) {
   const int64_t waves = (int64_t)a.T * a.parts;
-  hipLaunchKernelGGL((head_norm_kernel<LPH>), dim3((uint32_t)((waves + HN_WAVES - 1) / HN_WAVES)),
-                     dim3(HN_WAVES * 64), 0, stream, a);
+  const dim3 grid((uint32_t)((waves + HN_WAVES - 1) / HN_WAVES)), block(HN_WAVES * 64);
+  if (a.inter) hipLaunchKernelGGL((head_norm_kernel<LPH, true>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((head_norm_kernel<LPH, false>), grid, block, 0, stream, a);
   return hipGetLastError();
 }
 template <int LPH>
 hipError_t run_bwd(const HeadNormArgs& a, hipStream_t stream) {
-  if (a.nwg > 0)
-    hipLaunchKernelGGL((head_norm_bwd_kernel<LPH>), dim3(a.nwg), dim3(HN_WAVES * 64), 0, stream, a);
+  const dim3 grid(a.nwg), block(HN_WAVES * 64);
+  if (a.nwg > 0) {
+    if (a.inter) hipLaunchKernelGGL((head_norm_bwd_kernel<LPH, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((head_norm_bwd_kernel<LPH, false>), grid, block, 0, stream, a);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || (a.dwq == nullptr && a.dwk == nullptr)) return e;
-  hipLaunchKernelGGL(head_norm_dw_kernel, dim3(2 * 8 * LPH / 32), dim3(256), 0, stream, a, 8 * LPH);
+  hipLaunchKernelGGL(head_norm_dw_kernel, dim3(2 * 8 * LPH / 16), dim3(1024), 0, stream, a, 8 * LPH);
   return hipGetLastError();
 }
 
 }  // namespace
 
-// Workgroups of the gradient kernel: four per CU, or as many as the tokens fill.
+// Workgroups of the gradient kernel: four per CU, or as many as the tokens fill (for q and for k).
 int head_norm_bwd_workgroups(int T, int cus) {
-  const int need = (T + HN_WAVES - 1) / HN_WAVES;
+  const int need = 2 * ((T + HN_WAVES - 1) / HN_WAVES);
   return need < 4 * cus ? need : 4 * cus;
 }
 
@@ -306,7 +334,7 @@ hipError_t launch_head_norm(const HeadNormArgs& args, int D, hipStream_t stream)
   // a token's heads are shared by several waves while the tokens alone do not fill the chip
   const int nch = (a.Hq + 2 * a.Hk + 512 / D - 1) / (512 / D);
   a.parts = 1;
-  while (a.parts < nch && (int64_t)a.T * a.parts < 4096) a.parts *= 2;
+  while (a.parts < nch && (int64_t)a.T * a.parts < 16384) a.parts *= 2;
   switch (D) {
     case 32: return run_fwd<4>(a, stream);
     case 64: return run_fwd<8>(a, stream);
@@ -314,7 +342,9 @@ hipError_t launch_head_norm(const HeadNormArgs& args, int D, hipStream_t stream)
     default: return run_fwd<32>(a, stream);
   }
 }
-hipError_t launch_head_norm_bwd(const HeadNormArgs& a, int D, hipStream_t stream) {
+hipError_t launch_head_norm_bwd(const HeadNormArgs& args, int D, hipStream_t stream) {
+  HeadNormArgs a = args;
+  a.nwg_q = (int)((int64_t)a.nwg * a.Hq / (a.Hq + a.Hk));  // (k has at most q's heads: never all)
   switch (D) {
     case 32: return run_bwd<4>(a, stream);
     case 64: return run_bwd<8>(a, stream);

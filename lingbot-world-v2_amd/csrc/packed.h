@@ -41,8 +41,8 @@ struct HeadNormArgs {
   int parts;                  // waves that share one token's heads (forward)
   // gradient
   Rows dqo, dko;
-  float* part;                // [workgroups][2][D] partial weight gradients
-  int nwg;
+  float* part;                // [nwg][D] partial weight gradients
+  int nwg, nwg_q;             // workgroups of the gradient; the first nwg_q of them take q
   void* dwq;                  // [D] each, of the weights' type, or null
   void* dwk;
 };
