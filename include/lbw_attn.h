@@ -310,10 +310,14 @@ int lbw_head_norm_rope_bwd(const lbw_head_norm_rope_params* p, const lbw_head_no
  * number of heads and layers. A table of other lengths gives wrong results, but its items never lead a
  * kernel outside the q_tokens / k_tokens rows given. */
 #define LBW_PACKED_ITEM 8
+typedef struct lbw_packed_plan_info {
+  int64_t n_q_items, n_k_items;
+  int64_t q_tiles, q_tiles_max;    /* 64-key tiles of all query items, of the costliest */
+  int64_t k_tiles, k_tiles_max;    /* 64-query tiles (of one head) of all key items */
+} lbw_packed_plan_info;
 int lbw_attention_packed_plan(int32_t n_seqs, const int32_t* q_lens, const int32_t* k_lens,
                               int32_t causal, int32_t* q_items, int64_t q_items_cap,
-                              int64_t* n_q_items, int32_t* k_items, int64_t k_items_cap,
-                              int64_t* n_k_items);
+                              int32_t* k_items, int64_t k_items_cap, lbw_packed_plan_info* info);
 typedef struct lbw_packed_params {
   int32_t q_heads, k_heads, head_dim;
   int64_t q_tokens, k_tokens;      /* packed rows of q, out and of k, v */
@@ -325,8 +329,12 @@ typedef struct lbw_packed_params {
   float softmax_scale;             /* > 0; 0: 1 / sqrt(head_dim) */
   const int32_t* q_items; int32_t n_q_items;
   const int32_t* k_items; int32_t n_k_items; /* gradient only */
+  /* the plan's tile counts, by which long items are cut into pieces when there are few (0: never cut) */
+  int64_t q_tiles, q_tiles_max, k_tiles, k_tiles_max;
 } lbw_packed_params;
-int lbw_attention_packed_fwd(const lbw_packed_params* p, void* stream);
+size_t lbw_attention_packed_workspace_size(const lbw_packed_params* p);
+int lbw_attention_packed_fwd(const lbw_packed_params* p, void* workspace, size_t workspace_bytes,
+                             void* stream);
 
 /* Its gradient, from q, k, v, out and lse of the forward call: the same result on every run (no
  * atomics). dq, dk, dv have no overlap with anything. */

@@ -136,8 +136,10 @@ int fill_packed(const lbw_packed_params* p, PackedArgs* a) {
   LBW_TRY(check_scale(p->softmax_scale, p->head_dim, &scale));
   if (p->n_q_items < 0 || (p->n_q_items > 0 && p->q_items == nullptr))
     return fail(LBW_ERR_INVALID, "q_items missing");
-  if ((int64_t)p->n_q_items * p->q_heads > kMaxWorkgroups)
-    return fail(LBW_ERR_UNSUPPORTED, "%d query items x %d heads", p->n_q_items, p->q_heads);
+  if (p->q_tiles < 0 || p->q_tiles_max < 0 || p->k_tiles < 0 || p->k_tiles_max < 0 ||
+      std::max(std::max(p->q_tiles, p->q_tiles_max), std::max(p->k_tiles, p->k_tiles_max)) >
+          (int64_t(1) << 56) / p->q_heads)
+    return fail(LBW_ERR_INVALID, "the plan's tile counts are out of range");
   a->q = {static_cast<const uint16_t*>(p->q), p->q_stride_l, p->q_stride_h};
   a->k = {static_cast<const uint16_t*>(p->k), p->k_stride_l, p->k_stride_h};
   a->v = {static_cast<const uint16_t*>(p->v), p->v_stride_l, p->v_stride_h};
@@ -149,6 +151,54 @@ int fill_packed(const lbw_packed_params* p, PackedArgs* a) {
   a->q_items = p->q_items; a->n_q_items = p->n_q_items;
   a->k_items = p->k_items; a->n_k_items = p->n_k_items;
   return LBW_OK;
+}
+
+// How a kernel's items are cut. `slots` run at once; an item of `longest` tiles ends last when that is
+// more than half as much again as its share of all tiles: then items are cut into pieces of two thirds of
+// a share, `least` tiles at least.
+PackedSplit split_items(int64_t items, int64_t heads, int64_t tiles, int64_t longest, int64_t slots,
+                        int64_t least) {
+  PackedSplit s = {0, 1, 1};
+  if (tiles <= 0 || longest <= 0 || items <= 0) return s;
+  const int64_t share = tiles * heads / slots;
+  if (2 * longest <= 3 * share || longest < 2 * least) return s;
+  s.piece = (int)std::min<int64_t>(std::max<int64_t>(least, share * 2 / 3), 1 << 30);
+  s.smax = (int)std::min<int64_t>(16, (longest + s.piece - 1) / s.piece);
+  if (s.smax < 2) return PackedSplit{0, 1, 1};
+  // (the items longer than a piece come first in the table, and are no more than this)
+  s.n_split = (int)std::min<int64_t>(items, std::max<int64_t>(1, tiles / s.piece));
+  return s;
+}
+// two workgroups per CU; a piece's O is written and read in the time of about 6 tiles
+PackedSplit split_q(const lbw_packed_params* p) {
+  return split_items(p->n_q_items, p->q_heads, p->q_tiles, p->q_tiles_max, 2 * num_cus(), 8);
+}
+// one workgroup per CU, its tiles those of all heads of the group
+PackedSplit split_k(const lbw_packed_params* p) {
+  const int64_t group = p->q_heads / p->k_heads;
+  return split_items(p->n_k_items, p->k_heads, p->k_tiles * group, p->k_tiles_max * group, num_cus(), 24);
+}
+size_t part_bytes(const PackedSplit& s, int heads, int floats) {
+  return (size_t)s.n_split * heads * s.smax * floats * sizeof(float);
+}
+int check_grid(const PackedSplit& s, int64_t items, int64_t heads, int64_t limit) {
+  if (items + (int64_t)s.n_split * (s.smax - 1) > limit / heads)
+    return fail(LBW_ERR_UNSUPPORTED, "%lld work items x %lld heads", (long long)items, (long long)heads);
+  return LBW_OK;
+}
+void set_split(PackedArgs* a, const PackedSplit& s, void* part) {
+  a->n_split = s.n_split;
+  a->smax = s.smax;
+  a->piece = s.piece;
+  a->part = static_cast<float*>(part);
+}
+// delta and -lse of the gradient, rounded up to 16 bytes
+size_t stat_bytes(const lbw_packed_params* p) {
+  return (2 * (size_t)p->q_heads * (size_t)p->q_tokens * sizeof(float) + 15) / 16 * 16;
+}
+bool sane(const lbw_packed_params* p) {
+  return p != nullptr && p->q_heads >= 1 && p->k_heads >= 1 && p->q_heads % p->k_heads == 0 &&
+         p->q_tokens >= 0 && p->q_tokens <= 0x7fffffff;
 }
 
 int decode_pieces(const lbw_decode_params* p) {
@@ -246,12 +296,10 @@ int lbw_head_norm_rope_bwd(const lbw_head_norm_rope_params* p, const lbw_head_no
 
 int lbw_attention_packed_plan(int32_t n_seqs, const int32_t* q_lens, const int32_t* k_lens,
                               int32_t causal, int32_t* q_items, int64_t q_items_cap,
-                              int64_t* n_q_items, int32_t* k_items, int64_t k_items_cap,
-                              int64_t* n_k_items) {
+                              int32_t* k_items, int64_t k_items_cap, lbw_packed_plan_info* info) {
   if (n_seqs < 0 || (n_seqs > 0 && (q_lens == nullptr || k_lens == nullptr)))
     return fail(LBW_ERR_INVALID, "n_seqs %d needs q_lens and k_lens", n_seqs);
-  if (n_q_items == nullptr || n_k_items == nullptr)
-    return fail(LBW_ERR_INVALID, "n_q_items and n_k_items must not be NULL");
+  if (info == nullptr) return fail(LBW_ERR_INVALID, "info must not be NULL");
   int64_t tq = 0, tk = 0, nq = 0, nk = 0;
   for (int32_t s = 0; s < n_seqs; ++s) {
     if (q_lens[s] < 0 || k_lens[s] < 0)
@@ -264,8 +312,24 @@ int lbw_attention_packed_plan(int32_t n_seqs, const int32_t* q_lens, const int32
   if (tq > 0x7fffffff || tk > 0x7fffffff)
     return fail(LBW_ERR_UNSUPPORTED, "%lld query and %lld key rows: below 2^31", (long long)tq,
                 (long long)tk);
-  *n_q_items = nq;
-  *n_k_items = nk;
+  memset(info, 0, sizeof(*info));
+  info->n_q_items = nq;
+  info->n_k_items = nk;
+  for (int32_t s = 0; s < n_seqs; ++s) {
+    const int64_t lq = q_lens[s], lk = k_lens[s], shift = causal ? lk - lq : lk;
+    for (int64_t i = 0; i < lq; i += PK_BLOCK) {
+      const int64_t seen = std::clamp<int64_t>(std::min<int64_t>(i + PK_BLOCK, lq) + shift, 0, lk);
+      const int64_t t = (seen + 63) / 64;
+      info->q_tiles += t;
+      info->q_tiles_max = std::max(info->q_tiles_max, t);
+    }
+    for (int64_t j = 0; j < lk; j += PK_BLOCK) {
+      const int64_t first = std::clamp<int64_t>(j - shift, 0, lq);
+      const int64_t t = first < lq ? (lq + 63) / 64 - first / 64 : 0;
+      info->k_tiles += t;
+      info->k_tiles_max = std::max(info->k_tiles_max, t);
+    }
+  }
   if (q_items == nullptr && k_items == nullptr) return LBW_OK;
   if ((nq > 0 && q_items == nullptr) || (nk > 0 && k_items == nullptr) || q_items_cap < nq ||
       k_items_cap < nk)
@@ -304,17 +368,31 @@ int lbw_attention_packed_plan(int32_t n_seqs, const int32_t* q_lens, const int32
   return LBW_OK;
 }
 
-int lbw_attention_packed_fwd(const lbw_packed_params* p, void* stream) {
+size_t lbw_attention_packed_workspace_size(const lbw_packed_params* p) {
+  return sane(p) ? part_bytes(split_q(p), p->q_heads, PK_PART_FWD) : 0;
+}
+
+int lbw_attention_packed_fwd(const lbw_packed_params* p, void* workspace, size_t workspace_bytes,
+                             void* stream) {
   PackedArgs a;
   LBW_TRY(fill_packed(p, &a));
   if (a.n_q_items == 0) return LBW_OK;
+  const PackedSplit s = split_q(p);
+  LBW_TRY(check_grid(s, a.n_q_items, a.Hq, kMaxWorkgroups));
+  const size_t need = part_bytes(s, p->q_heads, PK_PART_FWD);
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
+    return fail(LBW_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need,
+                workspace_bytes);
+  set_split(&a, s, workspace);
   const hipError_t e = launch_packed_fwd(a, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? LBW_OK : hip_fail(e, "packed attention launch");
 }
 
+// delta and -lse, then the partial results of dQ and, after them, of dK and dV in the same place
 size_t lbw_attention_packed_bwd_workspace_size(const lbw_packed_params* p) {
-  if (p == nullptr || p->q_tokens <= 0 || p->q_heads <= 0) return 0;
-  return 2 * (size_t)p->q_heads * (size_t)p->q_tokens * sizeof(float);  // delta and -lse
+  if (!sane(p)) return 0;
+  return stat_bytes(p) + std::max(part_bytes(split_q(p), p->q_heads, PK_PART_DQ),
+                                  part_bytes(split_k(p), p->k_heads, PK_PART_DKV));
 }
 
 int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads* g,
@@ -324,8 +402,8 @@ int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads*
   if (g == nullptr) return fail(LBW_ERR_INVALID, "grads is NULL");
   if (p->n_k_items < 0 || (p->n_k_items > 0 && p->k_items == nullptr))
     return fail(LBW_ERR_INVALID, "k_items missing");
-  if ((int64_t)p->n_k_items * p->k_heads > kMaxWorkgroups)
-    return fail(LBW_ERR_UNSUPPORTED, "%d key items x %d heads", p->n_k_items, p->k_heads);
+  LBW_TRY(check_grid(split_q(p), p->n_q_items, p->q_heads, kMaxWorkgroups));
+  LBW_TRY(check_grid(split_k(p), p->n_k_items, p->k_heads, kMaxWorkgroups / 2));
   if (p->q_tokens > 0 && p->lse == nullptr) return fail(LBW_ERR_INVALID, "lse missing");
   LBW_TRY(check_rows("dout", g->dout, p->q_tokens, g->dout_stride_l, g->dout_stride_h, true));
   LBW_TRY(check_rows("dq", g->dq, p->q_tokens, g->dq_stride_l, g->dq_stride_h));
@@ -342,11 +420,14 @@ int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads*
   a.dq = {static_cast<uint16_t*>(g->dq), g->dq_stride_l, g->dq_stride_h};
   a.dk = {static_cast<uint16_t*>(g->dk), g->dk_stride_l, g->dk_stride_h};
   a.dv = {static_cast<uint16_t*>(g->dv), g->dv_stride_l, g->dv_stride_h};
+  void* const part = static_cast<char*>(workspace) + stat_bytes(p);
   if (a.n_q_items > 0) {
+    set_split(&a, split_q(p), part);
     const hipError_t e = launch_packed_dq(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "packed attention dQ launch");
   }
   if (a.n_k_items > 0) {
+    set_split(&a, split_k(p), part);
     const hipError_t e = launch_packed_dkv(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "packed attention dK/dV launch");
   }

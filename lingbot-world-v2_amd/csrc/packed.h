@@ -68,12 +68,22 @@ struct PackedArgs {
   const int32_t* q_items;
   const int32_t* k_items;
   int n_q_items, n_k_items;
+  // The first n_split items are cut into pieces of about `piece` tiles, at most smax, when they are
+  // longer; a piece leaves fp32 partial results in `part`, which a second kernel joins in their order.
+  int n_split, smax, piece;
+  float* part;
   // gradient
   Rows o, dout;
   float* delta;                // [Hq][Tq]: sum_d dout out
   float* nlse2;                // [Hq][Tq]: -lse log2(e), -inf for a query that sees no key
   RowsOut dq, dk, dv;
 };
+struct PackedSplit {
+  int n_split, smax, piece;
+};
+// Floats of a piece's partial result: forward (O, m, l), dQ, dK + dV of 128 rows x 128.
+constexpr int PK_PART_FWD = PK_BLOCK * 128 + 2 * PK_BLOCK, PK_PART_DQ = PK_BLOCK * 128,
+              PK_PART_DKV = 2 * PK_BLOCK * 128;
 hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t stream);
 hipError_t launch_packed_dq(const PackedArgs& a, hipStream_t stream);
 hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream);

@@ -9,7 +9,6 @@
 // walks the queries of all heads of its group: dK and dV (four products a tile).
 // Both recompute S; P and dS go to bf16 as operands, one rounding each.
 
-#include <stdlib.h>
 #include "packed_tiles.h"
 
 namespace lbw {
@@ -28,9 +27,14 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
   int h, kv;
-  pick_head(blockIdx.x % (uint32_t)a.Hq, a.Hk, a.Hq / a.Hk, h, kv);
-  const PackedItem it = load_item(a.q_items, blockIdx.x / (uint32_t)a.Hq);
+  const PackedShare sh = pick_share(a, blockIdx.x, a.Hq);
+  pick_head(sh.head, a.Hk, a.Hq / a.Hk, h, kv);
+  const PackedItem it = load_item(a.q_items, sh.item);
   if (!item_fits(it, a.Tq, a.Tk)) return;
+  const int n_tiles = (it.bound + BN - 1) / BN, pieces = pieces_of(a, sh, n_tiles);
+  if (sh.piece >= pieces) return;
+  const int t0 = (int)((int64_t)n_tiles * sh.piece / pieces);
+  const int T = (int)((int64_t)n_tiles * (sh.piece + 1) / pieces);
   const int r0 = 32 * wave, rows = it.rows - r0;
   const bool active = rows > 0;
 
@@ -52,7 +56,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
       const int64_t at = (int64_t)h * a.Tq + row + l32;
       const float x = a.lse[at];
       nlse2 = x == -INFINITY ? -INFINITY : -x * LOG2E;
-      if (hl == 0) {
+      if (hl == 0 && sh.piece == 0) {
         a.delta[at] = delta;
         a.nlse2[at] = nlse2;
       }
@@ -80,13 +84,12 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
 #pragma unroll
   for (int db = 0; db < 4; ++db) zero(acc[db]);
   const float c = a.scale_log2;
-  const int T = (it.bound + BN - 1) / BN;
-  if (T > 0) {
-    copy.issue(kb, ks, 0, it.other_len, dst);
-    copy.issue(vb, vs, 0, it.other_len, dst + V_AT);
+  if (t0 < T) {
+    copy.issue(kb, ks, t0 * BN, it.other_len, dst + (t0 & 1) * PK_TILE_B);
+    copy.issue(vb, vs, t0 * BN, it.other_len, dst + V_AT + (t0 & 1) * PK_TILE_B);
   }
 #pragma unroll 1
-  for (int u = 0; u < T; ++u) {
+  for (int u = t0; u < T; ++u) {
     const int st = (u & 1) * PK_TILE_B;
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     barrier_nofence();
@@ -127,23 +130,57 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
   __builtin_amdgcn_s_waitcnt(0x0070);
   barrier_nofence();
   if (!active) return;
+  if (pieces > 1) {
+    store_acc(part_of(a, sh, a.Hq, sh.piece, PK_PART_DQ), wave, lane, acc);
+    return;
+  }
   store_rows(lds + 8192 * wave, acc, a.scale, lane, rows, [&](int r) {
     return a.dq.p + (int64_t)(it.row0 + r0 + r) * a.dq.sl + h * a.dq.sh;
   });
 }
 
+// The pieces of a split query item added up, in their order.
+__global__ void __launch_bounds__(PK_WAVES * 64) packed_dq_join_kernel(const PackedArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[PK_WAVES * 8192];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const PackedShare sh = {(int)(blockIdx.x / (uint32_t)a.Hq), (int)(blockIdx.x % (uint32_t)a.Hq), 0, true};
+  int h, kv;
+  pick_head(sh.head, a.Hk, a.Hq / a.Hk, h, kv);
+  const PackedItem it = load_item(a.q_items, sh.item);
+  if (!item_fits(it, a.Tq, a.Tk)) return;
+  const int pieces = pieces_of(a, sh, (it.bound + BN - 1) / BN), rows = it.rows - 32 * wave;
+  if (pieces == 1 || rows <= 0) return;
+  floatx16 acc[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db) zero(acc[db]);
+  for (int s = 0; s < pieces; ++s) add_acc(part_of(a, sh, a.Hq, s, PK_PART_DQ), wave, lane, 1.0f, acc);
+  store_rows(lds + 8192 * wave, acc, a.scale, lane, rows, [&](int r) {
+    return a.dq.p + (int64_t)(it.row0 + 32 * wave + r) * a.dq.sl + h * a.dq.sh;
+  });
+}
+
 // ---- dK, dV: a lane holds one key's column of S = Q K^T and dP = dO V^T
-template <int GROUPS>
-__global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, GROUPS == 1 ? 2 : 1)
-packed_dkv_kernel(const PackedArgs a) {
+constexpr int GROUPS = 2;  // wave groups of a workgroup, each with its share of an item's query tiles
+constexpr int DKV_LDS = GROUPS * DKV_GROUP_B;
+__global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(const PackedArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63;
   const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = wave_id % PK_WAVES, grp = wave_id / PK_WAVES;
   const int hl = lane >> 5, l32 = lane & 31;
-  const int kv = blockIdx.x % (uint32_t)a.Hk, group = a.Hq / a.Hk;
-  const PackedItem it = load_item(a.k_items, blockIdx.x / (uint32_t)a.Hk);
+  const PackedShare sh = pick_share(a, blockIdx.x, a.Hk);
+  const int kv = sh.head, group = a.Hq / a.Hk;
+  const PackedItem it = load_item(a.k_items, sh.item);
   if (!item_fits(it, a.Tk, a.Tq)) return;
+  // query tiles of a head, and of the group's heads one after another; this piece's, this group's
+  const int t_first = it.bound / BN, t_end = (it.other_len + BN - 1) / BN;
+  const int per = it.bound < it.other_len ? t_end - t_first : 0;
+  const int all = per * group, pieces = pieces_of(a, sh, all);
+  if (sh.piece >= pieces) return;
+  const int p0 = (int)((int64_t)all * sh.piece / pieces);
+  const int mine = (int)((int64_t)all * (sh.piece + 1) / pieces) - p0;
+  const int n0 = p0 + mine * grp / GROUPS, T = p0 + mine * (grp + 1) / GROUPS;
+  const int Tmax = n0 + (mine + GROUPS - 1) / GROUPS;  // the loop's end, the same count in both groups
   const int r0 = 32 * wave, rows = it.rows - r0;
   const bool active = rows > 0;
 
@@ -174,11 +211,6 @@ packed_dkv_kernel(const PackedArgs a) {
     zero(dv[db]);
   }
   const float c = a.scale_log2;
-  const int t_first = it.bound / BN, t_end = (it.other_len + BN - 1) / BN;
-  const int per = it.bound < it.other_len ? t_end - t_first : 0;  // query tiles of a head
-  const int all = per * group;
-  const int n0 = all * grp / GROUPS, T = all * (grp + 1) / GROUPS;  // this group's share
-  const int Tmax = n0 + (all + GROUPS - 1) / GROUPS;
   const int64_t qs = a.q.sl * 2, gs = a.dout.sl * 2;
   // query tile n (head n / per of the group) into stage n % 2; waves 0 and 1 fetch its rows' -lse and
   // delta (rows past the sequence's end: the last one's)
@@ -249,7 +281,7 @@ packed_dkv_kernel(const PackedArgs a) {
   }
   __builtin_amdgcn_s_waitcnt(0x0070);
   barrier_nofence();
-  if constexpr (GROUPS == 2) {
+  {
     // group 1 hands its sums over in register order, 16 bytes per lane: dK through its own LDS, dV
     // through group 0's
     unsigned char* g1 = lds + DKV_GROUP_B + 16384 * wave;
@@ -282,6 +314,13 @@ packed_dkv_kernel(const PackedArgs a) {
   }
   if (!active) return;
   // (the lane index taken anew rather than kept, or spilled, across the loop)
+  if (pieces > 1) {
+    const int ln1 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    float* const part = part_of(a, sh, a.Hk, sh.piece, PK_PART_DKV);
+    store_acc(part, wave, ln1, dk);
+    store_acc(part + PK_BLOCK * 128, wave, ln1, dv);
+    return;
+  }
   const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
   store_rows(lds + 8192 * wave, dk, a.scale, ln, rows, [&](int r) {
     return a.dk.p + (int64_t)(it.row0 + r0 + r) * a.dk.sl + kv * a.dk.sh;
@@ -292,30 +331,57 @@ packed_dkv_kernel(const PackedArgs a) {
   });
 }
 
+// The pieces of a split key item added up, in their order.
+__global__ void __launch_bounds__(PK_WAVES * 64) packed_dkv_join_kernel(const PackedArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[PK_WAVES * 8192];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const PackedShare sh = {(int)(blockIdx.x / (uint32_t)a.Hk), (int)(blockIdx.x % (uint32_t)a.Hk), 0, true};
+  const PackedItem it = load_item(a.k_items, sh.item);
+  if (!item_fits(it, a.Tk, a.Tq)) return;
+  const int per = it.bound < it.other_len ? (it.other_len + BN - 1) / BN - it.bound / BN : 0;
+  const int pieces = pieces_of(a, sh, per * (a.Hq / a.Hk)), rows = it.rows - 32 * wave;
+  if (pieces == 1 || rows <= 0) return;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    floatx16 acc[4];
+#pragma unroll
+    for (int db = 0; db < 4; ++db) zero(acc[db]);
+    for (int s = 0; s < pieces; ++s)
+      add_acc(part_of(a, sh, a.Hk, s, PK_PART_DKV) + which * PK_BLOCK * 128, wave, lane, 1.0f, acc);
+    const RowsOut out = which == 0 ? a.dk : a.dv;
+    store_rows(lds + 8192 * wave, acc, which == 0 ? a.scale : 1.0f, lane, rows, [&](int r) {
+      return out.p + (int64_t)(it.row0 + 32 * wave + r) * out.sl + sh.head * out.sh;
+    });
+    wave_lds_fence();
+  }
+}
+
 }  // namespace
 
 hipError_t launch_packed_dq(const PackedArgs& a, hipStream_t stream) {
   static hipError_t attr = hipFuncSetAttribute((const void*)packed_dq_kernel,
                                                hipFuncAttributeMaxDynamicSharedMemorySize, BWD_LDS);
   if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL(packed_dq_kernel, dim3((uint32_t)a.n_q_items * a.Hq), dim3(PK_WAVES * 64),
-                     BWD_LDS, stream, a);
+  const uint32_t n = ((uint32_t)a.n_q_items + (uint32_t)a.n_split * (a.smax - 1)) * a.Hq;
+  hipLaunchKernelGGL(packed_dq_kernel, dim3(n), dim3(PK_WAVES * 64), BWD_LDS, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.n_split == 0) return e;
+  hipLaunchKernelGGL(packed_dq_join_kernel, dim3((uint32_t)a.n_split * a.Hq), dim3(PK_WAVES * 64), 0,
+                     stream, a);
   return hipGetLastError();
 }
 
-template <int GROUPS>
-static hipError_t run_dkv(const PackedArgs& a, hipStream_t stream) {
-  constexpr int bytes = GROUPS * DKV_GROUP_B;
-  static hipError_t attr = hipFuncSetAttribute((const void*)packed_dkv_kernel<GROUPS>,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL(packed_dkv_kernel<GROUPS>, dim3((uint32_t)a.n_k_items * a.Hk),
-                     dim3(GROUPS * PK_WAVES * 64), bytes, stream, a);
-  return hipGetLastError();
-}
 hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream) {
-  const char* e = getenv("LBW_G");
-  return e && e[0] == '1' ? run_dkv<1>(a, stream) : run_dkv<2>(a, stream);
+  static hipError_t attr = hipFuncSetAttribute((const void*)packed_dkv_kernel,
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, DKV_LDS);
+  if (attr != hipSuccess) return attr;
+  const uint32_t n = ((uint32_t)a.n_k_items + (uint32_t)a.n_split * (a.smax - 1)) * a.Hk;
+  hipLaunchKernelGGL(packed_dkv_kernel, dim3(n), dim3(GROUPS * PK_WAVES * 64), DKV_LDS, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.n_split == 0) return e;
+  hipLaunchKernelGGL(packed_dkv_join_kernel, dim3((uint32_t)a.n_split * a.Hk), dim3(PK_WAVES * 64), 0,
+                     stream, a);
+  return hipGetLastError();
 }
 
 }  // namespace lbw

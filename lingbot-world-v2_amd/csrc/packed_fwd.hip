@@ -12,33 +12,39 @@
 // O += V_{j-1}^T P_{j-1}^T and S_{j+1} = K_{j+1} Q^T. Online softmax in base 2 against a reference
 // that moves only when a row's sum in a step outgrows it; O and l share it, so the result is exact.
 
-#include <stdlib.h>
 #include "packed_tiles.h"
 
 namespace lbw {
 namespace {
 
 constexpr int V_AT = 2 * PK_TILE_B;              // V stages behind the K stages
-constexpr int GROUP_B = 4 * PK_TILE_B;           // LDS of a group of 4 waves
+constexpr int FWD_LDS = 4 * PK_TILE_B;
 constexpr int HALF_B = PK_TILE_B / 2;
 constexpr int AHEAD = 2;                         // MFMA pairs that LDS fragments are read ahead
 
 template <int N>
 using ic = std::integral_constant<int, N>;
 
-// GROUPS = 1: a workgroup is one group, two workgroups share a CU. GROUPS = 2: two groups share a work
-// item, each with half of its keys, and join their results in LDS.
-template <int GROUPS>
-__global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, GROUPS == 1 ? 2 : 1)
-packed_fwd_kernel(const PackedArgs a) {
+// A wave's rows from O, the reference and the sum (of both lane halves) to out and lse.
+__device__ __forceinline__ void finish(const PackedArgs& a, const PackedItem& it, int h, int wave,
+                                       int lane, int rows, const floatx16 (&o)[4], float m, float l,
+                                       unsigned char* lds) {
+  const int64_t row0 = it.row0 + 32 * wave;
+  if (a.lse != nullptr && lane < 32 && lane < rows)
+    a.lse[(int64_t)h * a.Tq + row0 + lane] = l > 0.0f ? m * a.scale + logf(l) : -INFINITY;
+  store_rows(lds + 8192 * wave, o, l > 0.0f ? 1.0f / l : 0.0f, lane, rows,
+             [&](int r) { return a.out.p + (row0 + r) * a.out.sl + h * a.out.sh; });
+}
+
+__global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const PackedArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63;
-  const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wave = wave_id % PK_WAVES, grp = wave_id / PK_WAVES;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
   int h, kv;
-  pick_head(blockIdx.x % (uint32_t)a.Hq, a.Hk, a.Hq / a.Hk, h, kv);
-  const PackedItem it = load_item(a.q_items, blockIdx.x / (uint32_t)a.Hq);
+  const PackedShare sh = pick_share(a, blockIdx.x, a.Hq);
+  pick_head(sh.head, a.Hk, a.Hq / a.Hk, h, kv);
+  const PackedItem it = load_item(a.q_items, sh.item);
   if (!item_fits(it, a.Tq, a.Tk)) return;
   const int r0 = 32 * wave;                       // this wave's first row of the item
   const int rows = it.rows - r0;                  // and how many it has
@@ -62,15 +68,15 @@ packed_fwd_kernel(const PackedArgs a) {
   };
   const int lim = limit(i0 + l32);
   const int lim_lo = limit(i0), lim_hi = limit(i0 + (rows < 32 ? rows : 32) - 1);
-  // this group's tiles [t0, t0 + T) of the item, of which this wave needs the first Tw; the loop
-  // runs Tmax times in every wave of the workgroup
-  const int n_tiles = (it.bound + BN - 1) / BN;
-  const int t0 = n_tiles * grp / GROUPS, T = n_tiles * (grp + 1) / GROUPS - t0;
-  const int Tmax = (n_tiles + GROUPS - 1) / GROUPS;
+  // this piece's tiles [t0, t0 + T), of which this wave needs the first Tw
+  const int n_tiles = (it.bound + BN - 1) / BN, pieces = pieces_of(a, sh, n_tiles);
+  if (sh.piece >= pieces) return;
+  const int t0 = (int)((int64_t)n_tiles * sh.piece / pieces);
+  const int T = (int)((int64_t)n_tiles * (sh.piece + 1) / pieces) - t0;
   int Tw = rows > 0 ? (lim_hi + BN - 1) / BN - t0 : 0;
   Tw = Tw < 0 ? 0 : (Tw < T ? Tw : T);
 
-  const int lds0 = (int)lds_addr(lds) + GROUP_B * grp;
+  const int lds0 = (int)lds_addr(lds);
   const int ka = row_address(lds0, l32, hl), va = tr_address(lds0 + V_AT, lane, hl);
   TileCopy copy;
   copy.init(wave, lane);
@@ -86,17 +92,14 @@ packed_fwd_kernel(const PackedArgs a) {
   float m = M_INIT, l = 0.0f;
   const float c = sreg(a.scale_log2);
 
-  if (Tmax > 0) {
-    if (T > 0) {
-      issue_k(0);
-      issue_v(0);
-      if (T > 1) issue_k(1);
-    }
+  if (T > 0) {
+    issue_k(0);
+    issue_v(0);
+    if (T > 1) issue_k(1);
     // the first step's "previous block" is the second half of V stage 1, with P = 0: zeros there
-    *reinterpret_cast<u32x4*>(lds + GROUP_B * grp + V_AT + PK_TILE_B + HALF_B + 1024 * 2 * wave + 16 * lane) =
-        u32x4{0u, 0u, 0u, 0u};
-    *reinterpret_cast<u32x4*>(lds + GROUP_B * grp + V_AT + PK_TILE_B + HALF_B + 1024 * (2 * wave + 1) + 16 * lane) =
-        u32x4{0u, 0u, 0u, 0u};
+    unsigned char* const zv = lds + V_AT + PK_TILE_B + HALF_B + 2048 * wave + 16 * lane;
+    *reinterpret_cast<u32x4*>(zv) = u32x4{0u, 0u, 0u, 0u};
+    *reinterpret_cast<u32x4*>(zv + 1024) = u32x4{0u, 0u, 0u, 0u};
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     barrier_nofence();
   }
@@ -209,68 +212,69 @@ packed_fwd_kernel(const PackedArgs a) {
     if (u < Tw) step(ic<SN * PK_TILE_B>{}, ic<ST * PK_TILE_B>{}, sB, sA, pB, pA, key0 + 32);
   };
 #pragma unroll 1
-  for (int u = 0; u < Tmax; u += 2) {
+  for (int u = 0; u < T; u += 2) {
     tile(ic<0>{}, u);
-    if (u + 1 < Tmax) tile(ic<1>{}, u + 1);
+    if (u + 1 < T) tile(ic<1>{}, u + 1);
   }
-  if (Tw == Tmax && Tw > 0) drain(Tw - 1);
+  if (Tw == T && Tw > 0) drain(Tw - 1);
   __builtin_amdgcn_s_waitcnt(0x0070);
   barrier_nofence();  // all waves are past their tile reads: the LDS is free for the output
-  float ls = wave_sum_xor32(l);
-  if constexpr (GROUPS == 2) {
-    // group 1 hands its O, m and l over in register order, 16 bytes per lane
-    unsigned char* og = lds + GROUP_B + 16384 * wave + 16 * lane;
-    float* ml = reinterpret_cast<float*>(lds + 32768 + 512 * wave);
-    if (grp == 1) {
-#pragma unroll
-      for (int x = 0; x < 16; ++x)
-        *reinterpret_cast<floatx4*>(og + 1024 * x) =
-            floatx4{o[x >> 2][4 * (x & 3)], o[x >> 2][4 * (x & 3) + 1], o[x >> 2][4 * (x & 3) + 2],
-                    o[x >> 2][4 * (x & 3) + 3]};
-      ml[lane] = m;
-      ml[64 + lane] = ls;
-    }
-    __syncthreads();
-    if (grp == 1) return;
-    const float m1 = ml[lane], l1 = ml[64 + lane];
-    const float mn = fmaxf(m, m1);  // (a half without keys: M_INIT, l = 0, O = 0)
-    const float f0 = fast_exp2((m - mn) * c), f1 = fast_exp2((m1 - mn) * c);
-#pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      const floatx4 y = *reinterpret_cast<const floatx4*>(og + 1024 * x);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float& z = reinterpret_cast<float*>(&o[x >> 2])[4 * (x & 3) + e];
-        z = z * f0 + y[e] * f1;
-      }
-    }
-    ls = ls * f0 + l1 * f1;
-    m = mn;
-  }
   if (rows <= 0) return;
-  if (a.lse != nullptr && hl == 0 && l32 < rows)
-    a.lse[(int64_t)h * a.Tq + it.row0 + r0 + l32] = ls > 0.0f ? m * a.scale + logf(ls) : -INFINITY;
-  store_rows(lds + 8192 * wave, o, ls > 0.0f ? 1.0f / ls : 0.0f, lane, rows, [&](int r) {
-    return a.out.p + (int64_t)(it.row0 + r0 + r) * a.out.sl + h * a.out.sh;
-  });
+  const float ls = wave_sum_xor32(l);
+  if (pieces > 1) {
+    float* const part = part_of(a, sh, a.Hq, sh.piece, PK_PART_FWD);
+    store_acc(part, wave, lane, o);
+    if (hl == 0) {
+      part[PK_BLOCK * 128 + r0 + l32] = ls > 0.0f ? m : -INFINITY;
+      part[PK_BLOCK * 128 + PK_BLOCK + r0 + l32] = ls;
+    }
+    return;
+  }
+  finish(a, it, h, wave, lane, rows, o, m, ls, lds);
 }
 
-template <int GROUPS>
-hipError_t run(const PackedArgs& a, hipStream_t stream) {
-  static hipError_t attr = hipFuncSetAttribute((const void*)packed_fwd_kernel<GROUPS>,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize,
-                                               GROUPS * GROUP_B);
-  if (attr != hipSuccess) return attr;
-  hipLaunchKernelGGL(packed_fwd_kernel<GROUPS>, dim3((uint32_t)a.n_q_items * a.Hq),
-                     dim3(GROUPS * PK_WAVES * 64), GROUPS * GROUP_B, stream, a);
-  return hipGetLastError();
+// The pieces of a split item joined, in their order.
+__global__ void __launch_bounds__(PK_WAVES * 64) packed_fwd_join_kernel(const PackedArgs a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[PK_WAVES * 8192];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  PackedShare sh = {(int)(blockIdx.x / (uint32_t)a.Hq), (int)(blockIdx.x % (uint32_t)a.Hq), 0, true};
+  int h, kv;
+  pick_head(sh.head, a.Hk, a.Hq / a.Hk, h, kv);
+  const PackedItem it = load_item(a.q_items, sh.item);
+  if (!item_fits(it, a.Tq, a.Tk)) return;
+  const int pieces = pieces_of(a, sh, (it.bound + BN - 1) / BN);
+  const int rows = it.rows - 32 * wave;
+  if (pieces == 1 || rows <= 0) return;
+  const int row = 32 * wave + (lane & 31);
+  float m = -INFINITY, l = 0.0f;
+  for (int s = 0; s < pieces; ++s)
+    m = fmaxf(m, part_of(a, sh, a.Hq, s, PK_PART_FWD)[PK_BLOCK * 128 + row]);
+  floatx16 o[4];
+#pragma unroll
+  for (int db = 0; db < 4; ++db) zero(o[db]);
+  for (int s = 0; s < pieces; ++s) {
+    const float* part = part_of(a, sh, a.Hq, s, PK_PART_FWD);
+    const float ms = part[PK_BLOCK * 128 + row];
+    const float f = ms == -INFINITY ? 0.0f : fast_exp2((ms - m) * a.scale_log2);
+    l += f * part[PK_BLOCK * 128 + PK_BLOCK + row];
+    add_acc(part, wave, lane, f, o);
+  }
+  finish(a, it, h, wave, lane, rows, o, m, l, lds);
 }
 
 }  // namespace
 
 hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t stream) {
-  const char* e = getenv("LBW_G");
-  return e && e[0] == '3' ? run<2>(a, stream) : run<1>(a, stream);
+  static hipError_t attr = hipFuncSetAttribute((const void*)packed_fwd_kernel,
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, FWD_LDS);
+  if (attr != hipSuccess) return attr;
+  const uint32_t n = ((uint32_t)a.n_q_items + (uint32_t)a.n_split * (a.smax - 1)) * a.Hq;
+  hipLaunchKernelGGL(packed_fwd_kernel, dim3(n), dim3(PK_WAVES * 64), FWD_LDS, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.n_split == 0) return e;
+  hipLaunchKernelGGL(packed_fwd_join_kernel, dim3((uint32_t)a.n_split * a.Hq), dim3(PK_WAVES * 64), 0,
+                     stream, a);
+  return hipGetLastError();
 }
 
 }  // namespace lbw

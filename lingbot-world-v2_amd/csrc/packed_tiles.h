@@ -46,6 +46,54 @@ __device__ __forceinline__ void pick_head(uint32_t c, int Hk, int group, int& h,
   h = kv * group + c / (uint32_t)Hk;
 }
 
+// A workgroup's item, head and piece. Split items come first, all pieces of the costliest ahead: item,
+// piece, head; then the others: item, head.
+struct PackedShare {
+  int item, head, piece;
+  bool split;  // the item may have several pieces
+};
+__device__ __forceinline__ PackedShare pick_share(const PackedArgs& a, uint32_t b, int heads) {
+  const uint32_t cut = (uint32_t)a.n_split * a.smax * heads;
+  PackedShare s;
+  if (b < cut) {
+    const uint32_t r = b % ((uint32_t)a.smax * heads);
+    s = {(int)(b / ((uint32_t)a.smax * heads)), (int)(r % heads), (int)(r / heads), true};
+  } else {
+    s = {a.n_split + (int)((b - cut) / heads), (int)((b - cut) % heads), 0, false};
+  }
+  return s;
+}
+__device__ __forceinline__ int pieces_of(const PackedArgs& a, const PackedShare& s, int tiles) {
+  if (!s.split) return 1;
+  const int n = (tiles + a.piece - 1) / a.piece;
+  return n < 1 ? 1 : (n < a.smax ? n : a.smax);
+}
+// Piece's partial result, `floats` of them for each.
+__device__ __forceinline__ float* part_of(const PackedArgs& a, const PackedShare& s, int heads, int piece,
+                                          int floats) {
+  return a.part + (((int64_t)s.item * heads + s.head) * a.smax + piece) * floats;
+}
+// 16 accumulator registers x 4 blocks of a wave to and from memory in register order: 16 bytes per
+// lane, a wave's kilobytes one after another.
+__device__ __forceinline__ void store_acc(float* p, int wave, int lane, const floatx16 (&acc)[4]) {
+  floatx4* d = reinterpret_cast<floatx4*>(p) + 1024 * wave + lane;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const floatx16& y = acc[x >> 2];
+    const int e = 4 * (x & 3);
+    d[64 * x] = floatx4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+  }
+}
+__device__ __forceinline__ void add_acc(const float* p, int wave, int lane, float f, floatx16 (&acc)[4]) {
+  const floatx4* d = reinterpret_cast<const floatx4*>(p) + 1024 * wave + lane;
+#pragma unroll
+  for (int x = 0; x < 16; ++x) {
+    const floatx4 v = d[64 * x];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[x >> 2][4 * (x & 3) + e] += f * v[e];
+  }
+}
+
 // This wave's share of a tile copied HBM -> LDS: rows first .. first + 63 of a sequence of `len`
 // rows at `base` (its row 0), row stride `stride_b` bytes; rows past the end copy the last row, so
 // a tile never touches another sequence.

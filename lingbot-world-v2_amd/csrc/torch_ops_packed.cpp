@@ -239,29 +239,31 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> head_norm_rope_bwd(
 
 // ---- packed attention
 
-std::tuple<Tensor, Tensor> packed_plan(const Tensor& q_lens, const Tensor& k_lens, bool causal) {
+// -> query items, key items, and the tile counts [q_tiles, q_tiles_max, k_tiles, k_tiles_max]
+std::tuple<Tensor, Tensor, std::vector<int64_t>> packed_plan(const Tensor& q_lens,
+                                                             const Tensor& k_lens, bool causal) {
   for (const Tensor* t : {&q_lens, &k_lens})
     TORCH_CHECK(t->device().is_cpu() && t->scalar_type() == at::kInt && t->dim() == 1 &&
                     t->is_contiguous() && t->numel() == q_lens.numel() &&
                     t->numel() < (int64_t(1) << 31),
                 "q_lens and k_lens must be int32 CPU vectors of one length");
   const int32_t n = (int32_t)q_lens.numel();
-  int64_t nq = 0, nk = 0;
-  check(lbw_attention_packed_plan(n, q_lens.data_ptr<int32_t>(), k_lens.data_ptr<int32_t>(), causal,
-                                  nullptr, 0, &nq, nullptr, 0, &nk),
+  const int32_t *ql = q_lens.data_ptr<int32_t>(), *kl = k_lens.data_ptr<int32_t>();
+  lbw_packed_plan_info info;
+  check(lbw_attention_packed_plan(n, ql, kl, causal, nullptr, 0, nullptr, 0, &info),
         "lbw_attention_packed_plan");
-  Tensor qi = at::empty({nq, LBW_PACKED_ITEM}, q_lens.options());
-  Tensor ki = at::empty({nk, LBW_PACKED_ITEM}, q_lens.options());
-  if (nq + nk > 0)
-    check(lbw_attention_packed_plan(n, q_lens.data_ptr<int32_t>(), k_lens.data_ptr<int32_t>(),
-                                    causal, qi.data_ptr<int32_t>(), nq, &nq,
-                                    ki.data_ptr<int32_t>(), nk, &nk),
+  Tensor qi = at::empty({info.n_q_items, LBW_PACKED_ITEM}, q_lens.options());
+  Tensor ki = at::empty({info.n_k_items, LBW_PACKED_ITEM}, q_lens.options());
+  if (info.n_q_items + info.n_k_items > 0)
+    check(lbw_attention_packed_plan(n, ql, kl, causal, qi.data_ptr<int32_t>(), info.n_q_items,
+                                    ki.data_ptr<int32_t>(), info.n_k_items, &info),
           "lbw_attention_packed_plan");
-  return {qi, ki};
+  return {qi, ki, {info.q_tiles, info.q_tiles_max, info.k_tiles, info.k_tiles_max}};
 }
 
 lbw_packed_params packed_params(const Tensor& q, const Tensor& k, const Tensor& v,
-                                const Tensor& q_items, const Tensor& k_items, double scale) {
+                                const Tensor& q_items, const Tensor& k_items,
+                                at::IntArrayRef tiles, double scale) {
   check_rows("q", q, q);
   check_rows("k", k, q);
   check_rows("v", v, q);
@@ -290,6 +292,11 @@ lbw_packed_params packed_params(const Tensor& q, const Tensor& k, const Tensor& 
   p.n_q_items = (int32_t)q_items.size(0);
   p.k_items = k_items.data_ptr<int32_t>();
   p.n_k_items = (int32_t)k_items.size(0);
+  TORCH_CHECK(tiles.size() == 4, "the plan's four tile counts are wanted");
+  p.q_tiles = tiles[0];
+  p.q_tiles_max = tiles[1];
+  p.k_tiles = tiles[2];
+  p.k_tiles_max = tiles[3];
   return p;
 }
 
@@ -299,14 +306,18 @@ Tensor new_lse(const Tensor& q) {
 
 std::tuple<Tensor, Tensor> attention_packed(const Tensor& q, const Tensor& k, const Tensor& v,
                                             const Tensor& q_items, const Tensor& k_items,
-                                            double scale, bool want_lse) {
+                                            at::IntArrayRef tiles, double scale, bool want_lse) {
   c10::DeviceGuard guard(q.device());
-  auto p = packed_params(q, k, v, q_items, k_items, scale);
+  auto p = packed_params(q, k, v, q_items, k_items, tiles, scale);
   Tensor out = at::empty(q.sizes(), q.options());
   Tensor lse = want_lse ? new_lse(q) : at::empty({0}, q.options().dtype(at::kFloat));
   p.out = out.data_ptr(); p.out_stride_l = out.stride(0); p.out_stride_h = out.stride(1);
   p.lse = want_lse ? lse.data_ptr<float>() : nullptr;
-  check(lbw_attention_packed_fwd(&p, stream_of(q)), "lbw_attention_packed_fwd");
+  const size_t bytes = lbw_attention_packed_workspace_size(&p);
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+  check(lbw_attention_packed_fwd(&p, bytes > 0 ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+        "lbw_attention_packed_fwd");
   return {out, lse};
 }
 
@@ -314,9 +325,10 @@ std::tuple<Tensor, Tensor, Tensor> attention_packed_bwd(const Tensor& dout_, con
                                                         const Tensor& k, const Tensor& v,
                                                         const Tensor& out, const Tensor& lse,
                                                         const Tensor& q_items,
-                                                        const Tensor& k_items, double scale) {
+                                                        const Tensor& k_items,
+                                                        at::IntArrayRef tiles, double scale) {
   c10::DeviceGuard guard(q.device());
-  auto p = packed_params(q, k, v, q_items, k_items, scale);
+  auto p = packed_params(q, k, v, q_items, k_items, tiles, scale);
   check_rows("out", out, q);
   TORCH_CHECK(dout_.sizes() == q.sizes() && dout_.scalar_type() == at::kBFloat16 &&
                   dout_.device() == q.device() && out.sizes() == q.sizes(),
@@ -412,14 +424,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> head_norm_rope_bwd_meta(
           wk.has_value() ? at::empty_like(*wk) : at::empty({0}, q.options())};
 }
 std::tuple<Tensor, Tensor> attention_packed_meta(const Tensor& q, const Tensor&, const Tensor&,
-                                                 const Tensor&, const Tensor&, double,
-                                                 bool want_lse) {
+                                                 const Tensor&, const Tensor&, at::IntArrayRef,
+                                                 double, bool want_lse) {
   return {at::empty(q.sizes(), q.options()),
           want_lse ? new_lse(q) : at::empty({0}, q.options().dtype(at::kFloat))};
 }
 std::tuple<Tensor, Tensor, Tensor> attention_packed_bwd_meta(
     const Tensor&, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&, const Tensor&,
-    const Tensor&, const Tensor&, double) {
+    const Tensor&, const Tensor&, at::IntArrayRef, double) {
   return {at::empty(q.sizes(), q.options()), at::empty(k.sizes(), k.options()),
           at::empty(v.sizes(), v.options())};
 }
@@ -528,19 +540,21 @@ std::tuple<Tensor, Tensor> head_norm_rope_autograd(const Tensor& q, const Tensor
 }
 
 auto call_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qi,
-                 const Tensor& ki, double scale, bool want_lse) {
+                 const Tensor& ki, at::IntArrayRef tiles, double scale, bool want_lse) {
   static auto op = handle<decltype(attention_packed)>("lbw::attention_packed");
-  return op.call(q, k, v, qi, ki, scale, want_lse);
+  return op.call(q, k, v, qi, ki, tiles, scale, want_lse);
 }
 
 struct PackedAttention : torch::autograd::Function<PackedAttention> {
   using Ctx = torch::autograd::AutogradContext;
   static torch::autograd::variable_list forward(Ctx* ctx, const Tensor& q, const Tensor& k,
                                                 const Tensor& v, const Tensor& qi,
-                                                const Tensor& ki, double scale) {
+                                                const Tensor& ki, std::vector<int64_t> tiles,
+                                                double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, lse] = call_packed(q, k, v, qi, ki, scale, true);
+    auto [out, lse] = call_packed(q, k, v, qi, ki, tiles, scale, true);
     ctx->save_for_backward({q, k, v, out, lse, qi, ki});
+    ctx->saved_data["tiles"] = tiles;
     ctx->saved_data["scale"] = scale;
     ctx->mark_non_differentiable({lse});
     return {out, lse};
@@ -549,23 +563,24 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     refuse_foreign_leaves();
     const auto s = ctx->get_saved_variables();
     const Tensor none;
-    if (!g[0].defined()) return {none, none, none, none, none, none};
+    if (!g[0].defined()) return {none, none, none, none, none, none, none};
     static auto op = handle<decltype(attention_packed_bwd)>("lbw::attention_packed_bwd");
     auto [dq, dk, dv] = op.call(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6],
+                                ctx->saved_data["tiles"].toIntVector(),
                                 ctx->saved_data["scale"].toDouble());
-    return {dq, dk, dv, none, none, none};
+    return {dq, dk, dv, none, none, none, none};
   }
 };
 
 std::tuple<Tensor, Tensor> attention_packed_autograd(const Tensor& q, const Tensor& k,
                                                      const Tensor& v, const Tensor& qi,
-                                                     const Tensor& ki, double scale,
-                                                     bool want_lse) {
+                                                     const Tensor& ki, at::IntArrayRef tiles,
+                                                     double scale, bool want_lse) {
   if (!any_grad({&q, &k, &v})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return call_packed(q, k, v, qi, ki, scale, want_lse);
+    return call_packed(q, k, v, qi, ki, tiles, scale, want_lse);
   }
-  auto r = PackedAttention::apply(q, k, v, qi, ki, scale);
+  auto r = PackedAttention::apply(q, k, v, qi, ki, tiles.vec(), scale);
   return {r[0], r[1]};
 }
 
@@ -581,11 +596,12 @@ TORCH_LIBRARY_FRAGMENT(lbw, m) {
   m.def("head_norm_rope_bwd(Tensor dq_out, Tensor dk_out, Tensor q, Tensor k, Tensor? wq, "
         "Tensor? wk, Tensor rope, int[] axes, bool interleaved, Tensor pos, float eps, "
         "float q_scale, float k_scale) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("packed_plan(Tensor q_lens, Tensor k_lens, bool causal) -> (Tensor, Tensor)");
+  m.def("packed_plan(Tensor q_lens, Tensor k_lens, bool causal) -> (Tensor, Tensor, int[])");
   m.def("attention_packed(Tensor q, Tensor k, Tensor v, Tensor q_items, Tensor k_items, "
-        "float softmax_scale=0., bool want_lse=True) -> (Tensor, Tensor)");
+        "int[] tiles, float softmax_scale=0., bool want_lse=True) -> (Tensor, Tensor)");
   m.def("attention_packed_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, "
-        "Tensor q_items, Tensor k_items, float softmax_scale=0.) -> (Tensor, Tensor, Tensor)");
+        "Tensor q_items, Tensor k_items, int[] tiles, float softmax_scale=0.) "
+        "-> (Tensor, Tensor, Tensor)");
   m.def("attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor lens, "
         "float softmax_scale=0., int num_splits=0) -> Tensor");
   m.def("attention_decode_out(Tensor q, Tensor k_cache, Tensor v_cache, Tensor lens, "

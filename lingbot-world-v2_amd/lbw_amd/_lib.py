@@ -120,6 +120,16 @@ class PackedParams(ctypes.Structure):
         ("lse", ctypes.c_void_p), ("softmax_scale", ctypes.c_float),
         ("q_items", ctypes.c_void_p), ("n_q_items", ctypes.c_int32),
         ("k_items", ctypes.c_void_p), ("n_k_items", ctypes.c_int32),
+        ("q_tiles", ctypes.c_int64), ("q_tiles_max", ctypes.c_int64),
+        ("k_tiles", ctypes.c_int64), ("k_tiles_max", ctypes.c_int64),
+    ]
+
+
+class PackedPlanInfo(ctypes.Structure):
+    _fields_ = [
+        ("n_q_items", ctypes.c_int64), ("n_k_items", ctypes.c_int64),
+        ("q_tiles", ctypes.c_int64), ("q_tiles_max", ctypes.c_int64),
+        ("k_tiles", ctypes.c_int64), ("k_tiles_max", ctypes.c_int64),
     ]
 
 
@@ -156,7 +166,7 @@ EXPORTS = (
     "lbw_qk_norm_rope",
     "lbw_kv_quant_fp8",
     "lbw_head_norm_rope", "lbw_head_norm_rope_bwd_workspace_size", "lbw_head_norm_rope_bwd",
-    "lbw_attention_packed_plan", "lbw_attention_packed_fwd",
+    "lbw_attention_packed_plan", "lbw_attention_packed_workspace_size", "lbw_attention_packed_fwd",
     "lbw_attention_packed_bwd_workspace_size", "lbw_attention_packed_bwd",
     "lbw_attention_decode_workspace_size", "lbw_attention_decode",
     "lbw_last_error", "lbw_abi_version",
@@ -204,10 +214,12 @@ def _declare(lib):
     lib.lbw_head_norm_rope_bwd.argtypes = [P(HeadNormRopeParams), P(HeadNormRopeGrads), vp,
                                            ctypes.c_size_t, vp]
     lib.lbw_head_norm_rope_bwd.restype = ctypes.c_int
-    lib.lbw_attention_packed_plan.argtypes = [i32, P(i32), P(i32), i32, P(i32), i64, P(i64),
-                                              P(i32), i64, P(i64)]
+    lib.lbw_attention_packed_plan.argtypes = [i32, P(i32), P(i32), i32, P(i32), i64,
+                                              P(i32), i64, P(PackedPlanInfo)]
     lib.lbw_attention_packed_plan.restype = ctypes.c_int
-    lib.lbw_attention_packed_fwd.argtypes = [P(PackedParams), vp]
+    lib.lbw_attention_packed_workspace_size.argtypes = [P(PackedParams)]
+    lib.lbw_attention_packed_workspace_size.restype = ctypes.c_size_t
+    lib.lbw_attention_packed_fwd.argtypes = [P(PackedParams), vp, ctypes.c_size_t, vp]
     lib.lbw_attention_packed_fwd.restype = ctypes.c_int
     lib.lbw_attention_packed_bwd_workspace_size.argtypes = [P(PackedParams)]
     lib.lbw_attention_packed_bwd_workspace_size.restype = ctypes.c_size_t

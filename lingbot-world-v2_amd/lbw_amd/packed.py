@@ -35,6 +35,7 @@ class PackedPlan:
     k_tokens: int
     q_items: torch.Tensor
     k_items: torch.Tensor
+    tiles: tuple
 
 
 def _lens(name, lens) -> tuple:
@@ -61,10 +62,11 @@ def packed_plan(q_lens: Sequence[int], k_lens: Sequence[int] | None = None, *, c
     kl = ql if k_lens is None else _lens("k_lens", k_lens)
     if len(ql) != len(kl):
         raise ValueError(f"{len(ql)} query and {len(kl)} key lengths")
-    qi, ki = ops.packed_plan(torch.tensor(ql, dtype=torch.int32), torch.tensor(kl, dtype=torch.int32),
+    qi, ki, tiles = ops.packed_plan(torch.tensor(ql, dtype=torch.int32), torch.tensor(kl, dtype=torch.int32),
                              bool(causal))
     device = torch.device("cuda") if device is None else torch.device(device)
-    return PackedPlan(ql, kl, bool(causal), sum(ql), sum(kl), qi.to(device), ki.to(device))
+    return PackedPlan(ql, kl, bool(causal), sum(ql), sum(kl), qi.to(device), ki.to(device),
+                      tuple(tiles))
 
 
 def _check(q, k, v, plan):
@@ -106,7 +108,7 @@ def attention_packed(q, k, v, plan: PackedPlan, *, softmax_scale: float | None =
     ops = _lib.ops()
     _check(q, k, v, plan)
     out, lse = ops.attention_packed(_unit(q), _unit(k), _unit(v), plan.q_items, plan.k_items,
-                                    _scale(softmax_scale), return_lse)
+                                    plan.tiles, _scale(softmax_scale), return_lse)
     return (out, lse) if return_lse else out
 
 
@@ -119,7 +121,7 @@ def attention_packed_backward(dout, q, k, v, out, lse, plan: PackedPlan, *,
     if dout.shape != q.shape or out.shape != q.shape or tuple(lse.shape) != (q.shape[1], q.shape[0]):
         raise ValueError("dout and out must have q's shape, lse [heads, tokens]")
     return ops.attention_packed_bwd(dout, _unit(q), _unit(k), _unit(v), _unit(out), lse,
-                                    plan.q_items, plan.k_items, _scale(softmax_scale))
+                                    plan.q_items, plan.k_items, plan.tiles, _scale(softmax_scale))
 
 
 def attention_decode(q, k_cache, v_cache, lens, *, softmax_scale: float | None = None,

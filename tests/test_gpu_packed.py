@@ -42,6 +42,9 @@ CASES = [  # q_lens, k_lens, heads, kv heads, causal
     ([200, 5], [37, 0], 2, 1, True), ([200, 5], [37, 0], 2, 1, False), ([0, 3], [9, 200], 2, 2, True),
     ([2, 130], [130, 2], 3, 3, True), ([640], [641], 1, 1, True), ([64, 32, 96], [64, 96, 32], 2, 1, True),
     ([1025, 3, 258], None, 8, 2, True), ([33] * 40, None, 1, 1, True),
+    # few rows over many keys, many queries over few keys: items cut into pieces (up to 16)
+    ([16], [3000], 2, 1, True), ([5, 2, 130], [2500, 10, 700], 1, 1, False), ([2200], [70], 6, 1, False),
+    ([1, 129], [9000, 129], 1, 1, True), ([5000, 40], [33, 40], 1, 1, True),
 ]
 
 
@@ -125,7 +128,8 @@ def test_rows_around_the_packed_ones_are_left_alone():
         setattr(s, n + "_stride_h", t.stride(1))
     lib = _lib.load()
     stream = _lib.stream_ptr()
-    _lib.check(lib.lbw_attention_packed_fwd(ctypes.byref(p), stream), "fwd")
+    assert lib.lbw_attention_packed_workspace_size(ctypes.byref(p)) == 0  # (no tile counts: never cut)
+    _lib.check(lib.lbw_attention_packed_fwd(ctypes.byref(p), None, 0, stream), "fwd")
     n = lib.lbw_attention_packed_bwd_workspace_size(ctypes.byref(p))
     ws = torch.empty(n, dtype=torch.uint8, device="cuda")
     assert lib.lbw_attention_packed_bwd(ctypes.byref(p), ctypes.byref(g), ws.data_ptr(), n - 1, stream) == 4
@@ -191,7 +195,8 @@ def test_a_plan_of_other_lengths_stays_inside_the_tensors():
     import lbw_amd
     big = lbw_amd.packed_plan([4000, 100])
     q, k, v, _ = _data([60], [60], 2, 1, 10)
-    out, _ = torch.ops.lbw.attention_packed(q, k, v, big.q_items, big.k_items, 0.0, True)
+    out, _ = torch.ops.lbw.attention_packed(q, k, v, big.q_items, big.k_items, big.tiles, 0.0,
+                                             True)
     torch.cuda.synchronize()
     assert out.shape == q.shape
     with pytest.raises(ValueError, match="the plan"):

@@ -49,6 +49,9 @@ def test_plan_covers_every_row_once_and_bounds_what_is_seen(ql, kl, causal):
     assert sorted(keys) == list(range(sum(kl)))
     cost = [x[5] for x in p.q_items.tolist()]
     assert cost == sorted(cost, reverse=True)
+    qt = [-(-x // 64) for x in cost]
+    kt = [-(-x[4] // 64) - x[5] // 64 if x[5] < x[4] else 0 for x in p.k_items.tolist()]
+    assert p.tiles == (sum(qt), max(qt, default=0), sum(kt), max(kt, default=0))
 
 
 def test_plan_refusals():
@@ -60,21 +63,20 @@ def test_plan_refusals():
         lbw().packed_plan([2 ** 30, 2 ** 30], device="cpu")
     from lbw_amd import _lib
     lib = _lib.load()
-    n = ctypes.c_int64()
+    n = ctypes.byref(_lib.PackedPlanInfo())
     lens = (ctypes.c_int32 * 1)(300)
     items = (ctypes.c_int32 * 8)()
-    assert lib.lbw_attention_packed_plan(1, lens, lens, 1, items, 1, ctypes.byref(n), items, 1,
-                                         ctypes.byref(n)) == 1
+    assert lib.lbw_attention_packed_plan(1, lens, lens, 1, items, 1, items, 1, n) == 1
     assert b"room for 3" in lib.lbw_last_error()
-    assert lib.lbw_attention_packed_plan(1, None, lens, 1, None, 0, ctypes.byref(n), None, 0,
-                                         ctypes.byref(n)) == 1
-    assert lib.lbw_attention_packed_plan(1, lens, lens, 1, None, 0, None, None, 0, None) == 1
+    assert lib.lbw_attention_packed_plan(1, None, lens, 1, None, 0, None, 0, n) == 1
+    assert lib.lbw_attention_packed_plan(1, lens, lens, 1, None, 0, None, 0, None) == 1
 
 
 @pytest.mark.parametrize("cname,pyname", [("lbw_head_norm_rope_params", "HeadNormRopeParams"),
                                           ("lbw_head_norm_rope_grads", "HeadNormRopeGrads"),
                                           ("lbw_packed_params", "PackedParams"),
                                           ("lbw_packed_grads", "PackedGrads"),
+                                          ("lbw_packed_plan_info", "PackedPlanInfo"),
                                           ("lbw_decode_params", "DecodeParams")])
 def test_struct_layouts_match_the_header(cname, pyname):
     from lbw_amd import _lib
@@ -228,24 +230,24 @@ def test_c_entries_refuse_before_any_gpu_call():
     d = _lib.DecodeParams(batch=1, q_heads=4, k_heads=2, head_dim=64, capacity=8)
     assert lib.lbw_attention_decode(ctypes.byref(d), None, 0, None) == 2
     p = _lib.PackedParams(q_heads=4, k_heads=3, head_dim=128, q_tokens=1, k_tokens=1)
-    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 1
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None, 0, None) == 1
     p = _lib.PackedParams(q_heads=4, k_heads=2, head_dim=128, q_tokens=1, k_tokens=1, q=8)
-    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 1
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None, 0, None) == 1
     assert b"16-byte" in lib.lbw_last_error()
     p = _lib.PackedParams(q_heads=4, k_heads=2, head_dim=128, q_tokens=1, k_tokens=1, q=16, k=16, v=16,
                           out=16, q_stride_l=12)
-    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 1
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None, 0, None) == 1
     assert b"multiples of 8" in lib.lbw_last_error()
     p.q_stride_l = 1 << 26
-    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 2
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None, 0, None) == 2
     p.q_stride_l = 512
     p.softmax_scale = -1.0
-    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None) == 1
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None, 0, None) == 1
     n = _lib.HeadNormRopeParams(tokens=1, q_heads=4, k_heads=2, head_dim=48)
     assert lib.lbw_head_norm_rope(ctypes.byref(n), None) == 2
     n = _lib.HeadNormRopeParams(tokens=1, q_heads=4, k_heads=2, head_dim=128, n_axes=2, rope_pairs=64)
     n.axis_pairs[0] = 60
     assert lib.lbw_head_norm_rope(ctypes.byref(n), None) == 1
     assert b"add up" in lib.lbw_last_error()
-    for f in (lib.lbw_attention_packed_fwd, lib.lbw_head_norm_rope):
-        assert f(None, None) == 1
+    assert lib.lbw_attention_packed_fwd(None, None, 0, None) == 1
+    assert lib.lbw_head_norm_rope(None, None) == 1
