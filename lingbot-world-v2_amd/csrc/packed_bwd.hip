@@ -79,14 +79,15 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
   int ra = row_address(lds0, l32, hl), ta = tr_address(lds0, lane, hl);
   TileCopy copy;
   copy.init(wave, lane);
+  const uint32_t koff = copy.row_offset(ks), voff = copy.row_offset(vs);
   const uint32_t dst = (uint32_t)lds0 + 1024 * PK_NDMA * wave;
   floatx16 acc[4];
 #pragma unroll
   for (int db = 0; db < 4; ++db) zero(acc[db]);
   const float c = a.scale_log2;
   if (t0 < T) {
-    copy.issue(kb, ks, t0 * BN, it.other_len, dst + (t0 & 1) * PK_TILE_B);
-    copy.issue(vb, vs, t0 * BN, it.other_len, dst + V_AT + (t0 & 1) * PK_TILE_B);
+    copy.issue(kb, ks, koff, t0 * BN, it.other_len, dst + (t0 & 1) * PK_TILE_B);
+    copy.issue(vb, vs, voff, t0 * BN, it.other_len, dst + V_AT + (t0 & 1) * PK_TILE_B);
   }
 #pragma unroll 1
   for (int u = t0; u < T; ++u) {
@@ -94,8 +95,8 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     barrier_nofence();
     if (u + 1 < T) {
-      copy.issue(kb, ks, (u + 1) * BN, it.other_len, dst + (PK_TILE_B - st));
-      copy.issue(vb, vs, (u + 1) * BN, it.other_len, dst + V_AT + (PK_TILE_B - st));
+      copy.issue(kb, ks, koff, (u + 1) * BN, it.other_len, dst + (PK_TILE_B - st));
+      copy.issue(vb, vs, voff, (u + 1) * BN, it.other_len, dst + V_AT + (PK_TILE_B - st));
     }
     if (!active || u * BN >= lim_hi) continue;
 #pragma unroll
@@ -160,8 +161,14 @@ __global__ void __launch_bounds__(PK_WAVES * 64) packed_dq_join_kernel(const Pac
 }
 
 // ---- dK, dV: a lane holds one key's column of S = Q K^T and dP = dO V^T
+// 192 of a wave's 256 registers hold dK, dV, K and V; S, dP and the fragments take 50 more. So nothing that
+// can be had again in a few instructions is kept across the loop: the lane index and what follows from it.
+__device__ __forceinline__ int lane_now() {
+  return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, (uint32_t)opaque(0)));
+}
 constexpr int GROUPS = 2;  // wave groups of a workgroup, each with its share of an item's query tiles
-constexpr int DKV_LDS = GROUPS * DKV_GROUP_B;
+constexpr int FRAG_AT = GROUPS * DKV_GROUP_B;    // each wave's last fragment of K and of V: 2 KB
+constexpr int DKV_LDS = FRAG_AT + GROUPS * PK_WAVES * 2048;
 __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(const PackedArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63;
@@ -190,19 +197,24 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
     load_rows(a.k.p + row * a.k.sl + kv * a.k.sh, a.k.sl, rows, l32, hl, kf);
     load_rows(a.v.p + row * a.v.sl + kv * a.v.sh, a.v.sl, rows, l32, hl, vf);
   }
+  // the eighth fragments wait in LDS rather than in registers
+  const int frag = (int)lds_addr(lds) + FRAG_AT + 2048 * wave_id;
+  {
+    unsigned char* const d = lds + FRAG_AT + 2048 * wave_id + 16 * lane;
+    *reinterpret_cast<u32x4*>(d) = kf[7];
+    *reinterpret_cast<u32x4*>(d + 1024) = vf[7];
+    wave_lds_fence();
+  }
   // first query that sees this lane's key, and the wave's smallest and largest such
   const int j0 = it.pos0 + r0;
   auto first = [&](int j) {
     const int64_t x = (int64_t)j - it.shift;
     return (int)(x < 0 ? 0 : (x < it.other_len ? x : it.other_len));
   };
-  const int lo = first(j0 + l32);
   const int lo_min = first(j0), lo_max = first(j0 + 31);
 
   const int lds0 = (int)lds_addr(lds) + DKV_GROUP_B * grp;
   const int ra0 = row_address(lds0, l32, hl), ta0 = tr_address(lds0, lane, hl);
-  TileCopy copy;
-  copy.init(wave, lane);
   const uint32_t dst = (uint32_t)lds0 + 1024 * PK_NDMA * wave;
   floatx16 dk[4], dv[4];
 #pragma unroll
@@ -212,22 +224,32 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
   }
   const float c = a.scale_log2;
   const int64_t qs = a.q.sl * 2, gs = a.dout.sl * 2;
-  // query tile n (head n / per of the group) into stage n % 2; waves 0 and 1 fetch its rows' -lse and
-  // delta (rows past the sequence's end: the last one's)
+  // The next query tile to fetch: head and tile of it, stepped along (no division per tile).
+  int nh = kv * group + (per > 0 ? n0 / per : 0), nt = t_first + (per > 0 ? n0 % per : 0);
+  // query tile n into stage n % 2; waves 0 and 1 fetch its rows' -lse and delta (rows past the sequence's
+  // end: the last one's)
   auto issue = [&](int n) {
-    const int h = kv * group + n / per, first_row = (t_first + n % per) * BN;
+    const int first_row = nt * BN, ln = lane_now();
+    TileCopy copy;
+    copy.init(wave, ln);
+    const uint32_t qoff = copy.row_offset(qs), goff = copy.row_offset(gs);
     const uint32_t to = dst + (n & 1) * PK_TILE_B;
     if (wave < 2) {
-      const int r = min(first_row + lane, it.other_len - 1);
-      const float* x = (wave == 0 ? a.nlse2 : a.delta) + (int64_t)h * a.Tq + it.other0 + r;
+      const int r = min(first_row + ln, it.other_len - 1);
+      const float* x = (wave == 0 ? a.nlse2 : a.delta) + (int64_t)nh * a.Tq + it.other0 + r;
       dma4((uint64_t)(uintptr_t)x, (uint32_t)lds0 + STAT_AT + ((n & 1) * 2 + wave) * BN * 4);
     }
-    copy.issue(reinterpret_cast<const unsigned char*>(a.q.p + (int64_t)it.other0 * a.q.sl + h * a.q.sh),
-               qs, first_row, it.other_len, to);
+    copy.issue(reinterpret_cast<const unsigned char*>(a.q.p + (int64_t)it.other0 * a.q.sl + nh * a.q.sh),
+               qs, qoff, first_row, it.other_len, to);
     copy.issue(reinterpret_cast<const unsigned char*>(a.dout.p + (int64_t)it.other0 * a.dout.sl +
-                                                      h * a.dout.sh),
-               gs, first_row, it.other_len, to + V_AT);
+                                                      nh * a.dout.sh),
+               gs, goff, first_row, it.other_len, to + V_AT);
+    if (++nt == t_end) {
+      nt = t_first;
+      ++nh;
+    }
   };
+  int ct = nt;  // the tile being worked on
   if (n0 < T) issue(n0);
 #pragma unroll 1
   for (int n = n0; n < Tmax; ++n) {
@@ -235,48 +257,76 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
     __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     barrier_nofence();
     if (n + 1 < T) issue(n + 1);
-    const int row0 = (t_first + n % per) * BN;
+    const int row0 = ct * BN;
+    ct = ct + 1 == t_end ? t_first : ct + 1;
     if (!active || n >= T || row0 + BN <= lo_min) continue;
 #pragma unroll 1
     for (int qb = 0; qb < 2; ++qb) {
-      const int at = 0;
-      const int ra = opaque(ra0 + st + qb * 32 * PK_ROWB), ta = opaque(ta0 + st + qb * 32 * PK_ROWB);
-      const int sa = lds0 + STAT_AT + (n & 1) * 2 * BN * 4 + (32 * qb + 4 * hl) * 4;
+      // (each product's fragment addresses are taken anew: kept for two of them, they spill others)
+      const int ra = opaque(ra0 + st + qb * 32 * PK_ROWB);
+      const int sa = lds0 + STAT_AT + (n & 1) * 2 * BN * 4 + 128 * qb + 16 * (lane_now() >> 5);
+      // S, then dP beside the exponentials, then dV beside dS, then dK: fragments two products ahead
       floatx16 s, dp;
       zero(s);
       zero(dp);
+      u32x4 f[3];
+      const int fa = frag + 16 * lane_now();
+      u32x4 last = lds_read_b128(fa);
+      f[0] = read_row(ra, 0, 0);
+      f[1] = read_row(ra, 1, 0);
 #pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        s = mfma32x32x16(read_row(ra, d, at), kf[d], s);
-        dp = mfma32x32x16(read_row(ra, d, at + V_AT), vf[d], dp);
+      for (int i = 0; i < 8; ++i) {
+        f[(i + 2) % 3] = i + 2 < 8 ? read_row(ra, i + 2, 0) : read_row(ra, i - 6, V_AT);
+        s = mfma32x32x16(f[i % 3], i < 7 ? kf[i] : last, s);
+        __builtin_amdgcn_sched_barrier(0);
       }
       const int i0 = row0 + 32 * qb;
       if (i0 < lo_max || i0 + 32 > it.other_len) {  // (register r is query i0 + 4 hl + acc_row(r))
-        const int skip = lo - (i0 + 4 * hl), end = it.other_len - (i0 + 4 * hl);
+        const int ln = lane_now(), q0 = i0 + 4 * (ln >> 5);
+        const int skip = first(j0 + (ln & 31)) - q0, end = it.other_len - q0;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           s[r] = acc_row(r) >= skip && acc_row(r) < end ? s[r] : -INFINITY;
       }
-      floatx16 p, ds;
+      // (fragment i of the 8 + 8 + 8 products from here on is in f[(i + 2) % 3])
+      const int rb = opaque(ra), ta = opaque(ta0 + st + qb * 32 * PK_ROWB);
+      u32x4 pf[2], df[2];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const u32x4 l4 = lds_read_b128(sa + 32 * g), d4 = lds_read_b128(sa + 32 * g + BN * 4);
+      for (int i = 0; i < 8; ++i) {
+        const u32x2 st = lds_read_b64(sa + 16 * (i & ~1) + 8 * (i & 1));
+        f[(i + 4) % 3] = i + 2 < 8 ? read_row(rb, i + 2, V_AT) : read_tr(ta, i - 6, 0, V_AT);
+        if (i == 4) last = lds_read_b128(fa + 1024);
+        dp = mfma32x32x16(f[(i + 2) % 3], i < 7 ? vf[i] : last, dp);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
-          p[r] = fast_exp2(__builtin_fmaf(s[r], c, __uint_as_float(l4[e])));
-          ds[r] = p[r] * (dp[r] - __uint_as_float(d4[e]));
-        }
+        for (int e = 0; e < 2; ++e)
+          s[2 * i + e] = fast_exp2(__builtin_fmaf(s[2 * i + e], c, __uint_as_float(st[e])));
+        if (i < 4) pf[0][i] = pack_bf16x2(s[2 * i], s[2 * i + 1]);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      const u32x4 pf[2] = {pack_half(p, 0), pack_half(p, 1)};
-      const u32x4 df[2] = {pack_half(ds, 0), pack_half(ds, 1)};
+      // products 8 .. 15: dV, k-half (i / 4) % 2, d-block i % 4; 16 .. 23: dK
+      const int tb = opaque(ta);
 #pragma unroll
-      for (int db = 0; db < 4; ++db)
+      for (int i = 8; i < 16; ++i) {
+        const int n = i + 2;
+        f[(i + 4) % 3] = read_tr(n < 16 ? ta : tb, n & 3, (n >> 2) & 1, n < 16 ? V_AT : 0);
+        dv[i & 3] = mfma32x32x16(f[(i + 2) % 3], pf[(i >> 2) & 1], dv[i & 3]);
+        const int w = i - 8;  // word w / 4, w % 4 of the operands
+        if (w < 4) pf[1][w] = pack_bf16x2(s[8 + 2 * w], s[8 + 2 * w + 1]);
+        const u32x2 st = lds_read_b64(sa + 16 * (w & ~1) + 8 * (w & 1) + BN * 4);
+        float x[2];
 #pragma unroll
-        for (int mm = 0; mm < 2; ++mm) {
-          dv[db] = mfma32x32x16(read_tr(ta, db, mm, at + V_AT), pf[mm], dv[db]);
-          dk[db] = mfma32x32x16(read_tr(ta, db, mm, at), df[mm], dk[db]);
-        }
+        for (int e = 0; e < 2; ++e)
+          x[e] = s[2 * w + e] * (dp[2 * w + e] - __uint_as_float(st[e]));
+        df[w >> 2][w & 3] = pack_bf16x2(x[0], x[1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int i = 16; i < 24; ++i) {
+        const int n = i + 2;
+        if (n < 24) f[(i + 4) % 3] = read_tr(tb, n & 3, (n >> 2) & 1, 0);
+        dk[i & 3] = mfma32x32x16(f[(i + 2) % 3], df[(i >> 2) & 1], dk[i & 3]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0070);
@@ -286,7 +336,7 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
     // through group 0's
     unsigned char* g1 = lds + DKV_GROUP_B + 16384 * wave;
     unsigned char* g0 = lds + 16384 * wave;
-    const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    const int ln = lane_now();
     if (grp == 1) {
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
@@ -313,15 +363,14 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
     if (grp == 1) return;
   }
   if (!active) return;
-  // (the lane index taken anew rather than kept, or spilled, across the loop)
   if (pieces > 1) {
-    const int ln1 = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+    const int ln1 = lane_now();
     float* const part = part_of(a, sh, a.Hk, sh.piece, PK_PART_DKV);
     store_acc(part, wave, ln1, dk);
     store_acc(part + PK_BLOCK * 128, wave, ln1, dv);
     return;
   }
-  const int ln = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+  const int ln = lane_now();
   store_rows(lds + 8192 * wave, dk, a.scale, ln, rows, [&](int r) {
     return a.dk.p + (int64_t)(it.row0 + r0 + r) * a.dk.sl + kv * a.dk.sh;
   });

@@ -80,10 +80,11 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
   const int ka = row_address(lds0, l32, hl), va = tr_address(lds0 + V_AT, lane, hl);
   TileCopy copy;
   copy.init(wave, lane);
+  const uint32_t koff = copy.row_offset(ks), voff = copy.row_offset(vs);
   const uint32_t dst = (uint32_t)lds0 + 1024 * PK_NDMA * wave;
-  auto issue_k = [&](int u) { copy.issue(kb, ks, (t0 + u) * BN, it.other_len, dst + (u & 1) * PK_TILE_B); };
+  auto issue_k = [&](int u) { copy.issue(kb, ks, koff, (t0 + u) * BN, it.other_len, dst + (u & 1) * PK_TILE_B); };
   auto issue_v = [&](int u) {
-    copy.issue(vb, vs, (t0 + u) * BN, it.other_len, dst + V_AT + (u & 1) * PK_TILE_B);
+    copy.issue(vb, vs, voff, (t0 + u) * BN, it.other_len, dst + V_AT + (u & 1) * PK_TILE_B);
   };
 
   floatx16 o[4];
