@@ -415,8 +415,8 @@ int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads*
                 workspace_bytes);
   a.o = {static_cast<const uint16_t*>(p->out), p->out_stride_l, p->out_stride_h};
   a.dout = {static_cast<const uint16_t*>(g->dout), g->dout_stride_l, g->dout_stride_h};
-  a.delta = static_cast<float*>(workspace);
-  a.nlse2 = a.delta + (size_t)p->q_heads * (size_t)p->q_tokens;
+  a.ndelta = static_cast<float*>(workspace);
+  a.nlse2 = a.ndelta + (size_t)p->q_heads * (size_t)p->q_tokens;
   a.dq = {static_cast<uint16_t*>(g->dq), g->dq_stride_l, g->dq_stride_h};
   a.dk = {static_cast<uint16_t*>(g->dk), g->dk_stride_l, g->dk_stride_h};
   a.dv = {static_cast<uint16_t*>(g->dv), g->dv_stride_l, g->dv_stride_h};

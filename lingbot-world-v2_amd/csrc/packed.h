@@ -74,7 +74,7 @@ struct PackedArgs {
   float* part;
   // gradient
   Rows o, dout;
-  float* delta;                // [Hq][Tq]: sum_d dout out
+  float* ndelta;               // [Hq][Tq]: -sum_d dout out
   float* nlse2;                // [Hq][Tq]: -lse log2(e), -inf for a query that sees no key
   RowsOut dq, dk, dv;
 };

@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
       const float x = a.lse[at];
       nlse2 = x == -INFINITY ? -INFINITY : -x * LOG2E;
       if (hl == 0 && sh.piece == 0) {
-        a.delta[at] = delta;
+        a.ndelta[at] = -delta;
         a.nlse2[at] = nlse2;
       }
     }
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
   const int64_t qs = a.q.sl * 2, gs = a.dout.sl * 2;
   // The next query tile to fetch: head and tile of it, stepped along (no division per tile).
   int nh = kv * group + (per > 0 ? n0 / per : 0), nt = t_first + (per > 0 ? n0 % per : 0);
-  // query tile n into stage n % 2; waves 0 and 1 fetch its rows' -lse and delta (rows past the sequence's
+  // query tile n into stage n % 2; waves 0 and 1 fetch its rows' -lse and -delta (rows past the sequence's
   // end: the last one's)
   auto issue = [&](int n) {
     const int first_row = nt * BN, ln = lane_now();
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
     const uint32_t to = dst + (n & 1) * PK_TILE_B;
     if (wave < 2) {
       const int r = min(first_row + ln, it.other_len - 1);
-      const float* x = (wave == 0 ? a.nlse2 : a.delta) + (int64_t)nh * a.Tq + it.other0 + r;
+      const float* x = (wave == 0 ? a.nlse2 : a.ndelta) + (int64_t)nh * a.Tq + it.other0 + r;
       dma4((uint64_t)(uintptr_t)x, (uint32_t)lds0 + STAT_AT + ((n & 1) * 2 + wave) * BN * 4);
     }
     copy.issue(reinterpret_cast<const unsigned char*>(a.q.p + (int64_t)it.other0 * a.q.sl + nh * a.q.sh),
@@ -265,10 +265,9 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
       // (each product's fragment addresses are taken anew: kept for two of them, they spill others)
       const int ra = opaque(ra0 + st + qb * 32 * PK_ROWB);
       const int sa = lds0 + STAT_AT + (n & 1) * 2 * BN * 4 + 128 * qb + 16 * (lane_now() >> 5);
-      // S, then dP beside the exponentials, then dV beside dS, then dK: fragments two products ahead
+      // S, then dP (from -delta on) beside the exponentials, then dV beside dS, then dK: fragments two products ahead
       floatx16 s, dp;
       zero(s);
-      zero(dp);
       u32x4 f[3];
       const int fa = frag + 16 * lane_now();
       u32x4 last = lds_read_b128(fa);
@@ -292,6 +291,12 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
       const int rb = opaque(ra), ta = opaque(ta0 + st + qb * 32 * PK_ROWB);
       u32x4 pf[2], df[2];
 #pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const u32x4 d4 = lds_read_b128(sa + 32 * g + BN * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dp[4 * g + e] = __uint_as_float(d4[e]);
+      }
+#pragma unroll
       for (int i = 0; i < 8; ++i) {
         const u32x2 st = lds_read_b64(sa + 16 * (i & ~1) + 8 * (i & 1));
         f[(i + 4) % 3] = i + 2 < 8 ? read_row(rb, i + 2, V_AT) : read_tr(ta, i - 6, 0, V_AT);
@@ -312,12 +317,7 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
         dv[i & 3] = mfma32x32x16(f[(i + 2) % 3], pf[(i >> 2) & 1], dv[i & 3]);
         const int w = i - 8;  // word w / 4, w % 4 of the operands
         if (w < 4) pf[1][w] = pack_bf16x2(s[8 + 2 * w], s[8 + 2 * w + 1]);
-        const u32x2 st = lds_read_b64(sa + 16 * (w & ~1) + 8 * (w & 1) + BN * 4);
-        float x[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          x[e] = s[2 * w + e] * (dp[2 * w + e] - __uint_as_float(st[e]));
-        df[w >> 2][w & 3] = pack_bf16x2(x[0], x[1]);
+        df[w >> 2][w & 3] = pack_bf16x2(s[2 * w] * dp[2 * w], s[2 * w + 1] * dp[2 * w + 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
