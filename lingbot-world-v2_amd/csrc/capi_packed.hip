@@ -51,6 +51,7 @@ int check_heads(int32_t hq, int32_t hk) {
 int check_scale(float s, int head_dim, float* scale) {
   if (!(s >= 0.0f) || isinf(s))
     return fail(LBW_ERR_INVALID, "softmax_scale must be positive and finite (0: 1/sqrt(head_dim))");
+  if (s > 0.0f && s < 1e-30f) return fail(LBW_ERR_UNSUPPORTED, "softmax_scale %g below 1e-30", s);
   *scale = s > 0.0f ? s : 1.0f / sqrtf((float)head_dim);
   return LBW_OK;
 }
@@ -416,7 +417,7 @@ int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads*
   a.o = {static_cast<const uint16_t*>(p->out), p->out_stride_l, p->out_stride_h};
   a.dout = {static_cast<const uint16_t*>(g->dout), g->dout_stride_l, g->dout_stride_h};
   a.ndelta = static_cast<float*>(workspace);
-  a.nlse2 = a.ndelta + (size_t)p->q_heads * (size_t)p->q_tokens;
+  a.nlse = a.ndelta + (size_t)p->q_heads * (size_t)p->q_tokens;
   a.dq = {static_cast<uint16_t*>(g->dq), g->dq_stride_l, g->dq_stride_h};
   a.dk = {static_cast<uint16_t*>(g->dk), g->dk_stride_l, g->dk_stride_h};
   a.dv = {static_cast<uint16_t*>(g->dv), g->dv_stride_l, g->dv_stride_h};

@@ -75,7 +75,7 @@ struct PackedArgs {
   // gradient
   Rows o, dout;
   float* ndelta;               // [Hq][Tq]: -sum_d dout out
-  float* nlse2;                // [Hq][Tq]: -lse log2(e), -inf for a query that sees no key
+  float* nlse;                 // [Hq][Tq]: -lse / scale, -inf for a query that sees no key
   RowsOut dq, dk, dv;
 };
 struct PackedSplit {

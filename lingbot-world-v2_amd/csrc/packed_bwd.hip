@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
       nlse2 = x == -INFINITY ? -INFINITY : -x * LOG2E;
       if (hl == 0 && sh.piece == 0) {
         a.ndelta[at] = -delta;
-        a.nlse2[at] = nlse2;
+        a.nlse[at] = x == -INFINITY ? -INFINITY : -x / a.scale;
       }
     }
   }
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
   const int64_t qs = a.q.sl * 2, gs = a.dout.sl * 2;
   // The next query tile to fetch: head and tile of it, stepped along (no division per tile).
   int nh = kv * group + (per > 0 ? n0 / per : 0), nt = t_first + (per > 0 ? n0 % per : 0);
-  // query tile n into stage n % 2; waves 0 and 1 fetch its rows' -lse and -delta (rows past the sequence's
+  // query tile n into stage n % 2; waves 0 and 1 fetch its rows' -lse / scale and -delta (rows past the sequence's
   // end: the last one's)
   auto issue = [&](int n) {
     const int first_row = nt * BN, ln = lane_now();
@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
     const uint32_t to = dst + (n & 1) * PK_TILE_B;
     if (wave < 2) {
       const int r = min(first_row + ln, it.other_len - 1);
-      const float* x = (wave == 0 ? a.nlse2 : a.ndelta) + (int64_t)nh * a.Tq + it.other0 + r;
+      const float* x = (wave == 0 ? a.nlse : a.ndelta) + (int64_t)nh * a.Tq + it.other0 + r;
       dma4((uint64_t)(uintptr_t)x, (uint32_t)lds0 + STAT_AT + ((n & 1) * 2 + wave) * BN * 4);
     }
     copy.issue(reinterpret_cast<const unsigned char*>(a.q.p + (int64_t)it.other0 * a.q.sl + nh * a.q.sh),
@@ -265,9 +265,17 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
       // (each product's fragment addresses are taken anew: kept for two of them, they spill others)
       const int ra = opaque(ra0 + st + qb * 32 * PK_ROWB);
       const int sa = lds0 + STAT_AT + (n & 1) * 2 * BN * 4 + 128 * qb + 16 * (lane_now() >> 5);
-      // S, then dP (from -delta on) beside the exponentials, then dV beside dS, then dK: fragments two products ahead
+      // S (from -lse / scale on), then dP (from -delta on) beside the exponentials, then dV beside dS, then dK: fragments two products ahead
       floatx16 s, dp;
-      zero(s);
+      auto start = [&](floatx16& x, int at) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const u32x4 v = lds_read_b128(sa + 32 * g + at);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[4 * g + e] = __uint_as_float(v[e]);
+        }
+      };
+      start(s, 0);
       u32x4 f[3];
       const int fa = frag + 16 * lane_now();
       u32x4 last = lds_read_b128(fa);
@@ -290,21 +298,14 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
       // (fragment i of the 8 + 8 + 8 products from here on is in f[(i + 2) % 3])
       const int rb = opaque(ra), ta = opaque(ta0 + st + qb * 32 * PK_ROWB);
       u32x4 pf[2], df[2];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const u32x4 d4 = lds_read_b128(sa + 32 * g + BN * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) dp[4 * g + e] = __uint_as_float(d4[e]);
-      }
+      start(dp, BN * 4);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const u32x2 st = lds_read_b64(sa + 16 * (i & ~1) + 8 * (i & 1));
         f[(i + 4) % 3] = i + 2 < 8 ? read_row(rb, i + 2, V_AT) : read_tr(ta, i - 6, 0, V_AT);
         if (i == 4) last = lds_read_b128(fa + 1024);
         dp = mfma32x32x16(f[(i + 2) % 3], i < 7 ? vf[i] : last, dp);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          s[2 * i + e] = fast_exp2(__builtin_fmaf(s[2 * i + e], c, __uint_as_float(st[e])));
+        for (int e = 0; e < 2; ++e) s[2 * i + e] = fast_exp2(s[2 * i + e] * c);
         if (i < 4) pf[0][i] = pack_bf16x2(s[2 * i], s[2 * i + 1]);
         __builtin_amdgcn_sched_barrier(0);
       }
