@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
   const int lim_lo = limit(i0), lim_hi = limit(i0 + (rows < 32 ? rows : 32) - 1);
 
   const int lds0 = (int)lds_addr(lds);
-  int ra = row_address(lds0, l32, hl), ta = tr_address(lds0, lane, hl);
+  const int ra0 = row_address(lds0, l32, hl), ta0 = tr_address(lds0, lane, hl);
   TileCopy copy;
   copy.init(wave, lane);
   const uint32_t koff = copy.row_offset(ks), voff = copy.row_offset(vs);
@@ -99,33 +99,74 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
       copy.issue(vb, vs, voff, (u + 1) * BN, it.other_len, dst + V_AT + (PK_TILE_B - st));
     }
     if (!active || u * BN >= lim_hi) continue;
-#pragma unroll
-    for (int kb32 = 0; kb32 < 2; ++kb32) {
-      const int at = st + kb32 * 32 * PK_ROWB;
-      floatx16 s, dp;
-      zero(s);
-      zero(dp);
-#pragma unroll
-      for (int d = 0; d < 8; ++d) {
-        s = mfma32x32x16(read_row(ra, d, at), qf[d], s);
-        dp = mfma32x32x16(read_row(ra, d, at + V_AT), gf[d], dp);
-      }
-      const int key0 = u * BN + 32 * kb32;
-      floatx16 ds;
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        ds[r] = fast_exp2(__builtin_fmaf(s[r], c, nlse2)) * (dp[r] - delta);
+    // The tile's two 32-key blocks: S0; dP0 beside exp(S0); S1 beside dS0; dQ's product with dS0 and dP1
+    // beside exp(S1); dS1; dQ's product with dS1. Fragments two products ahead.
+    const int ra = ra0 + st, ta = ta0 + st;
+    constexpr int B1 = 32 * PK_ROWB;
+    floatx16 s0, s1, dp;
+    u32x4 f[4], df[2];
+    auto mask = [&](floatx16& s, int key0) {
       if (key0 + 32 > lim_lo) {
         const int left = lim - (key0 + 4 * hl);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) ds[r] = acc_row(r) < left ? ds[r] : 0.0f;
+        for (int r = 0; r < 16; ++r) s[r] = acc_row(r) < left ? s[r] : -INFINITY;
       }
-      const u32x4 pf[2] = {pack_half(ds, 0), pack_half(ds, 1)};
+    };
+    auto exps = [&](floatx16& s, int i) {
 #pragma unroll
-      for (int db = 0; db < 4; ++db)
+      for (int e = 0; e < 2; ++e) s[2 * i + e] = fast_exp2(__builtin_fmaf(s[2 * i + e], c, nlse2));
+    };
+    auto grad = [&](const floatx16& p, int i) {
+      df[i >> 2][i & 3] = pack_bf16x2(p[2 * i] * (dp[2 * i] - delta), p[2 * i + 1] * (dp[2 * i + 1] - delta));
+    };
+    zero(s0);
+    f[0] = read_row(ra, 0, 0);
+    f[1] = read_row(ra, 1, 0);
 #pragma unroll
-        for (int mm = 0; mm < 2; ++mm)
-          acc[db] = mfma32x32x16(read_tr(ta, db, mm, at), pf[mm], acc[db]);
+    for (int i = 0; i < 8; ++i) {
+      f[(i + 2) & 3] = i + 2 < 8 ? read_row(ra, i + 2, 0) : read_row(ra, i - 6, V_AT);
+      s0 = mfma32x32x16(f[i & 3], qf[i], s0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    mask(s0, u * BN);
+    zero(dp);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[(i + 2) & 3] = i + 2 < 8 ? read_row(ra, i + 2, V_AT) : read_row(ra, i - 6, B1);
+      dp = mfma32x32x16(f[i & 3], gf[i], dp);
+      exps(s0, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    zero(s1);
+    u32x4 g[4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i + 2 < 8) f[(i + 2) & 3] = read_row(ra, i + 2, B1);
+      else g[i - 6] = read_tr(ta, i - 6, 0, 0);
+      s1 = mfma32x32x16(f[i & 3], qf[i], s1);
+      grad(s0, i);
+      if (i >= 6) f[(i + 2) & 3] = read_row(ra, i - 6, B1 + V_AT);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    mask(s1, u * BN + 32);
+    zero(dp);
+    // (fragment i of dQ's product: d-block i % 4, k-half i / 4)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i + 2 < 8) f[(i + 2) & 3] = read_row(ra, i + 2, B1 + V_AT);
+      g[(i + 2) & 3] = i + 2 < 8 ? read_tr(ta, (i + 2) & 3, (i + 2) >> 2, 0) : read_tr(ta, i - 6, 0, B1);
+      dp = mfma32x32x16(f[i & 3], gf[i], dp);
+      acc[i & 3] = mfma32x32x16(g[i & 3], df[i >> 2], acc[i & 3]);
+      exps(s1, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) grad(s1, i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i + 2 < 8) g[(i + 2) & 3] = read_tr(ta, (i + 2) & 3, (i + 2) >> 2, B1);
+      acc[i & 3] = mfma32x32x16(g[i & 3], df[i >> 2], acc[i & 3]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0070);
