@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
       exps(s0, i);
       __builtin_amdgcn_sched_barrier(0);
     }
+    asm volatile("" : "+v"(s0));  // (the exponentials stay here, not sunk to their use past a branch)
     zero(s1);
     u32x4 g[4];
 #pragma unroll
@@ -148,6 +149,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
       if (i >= 6) f[(i + 2) & 3] = read_row(ra, i - 6, B1 + V_AT);
       __builtin_amdgcn_sched_barrier(0);
     }
+    asm volatile("" : "+v"(df[0]), "+v"(df[1]));
     mask(s1, u * BN + 32);
     zero(dp);
     // (fragment i of dQ's product: d-block i % 4, k-half i / 4)
