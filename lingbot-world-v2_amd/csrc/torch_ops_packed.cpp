@@ -470,6 +470,15 @@ void refuse_foreign_leaves() {
   }
 }
 
+// A backward pass that builds no graph of its own calls the gradient operators below autograd (one that
+// does meets autograd's entry for them, which raises: they have no derivatives).
+struct BelowAutograd {
+  std::optional<at::AutoDispatchBelowADInplaceOrView> guard;
+  BelowAutograd() {
+    if (!at::GradMode::is_enabled()) guard.emplace();
+  }
+};
+
 bool any_grad(std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
@@ -510,6 +519,7 @@ struct HeadNorm : torch::autograd::Function<HeadNorm> {
   }
   static torch::autograd::variable_list backward(Ctx* ctx, torch::autograd::variable_list g) {
     refuse_foreign_leaves();
+    const BelowAutograd below;
     const auto s = ctx->get_saved_variables();
     const Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3];
     const Tensor dq_out = g[0].defined() ? g[0] : at::zeros_like(q);
@@ -561,6 +571,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   }
   static torch::autograd::variable_list backward(Ctx* ctx, torch::autograd::variable_list g) {
     refuse_foreign_leaves();
+    const BelowAutograd below;
     const auto s = ctx->get_saved_variables();
     const Tensor none;
     if (!g[0].defined()) return {none, none, none, none, none, none, none};
