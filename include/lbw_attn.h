@@ -360,7 +360,8 @@ typedef struct lbw_decode_params {
   const int32_t* lens;
   void* out; int64_t out_stride_b, out_stride_h;
   float softmax_scale;             /* > 0; 0: 1 / sqrt(head_dim) */
-  int32_t num_splits;              /* pieces of a sequence's keys; 0: chosen by the library */
+  int32_t num_splits;              /* 1: a workgroup per sequence and key/value head; n: the batch's keys in
+                                    * n * batch equal pieces, joined after; 0: chosen by the library */
 } lbw_decode_params;
 size_t lbw_attention_decode_workspace_size(const lbw_decode_params* p);
 int lbw_attention_decode(const lbw_decode_params* p, void* workspace, size_t workspace_bytes,

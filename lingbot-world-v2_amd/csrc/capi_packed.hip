@@ -202,9 +202,12 @@ bool sane(const lbw_packed_params* p) {
          p->q_tokens >= 0 && p->q_tokens <= 0x7fffffff;
 }
 
-int decode_pieces(const lbw_decode_params* p) {
-  return p->num_splits > 0 ? p->num_splits
-                           : decode_splits(p->batch, p->q_heads, p->k_heads, p->capacity, num_cus());
+int pieces_for(const lbw_decode_params* p) {
+  return decode_pieces(p->batch, p->q_heads, p->k_heads, p->capacity, p->num_splits, num_cus());
+}
+size_t decode_bytes(const lbw_decode_params* p, int pieces) {
+  return pieces > 0 ? (size_t)p->q_heads * ((size_t)pieces + p->batch) * (p->head_dim + 2) * sizeof(float)
+                    : 0;
 }
 
 int check_decode(const lbw_decode_params* p) {
@@ -437,9 +440,7 @@ int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads*
 
 size_t lbw_attention_decode_workspace_size(const lbw_decode_params* p) {
   if (check_decode(p) != LBW_OK || p->batch == 0) return 0;
-  const int s = decode_pieces(p);
-  if (s <= 1) return 0;
-  return (size_t)s * p->batch * p->q_heads * (p->head_dim + 2) * sizeof(float);
+  return decode_bytes(p, pieces_for(p));
 }
 
 int lbw_attention_decode(const lbw_decode_params* p, void* workspace, size_t workspace_bytes,
@@ -457,8 +458,8 @@ int lbw_attention_decode(const lbw_decode_params* p, void* workspace, size_t wor
   memset(&a, 0, sizeof(a));
   LBW_TRY(check_scale(p->softmax_scale, p->head_dim, &a.scale));
   if (B == 0) return LBW_OK;
-  a.splits = decode_pieces(p);
-  const size_t need = lbw_attention_decode_workspace_size(p);
+  a.pieces = pieces_for(p);
+  const size_t need = decode_bytes(p, a.pieces);
   if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need))
     return fail(LBW_ERR_WORKSPACE, "workspace of %zu bytes (16-byte aligned) needed, got %zu", need,
                 workspace_bytes);

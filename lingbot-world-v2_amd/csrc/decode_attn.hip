@@ -3,11 +3,18 @@
 //   out[b, h] = softmax(scale q[b, h] K^T) V over keys 0 .. len[b] - 1 of cache b, key/value head
 //   h / (Hq / Hk); a sequence of no keys gives 0.
 //
-// Bound by reading K and V once. A workgroup takes one key/value head of one sequence (its query
-// heads, up to 32, are the columns of S^T = K Q^T, so K and V are read once for the whole group)
-// and one piece of the keys; its 4 waves take 32-key tiles in turn, each through an LDS ring of
-// its own (two tiles of K and V, 32 KB), so no wave waits for another until the end, where the
-// four results are joined. Pieces are joined by a second kernel in a fixed order.
+// Bound by reading K and V once. A workgroup works for one key/value head: its query heads, up to 32,
+// are the columns of S^T = K Q^T, so K and V are read once for the whole group. Its 4 waves take 32-key
+// tiles in turn, each through 16 KB of LDS of its own (a tile of K, one of V: the next tile's K is
+// fetched while this one's V is worked on, and the other way round), so no wave waits for another until a
+// sequence ends, where the four results are joined; two workgroups share a CU.
+//
+// Either a workgroup has one whole sequence, or (few sequences, long caches) the keys of the whole batch,
+// laid end to end, are cut into equal pieces, as many as workgroups run at once: lengths are known on the
+// device only, and ragged ones then cost no time. A piece may end inside a sequence; what
+// belongs to one sequence is joined by a second kernel, in order.
+
+#include <algorithm>
 
 #include "packed_tiles.h"
 
@@ -17,15 +24,63 @@ namespace {
 constexpr int DW = 4;                       // waves per workgroup
 constexpr int DT = 32;                      // keys per tile
 constexpr int DT_B = DT * PK_ROWB;          // 8 KB
-constexpr int STAGE_B = 2 * DT_B;           // K, then V
-constexpr int RING_B = 2 * STAGE_B;         // per wave
+constexpr int RING_B = 2 * DT_B;            // per wave: K, V
 constexpr int DEC_LDS = DW * RING_B;
 constexpr int NCOPY = DT_B / 1024;          // copies per lane for K or V of a tile
 constexpr int HEADS = 32;                   // query heads per workgroup
 
-__global__ void __launch_bounds__(DW * 64, 1) decode_kernel(const DecodeArgs a) {
+// A value that every lane holds, in scalar registers.
+__device__ __forceinline__ int64_t scalar64(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ int tiles_of(const DecodeArgs& a, int b) {
+  const int n = a.lens[b];
+  return ((n < 0 ? 0 : (n > a.S ? a.S : n)) + DT - 1) / DT;
+}
+// Tiles of all sequences together and, with `upto`, of those before it.
+__device__ __forceinline__ void count_tiles_of(const DecodeArgs& a, int lane, int upto, int64_t& all,
+                                               int64_t& before) {
+  int64_t x = 0, y = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    const int n = tiles_of(a, b);
+    x += n;
+    if (b < upto) y += n;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    x += __shfl_xor(x, o);
+    y += __shfl_xor(y, o);
+  }
+  all = scalar64(x);
+  before = scalar64(y);
+}
+// The sequence that tile `t` belongs to (0 <= t < all), and the tiles before it.
+__device__ __forceinline__ int find_sequence(const DecodeArgs& a, int lane, int64_t t, int64_t& before) {
+  int64_t base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int n = b0 + lane < a.B ? tiles_of(a, b0 + lane) : 0;
+    int64_t sum = n;  // inclusive
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t y = __shfl_up(sum, o);
+      if (lane >= o) sum += y;
+    }
+    const uint64_t past = __ballot(base + sum > t);
+    if (past != 0) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      before = scalar64(base + __shfl(sum - n, l));
+      return __builtin_amdgcn_readfirstlane(b0 + l);
+    }
+    base += __shfl(sum, 63);
+  }
+  before = base;
+  return a.B;
+}
+
+__global__ void __launch_bounds__(DW * 64, 2) decode_kernel(const DecodeArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
-  __shared__ float sm[DW][HEADS], sl[DW][HEADS];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
@@ -33,198 +88,271 @@ __global__ void __launch_bounds__(DW * 64, 1) decode_kernel(const DecodeArgs a) 
   uint32_t id = blockIdx.x;
   const int kv = id % (uint32_t)a.Hk;
   id /= (uint32_t)a.Hk;
-  const int hb = id % (uint32_t)blocks;
-  id /= (uint32_t)blocks;
-  const int split = id % (uint32_t)a.splits, b = id / (uint32_t)a.splits;
+  const int hb = id % (uint32_t)blocks, piece = id / (uint32_t)blocks;
   const int h0 = kv * group + hb * HEADS;
   const int nh = min(HEADS, group - hb * HEADS);
 
-  int len = a.lens[b];
-  len = len < 0 ? 0 : (len > a.S ? a.S : len);
-  len = __builtin_amdgcn_readfirstlane(len);
-  const int tiles = (len + DT - 1) / DT;
-  const int t0 = (int)((int64_t)tiles * split / a.splits) + wave;
-  const int t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
-
-  u32x4 qf[8];
-  load_rows(a.q.p + b * a.q.sl + h0 * a.q.sh, a.q.sh, nh, l32, hl, qf);
-  const unsigned char* kb = reinterpret_cast<const unsigned char*>(a.k + b * a.ksb + kv * a.ksh);
-  const unsigned char* vb = reinterpret_cast<const unsigned char*>(a.v + b * a.vsb + kv * a.vsh);
+  // this workgroup's tiles [at, end) of the batch laid end to end, from sequence b on
+  int b = piece;
+  int64_t at = 0, end = 1, before = 0;
+  if (a.pieces > 0) {
+    int64_t all, none;
+    count_tiles_of(a, lane, 0, all, none);
+    // (no more pieces than tiles: an empty one between two parts of a sequence would leave a row unwritten)
+    const int64_t pieces = all < a.pieces ? all : a.pieces;
+    if (piece >= pieces) return;
+    at = all * piece / pieces;
+    end = all * (piece + 1) / pieces;
+    b = find_sequence(a, lane, at, before);
+    if (b >= a.B) return;
+  }
 
   const int ring = (int)lds_addr(lds) + RING_B * wave;
   const int ka = row_address(ring, l32, hl), va = tr_address(ring + DT_B, lane, hl);
-  int crow[NCOPY], ccol[NCOPY];
-#pragma unroll
-  for (int i = 0; i < NCOPY; ++i) {
-    crow[i] = 4 * i + (lane >> 4);
-    ccol[i] = ((lane & 15) ^ swz(crow[i])) * 16;
-  }
-  auto issue = [&](int t, int stage) {
-    const int64_t first = (int64_t)t * DT;
-    const int last = len - 1 - t * DT;  // (rows past the end copy the last valid one)
-    const unsigned char* kt = kb + first * a.ksl * 2;
-    const unsigned char* vt = vb + first * a.vsl * 2;
-    const uint32_t to = (uint32_t)ring + stage * STAGE_B;
-#pragma unroll
-    for (int i = 0; i < NCOPY; ++i) {
-      const int r = crow[i] < last ? crow[i] : last;
-      dma16_guarded(kt, (uint32_t)r * (uint32_t)(a.ksl * 2) + ccol[i], to + 1024 * i);
-      dma16_guarded(vt, (uint32_t)r * (uint32_t)(a.vsl * 2) + ccol[i], to + DT_B + 1024 * i);
-    }
-  };
+  // copy i of a tile: rows 4 i + lane / 16, chunk (lane % 16) ^ swz(row); rows i and i + 4 share the chunk
+  const int crow = lane >> 4, ccol = ((lane & 15) ^ swz(lane >> 4)) * 16;
+  const uint32_t koff = (uint32_t)crow * (uint32_t)(a.ksl * 2), voff = (uint32_t)crow * (uint32_t)(a.vsl * 2);
+  const float c = sreg(a.scale_log2);
 
-  floatx16 o[4];
+  do {
+    int len = a.lens[b];
+    len = __builtin_amdgcn_readfirstlane(len < 0 ? 0 : (len > a.S ? a.S : len));
+    const int tiles = (len + DT - 1) / DT;
+    // this sequence's tiles of the piece (without pieces: all of them)
+    const int s0 = a.pieces > 0 ? (int)(at - before) : 0;
+    const int s1 = a.pieces > 0 ? (int)(end - before < tiles ? end - before : tiles) : tiles;
+
+    u32x4 qf[8];
+    load_rows(a.q.p + b * a.q.sl + h0 * a.q.sh, a.q.sh, nh, l32, hl, qf);
+    const unsigned char* kb = reinterpret_cast<const unsigned char*>(a.k + b * a.ksb + kv * a.ksh);
+    const unsigned char* vb = reinterpret_cast<const unsigned char*>(a.v + b * a.vsb + kv * a.vsh);
+    auto issue = [&](const unsigned char* base, int64_t stride_b, uint32_t off, int t, uint32_t to) {
+      // (scalar: what the compiler cannot see is the same in every lane)
+      const unsigned char* p = reinterpret_cast<const unsigned char*>(
+          (uintptr_t)scalar64((int64_t)(uintptr_t)(base + (int64_t)t * DT * stride_b)));
+      const int last = len - 1 - t * DT;
+      if (last >= DT - 1) {
 #pragma unroll
-  for (int db = 0; db < 4; ++db) zero(o[db]);
-  float m = M_INIT, l = 0.0f;
-  const float c = a.scale_log2;
-  __builtin_amdgcn_s_waitcnt(0x0070);  // the query is there: only tile copies are counted below
-  if (t0 < t1) issue(t0, 0);
-  int stage = 0;
+        for (int i = 0; i < NCOPY; ++i)
+          dma16_guarded(p + 4 * i * stride_b, off + (ccol ^ ((i & 3) << 4)), to + 1024 * i);
+      } else {  // (rows past the end copy the last one)
+#pragma unroll
+        for (int i = 0; i < NCOPY; ++i) {
+          const int r = crow + 4 * i < last ? crow + 4 * i : last;
+          dma16_guarded(p, (uint32_t)r * (uint32_t)stride_b + (ccol ^ ((i & 3) << 4)), to + 1024 * i);
+        }
+      }
+    };
+    auto issue_k = [&](int t) { issue(kb, a.ksl * 2, koff, t, (uint32_t)ring); };
+    auto issue_v = [&](int t) { issue(vb, a.vsl * 2, voff, t, (uint32_t)ring + DT_B); };
+    static_assert(NCOPY == 8, "the counts below are a tile's copies");
+
+    floatx16 o[4];
+#pragma unroll
+    for (int db = 0; db < 4; ++db) zero(o[db]);
+    float m = M_INIT, l = 0.0f;
+    __builtin_amdgcn_s_waitcnt(0x0070);  // the query is there: only tile copies are counted below
+    int t = s0 + wave;
+    if (t < s1) {
+      issue_k(t);
+      issue_v(t);
+    }
 #pragma unroll 1
-  for (int t = t0; t < t1; t += DW, stage ^= 1) {
-    if (t + DW < t1) {
-      issue(t + DW, stage ^ 1);
-      static_assert(2 * NCOPY == 16, "the count below is a tile's copies");
-      asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-    } else {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (; t < s1; t += DW) {
+      const bool more = t + DW < s1;
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // K is there (V may be on its way)
+      floatx16 s;
+      zero(s);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) s = mfma32x32x16(read_row(ka, d, 0), qf[d], s);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its reads are over before K is overwritten
+      if (more) issue_k(t + DW);
+      if (t * DT + DT > len) {
+        const int left = len - (t * DT + 4 * hl);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = acc_row(r) < left ? s[r] : -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      mx = wave_max_xor32(mx);
+      const float mn = fmaxf(m, mx);
+      if (__any(mn > m)) {
+        const float alpha = fast_exp2((m - mn) * c);
+        scale_acc(o, alpha);
+        l *= alpha;
+        m = mn;
+      }
+      const float mc = -m * c;
+      floatx16 p;
+      float ls = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = fast_exp2(__builtin_fmaf(s[r], c, mc));
+        ls += p[r];
+      }
+      l += ls;
+      const u32x4 pf[2] = {pack_half(p, 0), pack_half(p, 1)};
+      if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V is there (the next K may not be)
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int mm = 0; mm < 2; ++mm) o[db] = mfma32x32x16(read_tr(va, db, mm, 0), pf[mm], o[db]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) issue_v(t + DW);
     }
-    const int at = stage * STAGE_B;
-    floatx16 s;
-    zero(s);
-#pragma unroll
-    for (int d = 0; d < 8; ++d) s = mfma32x32x16(read_row(ka, d, at), qf[d], s);
-    const int left = len - (t * DT + 4 * hl);
-    if (t * DT + DT > len) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = acc_row(r) < left ? s[r] : -INFINITY;
+    l = wave_sum_xor32(l);
+    // O^T as rows [head][128] fp32 into the wave's LDS, m and l behind the rings
+    float* const sm = reinterpret_cast<float*>(lds + DEC_LDS);
+    float* const sl = sm + DW * HEADS;
+    if (hl == 0) {
+      sm[wave * HEADS + l32] = l > 0.0f ? m : -INFINITY;
+      sl[wave * HEADS + l32] = l;
     }
-    float mx = s[0];
+    float* mine = reinterpret_cast<float*>(lds + RING_B * wave);
+    if (l32 < nh) {
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    mx = wave_max_xor32(mx);
-    const float mn = fmaxf(m, mx);
-    if (__any(mn > m)) {
-      const float alpha = fast_exp2((m - mn) * c);
-      scale_acc(o, alpha);
-      l *= alpha;
-      m = mn;
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          floatx4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = o[db][4 * g + e];
+          *reinterpret_cast<floatx4*>(mine + l32 * D + 32 * db + 8 * g + 4 * hl) = w;
+        }
     }
-    const float mc = -m * c;
-    floatx16 p;
-    float ls = 0.0f;
+    __syncthreads();
+    const bool whole = s1 - s0 == tiles;
+    for (int x = threadIdx.x; x < nh * (D / 4); x += DW * 64) {  // 4 values of one head at a time
+      const int hh = x / (D / 4), dq = 4 * (x % (D / 4));
+      float M = -INFINITY;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      p[r] = fast_exp2(__builtin_fmaf(s[r], c, mc));
-      ls += p[r];
+      for (int w = 0; w < DW; ++w) M = fmaxf(M, sm[w * HEADS + hh]);
+      float L = 0.0f;
+      floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < DW; ++w) {
+        const float mw = sm[w * HEADS + hh], f = mw == -INFINITY ? 0.0f : fast_exp2((mw - M) * c);
+        // (a wave without keys holds zeros)
+        L += f * sl[w * HEADS + hh];
+        acc += f * *reinterpret_cast<const floatx4*>(
+                       reinterpret_cast<const float*>(lds + RING_B * w) + hh * D + dq);
+      }
+      if (whole) {
+        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+        u32x2 w;
+        w[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+        w[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<u32x2*>(a.out.p + b * a.out.sl + (h0 + hh) * a.out.sh + dq) = w;
+      } else {
+        // (piece + b: the parts of a head in the order of their keys, each in a row of its own, as the
+        // next part has another piece or a later sequence, or both)
+        const int64_t rows = (int64_t)a.pieces + a.B, row = (h0 + hh) * rows + piece + b;
+        *reinterpret_cast<floatx4*>(a.part + row * D + dq) = acc;
+        if (dq == 0) {
+          float* st = a.part + a.Hq * rows * D;
+          st[row] = M;
+          st[a.Hq * rows + row] = L;
+        }
+      }
     }
-    l += ls;
-    const u32x4 pf[2] = {pack_half(p, 0), pack_half(p, 1)};
-#pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-      for (int mm = 0; mm < 2; ++mm) o[db] = mfma32x32x16(read_tr(va, db, mm, at), pf[mm], o[db]);
-    // its reads of this stage are over before the next turn's copies into it
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-  }
-  l = wave_sum_xor32(l);
-  if (hl == 0) {
-    sm[wave][l32] = l > 0.0f ? m : -INFINITY;
-    sl[wave][l32] = l;
-  }
-  // O^T as rows [head][128] fp32 into the wave's ring (16 KB)
-  float* mine = reinterpret_cast<float*>(lds + RING_B * wave);
-#pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      floatx4 w;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = o[db][4 * g + e];
-      *reinterpret_cast<floatx4*>(mine + l32 * D + 32 * db + 8 * g + 4 * hl) = w;
-    }
-  __syncthreads();
-  // thread: 4 values of one head at a time
-  const int64_t BH = (int64_t)a.B * a.Hq;
-  for (int x = threadIdx.x; x < nh * (D / 4); x += DW * 64) {
-    const int hh = x / (D / 4), dq = 4 * (x % (D / 4));
+    if (a.pieces == 0) return;
+    at = before + tiles;
+    if (at >= end) return;
+    // the next sequence with keys
+    before = at;
+    do {
+      b = __builtin_amdgcn_readfirstlane(b + 1);
+    } while (b < a.B && __builtin_amdgcn_readfirstlane(tiles_of(a, b)) == 0);
+    if (b >= a.B) return;
+    __syncthreads();  // the joined results are read: the rings are free
+  } while (true);
+}
+
+// One wave per (sequence, query head): a sequence that several pieces share is joined, in their order;
+// one of no keys gets zeros; the others are finished.
+__global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (id >= (int64_t)a.B * a.Hq) return;
+  const int b = (int)(id / a.Hq), h = (int)(id % a.Hq);
+  int64_t all, before;
+  count_tiles_of(a, lane, b, all, before);
+  const int tiles = __builtin_amdgcn_readfirstlane(tiles_of(a, b));
+  float x = 0.0f, y = 0.0f, L = 0.0f;
+  if (tiles > 0) {
+    // tile t is in piece j when floor(all j / pieces) <= t < floor(all (j + 1) / pieces)
+    const int64_t pieces = all < a.pieces ? all : a.pieces;
+    const int j0 = (int)(((before + 1) * pieces - 1) / all);
+    const int j1 = (int)(((before + tiles) * pieces - 1) / all);
+    if (j0 == j1) return;
+    const int64_t rows = (int64_t)a.pieces + a.B, row = h * rows + j0 + b;
+    const float* st = a.part + a.Hq * rows * D;
     float M = -INFINITY;
+    for (int i0 = 0; i0 <= j1 - j0; i0 += 64) {  // 64 parts at a time, their weights one per lane
+      const int n = min(64, j1 - j0 + 1 - i0);
+      float m = -INFINITY, l = 0.0f;
+      if (lane < n) {
+        m = st[row + i0 + lane];
+        l = st[a.Hq * rows + row + i0 + lane];
+      }
+      float mx = m;
 #pragma unroll
-    for (int w = 0; w < DW; ++w) M = fmaxf(M, sm[w][hh]);
-    float L = 0.0f;
-    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+      const float mn = fmaxf(M, mx);
+      if (mn == -INFINITY) continue;
+      const float f0 = M == -INFINITY ? 0.0f : fast_exp2((M - mn) * a.scale_log2);
+      const float w = m == -INFINITY ? 0.0f : fast_exp2((m - mn) * a.scale_log2);
+      x *= f0;
+      y *= f0;
+      L = L * f0 + wave_reduce_sum(w * l);
+      M = mn;
+      const float* p = a.part + (row + i0) * D + 2 * lane;
+      for (int i = 0; i < n; i += 8) {  // (lanes past n have weight 0; their rows are not read)
+        float2 v[8];
 #pragma unroll
-    for (int w = 0; w < DW; ++w) {
-      const float f = sm[w][hh] == -INFINITY ? 0.0f : fast_exp2((sm[w][hh] - M) * c);
-      // (a wave without keys holds zeros)
-      L += f * sl[w][hh];
-      acc += f * *reinterpret_cast<const floatx4*>(
-                     reinterpret_cast<const float*>(lds + RING_B * w) + hh * D + dq);
-    }
-    if (a.splits == 1) {
-      const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-      u32x2 w;
-      w[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-      w[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
-      *reinterpret_cast<u32x2*>(a.out.p + b * a.out.sl + (h0 + hh) * a.out.sh + dq) = w;
-    } else {
-      const int64_t row = (int64_t)split * BH + (int64_t)b * a.Hq + h0 + hh;
-      *reinterpret_cast<floatx4*>(a.part + row * D + dq) = acc;
-      if (dq == 0) {
-        float* st = a.part + (int64_t)a.splits * BH * D;
-        st[row] = M;
-        st[(int64_t)a.splits * BH + row] = L;
+        for (int u = 0; u < 8; ++u)
+          v[u] = i + u < n ? *reinterpret_cast<const float2*>(p + (int64_t)(i + u) * D) : float2{0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float f = __shfl(w, i + u);
+          x += f * v[u].x;
+          y += f * v[u].y;
+        }
       }
     }
   }
-}
-
-// One wave per (sequence, query head): the pieces joined in their order.
-__global__ void __launch_bounds__(256) decode_merge_kernel(const DecodeArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t BH = (int64_t)a.B * a.Hq, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= BH) return;
-  const float* st = a.part + (int64_t)a.splits * BH * D;
-  float M = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, st[s * BH + row]);
-  float L = 0.0f, x = 0.0f, y = 0.0f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float ms = st[s * BH + row];
-    const float f = ms == -INFINITY ? 0.0f : fast_exp2((ms - M) * a.scale_log2);
-    L += f * st[(int64_t)a.splits * BH + s * BH + row];
-    const float2 v = *reinterpret_cast<const float2*>(a.part + (s * BH + row) * D + 2 * lane);
-    x += f * v.x;
-    y += f * v.y;
-  }
   const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-  const int b = (int)(row / a.Hq), h = (int)(row % a.Hq);
   *reinterpret_cast<uint32_t*>(a.out.p + b * a.out.sl + h * a.out.sh + 2 * lane) =
       pack_bf16x2(x * inv, y * inv);
 }
 
 }  // namespace
 
-// Pieces of a sequence's keys: enough workgroups for every CU, pieces of 256 keys or more of the cache.
-int decode_splits(int64_t B, int Hq, int Hk, int64_t S, int cus) {
-  const int group = Hq / Hk;
-  const int64_t units = B * Hk * ((group + HEADS - 1) / HEADS);
-  int64_t s = (2 * cus + units - 1) / units;
-  if (s > S / 256) s = S / 256;
-  return (int)(s < 1 ? 1 : (s > 128 ? 128 : s));
+// Pieces per key/value head (and block of 32 of its query heads): none while whole sequences give work
+// enough or caches are short, else as many as run at once, two workgroups a CU, of 8 tiles or more.
+int decode_pieces(int64_t B, int Hq, int Hk, int64_t S, int num_splits, int cus) {
+  const int64_t units = (int64_t)Hk * ((Hq / Hk + HEADS - 1) / HEADS);
+  if (num_splits == 1) return 0;
+  if (num_splits > 1) return (int)std::min<int64_t>(num_splits * B, 1 << 20);
+  if (S <= 1024 || B * units >= 2 * cus) return 0;
+  const int64_t most = std::max<int64_t>(1, 2 * cus / units), tiles = B * ((S + DT - 1) / DT);
+  return (int)std::max<int64_t>(1, std::min(most, tiles / 8));
 }
 
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t stream) {
+  constexpr int bytes = DEC_LDS + 2 * DW * HEADS * 4;
   static hipError_t attr = hipFuncSetAttribute((const void*)decode_kernel,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, DEC_LDS);
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (attr != hipSuccess) return attr;
   const int group = a.Hq / a.Hk, blocks = (group + HEADS - 1) / HEADS;
-  const int64_t n = (int64_t)a.B * a.splits * blocks * a.Hk;
-  hipLaunchKernelGGL(decode_kernel, dim3((uint32_t)n), dim3(DW * 64), DEC_LDS, stream, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
+  const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B) * blocks * a.Hk;
+  hipLaunchKernelGGL(decode_kernel, dim3((uint32_t)n), dim3(DW * 64), bytes, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.pieces == 0) return e;
   const int64_t rows = (int64_t)a.B * a.Hq;
-  hipLaunchKernelGGL(decode_merge_kernel, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(decode_join_kernel, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 

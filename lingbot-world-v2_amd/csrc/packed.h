@@ -98,10 +98,11 @@ struct DecodeArgs {
   RowsOut out;                 // [B, Hq, D]
   int B, Hq, Hk, S;
   float scale, scale_log2;
-  int splits;                  // pieces of a sequence's keys
-  float* part;                 // splits > 1: [splits][B * Hq][D] then m, l [splits][B * Hq] each
+  int pieces;                  // 0: a workgroup per sequence; J: a key/value head's keys of the whole
+                               // batch in J equal pieces
+  float* part;                 // pieces: [Hq][pieces + B][D] partial O, then m and l, [Hq][pieces + B] each
 };
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t stream);
-int decode_splits(int64_t B, int Hq, int Hk, int64_t S, int cus);
+int decode_pieces(int64_t B, int Hq, int Hk, int64_t S, int num_splits, int cus);
 
 }  // namespace lbw

@@ -130,8 +130,8 @@ def attention_decode(q, k_cache, v_cache, lens, *, softmax_scale: float | None =
     ``[batch, capacity, kv_heads, 128]`` (strided views are fine), keys ``0 .. lens[b] - 1`` of
     sequence b -> ``[batch, heads, 128]`` (into ``out`` when given). ``lens`` int32 ``[batch]`` on q's device
     is read there (no host sync; limited to ``[0, capacity]``); rows behind a length may hold
-    anything. A sequence of no keys gives 0. ``num_splits``: pieces of each sequence's keys that run
-    side by side (0: by batch, heads and capacity)."""
+    anything. A sequence of no keys gives 0. ``num_splits`` 1: one workgroup per sequence and kv head; n: the whole batch's
+    keys cut into ``n * batch`` equal pieces that run side by side; 0: by batch, heads and capacity."""
     ops = _lib.ops()
     if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != HEAD_DIM:
         raise ValueError(f"q must be bf16 [batch, heads, {HEAD_DIM}], got {tuple(q.shape)} {q.dtype}")
