@@ -154,30 +154,36 @@ int fill_packed(const lbw_packed_params* p, PackedArgs* a) {
   return LBW_OK;
 }
 
-// How a kernel's items are cut. `slots` run at once; an item of `longest` tiles ends last when that is
-// more than half as much again as its share of all tiles: then items are cut into pieces of two thirds of
-// a share, `least` tiles at least.
+// How a kernel's items are cut. `slots` workgroups run at once; an item much longer than a slot's share of
+// all tiles ends last. A piece costs its partial results' way to memory and back and a share of a
+// second launch, about 10 tiles of its time, so pieces are long: one and a half shares, `least` tiles
+// at least (from 256 tiles a share on, where that cost is small beside an uncut item, two thirds of a share),
+// and nothing is cut that would give fewer than `times` / 2 pieces. Measured, uncut / cut: forward, 256 rows over
+// 4680 + 1816 + 3111 keys x 40/8 heads 83 / 71 us, 16 rows over 8192 keys 130 / 39, 5000 causal x 5/1
+// 90 / 62, but 2048 causal x 40/8 (32 tiles, 21 a share) 54 / 64; gradient of 2048 x 40/8 299 / 211, 4680 x 12/4
+// 446 / 334, 16384 x 16/2 4706 / 3690, but 8 x 512 x 40/8 (40 tiles, 25 a share) 131 / 185.
 PackedSplit split_items(int64_t items, int64_t heads, int64_t tiles, int64_t longest, int64_t slots,
-                        int64_t least) {
+                        int64_t least, int64_t times) {
   PackedSplit s = {0, 1, 1};
   if (tiles <= 0 || longest <= 0 || items <= 0) return s;
   const int64_t share = tiles * heads / slots;
-  if (2 * longest <= 3 * share || longest < 2 * least) return s;
-  s.piece = (int)std::min<int64_t>(std::max<int64_t>(least, share * 2 / 3), 1 << 30);
+  const int64_t piece = std::max<int64_t>(least, share < 256 ? share * 3 / 2 : share * 2 / 3);
+  if (2 * longest < times * piece) return s;
+  s.piece = (int)std::min<int64_t>(piece, 1 << 30);
   s.smax = (int)std::min<int64_t>(16, (longest + s.piece - 1) / s.piece);
   if (s.smax < 2) return PackedSplit{0, 1, 1};
   // (the items longer than a piece come first in the table, and are no more than this)
   s.n_split = (int)std::min<int64_t>(items, std::max<int64_t>(1, tiles / s.piece));
   return s;
 }
-// two workgroups per CU; a piece's O is written and read in the time of about 6 tiles
+// forward and dQ: two workgroups per CU
 PackedSplit split_q(const lbw_packed_params* p) {
-  return split_items(p->n_q_items, p->q_heads, p->q_tiles, p->q_tiles_max, 2 * num_cus(), 8);
+  return split_items(p->n_q_items, p->q_heads, p->q_tiles, p->q_tiles_max, 2 * num_cus(), 16, 4);
 }
-// one workgroup per CU, its tiles those of all heads of the group
+// dK and dV: one workgroup per CU, an item's tiles those of all heads of the group
 PackedSplit split_k(const lbw_packed_params* p) {
   const int64_t group = p->q_heads / p->k_heads;
-  return split_items(p->n_k_items, p->k_heads, p->k_tiles * group, p->k_tiles_max * group, num_cus(), 24);
+  return split_items(p->n_k_items, p->k_heads, p->k_tiles * group, p->k_tiles_max * group, num_cus(), 24, 3);
 }
 size_t part_bytes(const PackedSplit& s, int heads, int floats) {
   return (size_t)s.n_split * heads * s.smax * floats * sizeof(float);
