@@ -95,8 +95,9 @@ lbw_head_norm_rope_params head_norm_params(const Tensor& q, const Tensor& k, con
   const int64_t A = (int64_t)axes.size();
   TORCH_CHECK(A >= 1 && A <= LBW_MAX_AXES, "1 to ", LBW_MAX_AXES, " axes, got ", A);
   check_int32("pos", pos, q);
-  TORCH_CHECK(pos.dim() == 2 && pos.size(0) == q.size(0) && pos.size(1) == A &&
-                  (A == 1 || pos.stride(1) == 1) && pos.stride(0) >= 0,
+  TORCH_CHECK((pos.dim() == 2 ? pos.size(1) == A && (A == 1 || pos.stride(1) == 1)
+                              : pos.dim() == 1 && A == 1) &&
+                  pos.size(0) == q.size(0) && pos.stride(0) >= 0,
               "pos must be int32 [tokens, ", A, "] with contiguous rows");
   lbw_head_norm_rope_params p;
   std::memset(&p, 0, sizeof(p));
@@ -239,6 +240,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> head_norm_rope_bwd(
 
 // ---- packed attention
 
+// A tensor without a contiguous head dim is copied (in the forward above autograd, so that its gradient finds
+// the way back).
+Tensor unit(const Tensor& t) { return t.dim() != 3 || t.stride(2) == 1 ? t : t.contiguous(); }
+
+
 // -> query items, key items, and the tile counts [q_tiles, q_tiles_max, k_tiles, k_tiles_max]
 std::tuple<Tensor, Tensor, std::vector<int64_t>> packed_plan(const Tensor& q_lens,
                                                              const Tensor& k_lens, bool causal) {
@@ -263,7 +269,7 @@ std::tuple<Tensor, Tensor, std::vector<int64_t>> packed_plan(const Tensor& q_len
 
 lbw_packed_params packed_params(const Tensor& q, const Tensor& k, const Tensor& v,
                                 const Tensor& q_items, const Tensor& k_items,
-                                at::IntArrayRef tiles, double scale) {
+                                at::IntArrayRef info, double scale) {
   check_rows("q", q, q);
   check_rows("k", k, q);
   check_rows("v", v, q);
@@ -292,11 +298,13 @@ lbw_packed_params packed_params(const Tensor& q, const Tensor& k, const Tensor& 
   p.n_q_items = (int32_t)q_items.size(0);
   p.k_items = k_items.data_ptr<int32_t>();
   p.n_k_items = (int32_t)k_items.size(0);
-  TORCH_CHECK(tiles.size() == 4, "the plan's four tile counts are wanted");
-  p.q_tiles = tiles[0];
-  p.q_tiles_max = tiles[1];
-  p.k_tiles = tiles[2];
-  p.k_tiles_max = tiles[3];
+  TORCH_CHECK(info.size() == 6, "the plan's tokens and tile counts (6 values) are wanted");
+  TORCH_CHECK(q.size(0) == info[0] && k.size(0) == info[1], "the plan is for ", info[0], " query and ",
+              info[1], " key rows");
+  p.q_tiles = info[2];
+  p.q_tiles_max = info[3];
+  p.k_tiles = info[4];
+  p.k_tiles_max = info[5];
   return p;
 }
 
@@ -306,9 +314,9 @@ Tensor new_lse(const Tensor& q) {
 
 std::tuple<Tensor, Tensor> attention_packed(const Tensor& q, const Tensor& k, const Tensor& v,
                                             const Tensor& q_items, const Tensor& k_items,
-                                            at::IntArrayRef tiles, double scale, bool want_lse) {
+                                            at::IntArrayRef info, double scale, bool want_lse) {
   c10::DeviceGuard guard(q.device());
-  auto p = packed_params(q, k, v, q_items, k_items, tiles, scale);
+  auto p = packed_params(q, k, v, q_items, k_items, info, scale);
   Tensor out = at::empty(q.sizes(), q.options());
   Tensor lse = want_lse ? new_lse(q) : at::empty({0}, q.options().dtype(at::kFloat));
   p.out = out.data_ptr(); p.out_stride_l = out.stride(0); p.out_stride_h = out.stride(1);
@@ -321,14 +329,15 @@ std::tuple<Tensor, Tensor> attention_packed(const Tensor& q, const Tensor& k, co
   return {out, lse};
 }
 
-std::tuple<Tensor, Tensor, Tensor> attention_packed_bwd(const Tensor& dout_, const Tensor& q,
-                                                        const Tensor& k, const Tensor& v,
-                                                        const Tensor& out, const Tensor& lse,
+std::tuple<Tensor, Tensor, Tensor> attention_packed_bwd(const Tensor& dout_, const Tensor& q_,
+                                                        const Tensor& k_, const Tensor& v_,
+                                                        const Tensor& out_, const Tensor& lse,
                                                         const Tensor& q_items,
                                                         const Tensor& k_items,
-                                                        at::IntArrayRef tiles, double scale) {
+                                                        at::IntArrayRef info, double scale) {
+  const Tensor q = unit(q_), k = unit(k_), v = unit(v_), out = unit(out_);
   c10::DeviceGuard guard(q.device());
-  auto p = packed_params(q, k, v, q_items, k_items, tiles, scale);
+  auto p = packed_params(q, k, v, q_items, k_items, info, scale);
   check_rows("out", out, q);
   TORCH_CHECK(dout_.sizes() == q.sizes() && dout_.scalar_type() == at::kBFloat16 &&
                   dout_.device() == q.device() && out.sizes() == q.sizes(),
@@ -550,21 +559,21 @@ std::tuple<Tensor, Tensor> head_norm_rope_autograd(const Tensor& q, const Tensor
 }
 
 auto call_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qi,
-                 const Tensor& ki, at::IntArrayRef tiles, double scale, bool want_lse) {
+                 const Tensor& ki, at::IntArrayRef info, double scale, bool want_lse) {
   static auto op = handle<decltype(attention_packed)>("lbw::attention_packed");
-  return op.call(q, k, v, qi, ki, tiles, scale, want_lse);
+  return op.call(q, k, v, qi, ki, info, scale, want_lse);
 }
 
 struct PackedAttention : torch::autograd::Function<PackedAttention> {
   using Ctx = torch::autograd::AutogradContext;
   static torch::autograd::variable_list forward(Ctx* ctx, const Tensor& q, const Tensor& k,
                                                 const Tensor& v, const Tensor& qi,
-                                                const Tensor& ki, std::vector<int64_t> tiles,
+                                                const Tensor& ki, std::vector<int64_t> info,
                                                 double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, lse] = call_packed(q, k, v, qi, ki, tiles, scale, true);
+    auto [out, lse] = call_packed(q, k, v, qi, ki, info, scale, true);
     ctx->save_for_backward({q, k, v, out, lse, qi, ki});
-    ctx->saved_data["tiles"] = tiles;
+    ctx->saved_data["info"] = info;
     ctx->saved_data["scale"] = scale;
     ctx->mark_non_differentiable({lse});
     return {out, lse};
@@ -577,21 +586,22 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
     if (!g[0].defined()) return {none, none, none, none, none, none, none};
     static auto op = handle<decltype(attention_packed_bwd)>("lbw::attention_packed_bwd");
     auto [dq, dk, dv] = op.call(g[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6],
-                                ctx->saved_data["tiles"].toIntVector(),
+                                ctx->saved_data["info"].toIntVector(),
                                 ctx->saved_data["scale"].toDouble());
     return {dq, dk, dv, none, none, none, none};
   }
 };
 
-std::tuple<Tensor, Tensor> attention_packed_autograd(const Tensor& q, const Tensor& k,
-                                                     const Tensor& v, const Tensor& qi,
-                                                     const Tensor& ki, at::IntArrayRef tiles,
+std::tuple<Tensor, Tensor> attention_packed_autograd(const Tensor& q_, const Tensor& k_,
+                                                     const Tensor& v_, const Tensor& qi,
+                                                     const Tensor& ki, at::IntArrayRef info,
                                                      double scale, bool want_lse) {
+  const Tensor q = unit(q_), k = unit(k_), v = unit(v_);
   if (!any_grad({&q, &k, &v})) {
     at::AutoDispatchBelowADInplaceOrView below;
-    return call_packed(q, k, v, qi, ki, tiles, scale, want_lse);
+    return call_packed(q, k, v, qi, ki, info, scale, want_lse);
   }
-  auto r = PackedAttention::apply(q, k, v, qi, ki, tiles.vec(), scale);
+  auto r = PackedAttention::apply(q, k, v, qi, ki, info.vec(), scale);
   return {r[0], r[1]};
 }
 
@@ -609,9 +619,9 @@ TORCH_LIBRARY_FRAGMENT(lbw, m) {
         "float q_scale, float k_scale) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("packed_plan(Tensor q_lens, Tensor k_lens, bool causal) -> (Tensor, Tensor, int[])");
   m.def("attention_packed(Tensor q, Tensor k, Tensor v, Tensor q_items, Tensor k_items, "
-        "int[] tiles, float softmax_scale=0., bool want_lse=True) -> (Tensor, Tensor)");
+        "int[] info, float softmax_scale=0., bool want_lse=True) -> (Tensor, Tensor)");
   m.def("attention_packed_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor out, Tensor lse, "
-        "Tensor q_items, Tensor k_items, int[] tiles, float softmax_scale=0.) "
+        "Tensor q_items, Tensor k_items, int[] info, float softmax_scale=0.) "
         "-> (Tensor, Tensor, Tensor)");
   m.def("attention_decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor lens, "
         "float softmax_scale=0., int num_splits=0) -> Tensor");

@@ -58,6 +58,8 @@ def _rows(name, t, like=None):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
 
 
+# The ops check what they are given (and raise RuntimeError); a call they refuse is looked over once more
+# here, for a ValueError that names the argument. A call that passes pays for one set of checks.
 def _check(q, k, wq, wk, rope, pos):
     _rows("q", q)
     _rows("k", k)
@@ -76,7 +78,6 @@ def _check(q, k, wq, wk, rope, pos):
     if pos.dtype != torch.int32 or tuple(pos.shape) != (T, len(rope.axes)):
         raise ValueError(f"pos must be int32 [{T}, {len(rope.axes)}], got {tuple(pos.shape)} "
                          f"{pos.dtype}")
-    return pos if pos.shape[1] == 1 or pos.stride(1) == 1 else pos.contiguous()
 
 
 def qk_head_norm_rope(q, k, wq, wk, rope: AxisRope, pos, eps: float = 1e-6, *,
@@ -86,10 +87,12 @@ def qk_head_norm_rope(q, k, wq, wk, rope: AxisRope, pos, eps: float = 1e-6, *,
     256). ``wq``, ``wk``: ``[D]`` weights, both bf16 or both fp32, or None. ``pos``: int32
     ``[tokens, axes]`` (``[tokens]`` for one axis) on q's device; a position outside the table turns its
     pairs into NaN. Differentiable in q, k, wq and wk (first derivatives; the same bits every run)."""
-    ops = _lib.ops()
-    pos = _check(q, k, wq, wk, rope, pos)
-    return ops.head_norm_rope(q, k, wq, wk, rope.table, rope.axes, rope.interleaved, pos,
-                              float(eps), float(q_scale), float(k_scale))
+    try:
+        return _lib.ops().head_norm_rope(q, k, wq, wk, rope.table, rope.axes, rope.interleaved, pos,
+                                         eps, q_scale, k_scale)
+    except (RuntimeError, NotImplementedError):
+        _check(q, k, wq, wk, rope, pos)
+        raise
 
 
 def qk_head_norm_rope_(q, k, wq, wk, rope: AxisRope, pos, eps: float = 1e-6, *, q_out, k_out,
@@ -99,8 +102,17 @@ def qk_head_norm_rope_(q, k, wq, wk, rope: AxisRope, pos, eps: float = 1e-6, *, 
     newest one of sequence t: its k and v go to row ``rows[t]`` of the caches ``k_out``, ``v_out``
     ``[tokens, capacity, kv_heads, D]`` (strided views are fine), and are not written where that row
     is outside the cache. Not differentiable. Returns ``(q_out, k_out)``."""
-    ops = _lib.ops()
-    pos = _check(q, k, wq, wk, rope, pos)
+    try:
+        _lib.ops().head_norm_rope_(q, k, wq, wk, rope.table, rope.axes, rope.interleaved, pos, eps,
+                                   q_scale, k_scale, q_out, k_out, v, v_out, rows)
+    except (RuntimeError, NotImplementedError):
+        _check(q, k, wq, wk, rope, pos)
+        _check_out(q, k, q_out, k_out, v, v_out, rows)
+        raise
+    return q_out, k_out
+
+
+def _check_out(q, k, q_out, k_out, v, v_out, rows):
     _rows("q_out", q_out, q)
     if (v is None) != (v_out is None):
         raise ValueError("v and v_out: both or neither")
@@ -118,6 +130,3 @@ def qk_head_norm_rope_(q, k, wq, wk, rope: AxisRope, pos, eps: float = 1e-6, *, 
                              f"{t.dtype} strides {t.stride()}")
     if rows is not None and (rows.dtype != torch.int32 or tuple(rows.shape) != (q.shape[0],)):
         raise ValueError(f"rows must be int32 [{q.shape[0]}], got {tuple(rows.shape)} {rows.dtype}")
-    ops.head_norm_rope_(q, k, wq, wk, rope.table, rope.axes, rope.interleaved, pos, float(eps),
-                        float(q_scale), float(k_scale), q_out, k_out, v, v_out, rows)
-    return q_out, k_out

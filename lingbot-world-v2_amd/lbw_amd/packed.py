@@ -35,7 +35,7 @@ class PackedPlan:
     k_tokens: int
     q_items: torch.Tensor
     k_items: torch.Tensor
-    tiles: tuple
+    info: tuple  # q_tokens, k_tokens, and the items' tile counts
 
 
 def _lens(name, lens) -> tuple:
@@ -66,9 +66,11 @@ def packed_plan(q_lens: Sequence[int], k_lens: Sequence[int] | None = None, *, c
                              bool(causal))
     device = torch.device("cuda") if device is None else torch.device(device)
     return PackedPlan(ql, kl, bool(causal), sum(ql), sum(kl), qi.to(device), ki.to(device),
-                      tuple(tiles))
+                      (sum(ql), sum(kl), *tiles))
 
 
+# The ops check what they are given (and raise RuntimeError); a call they refuse is looked over once more
+# here, for a ValueError that names the argument. A call that passes pays for one set of checks.
 def _check(q, k, v, plan):
     for name, t, n in (("q", q, plan.q_tokens), ("k", k, plan.k_tokens), ("v", v, plan.k_tokens)):
         if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[2] != HEAD_DIM:
@@ -92,10 +94,6 @@ def _scale(softmax_scale) -> float:
     return s
 
 
-def _unit(t):
-    return t if t.stride(2) == 1 else t.contiguous()
-
-
 def attention_packed(q, k, v, plan: PackedPlan, *, softmax_scale: float | None = None,
                      return_lse: bool = False):
     """softmax(scale Q K^T) V of every sequence of ``plan``: q ``[q_tokens, heads, 128]``, k, v
@@ -105,10 +103,13 @@ def attention_packed(q, k, v, plan: PackedPlan, *, softmax_scale: float | None =
     sequence reaches another, whatever its values; inside a sequence a NaN or infinity may also reach
     rows that do not see it. Differentiable in q, k, v (first derivatives). A training step captured into
     a graph must not share leaves with a live eager graph of another stream: that backward raises."""
-    ops = _lib.ops()
-    _check(q, k, v, plan)
-    out, lse = ops.attention_packed(_unit(q), _unit(k), _unit(v), plan.q_items, plan.k_items,
-                                    plan.tiles, _scale(softmax_scale), return_lse)
+    scale = _scale(softmax_scale)
+    try:
+        out, lse = _lib.ops().attention_packed(q, k, v, plan.q_items, plan.k_items, plan.info, scale,
+                                               return_lse)
+    except (RuntimeError, NotImplementedError):
+        _check(q, k, v, plan)
+        raise
     return (out, lse) if return_lse else out
 
 
@@ -116,12 +117,16 @@ def attention_packed_backward(dout, q, k, v, out, lse, plan: PackedPlan, *,
                               softmax_scale: float | None = None):
     """``(dq, dk, dv)`` of :func:`attention_packed` from its inputs, ``out`` and ``lse``, without
     autograd."""
-    ops = _lib.ops()
-    _check(q, k, v, plan)
-    if dout.shape != q.shape or out.shape != q.shape or tuple(lse.shape) != (q.shape[1], q.shape[0]):
-        raise ValueError("dout and out must have q's shape, lse [heads, tokens]")
-    return ops.attention_packed_bwd(dout, _unit(q), _unit(k), _unit(v), _unit(out), lse,
-                                    plan.q_items, plan.k_items, plan.tiles, _scale(softmax_scale))
+    scale = _scale(softmax_scale)
+    try:
+        return _lib.ops().attention_packed_bwd(dout, q, k, v, out, lse, plan.q_items, plan.k_items,
+                                               plan.info, scale)
+    except (RuntimeError, NotImplementedError):
+        _check(q, k, v, plan)
+        if (dout.shape != q.shape or out.shape != q.shape
+                or tuple(lse.shape) != (q.shape[1], q.shape[0])):
+            raise ValueError("dout and out must have q's shape, lse [heads, tokens]") from None
+        raise
 
 
 def attention_decode(q, k_cache, v_cache, lens, *, softmax_scale: float | None = None,
@@ -132,7 +137,19 @@ def attention_decode(q, k_cache, v_cache, lens, *, softmax_scale: float | None =
     is read there (no host sync; limited to ``[0, capacity]``); rows behind a length may hold
     anything. A sequence of no keys gives 0. ``num_splits`` 1: one workgroup per sequence and kv head; n: the whole batch's
     keys cut into ``n * batch`` equal pieces that run side by side; 0: by batch, heads and capacity."""
-    ops = _lib.ops()
+    s = _scale(softmax_scale)
+    try:
+        ops = _lib.ops()
+        if out is None:
+            return ops.attention_decode(q, k_cache, v_cache, lens, s, num_splits)
+        ops.attention_decode_out(q, k_cache, v_cache, lens, s, num_splits, out)
+        return out
+    except (RuntimeError, NotImplementedError):
+        _check_decode(q, k_cache, v_cache, lens, num_splits, out)
+        raise
+
+
+def _check_decode(q, k_cache, v_cache, lens, num_splits, out):
     if q.dim() != 3 or q.dtype != torch.bfloat16 or q.shape[2] != HEAD_DIM:
         raise ValueError(f"q must be bf16 [batch, heads, {HEAD_DIM}], got {tuple(q.shape)} {q.dtype}")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
@@ -146,10 +163,5 @@ def attention_decode(q, k_cache, v_cache, lens, *, softmax_scale: float | None =
         raise ValueError(f"lens must be int32 [{q.shape[0]}], got {tuple(lens.shape)} {lens.dtype}")
     if not 0 <= num_splits <= 128:
         raise ValueError(f"num_splits {num_splits} not in [0, 128]")
-    s = _scale(softmax_scale)
-    if out is None:
-        return ops.attention_decode(_unit(q), k_cache, v_cache, lens, s, num_splits)
-    if out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1:
+    if out is not None and (out.shape != q.shape or out.dtype != torch.bfloat16 or out.stride(2) != 1):
         raise ValueError("out must be bf16 of q's shape with a contiguous head dim")
-    ops.attention_decode_out(_unit(q), k_cache, v_cache, lens, s, num_splits, out)
-    return out

@@ -179,6 +179,18 @@ def test_autograd_gives_the_explicit_gradients():
         assert not lbw_amd.attention_packed(*leaves, plan).requires_grad
 
 
+def test_head_dim_that_is_not_contiguous_is_copied():
+    import lbw_amd
+    ql = kl = [40, 9]
+    q, k, v, do = _data(ql, kl, 4, 2, 11)
+    want = _run(q, k, v, do, ql, kl, True)
+    leaves = [x.transpose(1, 2).contiguous().requires_grad_() for x in (q, k, v)]
+    out = lbw_amd.attention_packed(*[x.transpose(1, 2) for x in leaves], lbw_amd.packed_plan(ql))
+    assert torch.equal(out, want["out"])
+    for g, n in zip(torch.autograd.grad(out, leaves, do), ("dq", "dk", "dv")):
+        assert torch.equal(g.transpose(1, 2), want[n])
+
+
 def test_nothing_to_do():
     import lbw_amd
     q, k, v, do = _data([0], [5], 4, 2, 9)
@@ -191,14 +203,16 @@ def test_nothing_to_do():
 
 
 def test_a_plan_of_other_lengths_stays_inside_the_tensors():
-    """The ops themselves cannot see whose table they get: its items are skipped, not followed."""
+    """An op cannot see whose table it gets: items that do not fit are skipped, not followed."""
     import lbw_amd
     big = lbw_amd.packed_plan([4000, 100])
     q, k, v, _ = _data([60], [60], 2, 1, 10)
-    out, _ = torch.ops.lbw.attention_packed(q, k, v, big.q_items, big.k_items, big.tiles, 0.0,
-                                             True)
+    info = (60, 60) + big.info[2:]
+    out, _ = torch.ops.lbw.attention_packed(q, k, v, big.q_items, big.k_items, info, 0.0, True)
     torch.cuda.synchronize()
     assert out.shape == q.shape
+    with pytest.raises(RuntimeError, match="the plan is for 4100"):
+        torch.ops.lbw.attention_packed(q, k, v, big.q_items, big.k_items, big.info, 0.0, True)
     with pytest.raises(ValueError, match="the plan"):
         lbw_amd.attention_packed(q, k, v, big)
     with pytest.raises(ValueError, match="plan is on"):

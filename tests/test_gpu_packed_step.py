@@ -221,7 +221,7 @@ def test_traces_under_fake_tensors():
     with FakeTensorMode(allow_non_fake_inputs=True):
         q = torch.empty(16, HQ, D, dtype=BF, device="cuda")
         k = torch.empty(16, HK, D, dtype=BF, device="cuda")
-        out, lse = torch.ops.lbw.attention_packed(q, k, k, plan.q_items, plan.k_items, plan.tiles,
+        out, lse = torch.ops.lbw.attention_packed(q, k, k, plan.q_items, plan.k_items, plan.info,
                                                   0.0, True)
         assert out.shape == q.shape and lse.shape == (HQ, 16)
         kc = torch.empty(16, 30, HK, D, dtype=BF, device="cuda")

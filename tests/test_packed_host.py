@@ -51,7 +51,7 @@ def test_plan_covers_every_row_once_and_bounds_what_is_seen(ql, kl, causal):
     assert cost == sorted(cost, reverse=True)
     qt = [-(-x // 64) for x in cost]
     kt = [-(-x[4] // 64) - x[5] // 64 if x[5] < x[4] else 0 for x in p.k_items.tolist()]
-    assert p.tiles == (sum(qt), max(qt, default=0), sum(kt), max(kt, default=0))
+    assert p.info == (sum(ql), sum(kl), sum(qt), max(qt, default=0), sum(kt), max(kt, default=0))
 
 
 def test_plan_refusals():
