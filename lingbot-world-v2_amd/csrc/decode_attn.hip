@@ -4,10 +4,10 @@
 //   h / (Hq / Hk); a sequence of no keys gives 0.
 //
 // Bound by reading K and V once. A workgroup works for one key/value head: its query heads, up to 32,
-// are the columns of S^T = K Q^T, so K and V are read once for the whole group. Its 4 waves take 32-key
+// are the columns of S^T = K Q^T, so K and V are read once for the whole group. Its 4 or 8 waves take 32-key
 // tiles in turn, each through 16 KB of LDS of its own (a tile of K, one of V: the next tile's K is
 // fetched while this one's V is worked on, and the other way round), so no wave waits for another until a
-// sequence ends, where the four results are joined; two workgroups share a CU.
+// sequence ends, where their results are joined; two workgroups of 4 share a CU.
 //
 // Either a workgroup has one whole sequence, or (few sequences, long caches) the keys of the whole batch,
 // laid end to end, are cut into equal pieces, as many as workgroups run at once: lengths are known on the
@@ -16,16 +16,15 @@
 
 #include <algorithm>
 
+#include "capi_util.h"
 #include "packed_tiles.h"
 
 namespace lbw {
 namespace {
 
-constexpr int DW = 4;                       // waves per workgroup
 constexpr int DT = 32;                      // keys per tile
 constexpr int DT_B = DT * PK_ROWB;          // 8 KB
 constexpr int RING_B = 2 * DT_B;            // per wave: K, V
-constexpr int DEC_LDS = DW * RING_B;
 constexpr int NCOPY = DT_B / 1024;          // copies per lane for K or V of a tile
 constexpr int HEADS = 32;                   // query heads per workgroup
 
@@ -79,7 +78,9 @@ __device__ __forceinline__ int find_sequence(const DecodeArgs& a, int lane, int6
   return a.B;
 }
 
+template <int DW>  // waves per workgroup
 __global__ void __launch_bounds__(DW * 64, 2) decode_kernel(const DecodeArgs a) {
+  constexpr int DEC_LDS = DW * RING_B;
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -341,15 +342,24 @@ int decode_pieces(int64_t B, int Hq, int Hk, int64_t S, int num_splits, int cus)
   return (int)std::max<int64_t>(1, std::min(most, tiles / 8));
 }
 
-hipError_t launch_decode(const DecodeArgs& a, hipStream_t stream) {
-  constexpr int bytes = DEC_LDS + 2 * DW * HEADS * 4;
-  static hipError_t attr = hipFuncSetAttribute((const void*)decode_kernel,
+template <int DW>
+static hipError_t run(const DecodeArgs& a, hipStream_t stream) {
+  constexpr int bytes = DW * RING_B + 2 * DW * HEADS * 4;
+  static hipError_t attr = hipFuncSetAttribute((const void*)decode_kernel<DW>,
                                                hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (attr != hipSuccess) return attr;
   const int group = a.Hq / a.Hk, blocks = (group + HEADS - 1) / HEADS;
   const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B) * blocks * a.Hk;
-  hipLaunchKernelGGL(decode_kernel, dim3((uint32_t)n), dim3(DW * 64), bytes, stream, a);
-  const hipError_t e = hipGetLastError();
+  hipLaunchKernelGGL(decode_kernel<DW>, dim3((uint32_t)n), dim3(DW * 64), bytes, stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_decode(const DecodeArgs& a, hipStream_t stream) {
+  const int group = a.Hq / a.Hk, blocks = (group + HEADS - 1) / HEADS;
+  // whole sequences that leave every CU one workgroup at most: eight waves in it (one sequence of 500 keys
+  // x 40/8 heads 8.0 / 7.4 us with four / eight, of 1000 12.1 / 9.8; 64 of 500, two workgroups a CU, 28 / 31)
+  if (a.pieces == 0 && (int64_t)a.B * blocks * a.Hk <= num_cus()) return run<8>(a, stream);
+  const hipError_t e = run<4>(a, stream);
   if (e != hipSuccess || a.pieces == 0) return e;
   const int64_t rows = (int64_t)a.B * a.Hq;
   hipLaunchKernelGGL(decode_join_kernel, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, stream, a);
