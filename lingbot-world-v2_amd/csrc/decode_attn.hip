@@ -345,8 +345,8 @@ int decode_pieces(int64_t B, int Hq, int Hk, int64_t S, int num_splits, int cus)
 template <int DW>
 static hipError_t run(const DecodeArgs& a, hipStream_t stream) {
   constexpr int bytes = DW * RING_B + 2 * DW * HEADS * 4;
-  static hipError_t attr = hipFuncSetAttribute((const void*)decode_kernel<DW>,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static LdsAllowed allowed;
+  const hipError_t attr = allow_lds((const void*)decode_kernel<DW>, bytes, allowed);
   if (attr != hipSuccess) return attr;
   const int group = a.Hq / a.Hk, blocks = (group + HEADS - 1) / HEADS;
   const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B) * blocks * a.Hk;

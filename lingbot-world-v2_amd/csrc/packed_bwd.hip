@@ -9,6 +9,7 @@
 // walks the queries of all heads of its group: dK and dV (four products a tile).
 // Both recompute S; P and dS go to bf16 as operands, one rounding each.
 
+#include "capi_util.h"
 #include "packed_tiles.h"
 
 namespace lbw {
@@ -452,8 +453,8 @@ __global__ void __launch_bounds__(PK_WAVES * 64) packed_dkv_join_kernel(const Pa
 }  // namespace
 
 hipError_t launch_packed_dq(const PackedArgs& a, hipStream_t stream) {
-  static hipError_t attr = hipFuncSetAttribute((const void*)packed_dq_kernel,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, BWD_LDS);
+  static LdsAllowed allowed;
+  const hipError_t attr = allow_lds((const void*)packed_dq_kernel, BWD_LDS, allowed);
   if (attr != hipSuccess) return attr;
   const uint32_t n = ((uint32_t)a.n_q_items + (uint32_t)a.n_split * (a.smax - 1)) * a.Hq;
   hipLaunchKernelGGL(packed_dq_kernel, dim3(n), dim3(PK_WAVES * 64), BWD_LDS, stream, a);
@@ -465,8 +466,8 @@ hipError_t launch_packed_dq(const PackedArgs& a, hipStream_t stream) {
 }
 
 hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream) {
-  static hipError_t attr = hipFuncSetAttribute((const void*)packed_dkv_kernel,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, DKV_LDS);
+  static LdsAllowed allowed;
+  const hipError_t attr = allow_lds((const void*)packed_dkv_kernel, DKV_LDS, allowed);
   if (attr != hipSuccess) return attr;
   const uint32_t n = ((uint32_t)a.n_k_items + (uint32_t)a.n_split * (a.smax - 1)) * a.Hk;
   hipLaunchKernelGGL(packed_dkv_kernel, dim3(n), dim3(GROUPS * PK_WAVES * 64), DKV_LDS, stream, a);

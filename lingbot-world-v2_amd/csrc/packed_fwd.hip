@@ -12,6 +12,7 @@
 // O += V_{j-1}^T P_{j-1}^T and S_{j+1} = K_{j+1} Q^T. Online softmax in base 2 against a reference
 // that moves only when a row's sum in a step outgrows it; O and l share it, so the result is exact.
 
+#include "capi_util.h"
 #include "packed_tiles.h"
 
 namespace lbw {
@@ -266,8 +267,8 @@ __global__ void __launch_bounds__(PK_WAVES * 64) packed_fwd_join_kernel(const Pa
 }  // namespace
 
 hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t stream) {
-  static hipError_t attr = hipFuncSetAttribute((const void*)packed_fwd_kernel,
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, FWD_LDS);
+  static LdsAllowed allowed;
+  const hipError_t attr = allow_lds((const void*)packed_fwd_kernel, FWD_LDS, allowed);
   if (attr != hipSuccess) return attr;
   const uint32_t n = ((uint32_t)a.n_q_items + (uint32_t)a.n_split * (a.smax - 1)) * a.Hq;
   hipLaunchKernelGGL(packed_fwd_kernel, dim3(n), dim3(PK_WAVES * 64), FWD_LDS, stream, a);

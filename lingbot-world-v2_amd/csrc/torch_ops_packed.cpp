@@ -49,15 +49,36 @@ void check_int32(const char* name, const Tensor& t, const Tensor& like) {
               " must be int32 on q's device");
 }
 
-// An output that the caller gives: no two of its elements in one place, and apart from `others`
-// (or exactly one of them).
-void check_written(const char* name, const Tensor& out, std::initializer_list<const Tensor*> others) {
+// Whether two row tensors [n, heads, D] may share memory: by their address ranges, or, as column blocks of one
+// buffer with the same row stride, by their columns.
+bool may_overlap(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  auto span = [](const Tensor& t, int64_t from) {  // elements from the first to past the last, dims `from` on
+    int64_t n = 1;
+    for (int64_t d = from; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+    return n;
+  };
+  const int64_t pa = reinterpret_cast<intptr_t>(a.data_ptr()), pb = reinterpret_cast<intptr_t>(b.data_ptr());
+  if (pa + 2 * span(a, 0) <= pb || pb + 2 * span(b, 0) <= pa) return false;
+  const int64_t s = a.stride(0);
+  if (a.dim() != b.dim() || s != b.stride(0) || s <= 0) return true;
+  const int64_t wa = span(a, 1), wb = span(b, 1);
+  if (wa > s || wb > s || (pb - pa) % 2 != 0) return true;
+  int64_t d = (pb - pa) / 2 % s;  // b's first column from a's on
+  if (d < 0) d += s;
+  return !(d >= wa && d + wb <= s);
+}
+
+// An output that the caller gives: no two of its elements in one place, and apart from `others`, or exactly its
+// own input.
+void check_written(const char* name, const Tensor& out, const Tensor* own,
+                   std::initializer_list<const Tensor*> others) {
   TORCH_CHECK(at::has_internal_overlap(out) != at::MemOverlap::Yes, name,
               " has several elements in one place");
   for (const Tensor* t : others) {
     if (t == nullptr || !t->defined()) continue;
-    const auto s = at::get_overlap_status(out, *t);
-    TORCH_CHECK(s != at::MemOverlapStatus::Partial, name, " overlaps an input in part");
+    if (t == own && t->data_ptr() == out.data_ptr() && t->strides() == out.strides()) continue;
+    TORCH_CHECK(!may_overlap(out, *t), name, " overlaps another tensor of the call");
   }
 }
 
@@ -192,19 +213,9 @@ void head_norm_rope_(const Tensor& q, const Tensor& k, const OptT& wq, const Opt
     p.k_out_stride_b = k_out.stride(0);
     p.v_out_stride_b = v.has_value() ? vo.stride(0) : 0;
   }
-  check_written("q_out", q_out, {&q, &k, &vv});
-  check_written("k_out", k_out, {&q, &k, &vv});
-  TORCH_CHECK(at::get_overlap_status(q_out, k_out) != at::MemOverlapStatus::Full &&
-                  at::get_overlap_status(q_out, k_out) != at::MemOverlapStatus::Partial,
-              "q_out and k_out overlap");
-  if (v.has_value()) {
-    check_written("v_out", vo, {&q, &k, &vv});
-    for (const Tensor* t : {&q_out, &k_out}) {
-      const auto s = at::get_overlap_status(vo, *t);
-      TORCH_CHECK(s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial,
-                  "v_out overlaps another output");
-    }
-  }
+  check_written("q_out", q_out, &q, {&q, &k, &vv, &k_out, &vo});
+  check_written("k_out", k_out, &k, {&q, &k, &vv, &vo});
+  if (v.has_value()) check_written("v_out", vo, &vv, {&q, &k, &vv});
   check(lbw_head_norm_rope(&p, stream_of(q)), "lbw_head_norm_rope");
 }
 
@@ -383,10 +394,7 @@ void attention_decode_out(const Tensor& q, const Tensor& k, const Tensor& v, con
               "lens must be a contiguous int32 [batch] vector");
   TORCH_CHECK(q.size(0) < (int64_t(1) << 31) && q.size(1) < (1 << 30), "batch or heads too large");
   TORCH_CHECK(num_splits >= 0 && num_splits <= 128, "num_splits ", num_splits, " not in [0, 128]");
-  check_written("out", out, {&k, &v});
-  TORCH_CHECK(at::get_overlap_status(out, q) != at::MemOverlapStatus::Full &&
-                  at::get_overlap_status(out, q) != at::MemOverlapStatus::Partial,
-              "out overlaps q");
+  check_written("out", out, nullptr, {&q, &k, &v});
   lbw_decode_params p;
   std::memset(&p, 0, sizeof(p));
   p.batch = (int32_t)q.size(0);

@@ -158,6 +158,47 @@ def test_write_form_in_place_and_strided():
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, v0)
 
 
+def test_outputs_that_share_memory_with_other_tensors_are_refused():
+    import lbw_amd
+    T, h, d = 6, 2, 64
+    _, rope = _rope((32,), 8, True)
+    pos = torch.zeros(T, dtype=torch.int32, device="cuda")
+    buf = torch.zeros(T, 3 * h, d, dtype=BF, device="cuda")
+    q, k, v = buf.split([h, h, h], 1)
+    go = lambda q_, k_, qo, ko, **kw: lbw_amd.qk_head_norm_rope_(  # noqa: E731
+        q_, k_, None, None, rope, pos, q_out=qo, k_out=ko, **kw)
+    new = lambda: torch.zeros(T, h, d, dtype=BF, device="cuda")  # noqa: E731
+    go(q, k, q, k)                              # in place, column blocks of one buffer
+    go(q, k, new(), v)                          # k's result into v's columns (v is not read)
+    for bad in (lambda: go(q, q, q, new()),     # q's result over k, which other waves still read
+                lambda: go(q, k, k, new()), lambda: go(q, k, new(), q), lambda: go(q, k, v, v),
+                lambda: go(q, k, buf[:, 1:3], new()), lambda: go(q, k, new(), new(), v=v, v_out=q),
+                lambda: go(q, k, q, k, v=v, v_out=k)):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            bad()
+    cache = torch.zeros(T, 9, h, d, dtype=BF, device="cuda")
+    rows = torch.zeros(T, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="overlaps"):
+        go(q, k, new(), cache, v=v, v_out=cache, rows=rows)
+    with pytest.raises(RuntimeError, match="one place"):
+        go(q, k, new(), cache[:1].expand(T, 9, h, d), rows=rows)
+
+
+def test_more_than_2_31_elements():
+    import lbw_amd
+    T, hq, d = 270000, 63, 128
+    q = torch.zeros(T, hq, d, dtype=BF, device="cuda")
+    assert q.numel() > 1 << 31
+    q[-3:] = torch.randn(3, hq, d, device="cuda").to(BF)
+    k = torch.zeros(T, 1, d, dtype=BF, device="cuda")
+    ang, rope = _rope((64,), 50, True)
+    pos = torch.full((T,), 7, dtype=torch.int32, device="cuda")
+    q2, _ = lbw_amd.qk_head_norm_rope(q, k, None, None, rope, pos)
+    want = R.head_norm(q[-3:].double(), None, R.token_angles(ang, (64,), pos[-3:]), True, 1e-6, 1.0)
+    R.assert_within("q'", q2[-3:], want, R.head_norm_allow(want))
+    assert torch.all(q2[:-3] == 0)
+
+
 def test_refusals_on_the_device():
     import lbw_amd
     q, k, v, w = _data(8, 4, 2, 128, 11)

@@ -191,6 +191,24 @@ def test_head_dim_that_is_not_contiguous_is_copied():
         assert torch.equal(g.transpose(1, 2), want[n])
 
 
+def test_more_than_2_31_elements():
+    """Many sequences whose packed rows pass 2^31 elements of q: the last one against the definition."""
+    import lbw_amd
+    lens, hq = [90] * 3000, 63
+    n = sum(lens)
+    q = torch.empty(n, hq, 128, dtype=BF, device="cuda").normal_()
+    assert q.numel() > 1 << 31
+    k, v = torch.randn(n, 1, 128, device="cuda").to(BF), torch.randn(n, 1, 128, device="cuda").to(BF)
+    plan = lbw_amd.packed_plan(lens)
+    out, lse = lbw_amd.attention_packed(q, k, v, plan, return_lse=True)
+    dq, dk, dv = lbw_amd.attention_packed_backward(out, q, k, v, out, lse, plan)  # (dout = out)
+    s = slice(n - 90, n)
+    r = R.attention(q[s], k[s], v[s], [90], [90], True, SCALE, out[s])
+    R.assert_within("out", out[s], r["out"], r["out_a"])
+    for name, x in (("dq", dq), ("dk", dk), ("dv", dv)):
+        R.assert_within(name, x[s], r[name], r[name + "_a"])
+
+
 def test_nothing_to_do():
     import lbw_amd
     q, k, v, do = _data([0], [5], 4, 2, 9)
