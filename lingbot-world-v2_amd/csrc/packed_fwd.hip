@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
   zero(sB);
   u32x4 pA[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
   u32x4 pB[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
-  constexpr int R = AHEAD + 2;  // fragments of pair i in slot i % R (8 % R == 0)
+  constexpr int R = AHEAD + 1;  // fragments of pair i in slot i % R
   u32x4 kf[R], vf[R];
   auto load_k = [&](auto ko, int i) { kf[i % R] = read_row(ka, i, decltype(ko)::value); };
   auto load_v = [&](auto vo, int i) { vf[i % R] = read_tr(va, i >> 1, i & 1, decltype(vo)::value); };
@@ -137,6 +137,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
     }
     float mc = -m * c;
     zero(s_out);
+    float ls = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (i + AHEAD < 8) {
@@ -144,31 +145,13 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
         load_v(vo, i + AHEAD);
       }
       s_out = mfma32x32x16(kf[i % R], qf[i], s_out);
+      const float x0 = fast_exp2(__builtin_fmaf(s_in[2 * i], c, mc));
+      const float x1 = fast_exp2(__builtin_fmaf(s_in[2 * i + 1], c, mc));
       o[i >> 1] = mfma32x32x16(vf[i % R], p_in[i & 1], o[i >> 1]);
-    }
-    auto exps = [&]() {
-      float ls = 0.0f;
-#pragma unroll
-      for (int mm = 0; mm < 2; ++mm)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x0 = fast_exp2(__builtin_fmaf(s_in[8 * mm + 2 * e], c, mc));
-          const float x1 = fast_exp2(__builtin_fmaf(s_in[8 * mm + 2 * e + 1], c, mc));
-          p_out[mm][e] = pack_bf16x2(x0, x1);
-          ls += x0 + x1;
-        }
-      return ls;
-    };
-    float ls = exps();
-    // the step's order: the first fragments, then MFMA, 2 VALU, fragments AHEAD pairs on, MFMA, 2 VALU
-    __builtin_amdgcn_sched_group_barrier(0x100, 3 * AHEAD, 0);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
-      if (i + AHEAD < 8) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      p_out[i >> 2][i & 3] = pack_bf16x2(x0, x1);  // registers 2 i, 2 i + 1: word i of the operand
+      ls += x0 + x1;
+      // (two products and two exponentials a pair, in this order)
+      __builtin_amdgcn_sched_barrier(0);
     }
     asm volatile("" ::"v"(p_out[0]), "v"(p_out[1]), "v"(ls));
     // a sum past the limit (or not finite): some p outgrew the reference. Move it to the row's max
@@ -184,7 +167,14 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
       mc = -mn * c;
       scale_acc(o, alpha);
       l *= alpha;
-      ls = exps();
+      ls = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x0 = fast_exp2(__builtin_fmaf(s_in[2 * i], c, mc));
+        const float x1 = fast_exp2(__builtin_fmaf(s_in[2 * i + 1], c, mc));
+        p_out[i >> 2][i & 3] = pack_bf16x2(x0, x1);
+        ls += x0 + x1;
+      }
     }
     l += ls;
     asm volatile("" ::"v"(p_out[0]), "v"(p_out[1]), "v"(l));
