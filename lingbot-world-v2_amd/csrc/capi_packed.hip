@@ -180,10 +180,20 @@ PackedSplit split_items(int64_t items, int64_t heads, int64_t tiles, int64_t lon
 PackedSplit split_q(const lbw_packed_params* p) {
   return split_items(p->n_q_items, p->q_heads, p->q_tiles, p->q_tiles_max, 2 * num_cus(), 16, 4);
 }
-// dK and dV: one workgroup per CU, an item's tiles those of all heads of the group
+// dK and dV: one workgroup per CU, an item's tiles those of all heads of the group. Where items leave CUs idle
+// even at two workgroups each (halves_k), a tile takes half the time and a piece's cost twice as many:
+// least 24 / 48: causal 1024 x 40/8 112 / 97 us, 2048 x 8/1 171 / 135, 800 + 900 + 650 x 12/4 88 / 74.
 PackedSplit split_k(const lbw_packed_params* p) {
   const int64_t group = p->q_heads / p->k_heads;
-  return split_items(p->n_k_items, p->k_heads, p->k_tiles * group, p->k_tiles_max * group, num_cus(), 24, 3);
+  const int64_t least = 2 * (int64_t)p->n_k_items * p->k_heads <= num_cus() ? 48 : 24;
+  return split_items(p->n_k_items, p->k_heads, p->k_tiles * group, p->k_tiles_max * group, num_cus(), least, 3);
+}
+// Two workgroups for an item's (or a piece's) keys where that many run at once and have more than four tiles.
+// Gradient, one / two: 311 + 97 + 512 + 5 x 12/4 62 / 49 us, 1024 x 16 59 / 52, 16 x 256 x 12/4 (128 items,
+// 256 CUs) 53 / 48, but 5 x 60 x 12 (one tile) 18.6 / 20.2.
+bool halves_k(const lbw_packed_params* p, const PackedSplit& s) {
+  return 2 * (p->n_k_items + (int64_t)s.n_split * (s.smax - 1)) * p->k_heads <= num_cus() &&
+         p->k_tiles_max * (p->q_heads / p->k_heads) > 4;
 }
 size_t part_bytes(const PackedSplit& s, int heads, int floats) {
   return (size_t)s.n_split * heads * s.smax * floats * sizeof(float);
@@ -437,7 +447,9 @@ int lbw_attention_packed_bwd(const lbw_packed_params* p, const lbw_packed_grads*
     if (e != hipSuccess) return hip_fail(e, "packed attention dQ launch");
   }
   if (a.n_k_items > 0) {
-    set_split(&a, split_k(p), part);
+    const PackedSplit s = split_k(p);
+    set_split(&a, s, part);
+    a.halves = halves_k(p, s);
     const hipError_t e = launch_packed_dkv(a, static_cast<hipStream_t>(stream));
     if (e != hipSuccess) return hip_fail(e, "packed attention dK/dV launch");
   }

@@ -73,6 +73,7 @@ struct PackedArgs {
   int n_split, smax, piece;
   float* part;
   // gradient
+  bool halves;                 // dK, dV: 64 keys per workgroup
   Rows o, dout;
   float* ndelta;               // [Hq][Tq]: -sum_d dout out
   float* nlse;                 // [Hq][Tq]: -lse / scale, -inf for a query that sees no key

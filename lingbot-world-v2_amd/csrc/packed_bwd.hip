@@ -248,13 +248,16 @@ __device__ __forceinline__ int lane_now() {
 constexpr int GROUPS = 2;  // wave groups of a workgroup, each with its share of an item's query tiles
 constexpr int FRAG_AT = GROUPS * DKV_GROUP_B;    // each wave's last fragment of K and of V: 2 KB
 constexpr int DKV_LDS = FRAG_AT + GROUPS * PK_WAVES * 2048;
+// Where there are few items a workgroup takes HALF of one, 64 keys: two waves of a group share a block of 32
+// keys, each with every second block of 32 queries (12 tiles of 3 heads 43 to 30 us).
+template <bool HALF>
 __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(const PackedArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63;
   const int wave_id = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = wave_id % PK_WAVES, grp = wave_id / PK_WAVES;
   const int hl = lane >> 5, l32 = lane & 31;
-  const PackedShare sh = pick_share(a, blockIdx.x, a.Hk);
+  const PackedShare sh = pick_share(a, HALF ? blockIdx.x >> 1 : blockIdx.x, a.Hk);
   const int kv = sh.head, group = a.Hq / a.Hk;
   const PackedItem it = load_item(a.k_items, sh.item);
   if (!item_fits(it, a.Tk, a.Tq)) return;
@@ -267,7 +270,9 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
   const int mine = (int)((int64_t)all * (sh.piece + 1) / pieces) - p0;
   const int n0 = p0 + mine * grp / GROUPS, T = p0 + mine * (grp + 1) / GROUPS;
   const int Tmax = n0 + (mine + GROUPS - 1) / GROUPS;  // the loop's end, the same count in both groups
-  const int r0 = 32 * wave, rows = it.rows - r0;
+  const int part0 = HALF ? 64 * (int)(blockIdx.x & 1) : 0;
+  if (HALF && it.rows <= part0) return;
+  const int r0 = part0 + 32 * (HALF ? wave & 1 : wave), rows = it.rows - r0;
   const bool active = rows > 0;
 
   u32x4 kf[8], vf[8];
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
     ct = ct + 1 == t_end ? t_first : ct + 1;
     if (!active || n >= T || row0 + BN <= lo_min) continue;
 #pragma unroll 1
-    for (int qb = 0; qb < 2; ++qb) {
+    for (int qb = HALF ? wave >> 1 : 0; qb < (HALF ? (wave >> 1) + 1 : 2); ++qb) {
       // (each product's fragment addresses are taken anew: kept for two of them, they spill others)
       const int ra = opaque(ra0 + st + qb * 32 * PK_ROWB);
       const int sa = lds0 + STAT_AT + (n & 1) * 2 * BN * 4 + 128 * qb + 16 * (lane_now() >> 5);
@@ -412,42 +417,51 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
   __builtin_amdgcn_s_waitcnt(0x0070);
   barrier_nofence();
   {
-    // group 1 hands its sums over in register order, 16 bytes per lane: dK through its own LDS, dV
-    // through group 0's
-    unsigned char* g1 = lds + DKV_GROUP_B + 16384 * wave;
-    unsigned char* g0 = lds + 16384 * wave;
+    // Group 1 hands its sums over in register order, 16 bytes per lane: dK through its own LDS, dV
+    // through group 0's. Then, where two waves share keys, the second of group 0 does.
+    unsigned char* const g1 = lds + DKV_GROUP_B;
     const int ln = lane_now();
-    if (grp == 1) {
+    auto give = [&]() {
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
         const floatx16 &y = dk[x >> 2], &z = dv[x >> 2];
-        const int e = 4 * (x & 3);
-        *reinterpret_cast<floatx4*>(g1 + 1024 * x + 16 * ln) = floatx4{y[e], y[e + 1], y[e + 2], y[e + 3]};
-        *reinterpret_cast<floatx4*>(g0 + 1024 * x + 16 * ln) = floatx4{z[e], z[e + 1], z[e + 2], z[e + 3]};
+        const int e = 4 * (x & 3), at = 16384 * wave + 1024 * x + 16 * ln;
+        *reinterpret_cast<floatx4*>(g1 + at) = floatx4{y[e], y[e + 1], y[e + 2], y[e + 3]};
+        *reinterpret_cast<floatx4*>(lds + at) = floatx4{z[e], z[e + 1], z[e + 2], z[e + 3]};
       }
-    }
-    __syncthreads();
-    if (grp == 0) {
+    };
+    auto take = [&](int from) {
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        const floatx4 y = *reinterpret_cast<const floatx4*>(g1 + 1024 * x + 16 * ln);
-        const floatx4 z = *reinterpret_cast<const floatx4*>(g0 + 1024 * x + 16 * ln);
+        const int at = 16384 * from + 1024 * x + 16 * ln;
+        const floatx4 y = *reinterpret_cast<const floatx4*>(g1 + at);
+        const floatx4 z = *reinterpret_cast<const floatx4*>(lds + at);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           dk[x >> 2][4 * (x & 3) + e] += y[e];
           dv[x >> 2][4 * (x & 3) + e] += z[e];
         }
       }
+    };
+    if (grp == 1) give();
+    __syncthreads();
+    if (grp == 0) take(wave);
+    __syncthreads();  // the sums are read: the LDS is free again
+    if constexpr (HALF) {
+      if (grp == 0 && wave >= 2) give();
+      __syncthreads();
+      if (grp == 0 && wave < 2) take(wave + 2);
+      __syncthreads();
+      if (wave >= 2) return;
     }
-    __syncthreads();  // the sums are read: the LDS is free for staging
     if (grp == 1) return;
   }
   if (!active) return;
   if (pieces > 1) {
-    const int ln1 = lane_now();
+    const int ln1 = lane_now(), slot = part0 / 32 + wave;
     float* const part = part_of(a, sh, a.Hk, sh.piece, PK_PART_DKV);
-    store_acc(part, wave, ln1, dk);
-    store_acc(part + PK_BLOCK * 128, wave, ln1, dv);
+    store_acc(part, slot, ln1, dk);
+    store_acc(part + PK_BLOCK * 128, slot, ln1, dv);
     return;
   }
   const int ln = lane_now();
@@ -500,13 +514,20 @@ hipError_t launch_packed_dq(const PackedArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream) {
+namespace {
+template <bool HALF>
+hipError_t run_dkv(const PackedArgs& a, uint32_t n, hipStream_t stream) {
   static LdsAllowed allowed;
-  const hipError_t attr = allow_lds((const void*)packed_dkv_kernel, DKV_LDS, allowed);
+  const hipError_t attr = allow_lds((const void*)packed_dkv_kernel<HALF>, DKV_LDS, allowed);
   if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL(packed_dkv_kernel<HALF>, dim3(n), dim3(GROUPS * PK_WAVES * 64), DKV_LDS, stream, a);
+  return hipGetLastError();
+}
+}  // namespace
+
+hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream) {
   const uint32_t n = ((uint32_t)a.n_k_items + (uint32_t)a.n_split * (a.smax - 1)) * a.Hk;
-  hipLaunchKernelGGL(packed_dkv_kernel, dim3(n), dim3(GROUPS * PK_WAVES * 64), DKV_LDS, stream, a);
-  const hipError_t e = hipGetLastError();
+  const hipError_t e = a.halves ? run_dkv<true>(a, 2 * n, stream) : run_dkv<false>(a, n, stream);
   if (e != hipSuccess || a.n_split == 0) return e;
   hipLaunchKernelGGL(packed_dkv_join_kernel, dim3((uint32_t)a.n_split * a.Hk), dim3(PK_WAVES * 64), 0,
                      stream, a);

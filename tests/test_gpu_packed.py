@@ -45,6 +45,8 @@ CASES = [  # q_lens, k_lens, heads, kv heads, causal
     # few rows over many keys, many queries over few keys: items cut into pieces (up to 16)
     ([16], [3000], 2, 1, True), ([5, 2, 130], [2500, 10, 700], 1, 1, False), ([2200], [70], 6, 1, False),
     ([1, 129], [9000, 129], 1, 1, True), ([5000, 40], [33, 40], 1, 1, True),
+    # few items of keys: 64 of them per workgroup, whole and in pieces; items of 64 and 65 keys
+    ([448, 65], None, 3, 1, True), ([449], [320], 4, 2, False), ([1300], None, 8, 1, True),
 ]
 
 
