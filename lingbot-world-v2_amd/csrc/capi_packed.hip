@@ -209,7 +209,7 @@ void set_split(PackedArgs* a, const PackedSplit& s, void* part) {
   a->piece = s.piece;
   a->part = static_cast<float*>(part);
 }
-// delta and -lse of the gradient, rounded up to 16 bytes
+// -delta and -lse / scale of the gradient, rounded up to 16 bytes
 size_t stat_bytes(const lbw_packed_params* p) {
   return (2 * (size_t)p->q_heads * (size_t)p->q_tokens * sizeof(float) + 15) / 16 * 16;
 }
@@ -408,7 +408,7 @@ int lbw_attention_packed_fwd(const lbw_packed_params* p, void* workspace, size_t
   return e == hipSuccess ? LBW_OK : hip_fail(e, "packed attention launch");
 }
 
-// delta and -lse, then the partial results of dQ and, after them, of dK and dV in the same place
+// -delta and -lse / scale, then the partial results of dQ and, after them, of dK and dV in the same place
 size_t lbw_attention_packed_bwd_workspace_size(const lbw_packed_params* p) {
   if (!sane(p)) return 0;
   return stat_bytes(p) + std::max(part_bytes(split_q(p), p->q_heads, PK_PART_DQ),

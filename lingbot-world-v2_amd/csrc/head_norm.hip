@@ -9,7 +9,9 @@
 // Bound by memory: forward reads and writes each value once, the gradient reads two values and
 // writes one. D / 8 lanes hold a head, 16 bytes each, so a wave covers 512 / D heads and the sums
 // over a head are shuffles among its lanes. A wave keeps one token: its angles are read once into
-// registers (cos and signed sin of the lane's eight values) and serve all its heads.
+// registers (cos and signed sin of the lane's eight values) and serve all its heads. 32759 tokens x 12 + 12
+// heads of 128: forward 66.7 us (6.0 TB/s), gradient 134.7 us (4.5 TB/s; a large copy reaches 4.9);
+// one token 4.8 us, most of it the launch.
 
 #include "common.h"
 #include "packed.h"

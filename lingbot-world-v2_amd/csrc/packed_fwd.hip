@@ -11,6 +11,13 @@
 // Software pipeline (per wave, 32-key blocks): the softmax of block j (VALU) runs beside the MFMAs of
 // O += V_{j-1}^T P_{j-1}^T and S_{j+1} = K_{j+1} Q^T. Online softmax in base 2 against a reference
 // that moves only when a row's sum in a step outgrows it; O and l share it, so the result is exact.
+//
+// P goes to bf16 as the second product's operand: one rounding of each weight, which l does not see.
+//
+// Bound by the matrix cores at the clock that the chip holds under them: 4680 + 3600 + 1561 causal tokens x
+// 40/8 heads 394 us, 970 TFLOP/s (a library product of 16384^3 reaches 1364); the MFMA pipes are busy 55 % of
+// the cycles at 1.65 GHz. Two workgroups a CU hide each other's barriers: one of eight waves, half the keys to
+// each four, in step, took 522 us where two of four waves took 437.
 
 #include "capi_util.h"
 #include "packed_tiles.h"

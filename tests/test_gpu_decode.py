@@ -26,6 +26,7 @@ CASES = [  # lens, capacity, heads, kv heads
     ([1], 1, 1, 1), ([0], 8, 2, 1), ([5], 8, 40, 8), ([500], 1024, 40, 8), ([31, 32, 33, 0, 64], 64, 12, 4),
     ([1000, 1, 129, 1023], 1024, 5, 1), ([2000, 3], 2048, 6, 3), ([700], 700, 3, 3), ([100, 90], 100, 66, 1),
     ([97], 128, 40, 1), ([4096], 5000, 2, 2), ([300] * 20, 301, 4, 2),
+    ([7, 0, 40] * 50, 64, 2, 1),
 ]
 
 
