@@ -166,6 +166,16 @@ PackedSplit split_items(int64_t items, int64_t heads, int64_t tiles, int64_t lon
                         int64_t least, int64_t times) {
   PackedSplit s = {0, 1, 1};
   if (tiles <= 0 || longest <= 0 || items <= 0) return s;
+  // Nearly equal items in up to five rounds, the last not full: as many are cut as would be in it, into pieces
+  // for all slots, of 32 tiles or more (shorter ones: no gain at 25 tiles, the emptier chip clocks higher).
+  // Forward, uncut / cut: 6144 full x 12/4 294 / 251 us, 1800 rows over 20000 keys x 40/8 873 / 752, 3600 over
+  // 46800 3730 / 3509; gradient of 4680 over 9360 3140 / 2886.
+  const int64_t units = items * heads, rest = units % slots;
+  if (4 * items * longest <= 5 * tiles && units >= slots && units < 5 * slots && rest > 0) {
+    const int64_t n = (rest + heads - 1) / heads;
+    const int64_t c = std::min<int64_t>(std::min<int64_t>(16, slots / (n * heads)), longest / 32);
+    if (c >= 2) return PackedSplit{(int)n, (int)c, (int)((longest + c - 1) / c)};
+  }
   const int64_t share = tiles * heads / slots;
   const int64_t piece = std::max<int64_t>(least, share < 256 ? share * 3 / 2 : share * 2 / 3);
   if (2 * longest < times * piece) return s;

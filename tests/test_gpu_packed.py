@@ -47,6 +47,8 @@ CASES = [  # q_lens, k_lens, heads, kv heads, causal
     ([1, 129], [9000, 129], 1, 1, True), ([5000, 40], [33, 40], 1, 1, True),
     # few items of keys: 64 of them per workgroup, whole and in pieces; items of 64 and 65 keys
     ([448, 65], None, 3, 1, True), ([449], [320], 4, 2, False), ([1300], None, 8, 1, True),
+    # equal items, more than run at once: those of the last round are cut
+    ([129, 300], [4100, 4200], 130, 130, True), ([4200], [385], 65, 65, False),
 ]
 
 
