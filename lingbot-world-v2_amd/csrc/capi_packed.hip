@@ -156,12 +156,12 @@ int fill_packed(const lbw_packed_params* p, PackedArgs* a) {
 
 // How a kernel's items are cut. `slots` workgroups run at once; an item much longer than a slot's share of
 // all tiles ends last. A piece costs its partial results' way to memory and back and a share of a
-// second launch, about 10 tiles of its time, so pieces are long: one and a half shares, `least` tiles
+// second launch, some tiles of its time, so pieces are long: one and a half shares, `least` tiles
 // at least (from 256 tiles a share on, where that cost is small beside an uncut item, two thirds of a share),
 // and nothing is cut that would give fewer than `times` / 2 pieces. Measured, uncut / cut: forward, 256 rows over
-// 4680 + 1816 + 3111 keys x 40/8 heads 83 / 71 us, 16 rows over 8192 keys 130 / 39, 5000 causal x 5/1
-// 90 / 62, but 2048 causal x 40/8 (32 tiles, 21 a share) 54 / 64; gradient of 2048 x 40/8 299 / 211, 4680 x 12/4
-// 446 / 334, 16384 x 16/2 4706 / 3690, but 8 x 512 x 40/8 (40 tiles, 25 a share) 131 / 185.
+// 4680 + 1816 + 3111 keys x 40/8 heads 83 / 70 us, 16 rows over 8192 keys 130 / 32, 5000 causal x 5/1
+// 90 / 62, but 2048 causal x 40/8 (32 tiles, 21 a share) 54 / 64; gradient of 2048 x 40/8 299 / 190, 4680 x 12/4
+// 446 / 295, 16384 x 16/2 4706 / 3690, but 8 x 512 x 40/8 (40 tiles, 25 a share) 131 / 185.
 PackedSplit split_items(int64_t items, int64_t heads, int64_t tiles, int64_t longest, int64_t slots,
                         int64_t least, int64_t times) {
   PackedSplit s = {0, 1, 1};
@@ -171,10 +171,11 @@ PackedSplit split_items(int64_t items, int64_t heads, int64_t tiles, int64_t lon
   // Forward, uncut / cut: 6144 full x 12/4 294 / 251 us, 1800 rows over 20000 keys x 40/8 873 / 752, 3600 over
   // 46800 3730 / 3509; gradient of 4680 over 9360 3140 / 2886.
   const int64_t units = items * heads, rest = units % slots;
-  if (4 * items * longest <= 5 * tiles && units >= slots && units < 5 * slots && rest > 0) {
+  if (tiles / items >= longest - longest / 5 && units >= slots && units < 5 * slots && rest > 0) {
     const int64_t n = (rest + heads - 1) / heads;
     const int64_t c = std::min<int64_t>(std::min<int64_t>(16, slots / (n * heads)), longest / 32);
-    if (c >= 2) return PackedSplit{(int)n, (int)c, (int)((longest + c - 1) / c)};
+    if (c >= 2)
+      return PackedSplit{(int)n, (int)c, (int)std::min<int64_t>((longest + c - 1) / c, 1 << 30)};
   }
   const int64_t share = tiles * heads / slots;
   const int64_t piece = std::max<int64_t>(least, share < 256 ? share * 3 / 2 : share * 2 / 3);
@@ -186,16 +187,20 @@ PackedSplit split_items(int64_t items, int64_t heads, int64_t tiles, int64_t lon
   s.n_split = (int)std::min<int64_t>(items, std::max<int64_t>(1, tiles / s.piece));
   return s;
 }
-// forward and dQ: two workgroups per CU
+// forward and dQ: two workgroups per CU. Fewer items, more idle CUs: shorter pieces (least 16 / this rule: forward,
+// 12 items 31.5 / 19.8 us, 48 31.6 / 21.5, 64 23.1 / 20.2, 120 31.4 / 27.4; of 8 / 16 with 312 38.2 / 36.6).
 PackedSplit split_q(const lbw_packed_params* p) {
-  return split_items(p->n_q_items, p->q_heads, p->q_tiles, p->q_tiles_max, 2 * num_cus(), 16, 4);
+  return split_items(p->n_q_items, p->q_heads, p->q_tiles, p->q_tiles_max, 2 * num_cus(),
+                     std::clamp<int64_t>(p->n_q_items * (int64_t)p->q_heads / 10, 8, 16), 4);
 }
 // dK and dV: one workgroup per CU, an item's tiles those of all heads of the group. Where items leave CUs idle
-// even at two workgroups each (halves_k), a tile takes half the time and a piece's cost twice as many:
-// least 24 / 48: causal 1024 x 40/8 112 / 97 us, 2048 x 8/1 171 / 135, 800 + 900 + 650 x 12/4 88 / 74.
+// even at two workgroups each (halves_k), a tile takes half the time and a piece costs twice as many, and pieces
+// that leave no room for two workgroups each lose that half; so pieces get longer with the items (least 24 / 32 /
+// 48, gradient: 16 items 57 / 66 / 89 us, 48 items 81 / 71 / 93, 64 items 90 / 97 / 88).
 PackedSplit split_k(const lbw_packed_params* p) {
   const int64_t group = p->q_heads / p->k_heads;
-  const int64_t least = 2 * (int64_t)p->n_k_items * p->k_heads <= num_cus() ? 48 : 24;
+  const int64_t units = (int64_t)p->n_k_items * p->k_heads;
+  const int64_t least = 2 * units <= num_cus() ? std::clamp<int64_t>(units * 3 / 4, 24, 48) : 24;
   return split_items(p->n_k_items, p->k_heads, p->k_tiles * group, p->k_tiles_max * group, num_cus(), least, 3);
 }
 // Two workgroups for an item's (or a piece's) keys where that many run at once and have more than four tiles.

@@ -224,23 +224,23 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_dq_kernel(const Packe
   });
 }
 
-// The pieces of a split query item added up, in their order.
-__global__ void __launch_bounds__(PK_WAVES * 64) packed_dq_join_kernel(const PackedArgs a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[PK_WAVES * 8192];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const PackedShare sh = {(int)(blockIdx.x / (uint32_t)a.Hq), (int)(blockIdx.x % (uint32_t)a.Hq), 0, true};
+// The pieces of a split query item added up, in their order: a workgroup for 32 rows, a wave for 32 columns.
+__global__ void __launch_bounds__(256) packed_dq_join_kernel(const PackedArgs a) {
+  const int lane = threadIdx.x & 63, db = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t unit = blockIdx.x / PK_WAVES, wave = blockIdx.x % PK_WAVES;
+  const PackedShare sh = {(int)(unit / (uint32_t)a.Hq), (int)(unit % (uint32_t)a.Hq), 0, true};
   int h, kv;
   pick_head(sh.head, a.Hk, a.Hq / a.Hk, h, kv);
   const PackedItem it = load_item(a.q_items, sh.item);
   if (!item_fits(it, a.Tq, a.Tk)) return;
-  const int pieces = pieces_of(a, sh, (it.bound + BN - 1) / BN), rows = it.rows - 32 * wave;
+  const int pieces = pieces_of(a, sh, (it.bound + BN - 1) / BN), rows = it.rows - 32 * (int)wave;
   if (pieces == 1 || rows <= 0) return;
-  floatx16 acc[4];
-#pragma unroll
-  for (int db = 0; db < 4; ++db) zero(acc[db]);
-  for (int s = 0; s < pieces; ++s) add_acc(part_of(a, sh, a.Hq, s, PK_PART_DQ), wave, lane, 1.0f, acc);
-  store_rows(lds + 8192 * wave, acc, a.scale, lane, rows, [&](int r) {
-    return a.dq.p + (int64_t)(it.row0 + 32 * wave + r) * a.dq.sl + h * a.dq.sh;
+  floatx16 acc;
+  zero(acc);
+#pragma unroll 4
+  for (int s = 0; s < pieces; ++s) add_block(part_of(a, sh, a.Hq, s, PK_PART_DQ), wave, db, lane, 1.0f, acc);
+  store_block(acc, a.scale, db, lane, rows, [&](int r) {
+    return a.dq.p + (int64_t)(it.row0 + 32 * (int)wave + r) * a.dq.sl + h * a.dq.sh;
   });
 }
 
@@ -480,29 +480,25 @@ __global__ void __launch_bounds__(GROUPS * PK_WAVES * 64, 1) packed_dkv_kernel(c
   });
 }
 
-// The pieces of a split key item added up, in their order.
-__global__ void __launch_bounds__(PK_WAVES * 64) packed_dkv_join_kernel(const PackedArgs a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[PK_WAVES * 8192];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const PackedShare sh = {(int)(blockIdx.x / (uint32_t)a.Hk), (int)(blockIdx.x % (uint32_t)a.Hk), 0, true};
+// The pieces of a split key item added up, in their order: a workgroup for 32 rows of dK or dV.
+__global__ void __launch_bounds__(256) packed_dkv_join_kernel(const PackedArgs a) {
+  const int lane = threadIdx.x & 63, db = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t unit = blockIdx.x / (2 * PK_WAVES), which = blockIdx.x / PK_WAVES % 2, wave = blockIdx.x % PK_WAVES;
+  const PackedShare sh = {(int)(unit / (uint32_t)a.Hk), (int)(unit % (uint32_t)a.Hk), 0, true};
   const PackedItem it = load_item(a.k_items, sh.item);
   if (!item_fits(it, a.Tk, a.Tq)) return;
   const int per = it.bound < it.other_len ? (it.other_len + BN - 1) / BN - it.bound / BN : 0;
-  const int pieces = pieces_of(a, sh, per * (a.Hq / a.Hk)), rows = it.rows - 32 * wave;
+  const int pieces = pieces_of(a, sh, per * (a.Hq / a.Hk)), rows = it.rows - 32 * (int)wave;
   if (pieces == 1 || rows <= 0) return;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    floatx16 acc[4];
-#pragma unroll
-    for (int db = 0; db < 4; ++db) zero(acc[db]);
-    for (int s = 0; s < pieces; ++s)
-      add_acc(part_of(a, sh, a.Hk, s, PK_PART_DKV) + which * PK_BLOCK * 128, wave, lane, 1.0f, acc);
-    const RowsOut out = which == 0 ? a.dk : a.dv;
-    store_rows(lds + 8192 * wave, acc, which == 0 ? a.scale : 1.0f, lane, rows, [&](int r) {
-      return out.p + (int64_t)(it.row0 + 32 * wave + r) * out.sl + sh.head * out.sh;
-    });
-    wave_lds_fence();
-  }
+  floatx16 acc;
+  zero(acc);
+#pragma unroll 4
+  for (int s = 0; s < pieces; ++s)
+    add_block(part_of(a, sh, a.Hk, s, PK_PART_DKV) + which * PK_BLOCK * 128, wave, db, lane, 1.0f, acc);
+  const RowsOut out = which == 0 ? a.dk : a.dv;
+  store_block(acc, which == 0 ? a.scale : 1.0f, db, lane, rows, [&](int r) {
+    return out.p + (int64_t)(it.row0 + 32 * (int)wave + r) * out.sl + sh.head * out.sh;
+  });
 }
 
 }  // namespace
@@ -515,7 +511,7 @@ hipError_t launch_packed_dq(const PackedArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(packed_dq_kernel, dim3(n), dim3(PK_WAVES * 64), BWD_LDS, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.n_split == 0) return e;
-  hipLaunchKernelGGL(packed_dq_join_kernel, dim3((uint32_t)a.n_split * a.Hq), dim3(PK_WAVES * 64), 0,
+  hipLaunchKernelGGL(packed_dq_join_kernel, dim3((uint32_t)a.n_split * a.Hq * PK_WAVES), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
 }
@@ -535,7 +531,7 @@ hipError_t launch_packed_dkv(const PackedArgs& a, hipStream_t stream) {
   const uint32_t n = ((uint32_t)a.n_k_items + (uint32_t)a.n_split * (a.smax - 1)) * a.Hk;
   const hipError_t e = a.halves ? run_dkv<true>(a, 2 * n, stream) : run_dkv<false>(a, n, stream);
   if (e != hipSuccess || a.n_split == 0) return e;
-  hipLaunchKernelGGL(packed_dkv_join_kernel, dim3((uint32_t)a.n_split * a.Hk), dim3(PK_WAVES * 64), 0,
+  hipLaunchKernelGGL(packed_dkv_join_kernel, dim3((uint32_t)a.n_split * a.Hk * 2 * PK_WAVES), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
 }

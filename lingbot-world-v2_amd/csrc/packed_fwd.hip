@@ -33,15 +33,11 @@ constexpr int AHEAD = 2;                         // MFMA pairs that LDS fragment
 template <int N>
 using ic = std::integral_constant<int, N>;
 
-// A wave's rows from O, the reference and the sum (of both lane halves) to out and lse.
-__device__ __forceinline__ void finish(const PackedArgs& a, const PackedItem& it, int h, int wave,
-                                       int lane, int rows, const floatx16 (&o)[4], float m, float l,
-                                       unsigned char* lds) {
-  const int64_t row0 = it.row0 + 32 * wave;
+// A wave's rows of lse from the reference and the sum (of both lane halves).
+__device__ __forceinline__ void store_lse(const PackedArgs& a, int h, int64_t row0, int lane, int rows, float m,
+                                          float l) {
   if (a.lse != nullptr && lane < 32 && lane < rows)
     a.lse[(int64_t)h * a.Tq + row0 + lane] = l > 0.0f ? m * a.scale + logf(l) : -INFINITY;
-  store_rows(lds + 8192 * wave, o, l > 0.0f ? 1.0f / l : 0.0f, lane, rows,
-             [&](int r) { return a.out.p + (row0 + r) * a.out.sl + h * a.out.sh; });
 }
 
 __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const PackedArgs a) {
@@ -229,36 +225,42 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
     }
     return;
   }
-  finish(a, it, h, wave, lane, rows, o, m, ls, lds);
+  const int64_t row0 = it.row0 + 32 * wave;
+  store_lse(a, h, row0, lane, rows, m, ls);
+  store_rows(lds + 8192 * wave, o, ls > 0.0f ? 1.0f / ls : 0.0f, lane, rows,
+             [&](int r) { return a.out.p + (row0 + r) * a.out.sl + h * a.out.sh; });
 }
 
-// The pieces of a split item joined, in their order.
-__global__ void __launch_bounds__(PK_WAVES * 64) packed_fwd_join_kernel(const PackedArgs a) {
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[PK_WAVES * 8192];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  PackedShare sh = {(int)(blockIdx.x / (uint32_t)a.Hq), (int)(blockIdx.x % (uint32_t)a.Hq), 0, true};
+// The pieces of a split item joined, in their order: a workgroup for 32 rows, a wave for 32 columns.
+__global__ void __launch_bounds__(256) packed_fwd_join_kernel(const PackedArgs a) {
+  const int lane = threadIdx.x & 63, db = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t unit = blockIdx.x / PK_WAVES, wave = blockIdx.x % PK_WAVES;
+  const PackedShare sh = {(int)(unit / (uint32_t)a.Hq), (int)(unit % (uint32_t)a.Hq), 0, true};
   int h, kv;
   pick_head(sh.head, a.Hk, a.Hq / a.Hk, h, kv);
   const PackedItem it = load_item(a.q_items, sh.item);
   if (!item_fits(it, a.Tq, a.Tk)) return;
   const int pieces = pieces_of(a, sh, (it.bound + BN - 1) / BN);
-  const int rows = it.rows - 32 * wave;
+  const int rows = it.rows - 32 * (int)wave;
   if (pieces == 1 || rows <= 0) return;
   const int row = 32 * wave + (lane & 31);
   float m = -INFINITY, l = 0.0f;
   for (int s = 0; s < pieces; ++s)
     m = fmaxf(m, part_of(a, sh, a.Hq, s, PK_PART_FWD)[PK_BLOCK * 128 + row]);
-  floatx16 o[4];
-#pragma unroll
-  for (int db = 0; db < 4; ++db) zero(o[db]);
+  floatx16 o;
+  zero(o);
+#pragma unroll 4
   for (int s = 0; s < pieces; ++s) {
     const float* part = part_of(a, sh, a.Hq, s, PK_PART_FWD);
     const float ms = part[PK_BLOCK * 128 + row];
     const float f = ms == -INFINITY ? 0.0f : fast_exp2((ms - m) * a.scale_log2);
     l += f * part[PK_BLOCK * 128 + PK_BLOCK + row];
-    add_acc(part, wave, lane, f, o);
+    add_block(part, wave, db, lane, f, o);
   }
-  finish(a, it, h, wave, lane, rows, o, m, l, lds);
+  const int64_t row0 = it.row0 + 32 * (int)wave;
+  if (db == 0) store_lse(a, h, row0, lane, rows, m, l);
+  store_block(o, l > 0.0f ? 1.0f / l : 0.0f, db, lane, rows,
+              [&](int r) { return a.out.p + (row0 + r) * a.out.sl + h * a.out.sh; });
 }
 
 }  // namespace
@@ -271,7 +273,7 @@ hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t stream) {
   hipLaunchKernelGGL(packed_fwd_kernel, dim3(n), dim3(PK_WAVES * 64), FWD_LDS, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.n_split == 0) return e;
-  hipLaunchKernelGGL(packed_fwd_join_kernel, dim3((uint32_t)a.n_split * a.Hq), dim3(PK_WAVES * 64), 0,
+  hipLaunchKernelGGL(packed_fwd_join_kernel, dim3((uint32_t)a.n_split * a.Hq * PK_WAVES), dim3(256), 0,
                      stream, a);
   return hipGetLastError();
 }
