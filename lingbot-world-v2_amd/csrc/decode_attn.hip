@@ -274,17 +274,20 @@ __global__ void __launch_bounds__(DW * 64, 2) decode_kernel(const DecodeArgs a) 
   } while (true);
 }
 
-// One wave per (sequence, query head): a sequence that several pieces share is joined, in their order;
-// one of no keys gets zeros; the others are finished.
-__global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (id >= (int64_t)a.B * a.Hq) return;
-  const int b = (int)(id / a.Hq), h = (int)(id % a.Hq);
+// A workgroup per (sequence, query head): a sequence that several pieces share is joined, its waves taking 64 / JW
+// parts at a time in turn, then in the waves' order; one of no keys gets zeros; the others are finished. (One wave
+// for all parts, eight at a time: one sequence of 46000 keys x 12/4 heads 33.8 / 27.7 us in all, of 12000 x 40/8
+// 21.4 / 18.2; sixteen of 3000 43.3 / 43.9.)
+constexpr int JW = 4;
+__global__ void __launch_bounds__(JW * 64) decode_join_kernel(const DecodeArgs a) {
+  __shared__ float2 wx[JW][64];
+  __shared__ float wm[JW], wl[JW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = (int)(blockIdx.x / (uint32_t)a.Hq), h = (int)(blockIdx.x % (uint32_t)a.Hq);
   int64_t all, before;
   count_tiles_of(a, lane, b, all, before);
   const int tiles = __builtin_amdgcn_readfirstlane(tiles_of(a, b));
-  float x = 0.0f, y = 0.0f, L = 0.0f;
+  float x = 0.0f, y = 0.0f, L = 0.0f, M = -INFINITY;
   if (tiles > 0) {
     // tile t is in piece j when floor(all j / pieces) <= t < floor(all (j + 1) / pieces)
     const int64_t pieces = all < a.pieces ? all : a.pieces;
@@ -293,9 +296,14 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a) {
     if (j0 == j1) return;
     const int64_t rows = (int64_t)a.pieces + a.B, row = h * rows + j0 + b;
     const float* st = a.part + a.Hq * rows * D;
-    float M = -INFINITY;
-    for (int i0 = 0; i0 <= j1 - j0; i0 += 64) {  // 64 parts at a time, their weights one per lane
-      const int n = min(64, j1 - j0 + 1 - i0);
+    constexpr int N = 64 / JW;
+    for (int i0 = N * wave; i0 <= j1 - j0; i0 += 64) {  // N parts at a time, their weights one per lane
+      const int n = min(N, j1 - j0 + 1 - i0);
+      const float* p = a.part + (row + i0) * D + 2 * lane;
+      float2 v[N];
+#pragma unroll
+      for (int u = 0; u < N; ++u)
+        v[u] = u < n ? *reinterpret_cast<const float2*>(p + (int64_t)u * D) : float2{0.0f, 0.0f};
       float m = -INFINITY, l = 0.0f;
       if (lane < n) {
         m = st[row + i0 + lane];
@@ -312,20 +320,31 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a) {
       y *= f0;
       L = L * f0 + wave_reduce_sum(w * l);
       M = mn;
-      const float* p = a.part + (row + i0) * D + 2 * lane;
-      for (int i = 0; i < n; i += 8) {  // (lanes past n have weight 0; their rows are not read)
-        float2 v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          v[u] = i + u < n ? *reinterpret_cast<const float2*>(p + (int64_t)(i + u) * D) : float2{0.0f, 0.0f};
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float f = __shfl(w, i + u);
-          x += f * v[u].x;
-          y += f * v[u].y;
-        }
+      for (int u = 0; u < N; ++u) {  // (lanes past n have weight 0)
+        const float f = __shfl(w, u);
+        x += f * v[u].x;
+        y += f * v[u].y;
       }
     }
+  }
+  wx[wave][lane] = float2{x, y};
+  if (lane == 0) {
+    wm[wave] = M;
+    wl[wave] = L;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < JW; ++w) M = fmaxf(M, wm[w]);
+  x = y = L = 0.0f;
+#pragma unroll
+  for (int w = 0; w < JW; ++w) {
+    const float f = wm[w] == -INFINITY ? 0.0f : fast_exp2((wm[w] - M) * a.scale_log2);
+    L += f * wl[w];
+    x += f * wx[w][lane].x;
+    y += f * wx[w][lane].y;
   }
   const float inv = L > 0.0f ? 1.0f / L : 0.0f;
   *reinterpret_cast<uint32_t*>(a.out.p + b * a.out.sl + h * a.out.sh + 2 * lane) =
@@ -335,14 +354,15 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const DecodeArgs a) {
 }  // namespace
 
 // Pieces per key/value head (and block of 32 of its query heads): none while whole sequences give work
-// enough or caches are short, else as many as run at once, two workgroups a CU, of 8 tiles or more.
+// enough or caches are short, else as many as run at once, two workgroups a CU, of 6 tiles or more (of 4 / 6 / 8:
+// one sequence of 5000 keys x 40/8 heads 14.4 / 12.9 / 13.3 us, two of 5000 x 12/4 14.3 / 12.9 / 14.7).
 int decode_pieces(int64_t B, int Hq, int Hk, int64_t S, int num_splits, int cus) {
   const int64_t units = (int64_t)Hk * ((Hq / Hk + HEADS - 1) / HEADS);
   if (num_splits == 1) return 0;
   if (num_splits > 1) return (int)std::min<int64_t>(num_splits * B, 1 << 20);
   if (S <= 1024 || B * units >= 2 * cus) return 0;
   const int64_t most = std::max<int64_t>(1, 2 * cus / units), tiles = B * ((S + DT - 1) / DT);
-  return (int)std::max<int64_t>(1, std::min(most, tiles / 8));
+  return (int)std::max<int64_t>(1, std::min(most, tiles / 6));
 }
 
 template <int DW>
@@ -364,8 +384,7 @@ hipError_t launch_decode(const DecodeArgs& a, hipStream_t stream) {
   if (a.pieces == 0 && (int64_t)a.B * blocks * a.Hk <= num_cus()) return run<8>(a, stream);
   const hipError_t e = run<4>(a, stream);
   if (e != hipSuccess || a.pieces == 0) return e;
-  const int64_t rows = (int64_t)a.B * a.Hq;
-  hipLaunchKernelGGL(decode_join_kernel, dim3((uint32_t)((rows + 3) / 4)), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(decode_join_kernel, dim3((uint32_t)(a.B * a.Hq)), dim3(JW * 64), 0, stream, a);
   return hipGetLastError();
 }
 
