@@ -19,6 +19,8 @@ namespace {
 
 // hipLaunchKernel's limit: fewer than 2^32 threads in a grid
 constexpr int64_t kMaxWorkgroups = (int64_t(1) << 32) / 256 - 1;
+// packed rows: a tile past the last one still has a 32-bit index
+constexpr int64_t kMaxTokens = 0x7fffff00;
 
 // bf16 rows [n, heads, D]; n == 0: no pointer needed. `tile`: rows are copied in tiles of 64 with
 // 32-bit byte offsets.
@@ -126,7 +128,7 @@ int fill_packed(const lbw_packed_params* p, PackedArgs* a) {
   memset(a, 0, sizeof(*a));
   if (p->head_dim != 128) return fail(LBW_ERR_UNSUPPORTED, "head_dim %d: only 128", p->head_dim);
   LBW_TRY(check_heads(p->q_heads, p->k_heads));
-  if (p->q_tokens < 0 || p->k_tokens < 0 || p->q_tokens > 0x7fffffff || p->k_tokens > 0x7fffffff)
+  if (p->q_tokens < 0 || p->k_tokens < 0 || p->q_tokens > kMaxTokens || p->k_tokens > kMaxTokens)
     return fail(LBW_ERR_INVALID, "q_tokens %lld, k_tokens %lld", (long long)p->q_tokens,
                 (long long)p->k_tokens);
   LBW_TRY(check_rows("q", p->q, p->q_tokens, p->q_stride_l, p->q_stride_h, true));
@@ -230,7 +232,7 @@ size_t stat_bytes(const lbw_packed_params* p) {
 }
 bool sane(const lbw_packed_params* p) {
   return p != nullptr && p->q_heads >= 1 && p->k_heads >= 1 && p->q_heads % p->k_heads == 0 &&
-         p->q_tokens >= 0 && p->q_tokens <= 0x7fffffff;
+         p->q_tokens >= 0 && p->q_tokens <= kMaxTokens;
 }
 
 int pieces_for(const lbw_decode_params* p) {
@@ -344,8 +346,8 @@ int lbw_attention_packed_plan(int32_t n_seqs, const int32_t* q_lens, const int32
     nq += (q_lens[s] + (int64_t)PK_BLOCK - 1) / PK_BLOCK;
     nk += (k_lens[s] + (int64_t)PK_BLOCK - 1) / PK_BLOCK;
   }
-  if (tq > 0x7fffffff || tk > 0x7fffffff)
-    return fail(LBW_ERR_UNSUPPORTED, "%lld query and %lld key rows: below 2^31", (long long)tq,
+  if (tq > kMaxTokens || tk > kMaxTokens)
+    return fail(LBW_ERR_UNSUPPORTED, "%lld query and %lld key rows: at most 2^31 - 256", (long long)tq,
                 (long long)tk);
   memset(info, 0, sizeof(*info));
   info->n_q_items = nq;

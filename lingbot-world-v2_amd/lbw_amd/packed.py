@@ -46,8 +46,8 @@ def _lens(name, lens) -> tuple:
     lens = tuple(int(x) for x in lens)
     if any(x < 0 for x in lens):
         raise ValueError(f"{name} has a negative length")
-    if sum(lens) >= 1 << 31:
-        raise ValueError(f"{name} add up to {sum(lens)} tokens: below 2^31")
+    if sum(lens) > (1 << 31) - 256:
+        raise ValueError(f"{name} add up to {sum(lens)} tokens: at most 2^31 - 256")
     return lens
 
 

@@ -61,6 +61,8 @@ def test_plan_refusals():
         lbw().packed_plan([3], [3, 4], device="cpu")
     with pytest.raises(ValueError, match="2\\^31"):
         lbw().packed_plan([2 ** 30, 2 ** 30], device="cpu")
+    with pytest.raises(ValueError, match="2\\^31"):
+        lbw().packed_plan([1], [2 ** 31 - 255], device="cpu")
     from lbw_amd import _lib
     lib = _lib.load()
     n = ctypes.byref(_lib.PackedPlanInfo())
@@ -70,6 +72,9 @@ def test_plan_refusals():
     assert b"room for 3" in lib.lbw_last_error()
     assert lib.lbw_attention_packed_plan(1, None, lens, 1, None, 0, None, 0, n) == 1
     assert lib.lbw_attention_packed_plan(1, lens, lens, 1, None, 0, None, 0, None) == 1
+    long = (ctypes.c_int32 * 1)(2 ** 31 - 255)
+    assert lib.lbw_attention_packed_plan(1, lens, long, 1, None, 0, None, 0, n) != 0
+    assert b"2^31 - 256" in lib.lbw_last_error()
 
 
 @pytest.mark.parametrize("cname,pyname", [("lbw_head_norm_rope_params", "HeadNormRopeParams"),
