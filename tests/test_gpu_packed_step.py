@@ -227,3 +227,38 @@ def test_traces_under_fake_tensors():
         kc = torch.empty(16, 30, HK, D, dtype=BF, device="cuda")
         lens = torch.empty(16, dtype=torch.int32, device="cuda")
         assert torch.ops.lbw.attention_decode(q, kc, kc, lens).shape == q.shape
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_compiled_step_gives_the_same_bits(backend):
+    """One graph, no break: the training step with its gradients, and a decode step that writes the cache."""
+    import lbw_amd
+    lens = [70, 1, 33]
+    qkv, w, _, rope, pos, do = _setup(sum(lens), 9)
+    plan = lbw_amd.packed_plan(lens)
+
+    def forward(qkv, wq, wk):
+        q, k, v = qkv.split([HQ, HK, HK], 1)
+        q2, k2 = lbw_amd.qk_head_norm_rope(q, k, wq, wk, rope, pos)
+        return lbw_amd.attention_packed(q2, k2, v, plan)
+
+    def step(f):
+        x = _leaves(qkv, *w)
+        out = f(*x)
+        return (out,) + torch.autograd.grad(out, x, do)
+
+    def decode(q, k, v, kc, vc, rows):
+        lbw_amd.qk_head_norm_rope_(q, k, w[0], w[1], rope, pos[:3], q_out=q, k_out=kc, v=v, v_out=vc, rows=rows)
+        return lbw_amd.attention_decode(q, kc, vc, rows + 1)
+
+    def serve(f):
+        q, k, v = (t[:3].clone() for t in qkv.split([HQ, HK, HK], 1))
+        kc, vc = (torch.full((3, 20, HK, D), x, dtype=BF, device="cuda") for x in (0.5, 2.0))
+        rows = torch.tensor([0, 19, 7], dtype=torch.int32, device="cuda")
+        return f(q, k, v, kc, vc, rows), q, kc, vc
+
+    torch._dynamo.reset()
+    compiled = lambda f: torch.compile(f, backend=backend, fullgraph=True)  # noqa: E731
+    for run, f in ((step, forward), (serve, decode)):
+        for got, want in zip(run(compiled(f)), run(f)):
+            assert torch.equal(got, want)
