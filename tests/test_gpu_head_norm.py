@@ -221,3 +221,18 @@ def test_refusals_on_the_device():
     g, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.float().sum().backward()  # no second derivatives
+
+
+def test_no_rotation_and_a_column_of_positions():
+    import lbw_amd
+    q, k, _, w = _data(9, 4, 2, 128, 12)
+    none = lbw_amd.axis_rope(torch.empty(5, 0), device="cuda")
+    pos3 = torch.arange(27, dtype=torch.int32, device="cuda").view(9, 3)
+    got = lbw_amd.qk_head_norm_rope(q, k, *w, none, pos3[:, 1])
+    for y, x, wt in zip(got, (q, k), w):
+        want = R.head_norm(x.double(), wt.double(), torch.zeros(9, 0, dtype=torch.float64, device="cuda"), True, 1e-6, 1.0)
+        R.assert_within("y", y, want, R.head_norm_allow(want))
+    rope = lbw_amd.axis_rope(torch.randn(30, 64, generator=torch.Generator().manual_seed(1)), device="cuda")
+    a = lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos3[:, 1])
+    b = lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos3[:, 1:2].contiguous())
+    assert all(torch.equal(x, y) for x, y in zip(a, b))

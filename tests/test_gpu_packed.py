@@ -224,6 +224,26 @@ def test_nothing_to_do():
     assert lbw_amd.attention_packed(q, k[:0], v[:0], plan).shape == (0, 4, 128)
 
 
+def test_one_tensor_as_keys_and_values_and_heads_that_are_expanded():
+    import lbw_amd
+    ql = [70, 33]
+    q, k, _, do = _data(ql, ql, 4, 2, 13)
+    plan = lbw_amd.packed_plan(ql)
+    want = R.attention(q, k, k, ql, ql, True, SCALE, do)
+    x = k.detach().requires_grad_()
+    g, = torch.autograd.grad(lbw_amd.attention_packed(q, x, x, plan), x, do)
+    # two gradients, each within its allowance, and the rounding of their sum
+    total = want["dk"] + want["dv"]
+    R.assert_within("dk + dv", g, total, (1 + R.H) * (want["dk_a"] + want["dv_a"]) + R.H * total.abs())
+    one = k[:, :1].detach().requires_grad_()
+    wide = one.expand(-1, 2, -1)  # head stride 0
+    out = lbw_amd.attention_packed(q, wide, wide, plan)
+    same = lbw_amd.attention_packed(q, wide.detach().contiguous(), wide.detach().contiguous(), plan)
+    assert torch.equal(out, same)
+    g, = torch.autograd.grad(out, one, do)
+    assert g.shape == one.shape and torch.isfinite(g).all()
+
+
 def test_a_plan_of_other_lengths_stays_inside_the_tensors():
     """An op cannot see whose table it gets: items that do not fit are skipped, not followed."""
     import lbw_amd
