@@ -29,20 +29,12 @@ EPS = 1e-6
 BF16 = torch.bfloat16
 
 
-_lib = None
-
-
 def _lbw():
-    """The package, imported once, as a program that uses it imports it."""
-    global _lib
-    if _lib is not None:
-        return _lib
     pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
                        "lingbot-world-v2_amd")
     if pkg not in sys.path:
         sys.path.insert(0, pkg)
     import lbw_amd
-    _lib = lbw_amd
     return lbw_amd
 
 
