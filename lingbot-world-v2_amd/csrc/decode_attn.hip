@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(DW * 64, 2) decode_kernel(const DecodeArgs a) 
     // O^T as rows [head][128] fp32 into the wave's LDS, m and l behind the rings
     float* const sm = reinterpret_cast<float*>(lds + DEC_LDS);
     float* const sl = sm + DW * HEADS;
-    if (hl == 0) {
-      sm[wave * HEADS + l32] = l > 0.0f ? m : -INFINITY;
+    if (hl == 0) {  // (no keys: a reference of -inf, weight 0; a sum that is NaN keeps its own and stays)
+      sm[wave * HEADS + l32] = l == 0.0f ? -INFINITY : m;
       sl[wave * HEADS + l32] = l;
     }
     float* mine = reinterpret_cast<float*>(lds + RING_B * wave);
@@ -313,7 +313,6 @@ __global__ void __launch_bounds__(JW * 64) decode_join_kernel(const DecodeArgs a
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
       const float mn = fmaxf(M, mx);
-      if (mn == -INFINITY) continue;
       const float f0 = M == -INFINITY ? 0.0f : fast_exp2((M - mn) * a.scale_log2);
       const float w = m == -INFINITY ? 0.0f : fast_exp2((m - mn) * a.scale_log2);
       x *= f0;

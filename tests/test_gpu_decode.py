@@ -122,3 +122,32 @@ def test_no_sequences_and_refusals():
     out = lbw_amd.attention_decode(x, k, v, _lens([3, 3]))
     with pytest.raises(RuntimeError):
         out.float().sum().backward()
+
+
+@pytest.mark.parametrize("splits", [0, 1, 3, 128])
+def test_nan_and_infinite_scores_stay_in_their_heads(splits):
+    """A query, keys or values that are not finite give NaN in the heads that read them, cut into pieces or
+    not, and leave the bits of the others."""
+    import lbw_amd
+    lens = [2500, 0, 40, 1999]
+    q, k, v = _data(4, 8, 2, 2500, 6)
+    run = lambda q, k, v: lbw_amd.attention_decode(q, k, v, _lens(lens), num_splits=splits)  # noqa: E731
+    want = run(q, k, v)
+    q, k, v = q.clone(), k.clone(), v.clone()
+    nan = torch.zeros(4, 8, dtype=torch.bool, device="cuda")
+    q[0, 3] = float("nan")
+    q[0, 5] = 3e38                            # scores of both infinities
+    q[1, 0] = float("nan")                    # (no keys: 0 all the same)
+    k[2, :40, 1] = float("nan")               # every key of kv head 1
+    k[3, 512:1500, 0] = float("nan")          # whole pieces of kv head 0
+    v[3, 1600, 1] = float("nan")
+    nan[0, 3] = nan[0, 5] = True
+    nan[2, 4:] = True
+    nan[3] = True
+    got = run(q, k, v)
+    assert torch.equal(torch.isnan(got).all(-1), nan) and torch.equal(torch.isnan(got).any(-1), nan)
+    assert torch.equal(got[~nan], want[~nan])
+    # every key of every sequence
+    k[:] = float("nan")
+    got = run(*_data(4, 8, 2, 2500, 6)[:1], k, v)
+    assert torch.isnan(got[[0, 2, 3]]).all() and torch.all(got[1] == 0)
