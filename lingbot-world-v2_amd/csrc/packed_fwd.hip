@@ -33,11 +33,12 @@ constexpr int AHEAD = 2;                         // MFMA pairs that LDS fragment
 template <int N>
 using ic = std::integral_constant<int, N>;
 
-// A wave's rows of lse from the reference and the sum (of both lane halves).
+// A wave's rows of lse from the reference and the sum (of both lane halves): -inf for a sum of 0, a row that sees
+// no key; a sum that is NaN stays NaN.
 __device__ __forceinline__ void store_lse(const PackedArgs& a, int h, int64_t row0, int lane, int rows, float m,
                                           float l) {
   if (a.lse != nullptr && lane < 32 && lane < rows)
-    a.lse[(int64_t)h * a.Tq + row0 + lane] = l > 0.0f ? m * a.scale + logf(l) : -INFINITY;
+    a.lse[(int64_t)h * a.Tq + row0 + lane] = l == 0.0f ? -INFINITY : m * a.scale + logf(l);
 }
 
 __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const PackedArgs a) {
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(PK_WAVES * 64, 2) packed_fwd_kernel(const Pack
     float* const part = part_of(a, sh, a.Hq, sh.piece, PK_PART_FWD);
     store_acc(part, wave, lane, o);
     if (hl == 0) {
-      part[PK_BLOCK * 128 + r0 + l32] = ls > 0.0f ? m : -INFINITY;
+      part[PK_BLOCK * 128 + r0 + l32] = ls == 0.0f ? -INFINITY : m;
       part[PK_BLOCK * 128 + PK_BLOCK + r0 + l32] = ls;
     }
     return;

@@ -259,3 +259,26 @@ def test_a_plan_of_other_lengths_stays_inside_the_tensors():
         lbw_amd.attention_packed(q, k, v, big)
     with pytest.raises(ValueError, match="plan is on"):
         lbw_amd.attention_packed(q, k, v, lbw_amd.packed_plan([60], device="cpu"))
+
+
+@pytest.mark.parametrize("ql,kl", [([70], [70]), ([16], [3000]), ([200, 5], [37, 2])])
+def test_a_query_that_is_nan_has_a_nan_lse(ql, kl):
+    """Only a query that sees no key has lse -inf; the other rows stay within their allowance."""
+    import lbw_amd
+    q, k, v, _ = _data(ql, kl, 2, 1, 14)
+    want = R.attention(q, k, v, ql, kl, True, SCALE)
+    plan = lbw_amd.packed_plan(ql, kl)
+    rows = [0, ql[0] - 1]
+    q = q.clone()
+    q[rows, 1] = float("nan")
+    out, lse = lbw_amd.attention_packed(q, k, v, plan, return_lse=True)
+    for r in rows:
+        if want["lse"][1, r] == -math.inf:    # sees no key
+            assert lse[1, r] == -math.inf and torch.all(out[r, 1] == 0)
+        else:
+            assert torch.isnan(lse[1, r]) and torch.isnan(out[r, 1]).all()
+    keep = torch.ones(2, sum(ql), dtype=torch.bool, device="cuda")
+    keep[1, rows] = False
+    R.assert_within("out", out[keep.T], want["out"][keep.T], want["out_a"][keep.T])
+    keep &= want["lse"] != -math.inf
+    R.assert_within("lse", lse[keep], want["lse"][keep], want["lse_a"][keep])
