@@ -251,10 +251,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> head_norm_rope_bwd(
 
 // ---- packed attention
 
-// A tensor without a contiguous head dim is copied (in the forward above autograd, so that its gradient finds
-// the way back).
+// A tensor without a contiguous head dim is copied: in the forward above autograd, so that its gradient finds
+// the way back, and in the op itself, for calls that autograd does not see (inference mode).
 Tensor unit(const Tensor& t) { return t.dim() != 3 || t.stride(2) == 1 ? t : t.contiguous(); }
-
 
 // -> query items, key items, and the tile counts [q_tiles, q_tiles_max, k_tiles, k_tiles_max]
 std::tuple<Tensor, Tensor, std::vector<int64_t>> packed_plan(const Tensor& q_lens,
@@ -323,10 +322,11 @@ Tensor new_lse(const Tensor& q) {
   return at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
 }
 
-std::tuple<Tensor, Tensor> attention_packed(const Tensor& q, const Tensor& k, const Tensor& v,
+std::tuple<Tensor, Tensor> attention_packed(const Tensor& q_, const Tensor& k_, const Tensor& v_,
                                             const Tensor& q_items, const Tensor& k_items,
                                             at::IntArrayRef info, double scale, bool want_lse) {
-  c10::DeviceGuard guard(q.device());
+  c10::DeviceGuard guard(q_.device());
+  const Tensor q = unit(q_), k = unit(k_), v = unit(v_);
   auto p = packed_params(q, k, v, q_items, k_items, info, scale);
   Tensor out = at::empty(q.sizes(), q.options());
   Tensor lse = want_lse ? new_lse(q) : at::empty({0}, q.options().dtype(at::kFloat));
@@ -346,8 +346,8 @@ std::tuple<Tensor, Tensor, Tensor> attention_packed_bwd(const Tensor& dout_, con
                                                         const Tensor& q_items,
                                                         const Tensor& k_items,
                                                         at::IntArrayRef info, double scale) {
+  c10::DeviceGuard guard(q_.device());
   const Tensor q = unit(q_), k = unit(k_), v = unit(v_), out = unit(out_);
-  c10::DeviceGuard guard(q.device());
   auto p = packed_params(q, k, v, q_items, k_items, info, scale);
   check_rows("out", out, q);
   TORCH_CHECK(dout_.sizes() == q.sizes() && dout_.scalar_type() == at::kBFloat16 &&

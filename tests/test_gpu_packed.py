@@ -282,3 +282,17 @@ def test_a_query_that_is_nan_has_a_nan_lse(ql, kl):
     R.assert_within("out", out[keep.T], want["out"][keep.T], want["out_a"][keep.T])
     keep &= want["lse"] != -math.inf
     R.assert_within("lse", lse[keep], want["lse"][keep], want["lse_a"][keep])
+
+
+def test_head_dim_that_is_not_contiguous_is_copied_without_autograd_too():
+    import lbw_amd
+    ql = kl = [40, 9]
+    q, k, v, do = _data(ql, kl, 4, 2, 11)
+    want = _run(q, k, v, do, ql, kl, True)
+    plan = lbw_amd.packed_plan(ql)
+    with torch.inference_mode():
+        xs = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+        out, lse = lbw_amd.attention_packed(*xs, plan, return_lse=True)
+        grads = lbw_amd.attention_packed_backward(do.clone(), *xs, out, lse, plan)
+    for n, x in zip(("out", "lse", "dq", "dk", "dv"), (out, lse) + tuple(grads)):
+        assert torch.equal(x, want[n])
