@@ -248,14 +248,16 @@ __global__ void __launch_bounds__(HN_WAVES * 64) head_norm_bwd_kernel(const Head
         }
         ss = head_sum<LPH>(ss);
         dot = head_sum<LPH>(dot);
-        const float r = rsqrtf(ss * a.inv_d + a.eps);
+        const bool there = (it + u) * HPW + hsub < heads;
+        // (a lane past the last head holds zeros, and with eps = 0 their rsqrt is infinite)
+        const float r = there ? rsqrtf(ss * a.inv_d + a.eps) : 0.0f;
         const float m = r * r * dot * a.inv_d;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          gw[j] += g[j] * f[j] * r;  // (a lane past the last head holds zeros)
+          gw[j] += g[j] * f[j] * r;
           o[j] = r * (g[j] * wt[j] - f[j] * m);
         }
-        if ((it + u) * HPW + hsub < heads)
+        if (there)
           *reinterpret_cast<u32x4*>(ds + (int64_t)(it + u) * HPW * dst.sh + dof) = pack8(o);
       }
     }

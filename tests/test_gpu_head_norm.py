@@ -236,3 +236,36 @@ def test_no_rotation_and_a_column_of_positions():
     a = lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos3[:, 1])
     b = lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos3[:, 1:2].contiguous())
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def _gradient_allowance(X, W, a, inter, eps, s, dy):
+    """As in test_forward_and_gradient: 2^10 E of the sizes of the two terms, and the one rounding."""
+    r = torch.rsqrt(X.square().mean(-1, keepdim=True) + eps)
+    gw = R.rotate(dy.double(), a.cos(), -a.sin(), inter).abs() * s * W.abs()
+    size = r * (gw.amax(-1, keepdim=True) + (X.abs() * r).amax(-1, keepdim=True) *
+                (gw * X.abs() * r).mean(-1, keepdim=True))
+    terms = (R.rotate(dy.double(), a.cos(), -a.sin(), inter) * s * X * r).abs().sum((0, 1))
+    return 2 ** 10 * R.E * size, terms
+
+
+@pytest.mark.parametrize("hq,hk,d", [(4, 1, 128), (6, 3, 32), (5, 5, 256), (12, 4, 64)])
+def test_gradient_with_eps_0(hq, hk, d):
+    """Lanes past the last head hold zeros, whose rsqrt(0) must not reach the weights' gradient."""
+    import lbw_amd
+    T = 21
+    q, k, _, w = _data(T, hq, hk, d, 15)
+    ang, rope = _rope((d // 2,), 50, True)
+    pos = _pos(T, (d // 2,), 50)
+    leaves = [x.detach().requires_grad_() for x in (q, k, *w)]
+    y = lbw_amd.qk_head_norm_rope(*leaves, rope, pos, 0.0)
+    dy = [torch.randn(x.shape, generator=torch.Generator().manual_seed(n)).to(BF).cuda() for n, x in enumerate(y)]
+    grads = torch.autograd.grad(y, leaves, dy)
+    a = R.token_angles(ang, (d // 2,), pos)
+    for n in range(2):
+        X, W = leaves[n].detach().double().requires_grad_(), leaves[2 + n].detach().double().requires_grad_()
+        Y = R.head_norm(X, W, a, True, 0.0, 1.0)
+        R.assert_within("y", y[n], Y.detach(), R.head_norm_allow(Y.detach()))
+        G = torch.autograd.grad(Y, (X, W), dy[n].double())
+        allow, terms = _gradient_allowance(X.detach(), W.detach(), a, True, 0.0, 1.0, dy[n])
+        R.assert_within("dx", grads[n], G[0], R.H * G[0].abs() + allow)
+        R.assert_within("dw", grads[2 + n], G[1], R.H * G[1].abs() + (T + 200) * R.E * terms)
