@@ -9,12 +9,14 @@
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/util/SmallVector.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/graph_task.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstring>
 #include <unordered_set>
 #include <vector>
@@ -49,24 +51,48 @@ void check_int32(const char* name, const Tensor& t, const Tensor& like) {
               " must be int32 on q's device");
 }
 
-// Whether two row tensors [n, heads, D] may share memory: by their address ranges, or, as column blocks of one
-// buffer with the same row stride, by their columns.
+// Whether two bf16 tensors share an element, whatever their layouts. Elements i of a and j of b are one where the
+// sum over the strides s of t_s s is the distance c of their first elements, t_s = i - j along the dims of that
+// stride: an interval for each stride. Searched from the largest stride down, what is left of c within the
+// smaller ones' reach; layouts that nest leave one or two t a stride. A search that takes long counts as shared.
 bool may_overlap(const Tensor& a, const Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
-  auto span = [](const Tensor& t, int64_t from) {  // elements from the first to past the last, dims `from` on
-    int64_t n = 1;
-    for (int64_t d = from; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
-    return n;
+  struct Dim {
+    int64_t s, lo, hi;        // lo <= t <= hi
+    int64_t from, to;         // what this and the smaller strides add up to, at least and at most
   };
-  const int64_t pa = reinterpret_cast<intptr_t>(a.data_ptr()), pb = reinterpret_cast<intptr_t>(b.data_ptr());
-  if (pa + 2 * span(a, 0) <= pb || pb + 2 * span(b, 0) <= pa) return false;
-  const int64_t s = a.stride(0);
-  if (a.dim() != b.dim() || s != b.stride(0) || s <= 0) return true;
-  const int64_t wa = span(a, 1), wb = span(b, 1);
-  if (wa > s || wb > s || (pb - pa) % 2 != 0) return true;
-  int64_t d = (pb - pa) / 2 % s;  // b's first column from a's on
-  if (d < 0) d += s;
-  return !(d >= wa && d + wb <= s);
+  c10::SmallVector<Dim, 8> dims;
+  for (const Tensor* t : {&a, &b})
+    for (int64_t d = 0; d < t->dim(); ++d) {
+      const int64_t n = t->size(d) - 1, s = t->stride(d);
+      if (n == 0 || s == 0) continue;
+      auto at = std::find_if(dims.begin(), dims.end(), [&](const Dim& x) { return x.s == s; });
+      if (at == dims.end()) at = dims.insert(dims.end(), Dim{s, 0, 0, 0, 0});
+      if (t == &a) at->hi += n;
+      else at->lo -= n;
+    }
+  std::sort(dims.begin(), dims.end(), [](const Dim& x, const Dim& y) { return x.s > y.s; });
+  int64_t from = 0, to = 0;
+  for (size_t i = dims.size(); i-- > 0;) {
+    dims[i].from = from += dims[i].lo * dims[i].s;
+    dims[i].to = to += dims[i].hi * dims[i].s;
+  }
+  const int64_t bytes = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr());
+  if (bytes % 2 != 0) return from * 2 - 2 < bytes && bytes < to * 2 + 2;
+  int budget = 4096;
+  auto search = [&](auto& self, size_t i, int64_t c) -> bool {
+    if (i == dims.size()) return c == 0;
+    if (c < dims[i].from || c > dims[i].to) return false;
+    if (--budget < 0) return true;
+    const int64_t s = dims[i].s, lo = i + 1 < dims.size() ? dims[i + 1].from : 0,
+                  hi = i + 1 < dims.size() ? dims[i + 1].to : 0;
+    // (both divisions rounded towards zero: a t too many at each end, which the next level turns down)
+    const int64_t first = std::max(dims[i].lo, (c - hi) / s - 1), last = std::min(dims[i].hi, (c - lo) / s + 1);
+    for (int64_t t = first; t <= last; ++t)
+      if (self(self, i + 1, c - t * s)) return true;
+    return false;
+  };
+  return search(search, 0, bytes / 2);
 }
 
 // An output that the caller gives: no two of its elements in one place, and apart from `others`, or exactly its

@@ -269,3 +269,80 @@ def test_gradient_with_eps_0(hq, hk, d):
         allow, terms = _gradient_allowance(X.detach(), W.detach(), a, True, 0.0, 1.0, dy[n])
         R.assert_within("dx", grads[n], G[0], R.H * G[0].abs() + allow)
         R.assert_within("dw", grads[2 + n], G[1], R.H * G[1].abs() + (T + 200) * R.E * terms)
+
+
+def _cache_layouts(T, cap, hk, d):
+    new = lambda *s: torch.full(s, 7.0, dtype=BF, device="cuda")  # noqa: E731
+    a, b, c, e = new(T, cap, 2, hk, d), new(T, cap, hk, 2, d), new(T, 2, hk, cap, d), new(hk, cap, 2, T, d)
+    return {"K and V of a token": (a, a[:, :, 0], a[:, :, 1]), "K and V of a head": (b, b[..., 0, :], b[..., 1, :]),
+            "heads first": (c, c[:, 0].transpose(1, 2), c[:, 1].transpose(1, 2)),
+            "sequences last": (e, e[:, :, 0].permute(2, 1, 0, 3), e[:, :, 1].permute(2, 1, 0, 3))}
+
+
+@pytest.mark.parametrize("layout", ["K and V of a token", "K and V of a head", "heads first", "sequences last"])
+def test_write_form_into_interleaved_caches(layout):
+    import lbw_amd
+    T, hq, hk, d, cap = 5, 4, 2, 64, 9
+    q, k, v, w = _data(T, hq, hk, d, 16)
+    _, rope = _rope((32,), 40, False)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    rows = torch.tensor([0, 8, 3, -1, 5], dtype=torch.int32, device="cuda")
+    buf, kc, vc = _cache_layouts(T, cap, hk, d)[layout]
+    qo = torch.empty(T, hq, d, dtype=BF, device="cuda")
+    lbw_amd.qk_head_norm_rope_(q, k, *w, rope, pos, q_out=qo, k_out=kc, v=v, v_out=vc, rows=rows)
+    q2, k2 = lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos)
+    assert torch.equal(qo, q2)
+    want, wk, wv = _cache_layouts(T, cap, hk, d)[layout]
+    for t, r in enumerate(rows.tolist()):
+        if r >= 0:
+            wk[t, r], wv[t, r] = k2[t], v[t]
+    assert torch.equal(buf, want)
+
+
+def test_write_form_in_place_in_an_interleaved_projection():
+    import lbw_amd
+    T, h, d = 11, 3, 128
+    _, rope = _rope((64,), 40, True)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(17)
+    buf = torch.randn(T, h, 3, d, generator=g).to(BF).cuda()
+    want = buf.clone()
+    want[:, :, 0], want[:, :, 1] = lbw_amd.qk_head_norm_rope(buf[:, :, 0], buf[:, :, 1], None, None, rope, pos)
+    lbw_amd.qk_head_norm_rope_(buf[:, :, 0], buf[:, :, 1], None, None, rope, pos, q_out=buf[:, :, 0], k_out=buf[:, :, 1])
+    assert torch.equal(buf, want)
+
+
+def test_outputs_are_refused_exactly_when_they_share_an_element():
+    import random
+    import lbw_amd
+    rng = random.Random(18)
+    _, rope = _rope((16,), 8, True)
+    store = torch.zeros(8192, dtype=BF, device="cuda")
+    none = torch.zeros(8, 4, 32, dtype=BF, device="cuda")
+
+    def layout(own):
+        while True:
+            T, h = rng.randint(1, 6), rng.randint(1, 3)
+            s = [8 * rng.randint(0 if not own else 4, rng.choice([10, 60])) for _ in range(2)]
+            at = 8 * rng.randint(0, 100)
+            place = [at + t * s[0] + i * s[1] + x for t in range(T) for i in range(h) for x in range(32)]
+            if not own or len(set(place)) == len(place):
+                return (T, h, 32), (*s, 1), at, set(place)
+    seen = [0, 0]
+    for _ in range(300):
+        size, stride, at, mine = layout(True)
+        T, h, _ = size
+        _, kstride, kat, _ = layout(False)
+        place = {kat + t * kstride[0] + x for t in range(T) for x in range(32)}
+        q_out, k = store.as_strided(size, stride, at), store.as_strided((T, 1, 32), kstride, kat)
+        pos = torch.zeros(T, dtype=torch.int32, device="cuda")
+        call = lambda: lbw_amd.qk_head_norm_rope_(none[:T, :h], k, None, None, rope, pos, q_out=q_out,  # noqa: E731
+                                                  k_out=torch.empty(T, 1, 32, dtype=BF, device="cuda"))
+        shared = bool(mine & place)
+        seen[shared] += 1
+        if shared:
+            with pytest.raises(RuntimeError, match="overlaps"):
+                call()
+        else:
+            call()
+    assert min(seen) > 20
