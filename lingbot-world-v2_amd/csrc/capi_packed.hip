@@ -107,8 +107,6 @@ int fill_head_norm(const lbw_head_norm_rope_params* p, HeadNormArgs* a) {
   LBW_TRY(check_rows("k", p->k, p->tokens, p->k_stride_l, p->k_stride_h));
   LBW_TRY(check_head_strides("q", p->q_stride_h));
   LBW_TRY(check_head_strides("k", p->k_stride_h));
-  if ((int64_t)p->tokens * 32 / 4 >= kMaxWorkgroups)
-    return fail(LBW_ERR_UNSUPPORTED, "tokens %d", p->tokens);
   a->T = p->tokens; a->Hq = p->q_heads; a->Hk = p->k_heads;
   a->q = {static_cast<const uint16_t*>(p->q), p->q_stride_l, p->q_stride_h};
   a->k = {static_cast<const uint16_t*>(p->k), p->k_stride_l, p->k_stride_h};
@@ -267,6 +265,9 @@ extern "C" {
 int lbw_head_norm_rope(const lbw_head_norm_rope_params* p, void* stream) {
   HeadNormArgs a;
   LBW_TRY(fill_head_norm(p, &a));
+  // (a wave per token, where tokens are few up to 32767 in all; the gradient's grid does not grow with them)
+  if (p->tokens > HN_WAVES * kMaxWorkgroups)
+    return fail(LBW_ERR_UNSUPPORTED, "tokens %d above %lld", p->tokens, (long long)(HN_WAVES * kMaxWorkgroups));
   LBW_TRY(check_rows("q_out", p->q_out, p->tokens, p->q_out_stride_l, p->q_out_stride_h));
   LBW_TRY(check_rows("k_out", p->k_out, p->tokens, p->k_out_stride_l, p->k_out_stride_h));
   LBW_TRY(check_head_strides("q_out", p->q_out_stride_h));

@@ -19,8 +19,6 @@
 namespace lbw {
 namespace {
 
-constexpr int HN_WAVES = 4;  // waves per workgroup
-
 __device__ __forceinline__ void unpack8(const u32x4& v, float (&x)[8]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -329,8 +327,8 @@ hipError_t run_bwd(const HeadNormArgs& a, hipStream_t stream) {
 
 // Workgroups of the gradient kernel: four per CU, or as many as the tokens fill (for q and for k).
 int head_norm_bwd_workgroups(int T, int cus) {
-  const int need = 2 * ((T + HN_WAVES - 1) / HN_WAVES);
-  return need < 4 * cus ? need : 4 * cus;
+  const int64_t need = 2 * (((int64_t)T + HN_WAVES - 1) / HN_WAVES);
+  return need < 4 * cus ? (int)need : 4 * cus;
 }
 
 hipError_t launch_head_norm(const HeadNormArgs& args, int D, hipStream_t stream) {

@@ -8,6 +8,7 @@
 namespace lbw {
 
 constexpr int kMaxAxes = 4;
+constexpr int HN_WAVES = 4;    // per-head norm: waves per workgroup
 
 // One tensor of token rows: element strides of a token and of a head.
 struct Rows {

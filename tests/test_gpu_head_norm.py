@@ -346,3 +346,27 @@ def test_outputs_are_refused_exactly_when_they_share_an_element():
         else:
             call()
     assert min(seen) > 20
+
+
+def test_more_tokens_than_2_21():
+    import lbw_amd
+    T, d = (1 << 21) + 77, 32
+    g = torch.Generator(device="cuda").manual_seed(19)
+    q, k, dq, dk = (torch.randn(T, 1, d, generator=g, device="cuda").to(BF) for _ in range(4))
+    w = [(1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(BF) for _ in range(2)]
+    ang, rope = _rope((16,), 50, True)
+    pos = (torch.arange(T, device="cuda") % 50).int()
+    leaves = [x.requires_grad_() for x in (q, k, *w)]
+    y = lbw_amd.qk_head_norm_rope(*leaves, rope, pos, 1e-6)
+    grads = torch.autograd.grad(y, leaves, (dq, dk))
+    a = R.token_angles(ang, (16,), pos)
+    # each lane adds the tokens of its wave in turn: those of a quarter of a workgroup, at least one a CU for q and k
+    deep = T // (4 * torch.cuda.get_device_properties(0).multi_processor_count) + 200
+    for n, dy in enumerate((dq, dk)):
+        X, W = leaves[n].detach().double().requires_grad_(), leaves[2 + n].detach().double().requires_grad_()
+        Y = R.head_norm(X, W, a, True, 1e-6, 1.0)
+        R.assert_within("y", y[n], Y.detach(), R.head_norm_allow(Y.detach()))
+        G = torch.autograd.grad(Y, (X, W), dy.double())
+        allow, terms = _gradient_allowance(X.detach(), W.detach(), a, True, 1e-6, 1.0, dy)
+        R.assert_within("dx", grads[n], G[0], R.H * G[0].abs() + allow)
+        R.assert_within("dw", grads[2 + n], G[1], R.H * G[1].abs() + deep * R.E * terms)

@@ -256,3 +256,26 @@ def test_c_entries_refuse_before_any_gpu_call():
     assert b"add up" in lib.lbw_last_error()
     assert lib.lbw_attention_packed_fwd(None, None, 0, None) == 1
     assert lib.lbw_head_norm_rope(None, None) == 1
+
+
+def test_token_limits_of_the_head_norm():
+    """Forward: the grid of the tokens, four waves a workgroup, below 2^32 threads; gradient: none."""
+    from lbw_amd import _lib
+    lib = _lib.load()
+    most = 4 * ((1 << 24) - 1)
+
+    def params(tokens):
+        p = _lib.HeadNormRopeParams(tokens=tokens, q_heads=1, k_heads=1, head_dim=32, n_axes=1, pos=4)
+        for x in ("q", "k"):
+            setattr(p, x, 16)
+            setattr(p, x + "_stride_l", 32)
+        return ctypes.byref(p)
+    # (the next check after the tokens': an output's alignment)
+    for tokens in (1 << 21, (1 << 21) + 1, most):
+        assert lib.lbw_head_norm_rope(params(tokens), None) == 1
+        assert b"q_out must be" in lib.lbw_last_error()
+    assert lib.lbw_head_norm_rope(params(most + 1), None) == 2
+    assert str(most).encode() in lib.lbw_last_error()
+    for tokens in (1 << 21, most + 1, (1 << 31) - 1):
+        assert lib.lbw_head_norm_rope_bwd(params(tokens), ctypes.byref(_lib.HeadNormRopeGrads()), None, 0, None) == 1
+        assert b"dq_out must be" in lib.lbw_last_error()
