@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <limits>
 #include <unordered_set>
 #include <vector>
 
@@ -108,12 +109,13 @@ void check_written(const char* name, const Tensor& out, const Tensor* own,
   }
 }
 
-// A gradient as the kernels read it: 16-byte rows (an expanded or otherwise strided one is copied).
-Tensor grad_rows(const Tensor& g) {
+// A gradient as the kernels read it: 16-byte rows, heads less than `head_limit` elements apart (an expanded or
+// otherwise strided one is copied: its layout is the engine's choice, not the caller's).
+Tensor grad_rows(const Tensor& g, int64_t head_limit) {
   const bool ok = g.stride(2) == 1 && g.stride(0) % 8 == 0 && g.stride(1) % 8 == 0 &&
                   g.stride(0) >= 0 && g.stride(1) >= 0 &&
                   (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15u) == 0 &&
-                  g.stride(0) < (int64_t(1) << 31) / 128;
+                  g.stride(0) < (int64_t(1) << 31) / 128 && g.stride(1) < head_limit;
   return ok ? g : g.contiguous();
 }
 
@@ -255,7 +257,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> head_norm_rope_bwd(
                   dq_out_.scalar_type() == at::kBFloat16 && dk_out_.scalar_type() == at::kBFloat16 &&
                   dq_out_.device() == q.device() && dk_out_.device() == q.device(),
               "the outputs' gradients must be bf16 of q's and k's shape on their device");
-  const Tensor dq_out = grad_rows(dq_out_), dk_out = grad_rows(dk_out_);
+  const int64_t heads = int64_t(1) << 26;  // (the norm's kernels keep 32-bit offsets among a wave's heads)
+  const Tensor dq_out = grad_rows(dq_out_, heads), dk_out = grad_rows(dk_out_, heads);
   Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options());
   Tensor dwq = wq.has_value() ? at::empty_like(*wq) : at::empty({0}, q.options());
   Tensor dwk = wk.has_value() ? at::empty_like(*wk) : at::empty({0}, q.options());
@@ -382,7 +385,7 @@ std::tuple<Tensor, Tensor, Tensor> attention_packed_bwd(const Tensor& dout_, con
   TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.dim() == 2 &&
                   lse.size(0) == q.size(1) && lse.size(1) == q.size(0) && lse.is_contiguous(),
               "lse must be the forward call's fp32 [heads, tokens]");
-  const Tensor dout = grad_rows(dout_);
+  const Tensor dout = grad_rows(dout_, std::numeric_limits<int64_t>::max());
   p.out = out.data_ptr(); p.out_stride_l = out.stride(0); p.out_stride_h = out.stride(1);
   p.lse = lse.data_ptr<float>();
   Tensor dq = at::empty(q.sizes(), q.options());

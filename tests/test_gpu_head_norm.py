@@ -370,3 +370,20 @@ def test_more_tokens_than_2_21():
         allow, terms = _gradient_allowance(X.detach(), W.detach(), a, True, 1e-6, 1.0, dy)
         R.assert_within("dx", grads[n], G[0], R.H * G[0].abs() + allow)
         R.assert_within("dw", grads[2 + n], G[1], R.H * G[1].abs() + deep * R.E * terms)
+
+
+def test_gradients_with_far_heads_are_copied():
+    """Heads 2^26 elements apart, as a head-major gradient of 524288 tokens has them."""
+    import lbw_amd
+    T, d, far = 6, 128, 1 << 26
+    q, k, _, w = _data(T, 2, 2, d, 20)
+    _, rope = _rope((64,), 8, True)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    leaves = [x.detach().requires_grad_() for x in (q, k, *w)]
+    y = lbw_amd.qk_head_norm_rope(*leaves, rope, pos)
+    dy = torch.randn(T, 2, d, generator=torch.Generator().manual_seed(21)).to(BF).cuda()
+    g = torch.empty(far + T * d, dtype=BF, device="cuda").as_strided((T, 2, d), (d, far, 1))
+    g.copy_(dy)
+    want = torch.autograd.grad(y, leaves, (dy, dy), retain_graph=True)
+    got = torch.autograd.grad(y, leaves, (g, g))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
