@@ -516,12 +516,24 @@ void refuse_foreign_leaves() {
   }
 }
 
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+
+// The operators have reverse-mode derivatives only: a forward-mode tangent is refused, not dropped.
+void refuse_tangents(const char* name, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*t), name, ": forward-mode derivatives are not implemented");
+}
+
 // A backward pass that builds no graph of its own calls the gradient operators below autograd (one that
-// does meets autograd's entry for them, which raises: they have no derivatives).
+// does, or that has tangents, meets autograd's entry for them, which raises: they have no derivatives).
 struct BelowAutograd {
   std::optional<at::AutoDispatchBelowADInplaceOrView> guard;
-  BelowAutograd() {
-    if (!at::GradMode::is_enabled()) guard.emplace();
+  BelowAutograd(const torch::autograd::variable_list& g, const torch::autograd::variable_list& saved) {
+    if (at::GradMode::is_enabled()) return;
+    for (const auto* ts : {&g, &saved})
+      for (const Tensor& t : *ts)
+        if (has_tangent(t)) return;
+    guard.emplace();
   }
 };
 
@@ -565,8 +577,8 @@ struct HeadNorm : torch::autograd::Function<HeadNorm> {
   }
   static torch::autograd::variable_list backward(Ctx* ctx, torch::autograd::variable_list g) {
     refuse_foreign_leaves();
-    const BelowAutograd below;
     const auto s = ctx->get_saved_variables();
+    const BelowAutograd below(g, s);
     const Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3];
     const Tensor dq_out = g[0].defined() ? g[0] : at::zeros_like(q);
     const Tensor dk_out = g[1].defined() ? g[1] : at::zeros_like(k);
@@ -587,6 +599,7 @@ std::tuple<Tensor, Tensor> head_norm_rope_autograd(const Tensor& q, const Tensor
                                                    bool inter, const Tensor& pos, double eps,
                                                    double qs, double ks) {
   const Tensor w0 = value_or_none(wq), w1 = value_or_none(wk);
+  refuse_tangents("head_norm_rope", {&q, &k, &w0, &w1});
   if (!any_grad({&q, &k, &w0, &w1})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_head_norm(q, k, wq, wk, rope, axes, inter, pos, eps, qs, ks);
@@ -617,8 +630,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   }
   static torch::autograd::variable_list backward(Ctx* ctx, torch::autograd::variable_list g) {
     refuse_foreign_leaves();
-    const BelowAutograd below;
     const auto s = ctx->get_saved_variables();
+    const BelowAutograd below(g, s);
     const Tensor none;
     if (!g[0].defined()) return {none, none, none, none, none, none, none};
     static auto op = handle<decltype(attention_packed_bwd)>("lbw::attention_packed_bwd");
@@ -633,6 +646,7 @@ std::tuple<Tensor, Tensor> attention_packed_autograd(const Tensor& q_, const Ten
                                                      const Tensor& v_, const Tensor& qi,
                                                      const Tensor& ki, at::IntArrayRef info,
                                                      double scale, bool want_lse) {
+  refuse_tangents("attention_packed", {&q_, &k_, &v_});
   const Tensor q = unit(q_), k = unit(k_), v = unit(v_);
   if (!any_grad({&q, &k, &v})) {
     at::AutoDispatchBelowADInplaceOrView below;

@@ -262,3 +262,19 @@ def test_compiled_step_gives_the_same_bits(backend):
     for run, f in ((step, forward), (serve, decode)):
         for got, want in zip(run(compiled(f)), run(f)):
             assert torch.equal(got, want)
+
+
+def test_a_tangent_of_the_outputs_gradient_is_refused():
+    """Forward mode over a backward pass: raised, as in the forward calls, not a derivative without it."""
+    import lbw_amd
+    import torch.autograd.forward_ad as fw
+    qkv, w, _, rope, pos, do = _setup(40, 10)
+    plan = lbw_amd.packed_plan([40])
+    q, k, v = _leaves(*[t.contiguous() for t in qkv.split([HQ, HK, HK], 1)])
+    outs = [lbw_amd.attention_packed(q, k, v, plan), lbw_amd.qk_head_norm_rope(q, k, *w, rope, pos)[0]]
+    for out in outs:
+        want = torch.autograd.grad(out, q, do, retain_graph=True)[0]
+        with fw.dual_level():
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(out, q, fw.make_dual(do, torch.ones_like(do)), retain_graph=True)
+        assert torch.equal(torch.autograd.grad(out, q, do)[0], want)

@@ -279,3 +279,36 @@ def test_token_limits_of_the_head_norm():
     for tokens in (1 << 21, most + 1, (1 << 31) - 1):
         assert lib.lbw_head_norm_rope_bwd(params(tokens), ctypes.byref(_lib.HeadNormRopeGrads()), None, 0, None) == 1
         assert b"dq_out must be" in lib.lbw_last_error()
+
+
+# ---- autograd's view of the operators: tensors without memory take the same entries
+
+def _meta(*s):
+    return torch.zeros(*s, dtype=BF, device="meta")
+
+
+def _meta_calls():
+    """name -> (call, its differentiable inputs)."""
+    plan = lbw().packed_plan([3, 2], device="cpu")
+    qi, ki = plan.q_items.to("meta"), plan.k_items.to("meta")
+    rope = lbw().axis_rope(torch.zeros(8, 64), device="meta")
+    pos = torch.zeros(5, dtype=torch.int32, device="meta")
+    w = lambda: torch.ones(128, dtype=BF, device="meta")  # noqa: E731
+    qkv = lambda: [_meta(5, 4, 128), _meta(5, 2, 128), _meta(5, 2, 128)]  # noqa: E731
+    norm = lambda q, k, wq, wk: lbw().qk_head_norm_rope(q, k, wq, wk, rope, pos)[0]  # noqa: E731
+    packed = lambda q, k, v: torch.ops.lbw.attention_packed(q, k, v, qi, ki, plan.info)[0]  # noqa: E731
+    return {"norm": (norm, qkv()[:2] + [w(), w()]), "packed": (packed, qkv())}
+
+
+@pytest.mark.parametrize("name,at", [("norm", i) for i in range(4)] + [("packed", i) for i in range(3)])
+def test_forward_mode_derivatives_are_refused(name, at):
+    import torch.autograd.forward_ad as fw
+    call, xs = _meta_calls()[name]
+    with fw.dual_level():
+        ds = [fw.make_dual(x, torch.ones_like(x)) if i == at else x for i, x in enumerate(xs)]
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            call(*ds)
+        assert call(*xs).shape == xs[0].shape  # (no tangent: as ever)
+    f = lambda x: call(*xs[:at], x, *xs[at + 1:])  # noqa: E731
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(f, (xs[at],), (torch.ones_like(xs[at]),))
