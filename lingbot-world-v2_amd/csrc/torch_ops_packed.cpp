@@ -546,6 +546,15 @@ bool any_grad(std::initializer_list<const Tensor*> ts) {
 Tensor value_or_none(const OptT& t) { return t.has_value() ? *t : Tensor(); }
 OptT opt(const Tensor& t) { return t.defined() ? OptT(t) : OptT(); }
 
+// The write forms give no gradient: with one wanted the call raises, as the tensors it writes would go on
+// without it.
+void refuse_gradients(const char* name, std::initializer_list<const Tensor*> ts) {
+  bool wanted = any_grad(ts);
+  for (const Tensor* t : ts) wanted = wanted || has_tangent(*t);
+  TORCH_CHECK_NOT_IMPLEMENTED(!wanted, name, " is not differentiable: call it under torch.no_grad(), or with "
+                              "tensors that require no gradient");
+}
+
 template <typename Sig>
 auto handle(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
@@ -606,6 +615,24 @@ std::tuple<Tensor, Tensor> head_norm_rope_autograd(const Tensor& q, const Tensor
   }
   auto r = HeadNorm::apply(q, k, wq, wk, rope, axes.vec(), inter, pos, eps, qs, ks);
   return {r[0], r[1]};
+}
+
+void head_norm_rope__autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const OptT& wq,
+                              const OptT& wk, const Tensor& rope, at::IntArrayRef axes, bool inter,
+                              const Tensor& pos, double eps, double q_scale, double k_scale, const Tensor& q_out,
+                              const Tensor& k_out, const OptT& v, const OptT& v_out, const OptT& rows) {
+  const Tensor w0 = value_or_none(wq), w1 = value_or_none(wk), vv = value_or_none(v), vo = value_or_none(v_out);
+  refuse_gradients("head_norm_rope_", {&q, &k, &w0, &w1, &vv, &q_out, &k_out, &vo});
+  static auto op = handle<decltype(head_norm_rope_)>("lbw::head_norm_rope_");
+  op.redispatch(ks & c10::after_autograd_keyset, q, k, wq, wk, rope, axes, inter, pos, eps, q_scale, k_scale, q_out, k_out,
+                v, v_out, rows);
+}
+
+void attention_decode_out_autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v,
+                                   const Tensor& lens, double scale, int64_t num_splits, const Tensor& out) {
+  refuse_gradients("attention_decode with out", {&q, &k, &v, &out});
+  static auto op = handle<decltype(attention_decode_out)>("lbw::attention_decode_out");
+  op.redispatch(ks & c10::after_autograd_keyset, q, k, v, lens, scale, num_splits, out);
 }
 
 auto call_packed(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& qi,
@@ -705,10 +732,10 @@ TORCH_LIBRARY_IMPL(lbw, Meta, m) {
 TORCH_LIBRARY_IMPL(lbw, Autograd, m) {
   m.impl("head_norm_rope", &head_norm_rope_autograd);
   m.impl("attention_packed", &attention_packed_autograd);
-  // no second derivatives, and none through the write forms and single-token attention: they raise
-  m.impl("head_norm_rope_", torch::autograd::autogradNotImplementedFallback());
+  m.impl("head_norm_rope_", TORCH_FN(head_norm_rope__autograd));
+  m.impl("attention_decode_out", TORCH_FN(attention_decode_out_autograd));
+  // no second derivatives, and none through single-token attention: their backward pass raises
   m.impl("head_norm_rope_bwd", torch::autograd::autogradNotImplementedFallback());
   m.impl("attention_packed_bwd", torch::autograd::autogradNotImplementedFallback());
   m.impl("attention_decode", torch::autograd::autogradNotImplementedFallback());
-  m.impl("attention_decode_out", torch::autograd::autogradNotImplementedFallback());
 }

@@ -312,3 +312,50 @@ def test_forward_mode_derivatives_are_refused(name, at):
     f = lambda x: call(*xs[:at], x, *xs[at + 1:])  # noqa: E731
     with pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.jvp(f, (xs[at],), (torch.ones_like(xs[at]),))
+
+
+def _write_calls():
+    """name -> (call, inputs by name, written tensors by name)."""
+    rope = lbw().axis_rope(torch.zeros(8, 64), device="meta")
+    pos = torch.zeros(5, dtype=torch.int32, device="meta")
+    w = lambda: torch.ones(128, dtype=BF, device="meta")  # noqa: E731
+
+    def append(q, k, wq, wk, v, q_out, k_out, v_out):
+        lbw().qk_head_norm_rope_(q, k, wq, wk, rope, pos, q_out=q_out, k_out=k_out, v=v, v_out=v_out, rows=pos)
+
+    def decode(q, k_cache, v_cache, out):
+        lbw().attention_decode(q, k_cache, v_cache, pos, out=out)
+    return {"append": (append, dict(q=_meta(5, 4, 128), k=_meta(5, 2, 128), wq=w(), wk=w(), v=_meta(5, 2, 128)),
+                       dict(q_out=_meta(5, 4, 128), k_out=_meta(5, 9, 2, 128), v_out=_meta(5, 9, 2, 128))),
+            "decode": (decode, dict(q=_meta(5, 4, 128), k_cache=_meta(5, 9, 2, 128), v_cache=_meta(5, 9, 2, 128)),
+                       dict(out=_meta(5, 4, 128)))}
+
+
+@pytest.mark.parametrize("name,arg", [("append", a) for a in ("q", "k", "wq", "wk", "v", "q_out", "k_out", "v_out")] +
+                         [("decode", a) for a in ("q", "k_cache", "v_cache", "out")])
+def test_write_forms_refuse_tensors_that_require_a_gradient(name, arg):
+    import torch.autograd.forward_ad as fw
+    call, ins, outs = _write_calls()[name]
+    args = {**ins, **outs}
+    args[arg].requires_grad_()
+    with pytest.raises(NotImplementedError, match="not differentiable"):
+        call(**args)
+    with torch.no_grad():
+        call(**args)
+    args[arg] = args[arg] * 1                     # (of a graph, and not a leaf)
+    with pytest.raises(NotImplementedError, match="not differentiable"):
+        call(**args)
+    args[arg] = args[arg].detach()
+    call(**args)
+    with fw.dual_level():
+        args[arg] = fw.make_dual(args[arg], torch.ones_like(args[arg]))
+        with pytest.raises(NotImplementedError, match="not differentiable"):
+            call(**args)
+
+
+def test_in_place_in_a_graph_is_refused():
+    """q of a projection that is trained, overwritten: its gradient would miss the norm and the rotation."""
+    call, ins, outs = _write_calls()["append"]
+    q = _meta(5, 4, 128).requires_grad_() * 2
+    with pytest.raises(NotImplementedError, match="not differentiable"):
+        call(**{**ins, **outs, "q": q, "q_out": q})
