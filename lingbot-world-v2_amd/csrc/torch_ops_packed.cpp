@@ -23,6 +23,7 @@
 #include <vector>
 
 #include "lbw_attn.h"
+#include "torch_written.h"
 
 namespace {
 
@@ -738,4 +739,9 @@ TORCH_LIBRARY_IMPL(lbw, Autograd, m) {
   m.impl("head_norm_rope_bwd", torch::autograd::autogradNotImplementedFallback());
   m.impl("attention_packed_bwd", torch::autograd::autogradNotImplementedFallback());
   m.impl("attention_decode", torch::autograd::autogradNotImplementedFallback());
+}
+
+TORCH_LIBRARY_IMPL(lbw, ADInplaceOrView, m) {
+  LBW_COUNT_WRITES(m, head_norm_rope_);
+  LBW_COUNT_WRITES(m, attention_decode_out);
 }

@@ -359,3 +359,30 @@ def test_in_place_in_a_graph_is_refused():
     q = _meta(5, 4, 128).requires_grad_() * 2
     with pytest.raises(NotImplementedError, match="not differentiable"):
         call(**{**ins, **outs, "q": q, "q_out": q})
+
+
+@pytest.mark.parametrize("name", ["append", "decode"])
+@pytest.mark.parametrize("mode", [torch.enable_grad, torch.no_grad, torch.inference_mode])
+def test_writes_are_counted(name, mode):
+    call, ins, outs = _write_calls()[name]
+    before = {n: t._version for n, t in {**ins, **outs}.items()}
+    with mode():
+        call(**ins, **outs)
+    assert all(t._version == before[n] for n, t in ins.items())
+    assert all(t._version == before[n] + 1 for n, t in outs.items())
+    with torch.inference_mode():
+        outs = {n: torch.zeros_like(t) for n, t in outs.items()}
+        call(**ins, **outs)                       # inference tensors, which have no count
+    with torch.no_grad():
+        call(**ins, **outs)
+
+
+@pytest.mark.parametrize("name,out", [("append", "q_out"), ("append", "k_out"), ("append", "v_out"), ("decode", "out")])
+def test_backward_over_an_overwritten_tensor_raises(name, out):
+    call, ins, outs = _write_calls()[name]
+    h = torch.zeros_like(outs[out]).requires_grad_() * 1
+    y = (h * h).sum()
+    outs[out] = h.detach()
+    call(**ins, **outs)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
