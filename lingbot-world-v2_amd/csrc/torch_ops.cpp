@@ -22,6 +22,7 @@
 #include <vector>
 
 #include "lbw_attn.h"
+#include "torch_written.h"
 
 namespace {
 
@@ -710,4 +711,14 @@ TORCH_LIBRARY_IMPL(lbw, Meta, m) {
   m.impl("attention_merge_out", &attention_merge_out_meta);
   m.impl("qk_norm_rope_", &qk_norm_rope_meta);
   m.impl("kv_quant_fp8_", &kv_quant_fp8_meta);
+}
+
+TORCH_LIBRARY_IMPL(lbw, ADInplaceOrView, m) {
+  LBW_COUNT_WRITES(m, attention_out);
+  LBW_COUNT_WRITES(m, cross_attention_out);
+  LBW_COUNT_WRITES(m, attention_fp8kv_out);
+  LBW_COUNT_WRITES(m, attention_chain_out);
+  LBW_COUNT_WRITES(m, attention_merge_out);
+  LBW_COUNT_WRITES(m, qk_norm_rope_);
+  LBW_COUNT_WRITES(m, kv_quant_fp8_);
 }
