@@ -326,7 +326,7 @@ typedef struct lbw_packed_params {
   const void* v; int64_t v_stride_l, v_stride_h;
   void* out; int64_t out_stride_l, out_stride_h;
   float* lse;                      /* fp32 [q_heads][q_tokens], natural log; NULL: not wanted */
-  float softmax_scale;             /* > 0; 0: 1 / sqrt(head_dim) */
+  float softmax_scale;             /* 1e-30 to 1e6; 0: 1 / sqrt(head_dim) */
   const int32_t* q_items; int32_t n_q_items;
   const int32_t* k_items; int32_t n_k_items; /* gradient only */
   /* the plan's tile counts, by which long items are cut into pieces when there are few (0: never cut) */
@@ -359,7 +359,7 @@ typedef struct lbw_decode_params {
   const void* v; int64_t v_stride_b, v_stride_l, v_stride_h;
   const int32_t* lens;
   void* out; int64_t out_stride_b, out_stride_h;
-  float softmax_scale;             /* > 0; 0: 1 / sqrt(head_dim) */
+  float softmax_scale;             /* 1e-30 to 1e6; 0: 1 / sqrt(head_dim) */
   int32_t num_splits;              /* 1: a workgroup per sequence and key/value head; n: the batch's keys in
                                     * n * batch equal pieces, joined after; 0: chosen by the library */
 } lbw_decode_params;

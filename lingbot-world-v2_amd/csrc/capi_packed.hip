@@ -53,7 +53,11 @@ int check_heads(int32_t hq, int32_t hk) {
 int check_scale(float s, int head_dim, float* scale) {
   if (!(s >= 0.0f) || isinf(s))
     return fail(LBW_ERR_INVALID, "softmax_scale must be positive and finite (0: 1/sqrt(head_dim))");
-  if (s > 0.0f && s < 1e-30f) return fail(LBW_ERR_UNSUPPORTED, "softmax_scale %g below 1e-30", s);
+  // A row's exponents are taken against its reference times the scale, rounded to fp32: half a step of it is a
+  // factor that all of the row's weights have in common, as long as it does not leave fp32 (a scaled score up to
+  // 2^28 is off by 16 at most; at a scale of 1e8 ordinary scores gave sums of 0 and of infinity).
+  if (s > 0.0f && (s < 1e-30f || s > 1e6f))
+    return fail(LBW_ERR_UNSUPPORTED, "softmax_scale %g not in [1e-30, 1e6]", s);
   *scale = s > 0.0f ? s : 1.0f / sqrtf((float)head_dim);
   return LBW_OK;
 }

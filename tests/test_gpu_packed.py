@@ -296,3 +296,18 @@ def test_head_dim_that_is_not_contiguous_is_copied_without_autograd_too():
         grads = lbw_amd.attention_packed_backward(do.clone(), *xs, out, lse, plan)
     for n, x in zip(("out", "lse", "dq", "dk", "dv"), (out, lse) + tuple(grads)):
         assert torch.equal(x, want[n])
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-6, 1e3, 1e6, 1e8])
+def test_rows_without_keys_at_every_scale(scale):
+    import lbw_amd
+    ql, kl = [200, 5], [37, 2]
+    q, k, v, _ = _data(ql, kl, 4, 2, 15)
+    if scale > 1e6:  # ordinary scores times it leave what fp32 holds of an exponent: 0 and NaN
+        with pytest.raises(RuntimeError, match="softmax_scale"):
+            lbw_amd.attention_packed(q, k, v, lbw_amd.packed_plan(ql, kl), softmax_scale=scale)
+        return
+    out, lse = lbw_amd.attention_packed(q, k, v, lbw_amd.packed_plan(ql, kl), softmax_scale=scale, return_lse=True)
+    none = torch.zeros(205, dtype=torch.bool, device="cuda")
+    none[:163] = none[200:203] = True
+    assert torch.all(out[none] == 0) and torch.equal(lse == -math.inf, none.expand(4, 205))

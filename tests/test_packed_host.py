@@ -386,3 +386,20 @@ def test_backward_over_an_overwritten_tensor_raises(name, out):
     call(**ins, **outs)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("scale,status", [(1e-31, 2), (2e6, 2), (1e8, 2), (3e38, 2), (float("inf"), 1), (-1.0, 1)])
+def test_scales_that_leave_fp32_are_refused(scale, status):
+    """At 1e8 rows of ordinary scores gave 0 or NaN, from 3e8 on rows that see no key gave NaN."""
+    from lbw_amd import _lib
+    lib = _lib.load()
+    p = _lib.PackedParams(q_heads=4, k_heads=2, head_dim=128, softmax_scale=scale)
+    assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None, 0, None) == status
+    assert b"softmax_scale" in lib.lbw_last_error()
+    assert lib.lbw_attention_packed_bwd(ctypes.byref(p), ctypes.byref(_lib.PackedGrads()), None, 0, None) == status
+    d = _lib.DecodeParams(batch=0, q_heads=4, k_heads=2, head_dim=128, softmax_scale=scale)
+    assert lib.lbw_attention_decode(ctypes.byref(d), None, 0, None) == status
+    for ok in (1e-30, 0.0, 1e6):
+        p.softmax_scale = d.softmax_scale = ok
+        assert lib.lbw_attention_packed_fwd(ctypes.byref(p), None, 0, None) == 0
+        assert lib.lbw_attention_decode(ctypes.byref(d), None, 0, None) == 0
