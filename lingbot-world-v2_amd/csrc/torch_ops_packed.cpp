@@ -59,6 +59,14 @@ void check_int32(const char* name, const Tensor& t, const Tensor& like) {
 // smaller ones' reach; layouts that nest leave one or two t a stride. A search that takes long counts as shared.
 bool may_overlap(const Tensor& a, const Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return false;
+  const int64_t bytes = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr());
+  auto reach = [](const Tensor& t) {  // bytes from the first element's to past the last one's
+    int64_t n = 1;
+    for (int64_t d = 0; d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+    return 2 * n;
+  };
+  if (bytes >= reach(a) || -bytes >= reach(b)) return false;  // (as most are: tensors of their own)
+  if (bytes % 2 != 0) return true;
   struct Dim {
     int64_t s, lo, hi;        // lo <= t <= hi
     int64_t from, to;         // what this and the smaller strides add up to, at least and at most
@@ -79,8 +87,6 @@ bool may_overlap(const Tensor& a, const Tensor& b) {
     dims[i].from = from += dims[i].lo * dims[i].s;
     dims[i].to = to += dims[i].hi * dims[i].s;
   }
-  const int64_t bytes = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr());
-  if (bytes % 2 != 0) return from * 2 - 2 < bytes && bytes < to * 2 + 2;
   int budget = 4096;
   auto search = [&](auto& self, size_t i, int64_t c) -> bool {
     if (i == dims.size()) return c == 0;
