@@ -258,7 +258,8 @@ int lbw_kv_quant_fp8(const void* x, int32_t batch, int64_t len, int32_t heads,
  * Optional: v copied to v_out. With `rows` (int32 [tokens], device), token t is the new token of
  * sequence t and its k and v go to row rows[t] (0 <= rows[t] < row_count, else not written) of
  * k_out / v_out [tokens][row_count][k_heads][head_dim], whose sequences are *_stride_b apart.
- * Outputs may be the inputs themselves, and must not overlap them otherwise. */
+ * Outputs may be the inputs themselves, and must not share an element with them otherwise. At most 67108860
+ * tokens (the gradient: any number); a tensor's heads less than 2^26 elements apart. */
 #define LBW_MAX_AXES 4
 #define LBW_W_BF16 0
 #define LBW_W_FP32 1

@@ -355,6 +355,10 @@ __global__ void __launch_bounds__(JW * 64) decode_join_kernel(const DecodeArgs a
 // Pieces per key/value head (and block of 32 of its query heads): none while whole sequences give work
 // enough or caches are short, else as many as run at once, two workgroups a CU, of 6 tiles or more (of 4 / 6 / 8:
 // one sequence of 5000 keys x 40/8 heads 14.4 / 12.9 / 13.3 us, two of 5000 x 12/4 14.3 / 12.9 / 14.7).
+// Short, whole / cut, x 40/8 heads: one sequence of 500 keys 7.4 / 9.7 us, of 1000 9.9 / 9.8, of 1500 12.2 / 10.0;
+// four of 500 7.6 / 10.5, of 1000 10.6 / 11.2, of 1500 13.1 / 11.5; sixteen of 1000 15.7 / 18.9, of 1500 20.4 / 23.3.
+// The rule sees the capacity, as lengths are on the device: few keys in a long cache are cut (500 in 4096 rows: the
+// 9.7 us above), and from batch x units = 2 x CUs on one long sequence among short ones is not.
 int decode_pieces(int64_t B, int Hq, int Hk, int64_t S, int num_splits, int cus) {
   const int64_t units = (int64_t)Hk * ((Hq / Hk + HEADS - 1) / HEADS);
   if (num_splits == 1) return 0;

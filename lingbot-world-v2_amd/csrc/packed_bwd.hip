@@ -10,9 +10,10 @@
 // -lse / scale and its dP from -delta, so P and dS take one operation each from the accumulators.
 // Both recompute S; P and dS go to bf16 as operands, one rounding each.
 //
-// Bound by the matrix cores at the clock that the chip holds under them: 4680 + 3599 + 2340 causal tokens x
-// 40/8 heads dQ 568 us (1091 TFLOP/s of its three products, MFMA busy 66 % of the cycles at 1.5 GHz), dK and dV
-// 846 us (977 of its four, 58 % at 1.65 GHz; a library product of 16384^3 reaches 1364).
+// Bound by matrix products and by what stands between them: 4680 + 3599 + 2340 causal tokens x 40/8 heads dQ 568 us
+// (1091 TFLOP/s of its three products, MFMA busy 66 % of the cycles at 1.5 GHz), dK and dV 846 us (977 of its four,
+// 58 % at 1.65 GHz; a library product of 16384^3 reaches 1364). The formula needs five products; S and dP are made in
+// both kernels.
 
 #include "capi_util.h"
 #include "packed_tiles.h"

@@ -14,10 +14,13 @@
 //
 // P goes to bf16 as the second product's operand: one rounding of each weight, which l does not see.
 //
-// Bound by the matrix cores at the clock that the chip holds under them: 4680 + 3600 + 1561 causal tokens x
-// 40/8 heads 394 us, 970 TFLOP/s (a library product of 16384^3 reaches 1364); the MFMA pipes are busy 55 % of
-// the cycles at 1.65 GHz. Two workgroups a CU hide each other's barriers: one of eight waves, half the keys to
-// each four, in step, took 522 us where two of four waves took 437.
+// 4680 + 3600 + 1561 causal tokens x 40/8 heads 394 us, 970 TFLOP/s (a library product of 16384^3 reaches 1364);
+// the MFMA pipes are busy 55 % of the cycles at 1.65 GHz. That is not their limit: on the same products (3600 rows
+// over 46800 keys x 40 heads, full, one run) the chunk attention kernel keeps them busy 65 % of the cycles at 1.70
+// GHz, this one 58 % at 1.51 GHz (3278 / 4121 us). It has 17 % fewer vector instructions, three stages and counted
+// waits where this one waits for all copies at every tile, and 256 queries to a tile of K and V where this one has
+// 128; which of these costs what is not measured. Two workgroups a CU hide each other's barriers: one of eight
+// waves, half the keys to each four, in step, took 522 us where two of four waves took 437.
 
 #include "capi_util.h"
 #include "packed_tiles.h"

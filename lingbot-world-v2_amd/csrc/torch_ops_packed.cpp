@@ -631,8 +631,8 @@ void head_norm_rope__autograd(c10::DispatchKeySet ks, const Tensor& q, const Ten
   const Tensor w0 = value_or_none(wq), w1 = value_or_none(wk), vv = value_or_none(v), vo = value_or_none(v_out);
   refuse_gradients("head_norm_rope_", {&q, &k, &w0, &w1, &vv, &q_out, &k_out, &vo});
   static auto op = handle<decltype(head_norm_rope_)>("lbw::head_norm_rope_");
-  op.redispatch(ks & c10::after_autograd_keyset, q, k, wq, wk, rope, axes, inter, pos, eps, q_scale, k_scale, q_out, k_out,
-                v, v_out, rows);
+  op.redispatch(ks & c10::after_autograd_keyset, q, k, wq, wk, rope, axes, inter, pos, eps, q_scale, k_scale,
+                q_out, k_out, v, v_out, rows);
 }
 
 void attention_decode_out_autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v,

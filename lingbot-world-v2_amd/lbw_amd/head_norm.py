@@ -86,7 +86,8 @@ def qk_head_norm_rope(q, k, wq, wk, rope: AxisRope, pos, eps: float = 1e-6, *,
     with a contiguous head dim are fine, e.g. column blocks of a fused projection; D 32, 64, 128 or
     256). ``wq``, ``wk``: ``[D]`` weights, both bf16 or both fp32, or None. ``pos``: int32
     ``[tokens, axes]`` (``[tokens]`` for one axis) on q's device; a position outside the table turns its
-    pairs into NaN. Differentiable in q, k, wq and wk (first derivatives; the same bits every run)."""
+    pairs into NaN. Differentiable in q, k, wq and wk (first derivatives, reverse mode; the same bits every
+    run)."""
     try:
         return _lib.ops().head_norm_rope(q, k, wq, wk, rope.table, rope.axes, rope.interleaved, pos,
                                          eps, q_scale, k_scale)
@@ -101,7 +102,9 @@ def qk_head_norm_rope_(q, k, wq, wk, rope: AxisRope, pos, eps: float = 1e-6, *, 
     copied to ``v_out`` when given. With ``rows`` (int32 ``[tokens]`` on q's device) token t is the
     newest one of sequence t: its k and v go to row ``rows[t]`` of the caches ``k_out``, ``v_out``
     ``[tokens, capacity, kv_heads, D]`` (strided views are fine), and are not written where that row
-    is outside the cache. Not differentiable. Returns ``(q_out, k_out)``."""
+    is outside the cache. Outputs may interleave with other tensors of the call, not share an element with
+    one. Not differentiable: raises while gradients are recorded and one of the tensors, weights included,
+    requires one (``torch.no_grad`` takes it). Returns ``(q_out, k_out)``."""
     try:
         _lib.ops().head_norm_rope_(q, k, wq, wk, rope.table, rope.axes, rope.interleaved, pos, eps,
                                    q_scale, k_scale, q_out, k_out, v, v_out, rows)

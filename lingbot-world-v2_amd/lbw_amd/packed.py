@@ -98,10 +98,10 @@ def attention_packed(q, k, v, plan: PackedPlan, *, softmax_scale: float | None =
                      return_lse: bool = False):
     """softmax(scale Q K^T) V of every sequence of ``plan``: q ``[q_tokens, heads, 128]``, k, v
     ``[k_tokens, kv_heads, 128]`` bf16 (strided views are fine, 16-byte rows) -> out like q; scale
-    default 1/sqrt(128). ``return_lse``: also lse fp32 ``[heads, q_tokens]`` (natural log; no gradient
+    default 1/sqrt(128), at most 1e6. ``return_lse``: also lse fp32 ``[heads, q_tokens]`` (natural log; no gradient
     flows through it). A query that sees no key gives 0, lse -inf and no gradient. Nothing of one
     sequence reaches another, whatever its values; inside a sequence a NaN or infinity may also reach
-    rows that do not see it. Differentiable in q, k, v (first derivatives). A training step captured into
+    rows that do not see it. Differentiable in q, k, v (first derivatives, reverse mode). A training step captured into
     a graph must not share leaves with a live eager graph of another stream: that backward raises."""
     scale = _scale(softmax_scale)
     try:
@@ -135,7 +135,8 @@ def attention_decode(q, k_cache, v_cache, lens, *, softmax_scale: float | None =
     ``[batch, capacity, kv_heads, 128]`` (strided views are fine), keys ``0 .. lens[b] - 1`` of
     sequence b -> ``[batch, heads, 128]`` (into ``out`` when given). ``lens`` int32 ``[batch]`` on q's device
     is read there (no host sync; limited to ``[0, capacity]``); rows behind a length may hold
-    anything. A sequence of no keys gives 0. ``num_splits`` 1: one workgroup per sequence and kv head; n: the whole batch's
+    anything. A sequence of no keys gives 0. Not differentiable; with ``out`` it raises while gradients are
+    recorded and one of the tensors requires one. ``num_splits`` 1: one workgroup per sequence and kv head; n: the whole batch's
     keys cut into ``n * batch`` equal pieces that run side by side; 0: by batch, heads and capacity."""
     s = _scale(softmax_scale)
     try:
