@@ -368,6 +368,88 @@ size_t lbw_attention_decode_workspace_size(const lbw_decode_params* p);
 int lbw_attention_decode(const lbw_decode_params* p, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* ---- A paged key/value cache: serving beside the per-sequence caches above.
+ *
+ * A page holds page_size consecutive tokens (a power of two, 16 to 1024) of one sequence, k and v bf16
+ * [pages][page_size][k_heads][head_dim] with any strides that are multiples of 8 elements (token strides below 2^24);
+ * table int32 [batch][table_width] on the device: entry j of a row is the page of the sequence's tokens
+ * j * page_size ... Sequences may share pages that none of them writes to any more. bounds, optional: bf16
+ * [pages][k_heads][2][head_dim], contiguous, the smallest and the largest value of each key component of a page.
+ * Entries behind a sequence's length are not read. A page outside the cache is never followed: what would go there is
+ * not written, keys that would come from there make the result NaN, and it counts as the highest when pages are
+ * selected. */
+typedef struct lbw_paged_kv {
+  void* k; int64_t k_stride_p, k_stride_l, k_stride_h; /* page, token, head */
+  void* v; int64_t v_stride_p, v_stride_l, v_stride_h;
+  void* bounds;
+  int32_t pages, page_size;
+  const int32_t* table; int64_t table_stride;
+  int32_t table_width;
+} lbw_paged_kv;
+
+/* New tokens: q and k normalised per head (norm != 0, as lbw_head_norm_rope) or not, their pairs turned by the tokens'
+ * positions (pos; NULL: a token's row in its sequence, one axis), q into q_out, k and v into their rows of the cache,
+ * the bounds kept up. Token t of sequence b (starts[b] <= t < starts[b + 1], int32 [batch + 1] on the device; NULL:
+ * token t is sequence t's, batch == tokens) goes to row lens[b] + t - starts[b]; a row outside the table is not
+ * written. Tokens outside every sequence are left alone, their q_out too. q_out may be q itself. A page that gets its
+ * row 0 starts its bounds anew. No two sequences may be given tokens for one page. */
+typedef struct lbw_paged_append_params {
+  lbw_paged_kv cache;
+  int32_t tokens, batch, q_heads, k_heads, head_dim;
+  const void* q; int64_t q_stride_l, q_stride_h;
+  const void* k; int64_t k_stride_l, k_stride_h;
+  const void* v; int64_t v_stride_l, v_stride_h;
+  const void* wq; const void* wk;  /* [head_dim] or NULL (1); norm only */
+  int32_t w_dtype, norm;
+  float eps;
+  const float* rope; int64_t rope_rows;
+  int32_t rope_pairs, n_axes;
+  int32_t axis_pairs[LBW_MAX_AXES];
+  int32_t interleaved;
+  const int32_t* pos; int64_t pos_stride;
+  const int32_t* starts;
+  const int32_t* lens;             /* int32 [batch], device: rows so far */
+  void* q_out; int64_t q_out_stride_l, q_out_stride_h;
+  float q_out_scale, k_out_scale;
+} lbw_paged_append_params;
+int lbw_paged_append(const lbw_paged_append_params* p, void* stream);
+
+/* One query token per sequence over its pages: as lbw_attention_decode. With `selected` (int32
+ * [batch][k_heads][n_selected], device, contiguous) a key/value head attends to the table entries it names, up to the
+ * first negative one (an entry named twice counts twice). With a prefix (int32 [prefix_width] pages, min(*prefix_len,
+ * prefix_keys) keys; prefix_len NULL: prefix_keys) those keys come before every sequence's own and are read once for
+ * the batch. */
+typedef struct lbw_attention_paged_params {
+  lbw_paged_kv cache;
+  int32_t batch, q_heads, k_heads, head_dim;
+  const void* q; int64_t q_stride_b, q_stride_h;
+  const int32_t* lens;             /* int32 [batch], device: keys, limited to [0, table_width * page_size] */
+  const int32_t* selected; int32_t n_selected;
+  const int32_t* prefix_table; int32_t prefix_width;
+  const int32_t* prefix_len;       /* int32 [1], device */
+  int64_t prefix_keys;             /* at most prefix_width * page_size; 0: no prefix */
+  void* out; int64_t out_stride_b, out_stride_h;
+  float softmax_scale;             /* 1e-30 to 1e6; 0: 1 / sqrt(head_dim) */
+  int32_t num_splits;              /* as lbw_attention_decode; selected pages, prefix: cut into so many pieces */
+} lbw_attention_paged_params;
+size_t lbw_attention_paged_workspace_size(const lbw_attention_paged_params* p);
+int lbw_attention_paged(const lbw_attention_paged_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The pages a query token should look at, int32 [batch][k_heads][count], ascending, -1 behind them: a sequence's `first`
+ * first and `last` last pages, then those of the highest max over the group's heads of
+ * sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d (ties: the lower entry; NaN counts as infinity; sums in 64 bits). All
+ * pages when there are no more than count. first + last <= count. */
+typedef struct lbw_paged_select_params {
+  lbw_paged_kv cache;              /* k and v are not read */
+  int32_t batch, q_heads, k_heads, head_dim;
+  const void* q; int64_t q_stride_b, q_stride_h;
+  const int32_t* lens;
+  int32_t count, first, last;
+  int32_t* selected;
+} lbw_paged_select_params;
+size_t lbw_paged_select_workspace_size(const lbw_paged_select_params* p);
+int lbw_paged_select(const lbw_paged_select_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
 const char* lbw_last_error(void);
 int lbw_abi_version(void);
 

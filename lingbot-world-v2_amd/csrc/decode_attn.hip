@@ -21,6 +21,7 @@
 
 #include "capi_util.h"
 #include "packed_tiles.h"
+#include "sequence_tiles.h"
 
 namespace lbw {
 namespace {
@@ -31,54 +32,9 @@ constexpr int RING_B = 2 * DT_B;            // per wave: K, V
 constexpr int NCOPY = DT_B / 1024;          // copies per lane for K or V of a tile
 constexpr int HEADS = 32;                   // query heads per workgroup
 
-// A value that every lane holds, in scalar registers.
-__device__ __forceinline__ int64_t scalar64(int64_t x) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
-  return (int64_t)(((uint64_t)hi << 32) | lo);
-}
 __device__ __forceinline__ int tiles_of(const DecodeArgs& a, int b) {
   const int n = a.lens[b];
   return ((n < 0 ? 0 : (n > a.S ? a.S : n)) + DT - 1) / DT;
-}
-// Tiles of all sequences together and, with `upto`, of those before it.
-__device__ __forceinline__ void count_tiles_of(const DecodeArgs& a, int lane, int upto, int64_t& all,
-                                               int64_t& before) {
-  int64_t x = 0, y = 0;
-  for (int b = lane; b < a.B; b += 64) {
-    const int n = tiles_of(a, b);
-    x += n;
-    if (b < upto) y += n;
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    x += __shfl_xor(x, o);
-    y += __shfl_xor(y, o);
-  }
-  all = scalar64(x);
-  before = scalar64(y);
-}
-// The sequence that tile `t` belongs to (0 <= t < all), and the tiles before it.
-__device__ __forceinline__ int find_sequence(const DecodeArgs& a, int lane, int64_t t, int64_t& before) {
-  int64_t base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int n = b0 + lane < a.B ? tiles_of(a, b0 + lane) : 0;
-    int64_t sum = n;  // inclusive
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t y = __shfl_up(sum, o);
-      if (lane >= o) sum += y;
-    }
-    const uint64_t past = __ballot(base + sum > t);
-    if (past != 0) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      before = scalar64(base + __shfl(sum - n, l));
-      return __builtin_amdgcn_readfirstlane(b0 + l);
-    }
-    base += __shfl(sum, 63);
-  }
-  before = base;
-  return a.B;
 }
 
 template <int DW>  // waves per workgroup
@@ -101,13 +57,13 @@ __global__ void __launch_bounds__(DW * 64, 2) decode_kernel(const DecodeArgs a) 
   int64_t at = 0, end = 1, before = 0;
   if (a.pieces > 0) {
     int64_t all, none;
-    count_tiles_of(a, lane, 0, all, none);
+    count_tiles_of(a.B, [&](int s) { return tiles_of(a, s); }, lane, 0, all, none);
     // (no more pieces than tiles: an empty one between two parts of a sequence would leave a row unwritten)
     const int64_t pieces = all < a.pieces ? all : a.pieces;
     if (piece >= pieces) return;
     at = all * piece / pieces;
     end = all * (piece + 1) / pieces;
-    b = find_sequence(a, lane, at, before);
+    b = find_sequence(a.B, [&](int s) { return tiles_of(a, s); }, lane, at, before);
     if (b >= a.B) return;
   }
 
@@ -285,7 +241,7 @@ __global__ void __launch_bounds__(JW * 64) decode_join_kernel(const DecodeArgs a
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int b = (int)(blockIdx.x / (uint32_t)a.Hq), h = (int)(blockIdx.x % (uint32_t)a.Hq);
   int64_t all, before;
-  count_tiles_of(a, lane, b, all, before);
+  count_tiles_of(a.B, [&](int s) { return tiles_of(a, s); }, lane, b, all, before);
   const int tiles = __builtin_amdgcn_readfirstlane(tiles_of(a, b));
   float x = 0.0f, y = 0.0f, L = 0.0f, M = -INFINITY;
   if (tiles > 0) {

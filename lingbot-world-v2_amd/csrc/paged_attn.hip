@@ -1,0 +1,438 @@
+// Attention of one query token per sequence over a paged cache (gfx950).
+//
+//   out[b, h] = softmax(scale q[b, h] K^T) V over the keys of a common prefix (if any), then the sequence's own:
+//   all keys 0 .. len[b] - 1, or those of the selected pages; key/value head h / (Hq / Hk); no keys give 0.
+//
+// Bound by reading K and V once. The work of a workgroup is as in the single-token attention over whole caches: one
+// key/value head, up to 32 query rows as the columns of S^T = K Q^T, 4 or 8 waves that take 32-key tiles in turn,
+// each through 16 KB of LDS of its own, and join their results at the end. Here a tile is two halves of 16
+// tokens, each inside one page (pages are 16 tokens or more). The pages of a wave's next 32 tiles are looked
+// up at once, one half a lane, and handed to the scalar side a tile ahead.
+//
+// The prefix's keys are the same for the whole batch: its query rows are those of all sequences, 32 at a time.
+//
+// A half's rows past its last key copy that key (or the other half's), so the products never meet what lies
+// behind a sequence. A page outside the cache makes its keys' scores NaN.
+
+#include <algorithm>
+
+#include "capi_util.h"
+#include "packed_tiles.h"
+#include "paged.h"
+#include "sequence_tiles.h"
+
+namespace lbw {
+namespace {
+
+constexpr int DT = 32;                      // keys per tile
+constexpr int HT = DT / 2;                  // keys per half
+static_assert(HT == HALF_KEYS, "half_at looks up half a tile");
+constexpr int DT_B = DT * PK_ROWB;          // 8 KB
+constexpr int RING_B = 2 * DT_B;            // per wave: K, V
+constexpr int NCOPY = DT_B / 1024;          // copies per lane for K or V of a tile
+constexpr int HEADS = 32;                   // query rows per workgroup
+enum Kind { DENSE, SPARSE, PREFIX };
+
+// A sequence's keys: its length, limited to what its row of the table holds.
+__device__ __forceinline__ int keys_of(const PagedAttnArgs& a, int b) {
+  const int64_t cap = (int64_t)a.pt.width << a.pt.shift;
+  const int n = a.lens[b];
+  return n < 0 ? 0 : (n > cap ? (int)cap : n);
+}
+__device__ __forceinline__ int tiles_of(const PagedAttnArgs& a, int b) { return (int)(((int64_t)keys_of(a, b) + DT - 1) / DT); }
+__device__ __forceinline__ int64_t prefix_keys(const PagedAttnArgs& a) {
+  int64_t n = a.p_len != nullptr ? a.p_len[0] : a.p_max;
+  return n < 0 ? 0 : (n > a.p_max ? a.p_max : n);
+}
+// Entries of a list of selected pages: those before the first negative one.
+__device__ __forceinline__ int list_length(const int32_t* sel, int n, int lane) {
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const uint64_t stop = __ballot(i0 + lane < n && sel[i0 + lane] < 0);
+    if (stop != 0) return i0 + __ffsll((unsigned long long)stop) - 1;
+  }
+  return n;
+}
+
+template <int DW, Kind KIND>  // waves per workgroup
+__global__ void __launch_bounds__(DW * 64, 2) paged_kernel(const PagedAttnArgs a) {
+  constexpr int DEC_LDS = DW * RING_B;
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hl = lane >> 5, l32 = lane & 31;
+  const int group = a.Hq / a.Hk;
+  const int64_t rows_all = KIND == PREFIX ? (int64_t)a.B * group : group;  // query rows of a key/value head
+  const uint32_t blocks = (uint32_t)((rows_all + HEADS - 1) / HEADS);
+  uint32_t id = blockIdx.x;
+  const int kv = id % (uint32_t)a.Hk;
+  id /= (uint32_t)a.Hk;
+  const int64_t r0 = (int64_t)(id % blocks) * HEADS;
+  const int piece = id / blocks;
+  const int nr = (int)(rows_all - r0 < HEADS ? rows_all - r0 : HEADS);
+  const bool end_to_end = KIND == DENSE && a.pieces > 0;
+  const int splits = KIND == PREFIX ? a.p_splits : a.splits;
+
+  // this workgroup's tiles [at, end) of the batch laid end to end, from sequence b on
+  int b = KIND == PREFIX ? 0 : piece / (end_to_end ? 1 : splits);
+  const int split = end_to_end ? 0 : (KIND == PREFIX ? piece : piece % splits);
+  int64_t at = 0, end = 1, before = 0;
+  if (end_to_end) {
+    int64_t all, none;
+    count_tiles_of(a.B, [&](int s) { return tiles_of(a, s); }, lane, 0, all, none);
+    // (no more pieces than tiles: an empty one between two parts of a sequence would leave a row unwritten)
+    const int64_t pieces = all < a.pieces ? all : a.pieces;
+    if (piece >= pieces) return;
+    at = all * piece / pieces;
+    end = all * (piece + 1) / pieces;
+    b = find_sequence(a.B, [&](int s) { return tiles_of(a, s); }, lane, at, before);
+    if (b >= a.B) return;
+  }
+
+  const int ring = (int)lds_addr(lds) + RING_B * wave;
+  const int ka = row_address(ring, l32, hl), va = tr_address(ring + DT_B, lane, hl);
+  // copy i of a tile: rows 4 i + lane / 16, chunk (lane % 16) ^ swz(row); rows i and i + 4 share the chunk
+  const int crow = lane >> 4, ccol = ((lane & 15) ^ swz(lane >> 4)) * 16;
+  const float c = sreg(a.scale_log2);
+  const int shift = a.pt.shift, mask = (1 << shift) - 1;
+  const int64_t own = own_rows(a), rows = all_rows(a);
+
+  do {
+    // the list of this sequence's pages: `count` entries of 2^shift tokens, `len` keys in all
+    const int64_t len = KIND == PREFIX ? scalar64(prefix_keys(a)) : __builtin_amdgcn_readfirstlane(keys_of(a, b));
+    const int32_t* const table = KIND == PREFIX ? a.p_table : a.pt.p + b * a.pt.sb;
+    const int32_t* const sel = KIND == SPARSE ? a.sel + ((int64_t)b * a.Hk + kv) * a.n_sel : nullptr;
+    const int64_t span = KIND == SPARSE
+                             ? (len > 0 ? (int64_t)__builtin_amdgcn_readfirstlane(list_length(sel, a.n_sel, lane)) << shift : 0)
+                             : len;
+    const int tiles = (int)((span + DT - 1) / DT);
+    // this sequence's tiles of the piece
+    const int s0 = end_to_end ? (int)(at - before) : (int)((int64_t)tiles * split / splits);
+    const int s1 = end_to_end ? (int)(end - before < tiles ? end - before : tiles)
+                              : (int)((int64_t)tiles * (split + 1) / splits);
+
+    // query row x of the workgroup: its sequence and head
+    auto seq_of = [&](int x) { return KIND == PREFIX ? (int)((r0 + x) / group) : b; };
+    auto head_of = [&](int x) { return kv * group + (int)(KIND == PREFIX ? (r0 + x) % group : r0 + x); };
+    u32x4 qf[8];
+    {
+      const int x = l32 < nr ? l32 : nr - 1;
+      const uint16_t* p = a.q.p + seq_of(x) * a.q.sl + head_of(x) * a.q.sh + 8 * hl;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const u32x4*>(p + 16 * s);
+    }
+    // halves of tiles base, base + DW, ..: tile i's first half in lane i, its second in lane 32 + i
+    auto look_up = [&](int base) {
+      return half_at(sel, span, table, KIND == PREFIX ? a.p_width : a.pt.width, shift, a.pt.pages, len,
+                     ((int64_t)base + (int64_t)l32 * DW) * DT + HT * hl);
+    };
+    Half list = {0, 0}, h0, h1;  // h0, h1: the halves of the tile that is fetched next, scalar
+    int listed = 0;              // tiles of the list that are used up
+    auto next_halves = [&](int t) {
+      if ((listed & 31) == 0) {
+        list = look_up(t);
+        // (waited for here, once in 32 tiles: a load that may be pending after the branch would be waited for, and
+        // the copies with it, at every tile)
+        asm volatile("" : "+v"(list.page), "+v"(list.keys));
+      }
+      const int i = listed & 31;
+      h0.page = __builtin_amdgcn_readlane(list.page, i);
+      h0.keys = __builtin_amdgcn_readlane(list.keys, i);
+      h1.page = __builtin_amdgcn_readlane(list.page, i + 32);
+      h1.keys = __builtin_amdgcn_readlane(list.keys, i + 32);
+      ++listed;
+    };
+    auto issue = [&](const PageRows& src, int t, uint32_t to) {
+      const unsigned char* base = reinterpret_cast<const unsigned char*>(src.p + kv * src.sh);
+      const int64_t sl = src.sl * 2, sp = src.sp * 2;
+      const int in = (int)(((int64_t)t * DT) & mask), in1 = (in + HT) & mask;
+      const int n0 = h0.keys & (BAD_PAGE - 1), n1 = h1.keys & (BAD_PAGE - 1);
+      const unsigned char* p0 = base + h0.page * sp + in * sl;
+      const unsigned char* p1 = base + h1.page * sp + in1 * sl;
+      // a half without keys copies the other's last one (a tile without any: anything, it is not used)
+      const unsigned char* b0 = (const unsigned char*)(uintptr_t)scalar64((int64_t)(uintptr_t)(n0 > 0 || n1 == 0 ? p0 : p1));
+      const unsigned char* b1 = (const unsigned char*)(uintptr_t)scalar64((int64_t)(uintptr_t)(n1 > 0 || n0 == 0 ? p1 : p0));
+      const int last0 = (n0 > 0 ? n0 : (n1 > 0 ? n1 : 1)) - 1, last1 = (n1 > 0 ? n1 : (n0 > 0 ? n0 : 1)) - 1;
+#pragma unroll
+      for (int i = 0; i < NCOPY; ++i) {
+        const int x = crow + 4 * (i & 3), last = i < 4 ? last0 : last1;
+        const int r = x < last ? x : last;
+        dma16_guarded(i < 4 ? b0 : b1, (uint32_t)r * (uint32_t)sl + (ccol ^ ((i & 3) << 4)), to + 1024 * i);
+      }
+    };
+    auto issue_k = [&](int t) { issue(a.k, t, (uint32_t)ring); };
+    auto issue_v = [&](int t) { issue(a.v, t, (uint32_t)ring + DT_B); };
+    static_assert(NCOPY == 8, "the counts below are a tile's copies");
+
+    floatx16 o[4];
+#pragma unroll
+    for (int db = 0; db < 4; ++db) zero(o[db]);
+    float m = M_INIT, l = 0.0f;
+    __builtin_amdgcn_s_waitcnt(0x0070);  // the query is there: only tile copies are counted below
+    int t = s0 + wave, k0 = 0, k1 = 0;   // keys of the current tile's halves
+    if (t < s1) {
+      next_halves(t);
+      issue_k(t);
+      issue_v(t);
+    }
+#pragma unroll 1
+    for (; t < s1; t += DW) {
+      const bool more = t + DW < s1;
+      k0 = h0.keys;
+      k1 = h1.keys;
+      if (more) next_halves(t + DW);
+      asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // K is there (V may be on its way)
+      floatx16 s;
+      zero(s);
+#pragma unroll
+      for (int d = 0; d < 8; ++d) s = mfma32x32x16(read_row(ka, d, 0), qf[d], s);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its reads are over before K is overwritten
+      if (more) issue_k(t + DW);
+      if (k0 != HT || k1 != HT) {
+        // registers 0 .. 7 are keys of the first half, 8 .. 15 of the second
+        const int n0 = (k0 & (BAD_PAGE - 1)) - 4 * hl, n1 = (k1 & (BAD_PAGE - 1)) - 4 * hl;
+        const float bad0 = k0 >= BAD_PAGE ? __uint_as_float(0x7fc00000u) : 0.0f;
+        const float bad1 = k1 >= BAD_PAGE ? __uint_as_float(0x7fc00000u) : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[r] = acc_row(r & 7) < (r < 8 ? n0 : n1) ? s[r] + (r < 8 ? bad0 : bad1) : -INFINITY;
+      }
+      float mx = s[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+      mx = wave_max_xor32(mx);
+      const float mn = fmaxf(m, mx);
+      if (__any(mn > m)) {
+        const float alpha = fast_exp2((m - mn) * c);
+        scale_acc(o, alpha);
+        l *= alpha;
+        m = mn;
+      }
+      const float mc = -m * c;
+      floatx16 p;
+      float ls = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        p[r] = fast_exp2(__builtin_fmaf(s[r], c, mc));
+        ls += p[r];
+      }
+      l += ls;
+      const u32x4 pf[2] = {pack_half(p, 0), pack_half(p, 1)};
+      if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V is there (the next K may not be)
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (((k0 | k1) & (2 * BAD_PAGE - 1)) != 0) {  // (a tile without keys holds anything)
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int mm = 0; mm < 2; ++mm) o[db] = mfma32x32x16(read_tr(va, db, mm, 0), pf[mm], o[db]);
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) issue_v(t + DW);
+    }
+    l = wave_sum_xor32(l);
+    // O^T as rows [row][128] fp32 into the wave's LDS, m and l behind the rings
+    float* const sm = reinterpret_cast<float*>(lds + DEC_LDS);
+    float* const sl = sm + DW * HEADS;
+    if (hl == 0) {  // (no keys: a reference of -inf, weight 0; a sum that is NaN keeps its own and stays)
+      sm[wave * HEADS + l32] = l == 0.0f ? -INFINITY : m;
+      sl[wave * HEADS + l32] = l;
+    }
+    float* mine = reinterpret_cast<float*>(lds + RING_B * wave);
+    if (l32 < nr) {
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          floatx4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = o[db][4 * g + e];
+          *reinterpret_cast<floatx4*>(mine + l32 * D + 32 * db + 8 * g + 4 * hl) = w;
+        }
+    }
+    __syncthreads();
+    const bool whole = KIND != PREFIX && s1 - s0 == tiles && a.p_splits == 0 && (end_to_end || splits == 1);
+    for (int x = threadIdx.x; x < nr * (D / 4); x += DW * 64) {  // 4 values of one row at a time
+      const int hh = x / (D / 4), dq = 4 * (x % (D / 4));
+      float M = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < DW; ++w) M = fmaxf(M, sm[w * HEADS + hh]);
+      float L = 0.0f;
+      floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < DW; ++w) {
+        const float mw = sm[w * HEADS + hh], f = mw == -INFINITY ? 0.0f : fast_exp2((mw - M) * c);
+        // (a wave without keys holds zeros)
+        L += f * sl[w * HEADS + hh];
+        acc += f * *reinterpret_cast<const floatx4*>(
+                       reinterpret_cast<const float*>(lds + RING_B * w) + hh * D + dq);
+      }
+      const int sq = seq_of(hh), head = head_of(hh);
+      if (whole) {
+        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+        u32x2 w;
+        w[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+        w[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
+        *reinterpret_cast<u32x2*>(a.out.p + sq * a.out.sl + head * a.out.sh + dq) = w;
+      } else {
+        // (end to end: piece + b, the parts of a head in the order of their keys, each in a row of its own, as the
+        // next part has another piece or a later sequence, or both)
+        const int64_t part = KIND == PREFIX ? own + (int64_t)sq * splits + split
+                                            : (end_to_end ? (int64_t)piece + b : (int64_t)b * splits + split);
+        const int64_t row = head * rows + part;
+        *reinterpret_cast<floatx4*>(a.part + row * D + dq) = acc;
+        if (dq == 0) {
+          float* st = a.part + a.Hq * rows * D;
+          st[row] = M;
+          st[a.Hq * rows + row] = L;
+        }
+      }
+    }
+    if (!end_to_end) return;
+    at = before + tiles;
+    if (at >= end) return;
+    // the next sequence with keys
+    before = at;
+    do {
+      b = __builtin_amdgcn_readfirstlane(b + 1);
+    } while (b < a.B && __builtin_amdgcn_readfirstlane(tiles_of(a, b)) == 0);
+    if (b >= a.B) return;
+    __syncthreads();  // the joined results are read: the rings are free
+  } while (true);
+}
+
+// A workgroup per (sequence, query head): the parts of its own keys, then the prefix's, joined, its waves taking
+// 64 / JW parts at a time in turn, then in the waves' order. No parts: zeros (or, end to end without a prefix, a
+// result that one piece has written already).
+constexpr int JW = 4;
+__global__ void __launch_bounds__(JW * 64) paged_join_kernel(const PagedAttnArgs a) {
+  __shared__ float2 wx[JW][64];
+  __shared__ float wm[JW], wl[JW];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = (int)(blockIdx.x / (uint32_t)a.Hq), h = (int)(blockIdx.x % (uint32_t)a.Hq);
+  const int64_t own = own_rows(a), rows = all_rows(a);
+  int64_t first = (int64_t)b * a.splits;  // own parts [first, first + n_own)
+  int n_own = a.splits;
+  if (a.pieces > 0) {
+    int64_t all, before;
+    count_tiles_of(a.B, [&](int s) { return tiles_of(a, s); }, lane, b, all, before);
+    const int tiles = __builtin_amdgcn_readfirstlane(tiles_of(a, b));
+    n_own = 0;
+    if (tiles > 0) {
+      // tile t is in piece j when floor(all j / pieces) <= t < floor(all (j + 1) / pieces)
+      const int64_t pieces = all < a.pieces ? all : a.pieces;
+      const int j0 = (int)(((before + 1) * pieces - 1) / all);
+      const int j1 = (int)(((before + tiles) * pieces - 1) / all);
+      if (j0 == j1 && a.p_splits == 0) return;
+      first = j0 + b;
+      n_own = j1 - j0 + 1;
+    }
+  }
+  const int n_all = n_own + a.p_splits;
+  // part i's row
+  auto row_of = [&](int i) {
+    return h * rows + (i < n_own ? first + i : own + (int64_t)b * a.p_splits + (i - n_own));
+  };
+  const float* st = a.part + a.Hq * rows * D;
+  float x = 0.0f, y = 0.0f, L = 0.0f, M = -INFINITY;
+  constexpr int N = 64 / JW;
+  for (int i0 = N * wave; i0 < n_all; i0 += 64) {  // N parts at a time, their weights one per lane
+    const int n = min(N, n_all - i0);
+    float2 v[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+      v[u] = u < n ? *reinterpret_cast<const float2*>(a.part + row_of(i0 + u) * D + 2 * lane) : float2{0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    if (lane < n) {
+      m = st[row_of(i0 + lane)];
+      l = st[a.Hq * rows + row_of(i0 + lane)];
+    }
+    float mx = m;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    const float mn = fmaxf(M, mx);
+    const float f0 = M == -INFINITY ? 0.0f : fast_exp2((M - mn) * a.scale_log2);
+    const float w = m == -INFINITY ? 0.0f : fast_exp2((m - mn) * a.scale_log2);
+    x *= f0;
+    y *= f0;
+    L = L * f0 + wave_reduce_sum(w * l);
+    M = mn;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {  // (lanes past n have weight 0)
+      const float f = __shfl(w, u);
+      x += f * v[u].x;
+      y += f * v[u].y;
+    }
+  }
+  wx[wave][lane] = float2{x, y};
+  if (lane == 0) {
+    wm[wave] = M;
+    wl[wave] = L;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < JW; ++w) M = fmaxf(M, wm[w]);
+  x = y = L = 0.0f;
+#pragma unroll
+  for (int w = 0; w < JW; ++w) {
+    const float f = wm[w] == -INFINITY ? 0.0f : fast_exp2((wm[w] - M) * a.scale_log2);
+    L += f * wl[w];
+    x += f * wx[w][lane].x;
+    y += f * wx[w][lane].y;
+  }
+  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  *reinterpret_cast<uint32_t*>(a.out.p + b * a.out.sl + h * a.out.sh + 2 * lane) =
+      pack_bf16x2(x * inv, y * inv);
+}
+
+template <int DW, Kind KIND>
+hipError_t run(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
+  constexpr int bytes = DW * RING_B + 2 * DW * HEADS * 4;
+  static LdsAllowed allowed;
+  const hipError_t attr = allow_lds((const void*)paged_kernel<DW, KIND>, bytes, allowed);
+  if (attr != hipSuccess) return attr;
+  hipLaunchKernelGGL((paged_kernel<DW, KIND>), dim3((uint32_t)(units * a.Hk)), dim3(DW * 64), bytes, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+// How the keys are cut: own ones as the single-token attention over whole caches cuts them (whole sequences where they
+// give work enough, else the batch's keys in equal pieces), selected and the prefix's in equal pieces for two
+// workgroups a CU, of 6 tiles or more.
+void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
+  const int64_t group = a->Hq / a->Hk, units = a->Hk * ((group + HEADS - 1) / HEADS);
+  a->splits = 1;
+  a->pieces = a->p_splits = 0;
+  auto cut = [&](int64_t tiles, int64_t busy) {
+    if (num_splits > 0) return (int)num_splits;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / busy, tiles / 6));
+  };
+  if (a->B == 0) return;
+  if (a->sel != nullptr) {
+    a->splits = cut((((int64_t)a->n_sel << a->pt.shift) + DT - 1) / DT, a->B * units);
+  } else {
+    a->pieces = decode_pieces(a->B, a->Hq, a->Hk, (int64_t)a->pt.width << a->pt.shift, num_splits, cus);
+  }
+  if (a->p_max > 0)
+    a->p_splits = cut((a->p_max + DT - 1) / DT, a->Hk * ((a->B * group + HEADS - 1) / HEADS));
+}
+
+hipError_t launch_paged(const PagedAttnArgs& a, hipStream_t stream) {
+  const int group = a.Hq / a.Hk, blocks = (group + HEADS - 1) / HEADS;
+  hipError_t e;
+  if (a.p_splits > 0) {
+    e = run<4, PREFIX>(a, a.p_splits * (((int64_t)a.B * group + HEADS - 1) / HEADS), stream);
+    if (e != hipSuccess) return e;
+  }
+  const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B * a.splits) * blocks;
+  // whole sequences that leave every CU one workgroup at most: eight waves in it
+  const bool wide = a.pieces == 0 && n * a.Hk <= num_cus();
+  if (a.sel != nullptr) e = wide ? run<8, SPARSE>(a, n, stream) : run<4, SPARSE>(a, n, stream);
+  else e = wide ? run<8, DENSE>(a, n, stream) : run<4, DENSE>(a, n, stream);
+  if (e != hipSuccess || !has_parts(a)) return e;
+  hipLaunchKernelGGL(paged_join_kernel, dim3((uint32_t)((int64_t)a.B * a.Hq)), dim3(JW * 64), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace lbw

@@ -16,6 +16,7 @@ from .head_norm import AxisRope, axis_rope, qk_head_norm_rope, qk_head_norm_rope
 from .layer import WanCrossAttention, WanSelfAttention
 from .packed import (PackedPlan, attention_decode, attention_packed, attention_packed_backward,
                      packed_plan)
+from .paged import PagedKV, attention_paged, paged_append_, paged_kv, paged_select
 from .qk_post import (qk_norm_rope, qk_norm_rope3, qk_norm_rope_, qk_norm_rope_t, qk_norm_rope_t3,
                       x_norm_rope, x_norm_rope_t3)
 from .rope import RopeTables, causal_rope_tables, rope_params, wan_rope_freqs
@@ -32,4 +33,5 @@ __all__ = [
     "WanCrossAttention",
     "AxisRope", "axis_rope", "qk_head_norm_rope", "qk_head_norm_rope_",
     "PackedPlan", "packed_plan", "attention_packed", "attention_packed_backward", "attention_decode",
+    "PagedKV", "paged_kv", "paged_append_", "attention_paged", "paged_select",
 ]

@@ -157,6 +157,64 @@ class DecodeParams(ctypes.Structure):
     ]
 
 
+class PagedKv(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("k_stride_p", ctypes.c_int64), ("k_stride_l", ctypes.c_int64),
+        ("k_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride_p", ctypes.c_int64), ("v_stride_l", ctypes.c_int64),
+        ("v_stride_h", ctypes.c_int64),
+        ("bounds", ctypes.c_void_p), ("pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+        ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("table_width", ctypes.c_int32),
+    ]
+
+
+class PagedAppendParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedKv),
+        ("tokens", ctypes.c_int32), ("batch", ctypes.c_int32), ("q_heads", ctypes.c_int32),
+        ("k_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("q_stride_l", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_stride_l", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride_l", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+        ("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p), ("w_dtype", ctypes.c_int32),
+        ("norm", ctypes.c_int32), ("eps", ctypes.c_float),
+        ("rope", ctypes.c_void_p), ("rope_rows", ctypes.c_int64),
+        ("rope_pairs", ctypes.c_int32), ("n_axes", ctypes.c_int32),
+        ("axis_pairs", ctypes.c_int32 * 4), ("interleaved", ctypes.c_int32),
+        ("pos", ctypes.c_void_p), ("pos_stride", ctypes.c_int64),
+        ("starts", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p), ("q_out_stride_l", ctypes.c_int64), ("q_out_stride_h", ctypes.c_int64),
+        ("q_out_scale", ctypes.c_float), ("k_out_scale", ctypes.c_float),
+    ]
+
+
+class AttentionPagedParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedKv),
+        ("batch", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("q_stride_b", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("lens", ctypes.c_void_p),
+        ("selected", ctypes.c_void_p), ("n_selected", ctypes.c_int32),
+        ("prefix_table", ctypes.c_void_p), ("prefix_width", ctypes.c_int32),
+        ("prefix_len", ctypes.c_void_p), ("prefix_keys", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_stride_b", ctypes.c_int64), ("out_stride_h", ctypes.c_int64),
+        ("softmax_scale", ctypes.c_float), ("num_splits", ctypes.c_int32),
+    ]
+
+
+class PagedSelectParams(ctypes.Structure):
+    _fields_ = [
+        ("cache", PagedKv),
+        ("batch", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("k_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("q_stride_b", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("lens", ctypes.c_void_p),
+        ("count", ctypes.c_int32), ("first", ctypes.c_int32), ("last", ctypes.c_int32),
+        ("selected", ctypes.c_void_p),
+    ]
+
+
 EXPORTS = (
     "lbw_attention_workspace_size", "lbw_attention_fp8kv_workspace_size", "lbw_attention_fwd",
     "lbw_cross_attention_fwd",
@@ -169,6 +227,8 @@ EXPORTS = (
     "lbw_attention_packed_plan", "lbw_attention_packed_workspace_size", "lbw_attention_packed_fwd",
     "lbw_attention_packed_bwd_workspace_size", "lbw_attention_packed_bwd",
     "lbw_attention_decode_workspace_size", "lbw_attention_decode",
+    "lbw_paged_append", "lbw_attention_paged_workspace_size", "lbw_attention_paged",
+    "lbw_paged_select_workspace_size", "lbw_paged_select",
     "lbw_last_error", "lbw_abi_version",
 )
 
@@ -230,6 +290,16 @@ def _declare(lib):
     lib.lbw_attention_decode_workspace_size.restype = ctypes.c_size_t
     lib.lbw_attention_decode.argtypes = [P(DecodeParams), vp, ctypes.c_size_t, vp]
     lib.lbw_attention_decode.restype = ctypes.c_int
+    lib.lbw_paged_append.argtypes = [P(PagedAppendParams), vp]
+    lib.lbw_paged_append.restype = ctypes.c_int
+    lib.lbw_attention_paged_workspace_size.argtypes = [P(AttentionPagedParams)]
+    lib.lbw_attention_paged_workspace_size.restype = ctypes.c_size_t
+    lib.lbw_attention_paged.argtypes = [P(AttentionPagedParams), vp, ctypes.c_size_t, vp]
+    lib.lbw_attention_paged.restype = ctypes.c_int
+    lib.lbw_paged_select_workspace_size.argtypes = [P(PagedSelectParams)]
+    lib.lbw_paged_select_workspace_size.restype = ctypes.c_size_t
+    lib.lbw_paged_select.argtypes = [P(PagedSelectParams), vp, ctypes.c_size_t, vp]
+    lib.lbw_paged_select.restype = ctypes.c_int
     lib.lbw_last_error.argtypes = []
     lib.lbw_last_error.restype = ctypes.c_char_p
     lib.lbw_abi_version.argtypes = []
