@@ -131,8 +131,8 @@ int lbw_paged_append(const lbw_paged_append_params* p, void* stream) {
     return fail(LBW_ERR_INVALID, "pos missing: rows are positions on one axis only, not on %d", p->n_axes);
   if (p->starts == nullptr && p->batch != p->tokens)
     return fail(LBW_ERR_INVALID, "%d tokens of %d sequences need starts", p->tokens, p->batch);
-  if (p->tokens > HN_WAVES * kMaxWorkgroups)
-    return fail(LBW_ERR_UNSUPPORTED, "tokens %d above %lld", p->tokens, (long long)(HN_WAVES * kMaxWorkgroups));
+  if (p->tokens > 2 * kMaxWorkgroups)
+    return fail(LBW_ERR_UNSUPPORTED, "tokens %d above %lld", p->tokens, (long long)(2 * kMaxWorkgroups));
   LBW_TRY(fill_table(p->cache, p->batch, &a.pt));
   LBW_TRY(fill_cache(p->cache, &a.kp, &a.vp));
   LBW_TRY(check_head_strides("the cache's k", a.kp.sh));
@@ -144,7 +144,8 @@ int lbw_paged_append(const lbw_paged_append_params* p, void* stream) {
   if (p->batch > 0 && p->lens == nullptr) return fail(LBW_ERR_INVALID, "lens missing");
   if (p->cache.bounds != nullptr && !aligned16(p->cache.bounds))
     return fail(LBW_ERR_INVALID, "bounds must be a 16-byte aligned device pointer");
-  if (p->cache.bounds != nullptr && (p->tokens / 16 + 1) * (int64_t)p->k_heads > kMaxWorkgroups)
+  // (a workgroup of 512 for one token and 2 heads, at most)
+  if (p->cache.bounds != nullptr && p->tokens * (int64_t)p->k_heads > kMaxWorkgroups)
     return fail(LBW_ERR_UNSUPPORTED, "tokens %d x %d heads", p->tokens, p->k_heads);
   a.B = p->batch;
   a.norm = p->norm != 0;

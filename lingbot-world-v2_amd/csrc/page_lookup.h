@@ -31,21 +31,18 @@ struct Half {
 // those of the table entries that sel names, 2^shift places each. `len`: the sequence's keys.
 LBW_LOOKUP Half half_at(const int32_t* sel, int64_t span, const int32_t* entries, int width, int shift, int pages,
                         int64_t len, int64_t pos) {
-  Half h = {0, 0};
-  if (pos >= span) return h;
+  // (the entry is read whatever the length, so that both can be on their way at once)
   int64_t row = pos;
   if (sel != nullptr) {
+    if (pos >= span) return Half{0, 0};
     const int64_t entry = sel[pos >> shift];
-    if (entry < 0) return h;
-    row = (entry << shift) + (pos & ((1 << shift) - 1));
+    row = entry < 0 ? len : (entry << shift) + (pos & ((1 << shift) - 1));
   }
-  const int64_t left = len - row;
-  if (left <= 0) return h;
-  h.keys = left < HALF_KEYS ? (int)left : HALF_KEYS;
   const int page = page_at(entries, width, shift, pages, row);
-  if (page >= 0) h.page = page;
-  else h.keys += BAD_PAGE;
-  return h;
+  const int64_t left = (sel != nullptr || pos < span ? len - row : 0);
+  if (left <= 0) return Half{0, 0};
+  const int keys = left < HALF_KEYS ? (int)left : HALF_KEYS;
+  return page >= 0 ? Half{page, keys} : Half{0, keys + BAD_PAGE};
 }
 
 }  // namespace lbw

@@ -6,7 +6,8 @@
 //   bounds[page] = (min, max) over the page's rows so far, of the rounded values: exact, so their order is free.
 //
 // Bound by memory: every value is read once and written once. As in the per-head norm a wave keeps a token, its
-// angles in registers, and walks its heads.
+// angles in registers, and walks its heads. 4680 + 3600 + 1561 tokens x 40/8 heads of 128, normed, 54 us (5.2 TB/s; a
+// large copy reaches 4.9), their pages' bounds 8 us; one token 4.3 us, most of it the launch.
 
 #include "head_rows.h"
 #include "paged.h"
@@ -15,45 +16,50 @@ namespace lbw {
 namespace {
 
 constexpr int AP_WAVES = 4;
-constexpr int AP_BLOCK = 16;  // tokens whose pages a workgroup of the bounds kernel looks after
+constexpr int EDGE_WAVES = 8;  // of the bounds kernel
 
-// The sequence of token t: the last one that starts at or before it (64 starts at a time); -1: none.
-__device__ __forceinline__ int find_start(const int32_t* starts, int B, int t, int lane) {
-  int base = 0, n = B;
-  do {
-    const int step = (n + 63) >> 6;
-    const int off = lane * step;
-    const uint64_t past = __ballot(off < n && starts[base + off] <= t);
-    if (past == 0) return -1;
-    const int c = (63 - __clzll((unsigned long long)past)) * step;
-    base += c;
-    n = n - c < step ? n - c : step;
-  } while (n > 1);
-  return __builtin_amdgcn_readfirstlane(base);
-}
-
-// Where a token goes: its sequence, row and page (-1: nowhere).
+// Where a token goes: its sequence (-1: none), row and page (-1: nowhere).
 struct Place {
   int b;
   int64_t row;
   int page;
-  int end;  // one past the sequence's last token
+  int start, end;  // the sequence's tokens
 };
 __device__ __forceinline__ Place place_of(const AppendArgs& a, int t, int lane) {
-  Place w = {t, 0, -1, t + 1};
-  int at = t;
-  if (a.starts != nullptr) {
-    w.b = find_start(a.starts, a.B, t, lane);
-    if (w.b < 0) return w;
-    at = __builtin_amdgcn_readfirstlane(a.starts[w.b]);
-    w.end = __builtin_amdgcn_readfirstlane(a.starts[w.b + 1]);
-    w.end = w.end < a.T ? w.end : a.T;
-    if (t >= w.end) {  // behind the last sequence
-      w.b = -1;
-      return w;
+  Place w = {t, 0, -1, t, t + 1};
+  int len;
+  if (a.starts == nullptr) {
+    len = __builtin_amdgcn_readfirstlane(a.lens[t]);
+  } else {
+    // the last sequence that starts at or before the token: 64 starts at a time, and at the end all that is wanted
+    // of the sequence in one go
+    int base = 0, n = a.B;
+    while (n > 64) {
+      const int step = (n + 63) >> 6, off = lane * step;
+      const uint64_t past = __ballot(off < n && a.starts[base + off] <= t);
+      if (past == 0) break;
+      const int c = (63 - __clzll((unsigned long long)past)) * step;
+      base += c;
+      n = n - c < step ? n - c : step;
     }
+    int s = 0, e = 0, l = 0;
+    const bool mine = lane < n;
+    if (mine) {
+      s = a.starts[base + lane];
+      e = a.starts[base + lane + 1];
+      l = a.lens[base + lane];
+    }
+    const uint64_t past = __ballot(mine && s <= t);
+    const int c = past == 0 ? 0 : 63 - __clzll((unsigned long long)past);
+    w.b = past == 0 ? -1 : base + c;
+    w.start = __builtin_amdgcn_readlane(s, c);
+    w.end = __builtin_amdgcn_readlane(e, c);
+    w.end = w.end < a.T ? w.end : a.T;
+    len = __builtin_amdgcn_readlane(l, c);
+    if (t >= w.end) w.b = -1;  // behind the last sequence
+    if (w.b < 0) return w;
   }
-  w.row = (int64_t)__builtin_amdgcn_readfirstlane(a.lens[w.b]) + ((int64_t)t - at);
+  w.row = (int64_t)len + ((int64_t)t - w.start);
   w.page = __builtin_amdgcn_readfirstlane(
       page_at(a.pt.p + (int64_t)w.b * a.pt.sb, a.pt.width, a.pt.shift, a.pt.pages, w.row));
   return w;
@@ -63,8 +69,27 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int t, int lane) 
 __device__ __forceinline__ float min_nan(float x, float y) { return __builtin_elementwise_minimum(x, y); }
 __device__ __forceinline__ float max_nan(float x, float y) { return __builtin_elementwise_maximum(x, y); }
 
-// Chunks first, first + step, .. of a token's heads, normed and turned; `bounds` (of the token's page, or null): the
-// page's, started anew if `fresh`.
+// Eight values of a head: normed (or not), turned, scaled, rounded.
+template <int LPH, bool INTER>
+__device__ __forceinline__ u32x4 turn_chunk(const AppendArgs& a, const u32x4& x, const float (&wt)[8], float scale,
+                                            const Turn& rot) {
+  float f[8], o[8];
+  unpack8(x, f);
+  float r = scale;
+  if (a.norm) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
+    r = rsqrtf(head_sum<LPH>(ss) * a.inv_d + a.eps) * scale;
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] *= r * wt[j];
+  turn<INTER, false>(rot, f, o);
+  return pack8(o);
+}
+
+// Chunks first, first + step, .. of a token's heads; `bounds` (of the token's page, or null): the page's, started anew
+// if `fresh`.
 template <int LPH, bool INTER>
 __device__ __forceinline__ void turn_rows(const AppendArgs& a, const uint16_t* src, int64_t ssh, uint16_t* dst,
                                           int64_t dsh, int heads, int first, int step, int e0, int hsub,
@@ -87,19 +112,7 @@ __device__ __forceinline__ void turn_rows(const AppendArgs& a, const uint16_t* s
     for (int u = 0; u < U; ++u) {
       const int ch = it + u * step;
       if (ch >= nch) break;
-      float f[8], o[8];
-      unpack8(x[u], f);
-      float r = scale;
-      if (a.norm) {
-        float ss = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss += f[j] * f[j];
-        r = rsqrtf(head_sum<LPH>(ss) * a.inv_d + a.eps) * scale;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= r * wt[j];
-      turn<INTER, false>(rot, f, o);
-      const u32x4 out = pack8(o);
+      const u32x4 out = turn_chunk<LPH, INTER>(a, x[u], wt, scale, rot);
       if (ch * HPW + hsub >= heads) continue;
       *reinterpret_cast<u32x4*>(dst + (int64_t)ch * HPW * dsh + dof) = out;
       if (bounds == nullptr) continue;
@@ -144,6 +157,18 @@ __device__ __forceinline__ void copy_rows(const uint16_t* src, int64_t ssh, uint
   }
 }
 
+// The rotation of token t, at `row` of its sequence.
+template <bool INTER>
+__device__ __forceinline__ void load_rotation(const AppendArgs& a, int t, int64_t row, int e0, int lane, Turn& rot) {
+  if (a.pos != nullptr) {
+    load_turn<INTER>(a, t, e0, lane, rot);
+  } else {
+    // (a row past 31 bits is outside every table)
+    const int p = row >= 0 && row < a.P ? (int)row : -1;
+    load_turn_at<INTER>(a, p, p, p, p, e0, lane, rot);
+  }
+}
+
 template <int LPH, bool INTER>
 __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs a) {
   constexpr int HPW = 64 / LPH, D = 8 * LPH;
@@ -156,13 +181,7 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs 
   const Place w = place_of(a, t, lane);
   if (w.b < 0) return;  // a row behind the last sequence: left as it was
   Turn rot;
-  if (a.pos != nullptr) {
-    load_turn<INTER>(a, t, e0, lane, rot);
-  } else {
-    // (a row past 31 bits is outside every table)
-    const int p = w.row >= 0 && w.row < a.P ? (int)w.row : -1;
-    load_turn_at<INTER>(a, p, p, p, p, e0, lane, rot);
-  }
+  load_rotation<INTER>(a, t, w.row, e0, lane, rot);
   // the token's chunks, q's, k's, v's, in turn to the waves that share it
   const int cq = (a.Hq + HPW - 1) / HPW, ck = (a.Hk + HPW - 1) / HPW;
   auto first = [&](int before) {
@@ -182,19 +201,21 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs 
                  first(cq + ck), a.parts, e0, hsub);
 }
 
-// Bounds of the pages that several tokens were put into: blockIdx.x counts blocks of AP_BLOCK tokens, blockIdx.y
-// chunks of heads. The workgroup whose block holds a page's first new token reads the page's new rows back (from
+// Bounds of the pages that several tokens were put into: blockIdx.x counts blocks of a.run_block tokens, blockIdx.y
+// chunks of heads. The workgroup whose block holds a page's first new token reads the page's new keys back (from
 // cache: they were written just before), its waves in turn, and joins them with the old bounds where the page was
-// begun before: every page has one owner, no atomics.
+// begun before: every page has one owner, no atomics. (One kernel, in which the workgroup that makes a page's bounds
+// turns its keys: 4680 + 3600 + 1561 tokens x 40/8 heads 69 to 90 us against 54 + 8, as a page's tokens follow one
+// another.)
 template <int LPH>
-__global__ void __launch_bounds__(AP_WAVES * 64) append_bounds_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(EDGE_WAVES * 64) append_bounds_kernel(const AppendArgs a) {
   constexpr int HPW = 64 / LPH, D = 8 * LPH, U = 8;
-  __shared__ float red[AP_WAVES][2][64 * 8];
+  __shared__ u32x4 red[2][EDGE_WAVES][64];  // (bf16: what was rounded once stays)
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int e0 = 8 * (lane % LPH), head = (int)blockIdx.y * HPW + lane / LPH;
-  const int hh = head < a.Hk ? head : a.Hk - 1;
-  const int64_t t0 = (int64_t)blockIdx.x * AP_BLOCK;
-  const int t1 = (int)(t0 + AP_BLOCK < a.T ? t0 + AP_BLOCK : a.T);
+  const int hh = head < a.Hk ? head : a.Hk - 1;  // (lanes past the last head do its work again and write nothing)
+  const int64_t t0 = (int64_t)blockIdx.x * a.run_block;
+  const int t1 = (int)(t0 + a.run_block < a.T ? t0 + a.run_block : a.T);
   const int mask = (1 << a.pt.shift) - 1;
   for (int t = (int)t0; t < t1;) {
     const Place w = place_of(a, t, lane);
@@ -202,25 +223,27 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_bounds_kernel(const Appe
       ++t;
       continue;
     }
-    const int in = (int)(w.row & mask), at = __builtin_amdgcn_readfirstlane(a.starts[w.b]);
+    const int in = (int)(w.row & mask);
     const int n = w.end - t < mask + 1 - in ? w.end - t : mask + 1 - in;  // this page's tokens from t on
-    if (w.page < 0 || (in != 0 && t != at)) {  // nowhere, or not its first new token
+    if (w.page < 0 || (in != 0 && t != w.start)) {  // nowhere, or not its first new token
       t += n;
       continue;
     }
-    const uint16_t* rows = a.kp.p + w.page * a.kp.sp + hh * a.kp.sh + e0;
+    const uint16_t* const rows = a.kp.p + w.page * a.kp.sp + in * a.kp.sl + hh * a.kp.sh + e0;
+    uint16_t* const edge = a.bounds + ((int64_t)w.page * a.Hk + hh) * 2 * D + (wave & 1) * D + e0;
+    const u32x4 before = load16(edge);
     float lo[8], hi[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       lo[j] = INFINITY;
       hi[j] = -INFINITY;
     }
-    for (int r = wave; r < n; r += AP_WAVES * U) {
+    for (int r = wave; r < n; r += EDGE_WAVES * U) {
       u32x4 x[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {  // (past the end: the last row once more)
-        const int rr = r + u * AP_WAVES < n ? r + u * AP_WAVES : n - 1;
-        x[u] = load16(rows + (int64_t)(in + rr) * a.kp.sl);
+        const int rr = r + u * EDGE_WAVES < n ? r + u * EDGE_WAVES : n - 1;
+        x[u] = load16(rows + (int64_t)rr * a.kp.sl);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -234,37 +257,26 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_bounds_kernel(const Appe
       }
     }
     __syncthreads();  // the last page's results are read
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      red[wave][0][64 * j + lane] = lo[j];
-      red[wave][1][64 * j + lane] = hi[j];
-    }
+    red[0][wave][lane] = pack8(lo);
+    red[1][wave][lane] = pack8(hi);
     __syncthreads();
     if (wave < 2 && head < a.Hk) {  // one wave for the smallest values, one for the largest
-      uint16_t* const p = a.bounds + ((int64_t)w.page * a.Hk + head) * 2 * D + wave * D + e0;
-      float m[8], old[8];
+      float m[8], y[8];
+      unpack8(in != 0 ? before : red[wave][0][lane], m);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        m[j] = red[0][wave][64 * j + lane];
+      for (int x = 0; x < EDGE_WAVES; ++x) {
+        unpack8(red[wave][x][lane], y);
 #pragma unroll
-        for (int x = 1; x < AP_WAVES; ++x) {
-          const float y = red[x][wave][64 * j + lane];
-          m[j] = wave == 0 ? min_nan(m[j], y) : max_nan(m[j], y);
-        }
+        for (int j = 0; j < 8; ++j) m[j] = wave == 0 ? min_nan(m[j], y[j]) : max_nan(m[j], y[j]);
       }
-      if (in != 0) {
-        unpack8(load16(p), old);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) m[j] = wave == 0 ? min_nan(m[j], old[j]) : max_nan(m[j], old[j]);
-      }
-      *reinterpret_cast<u32x4*>(p) = pack8(m);
+      *reinterpret_cast<u32x4*>(edge) = pack8(m);
     }
     t += n;
   }
 }
 
 template <int LPH>
-hipError_t run(const AppendArgs& a, hipStream_t stream) {
+hipError_t run(AppendArgs a, hipStream_t stream) {
   constexpr int HPW = 64 / LPH;
   const int64_t waves = (int64_t)a.T * a.parts;
   const dim3 grid((uint32_t)((waves + AP_WAVES - 1) / AP_WAVES)), block(AP_WAVES * 64);
@@ -272,8 +284,13 @@ hipError_t run(const AppendArgs& a, hipStream_t stream) {
   else hipLaunchKernelGGL((append_kernel<LPH, false>), grid, block, 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.bounds == nullptr || a.starts == nullptr) return e;
-  hipLaunchKernelGGL(append_bounds_kernel<LPH>, dim3((a.T + AP_BLOCK - 1) / AP_BLOCK, (a.Hk + HPW - 1) / HPW), block,
-                     0, stream, a);
+  // as many tokens as a page has, so that a workgroup finds one page to look after, or fewer where sequences are
+  // shorter or workgroups few (a page takes its workgroup some microseconds, most of them waiting)
+  a.run_block = 1;
+  while (a.run_block < (1 << a.pt.shift) && (int64_t)2 * a.run_block * a.B <= a.T && a.T / a.run_block > 512)
+    a.run_block *= 2;
+  const dim3 runs((a.T + a.run_block - 1) / a.run_block, (a.Hk + HPW - 1) / HPW);
+  hipLaunchKernelGGL(append_bounds_kernel<LPH>, runs, dim3(EDGE_WAVES * 64), 0, stream, a);
   return hipGetLastError();
 }
 

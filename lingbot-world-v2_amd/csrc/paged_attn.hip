@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(DW * 64, 2) paged_kernel(const PagedAttnArgs a
   const int64_t r0 = (int64_t)(id % blocks) * HEADS;
   const int piece = id / blocks;
   const int nr = (int)(rows_all - r0 < HEADS ? rows_all - r0 : HEADS);
-  const bool end_to_end = KIND == DENSE && a.pieces > 0;
+  const bool end_to_end = KIND == DENSE && DW == 4 && a.pieces > 0;  // (eight waves: whole sequences)
   const int splits = KIND == PREFIX ? a.p_splits : a.splits;
 
   // this workgroup's tiles [at, end) of the batch laid end to end, from sequence b on

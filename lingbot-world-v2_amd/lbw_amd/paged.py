@@ -98,7 +98,7 @@ def paged_append_(cache: PagedKV, q, k, v, table, lens, rope: AxisRope, pos=None
     if q_out is None:
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     try:
-        _lib.ops().paged_append_(q, k, v, wq, wk, rope.table, rope.axes, rope.interleaved, pos, eps is not None,
+        _lib.ops().paged_append_.default(q, k, v, wq, wk, rope.table, rope.axes, rope.interleaved, pos, eps is not None,
                                  0.0 if eps is None else eps, q_scale, k_scale, table, lens, starts, q_out, cache.k,
                                  cache.v, cache.bounds)
     except (RuntimeError, NotImplementedError):
@@ -163,9 +163,9 @@ def attention_paged(q, cache: PagedKV, table, lens, *, selected=None, prefix_tab
     try:
         ops = _lib.ops()
         if out is None:
-            return ops.attention_paged(q, cache.k, cache.v, table, lens, selected, prefix_table, prefix_len, keys, s,
+            return ops.attention_paged.default(q, cache.k, cache.v, table, lens, selected, prefix_table, prefix_len, keys, s,
                                        num_splits)
-        ops.attention_paged_out(q, cache.k, cache.v, table, lens, selected, prefix_table, prefix_len, keys, s,
+        ops.attention_paged_out.default(q, cache.k, cache.v, table, lens, selected, prefix_table, prefix_len, keys, s,
                                 num_splits, out)
         return out
     except (RuntimeError, NotImplementedError):
@@ -214,7 +214,7 @@ def paged_select(q, cache: PagedKV, table, lens, count: int, *, first: int = 1, 
     if cache.bounds is None:
         raise ValueError("the cache has no bounds: paged_kv(..., bounds=True)")
     try:
-        return _lib.ops().paged_select(q, cache.bounds, table, lens, cache.k.shape[1], count, first, last)
+        return _lib.ops().paged_select.default(q, cache.bounds, table, lens, cache.k.shape[1], count, first, last)
     except (RuntimeError, NotImplementedError):
         heads = cache.k.shape[2] if cache.k.dim() == 4 else 0
         _check_query(q, heads)

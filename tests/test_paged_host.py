@@ -101,7 +101,7 @@ KV = [({"cache.k": None}, "cache's k"), ({"cache.v": ADDR + 2}, "cache's v"), ({
     ({"wq": ADDR + 4, "norm": 1}, "weights"), ({"pos": None, "n_axes": 2}, "pos missing"),
     ({"v": None}, "v must be"), ({"q_out": ADDR + 4}, "q_out must be"), ({"q_out_stride_h": 1 << 26}, "head stride"),
     ({"cache.k_stride_h": 1 << 26}, "head stride"), ({"cache.bounds": ADDR + 8}, "bounds"),
-    ({"tokens": 67108861, "batch": 67108861}, "above")])
+    ({"tokens": 33554431, "batch": 33554431}, "above")])
 def test_append_refusals(kw, message):
     from lbw_amd import _lib
     lib = _lib.load()
