@@ -102,9 +102,9 @@ int fill_select(const lbw_paged_select_params* p, SelectArgs* a) {
   if (p->cache.bounds == nullptr || !aligned16(p->cache.bounds))
     return fail(LBW_ERR_INVALID, "bounds must be a 16-byte aligned device pointer");
   if (p->batch > 0 && p->selected == nullptr) return fail(LBW_ERR_INVALID, "selected missing");
-  // (a workgroup of 256 per 32 pages, and one of 1024)
+  // (a workgroup for 32 pages, and one for all)
   const int64_t rows = (int64_t)p->batch * p->k_heads;
-  if (rows > kMaxWorkgroups / 4 || rows > kMaxWorkgroups / (p->cache.table_width / 32 + 1))
+  if (rows > kMaxWorkgroups || rows > kMaxWorkgroups / (p->cache.table_width / 32 + 1))
     return fail(LBW_ERR_UNSUPPORTED, "batch %d x %d heads x %d pages", p->batch, p->k_heads, p->cache.table_width);
   a->bounds = static_cast<const uint16_t*>(p->cache.bounds);
   a->count = p->count; a->first = p->first; a->last = p->last;

@@ -93,6 +93,7 @@ struct SelectArgs {
   PageTable pt;
   const int32_t* lens;
   int B, Hq, Hk, count, first, last;
+  int chunk;                  // pages that a workgroup of the score kernel takes
   uint64_t* score;            // [B][Hk][width] order-preserving images of the scores
   int32_t* sel;               // [B][Hk][count]
 };

@@ -12,7 +12,8 @@
 //
 // A wave scores four pages at a time: 16 lanes a page, 8 components each, with q's positive and negative parts in
 // registers. The second kernel has a workgroup per sequence and key/value head: it narrows the range of scores that
-// holds the last chosen one, 1024 equal bins at a time, until the choice is settled (a few rounds).
+// holds the last chosen one, 1024 equal bins at a time, until no more than 256 are left (one round mostly), whose ranks
+// are counted one against another.
 
 #include "capi_util.h"
 #include "head_rows.h"
@@ -22,15 +23,15 @@ namespace lbw {
 namespace {
 
 constexpr int SEL_D = 128;
-constexpr int SC_PAGES = 32;      // pages of a workgroup of the score kernel
 constexpr int SC_G = 5;           // query heads at a time, at most (64 registers of q each two)
-constexpr int TOP_T = 1024;       // threads of the choice, and bins
-constexpr int TOP_U = 4;          // scores per thread in registers
+constexpr int TOP_T = 256;        // threads of the choice
+constexpr int TOP_U = 16;         // scores per thread in registers
+constexpr int TOP_W = TOP_T / 64;
+constexpr int BINS = 1024;
 constexpr uint64_t INF_IMAGE = 0xfff0000000000000ull;
 
-// Order-preserving image of a score: -0 as 0, NaN as infinity.
+// Order-preserving image of a score that is not NaN, -0 as 0; never 0. (NaN counts as infinity.)
 __device__ __forceinline__ uint64_t image(double x) {
-  if (x != x) return INF_IMAGE;
   const uint64_t u = (uint64_t)__double_as_longlong(x + 0.0);
   return (u >> 63) ? ~u : u | (1ull << 63);
 }
@@ -61,14 +62,14 @@ __device__ __forceinline__ int pages_of(const SelectArgs& a, int b) {
 template <int G>
 __global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t chunks = (uint32_t)((a.pt.width + SC_PAGES - 1) / SC_PAGES);
+  const uint32_t chunks = (uint32_t)((a.pt.width + a.chunk - 1) / a.chunk);
   const int chunk = blockIdx.x % chunks, kv = (blockIdx.x / chunks) % (uint32_t)a.Hk,
             b = blockIdx.x / chunks / (uint32_t)a.Hk;
-  const int n = pages_of(a, b);
-  if (n <= a.count || chunk * SC_PAGES >= n) return;  // (all pages are chosen, or none is here)
   const int group = a.Hq / a.Hk, e0 = 8 * (lane & 15), sub = lane >> 4;
   const int32_t* const table = a.pt.p + b * a.pt.sb;
   uint64_t* const score = a.score + ((int64_t)b * a.Hk + kv) * a.pt.width;
+  const int n = pages_of(a, b);
+  if (n <= a.count || chunk * a.chunk >= n) return;  // (all pages are chosen, or none is here)
   for (int h0 = 0; h0 < group; h0 += G) {
     double up[G][8], down[G][8];
 #pragma unroll
@@ -82,17 +83,27 @@ __global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
         down[g][j] = f[j] < 0.0f ? (double)f[j] : 0.0;
       }
     }
-#pragma unroll
-    for (int i = 0; i < SC_PAGES / 16; ++i) {
-      const int page = chunk * SC_PAGES + 16 * i + 4 * wave + sub;
+    // the next pages' bounds are fetched while these are summed
+    int page = chunk * a.chunk + 4 * wave + sub;
+    const int end = min(n, (chunk + 1) * a.chunk);
+    u32x4 lw, hw;
+    bool bad = false;
+    auto fetch = [&](int i) {
       // (pages past the last are scored too, as page 0, and not written)
-      int at = page < n ? page_at(table, a.pt.width, a.pt.shift, a.pt.pages, (int64_t)page << a.pt.shift) : 0;
-      const bool bad = at < 0;
+      int at = i < end ? page_at(table, a.pt.width, a.pt.shift, a.pt.pages, (int64_t)i << a.pt.shift) : 0;
+      bad = at < 0;
       at = bad ? 0 : at;
       const uint16_t* p = a.bounds + ((int64_t)at * a.Hk + kv) * 2 * SEL_D + e0;
+      lw = load16(p);
+      hw = load16(p + SEL_D);
+    };
+    fetch(page);
+    for (; __any(page < end); page += 16) {
       float lo[8], hi[8];
-      unpack8(load16(p), lo);
-      unpack8(load16(p + SEL_D), hi);
+      unpack8(lw, lo);
+      unpack8(hw, hi);
+      const bool is_bad = bad;
+      fetch(page + 16);
       double x[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) x[g] = 0.0;
@@ -102,14 +113,16 @@ __global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
 #pragma unroll
         for (int g = 0; g < G; ++g) x[g] = __builtin_fma(down[g][j], l, __builtin_fma(up[g][j], h, x[g]));
       }
-      uint64_t best = 0;
+      double most = -INFINITY;
+      bool nan = is_bad;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
-        const uint64_t u = image(row_sum(x[g]));
-        best = u > best ? u : best;
+        const double y = row_sum(x[g]);
+        nan |= y != y;
+        most = fmax(most, y);
       }
-      if (bad) best = INF_IMAGE;
-      if (page < n && (lane & 15) == 0) {
+      uint64_t best = nan ? INF_IMAGE : image(most);
+      if (page < end && (lane & 15) == 0) {
         if (h0 > 0 && score[page] > best) best = score[page];
         score[page] = best;
       }
@@ -117,24 +130,11 @@ __global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
   }
 }
 
-// Reductions over a workgroup of 16 waves.
-template <typename F>
-__device__ __forceinline__ uint64_t reduce64(uint64_t x, F f, uint64_t* red, int lane, int wave) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x = f(x, (uint64_t)__shfl_xor((unsigned long long)x, o));
-  __syncthreads();
-  if (lane == 0) red[wave] = x;
-  __syncthreads();
-  uint64_t y = red[0];
-#pragma unroll
-  for (int w = 1; w < TOP_T / 64; ++w) y = f(y, red[w]);
-  return y;
-}
-
 __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
-  __shared__ uint32_t hist[TOP_T], sums[TOP_T / 64][2];
-  __shared__ uint64_t red[TOP_T / 64];
-  __shared__ uint32_t found[3];
+  __shared__ uint32_t hist[BINS], sums[TOP_W], counts[TOP_U * TOP_W][2];
+  __shared__ uint64_t range[TOP_W][2], cand[TOP_T], border;
+  __shared__ int32_t place[TOP_T];
+  __shared__ uint32_t found[3], collected;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kv = blockIdx.x % (uint32_t)a.Hk, b = blockIdx.x / (uint32_t)a.Hk;
   const int n = pages_of(a, b);
@@ -145,29 +145,52 @@ __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
   }
   const uint64_t* const score = a.score + ((int64_t)b * a.Hk + kv) * a.pt.width;
   auto kept = [&](int i) { return i < a.first || i >= n - a.last; };
+  // 0 for a page that is kept anyway, or is none
+  auto score_of = [&](int i) { return i < n && !kept(i) ? score[i] : 0; };
+  // page j * TOP_T + tid in mine[j]; those past TOP_U * TOP_T are read anew each time
   uint64_t mine[TOP_U];
 #pragma unroll
-  for (int j = 0; j < TOP_U; ++j) mine[j] = j * TOP_T + tid < n ? score[j * TOP_T + tid] : 0;
-  // f(score) of every page that is not kept anyway
+  for (int j = 0; j < TOP_U; ++j) mine[j] = j * TOP_T < n ? score_of(j * TOP_T + tid) : 0;
   auto each = [&](auto f) {
 #pragma unroll
     for (int j = 0; j < TOP_U; ++j) {
-      const int i = j * TOP_T + tid;
-      if (i < n && !kept(i)) f(mine[j]);
+      if (j * TOP_T >= n) break;
+      f(mine[j], j * TOP_T + tid);
     }
-    for (int i = TOP_U * TOP_T + tid; i < n; i += TOP_T)
-      if (!kept(i)) f(score[i]);
+    for (int i = TOP_U * TOP_T + tid; i < n; i += TOP_T) f(score_of(i), i);
+  };
+  auto clear = [&] {
+#pragma unroll
+    for (int i = 0; i < BINS / TOP_T; ++i) hist[i * TOP_T + tid] = 0;
   };
   uint32_t need = (uint32_t)(a.count - a.first - a.last);  // (n > count: first and last do not meet)
-  uint64_t over = ~0ull;  // chosen: scores above this, and `need` of those that equal it
+  uint64_t over = ~0ull;  // chosen: scores above this, and the first `need` of those that equal it
   if (need > 0) {
     uint64_t lo = ~0ull, hi = 0;
-    each([&](uint64_t u) {
-      lo = u < lo ? u : lo;
+    each([&](uint64_t u, int) {
+      lo = u - 1 < lo ? u - 1 : lo;  // (0 becomes the largest)
       hi = u > hi ? u : hi;
     });
-    lo = reduce64(lo, [](uint64_t x, uint64_t y) { return x < y ? x : y; }, red, lane, wave);
-    hi = reduce64(hi, [](uint64_t x, uint64_t y) { return x > y ? x : y; }, red, lane, wave);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      const uint64_t x = (uint64_t)__shfl_xor((unsigned long long)lo, o);
+      const uint64_t y = (uint64_t)__shfl_xor((unsigned long long)hi, o);
+      lo = x < lo ? x : lo;
+      hi = y > hi ? y : hi;
+    }
+    if (lane == 0) {
+      range[wave][0] = lo;
+      range[wave][1] = hi;
+    }
+    if (tid == 0) collected = 0;
+    clear();
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < TOP_W; ++w) {
+      lo = range[w][0] < lo ? range[w][0] : lo;
+      hi = range[w][1] > hi ? range[w][1] : hi;
+    }
+    ++lo;
     // the last chosen score is in [lo, hi], the need-th highest of those there
     while (true) {
       if (lo == hi) {
@@ -175,82 +198,142 @@ __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
         break;
       }
       const int bits = 64 - __clzll((unsigned long long)(hi - lo)), shift = bits > 10 ? bits - 10 : 0;
-      hist[tid] = 0;
-      __syncthreads();
-      each([&](uint64_t u) {
+      each([&](uint64_t u, int) {
         if (u >= lo && u <= hi) atomicAdd(&hist[(u - lo) >> shift], 1u);
       });
       __syncthreads();
-      // bin tid from the top: how many scores are in it and in those above it
-      const uint32_t own = hist[TOP_T - 1 - tid];
-      uint32_t sum = own;
+      // four bins a thread, from the top: how many scores are in them and in those above
+      constexpr int BPT = BINS / TOP_T;
+      uint32_t own[BPT], sum = 0;
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) sum += own[i] = hist[BINS - 1 - (tid * BPT + i)];
+      uint32_t upto = sum;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t y = __shfl_up(sum, o);
-        if (lane >= o) sum += y;
+        const uint32_t y = __shfl_up(upto, o);
+        if (lane >= o) upto += y;
       }
-      if (lane == 63) sums[wave][0] = sum;
+      if (lane == 63) sums[wave] = upto;
       __syncthreads();
 #pragma unroll
-      for (int w = 0; w < TOP_T / 64 - 1; ++w) sum += w < wave ? sums[w][0] : 0;
-      if (sum >= need && sum - own < need) {  // one thread: counts reach `need` once
-        found[0] = TOP_T - 1 - tid;
-        found[1] = own;
-        found[2] = need - (sum - own);
+      for (int w = 0; w < TOP_W - 1; ++w) upto += w < wave ? sums[w] : 0;
+      upto -= sum;
+#pragma unroll
+      for (int i = 0; i < BPT; ++i) {
+        if (upto < need && upto + own[i] >= need) {  // one bin: counts reach `need` once
+          found[0] = BINS - 1 - (tid * BPT + i);
+          found[1] = own[i];
+          found[2] = need - upto;
+        }
+        upto += own[i];
       }
+      clear();
       __syncthreads();
-      const uint64_t l = lo + ((uint64_t)found[0] << shift), h = l + ((1ull << shift) - 1);
-      need = found[2];
-      const bool all = need == found[1];
-      lo = l;
+      lo += (uint64_t)found[0] << shift;
+      const uint64_t h = lo + ((1ull << shift) - 1);
       hi = h < hi ? h : hi;
-      if (all) {  // every score of the bin
+      need = found[2];
+      const uint32_t in_bin = found[1];
+      if (need == in_bin) {  // every score of the bin
         over = lo - 1;
         need = 0;
+        break;
+      }
+      if (in_bin <= TOP_T) {
+        each([&](uint64_t u, int i) {
+          if (u >= lo && u <= hi) {
+            const uint32_t at = atomicAdd(&collected, 1u);
+            cand[at] = u;
+            place[at] = i;
+          }
+        });
+        __syncthreads();
+        if (tid < (int)in_bin) {  // (their order differs from run to run, their ranks do not)
+          const uint64_t u = cand[tid];
+          const int32_t i = place[tid];
+          uint32_t above = 0, rank = 0;
+          for (uint32_t j = 0; j < in_bin; ++j) {
+            above += cand[j] > u;
+            rank += cand[j] > u || (cand[j] == u && place[j] < i);
+          }
+          if (rank == need - 1) {
+            border = u;
+            found[2] = need - above;
+          }
+        }
+        __syncthreads();
+        over = border;
+        need = found[2];
         break;
       }
       __syncthreads();  // found is read
     }
   }
-  // in ascending order: kept pages and scores above come first-come, of equal ones the first `need`
-  uint32_t above0 = 0, equal0 = 0;
+  // in ascending order: kept pages and scores above, of equal ones the first `need`
   const uint64_t before = ((uint64_t)1 << lane) - 1;
-  auto put = [&](int i, uint64_t u) {
-    const bool is_kept = i < n && kept(i);
-    const bool above = is_kept || (i < n && u > over), equal = i < n && !is_kept && u == over;
-    const uint64_t ma = __ballot(above), me = __ballot(equal);
-    __syncthreads();  // the last sums are read
-    if (lane == 0) {
-      sums[wave][0] = __popcll(ma);
-      sums[wave][1] = __popcll(me);
+  uint32_t above0 = 0, equal0 = 0;
+  for (int base = 0; base < n; base += TOP_U * TOP_T) {
+    // a page's: bit 16 above, bit 17 equal, and how many above (bits 0 ..) and equal ones (bits 8 ..) the wave's lower
+    // lanes hold
+    uint32_t turn[TOP_U];
+#pragma unroll
+    for (int j = 0; j < TOP_U; ++j) {
+      turn[j] = 0;
+      if (base + j * TOP_T >= n) continue;
+      const int i = base + j * TOP_T + tid;
+      const uint64_t u = base == 0 ? mine[j] : score_of(i);
+      const bool above = (i < n && kept(i)) || u > over, equal = u == over;
+      const uint64_t ma = __ballot(above), me = __ballot(equal);
+      turn[j] = (uint32_t)__popcll(ma & before) | (uint32_t)__popcll(me & before) << 8 | (above ? 1u << 16 : 0) |
+                (equal ? 1u << 17 : 0);
+      if (lane == 0) {
+        counts[j * TOP_W + wave][0] = __popcll(ma);
+        counts[j * TOP_W + wave][1] = __popcll(me);
+      }
     }
     __syncthreads();
-    uint32_t na = above0 + __popcll(ma & before), ne = equal0 + __popcll(me & before);
+    // lane x: how many are in the first x + 1 of the waves' turns
+    static_assert(TOP_U * TOP_W == 64, "a lane for each turn of each wave");
+    const bool there = base + (lane / TOP_W) * TOP_T < n;
+    const uint32_t na = there ? counts[lane][0] : 0, ne = there ? counts[lane][1] : 0;
+    uint32_t sa = na, se = ne;
 #pragma unroll
-    for (int w = 0; w < TOP_T / 64; ++w) {
-      na += w < wave ? sums[w][0] : 0;
-      ne += w < wave ? sums[w][1] : 0;
-      above0 += sums[w][0];
-      equal0 += sums[w][1];
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t x = __shfl_up(sa, o), y = __shfl_up(se, o);
+      if (lane >= o) {
+        sa += x;
+        se += y;
+      }
     }
-    if (above || (equal && ne < need)) sel[na + (ne < need ? ne : need)] = i;
-  };
 #pragma unroll
-  for (int j = 0; j < TOP_U; ++j)
-    if (j * TOP_T < n) put(j * TOP_T + tid, mine[j]);
-  for (int i0 = TOP_U * TOP_T; i0 < n; i0 += TOP_T) put(i0 + tid, i0 + tid < n ? score[i0 + tid] : 0);
+    for (int j = 0; j < TOP_U; ++j) {
+      if (base + j * TOP_T >= n) continue;
+      const int x = j * TOP_W + wave;
+      const uint32_t pa = above0 + __builtin_amdgcn_readlane(sa - na, x) + (turn[j] & 255);
+      const uint32_t pe = equal0 + __builtin_amdgcn_readlane(se - ne, x) + (turn[j] >> 8 & 255);
+      if ((turn[j] >> 16 & 1) || ((turn[j] >> 17) && pe < need))
+        sel[pa + (pe < need ? pe : need)] = base + j * TOP_T + tid;
+    }
+    above0 += __shfl(sa, 63);
+    equal0 += __shfl(se, 63);
+    __syncthreads();  // the counts are read
+  }
 }
 
 template <int G>
 void score(const SelectArgs& a, hipStream_t stream) {
-  const int64_t chunks = (a.pt.width + SC_PAGES - 1) / SC_PAGES;
+  const int64_t chunks = (a.pt.width + a.chunk - 1) / a.chunk;
   hipLaunchKernelGGL(select_score_kernel<G>, dim3((uint32_t)(chunks * a.Hk * a.B)), dim3(256), 0, stream, a);
 }
 
 }  // namespace
 
-hipError_t launch_select(const SelectArgs& a, hipStream_t stream) {
+hipError_t launch_select(const SelectArgs& args, hipStream_t stream) {
+  SelectArgs a = args;
   if (a.pt.width > a.count) {  // (else every page is chosen)
+    // pages of a workgroup: 32, more once that gives eight workgroups a CU (each turns its q into 64 bits first)
+    a.chunk = 32;
+    while (a.chunk < 256 && (int64_t)a.B * a.Hk * a.pt.width > (int64_t)8 * num_cus() * a.chunk) a.chunk *= 2;
     // a group's heads in equal turns of five at most
     const int group = a.Hq / a.Hk, turns = (group + SC_G - 1) / SC_G;
     switch ((group + turns - 1) / turns) {

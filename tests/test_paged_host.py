@@ -132,7 +132,7 @@ def test_attention_refusals(kw, message):
     ({"count": 0}, "count"), ({"first": -1}, "count"), ({"last": 2}, "count"),
     ({"first": 2147483647, "last": 2147483647, "count": 2147483647}, "count"), ({"cache.bounds": None}, "bounds"),
     ({"cache.bounds": ADDR + 8}, "bounds"), ({"selected": None}, "selected"), ({"head_dim": 256}, "only 128"),
-    ({"batch": 1 << 22}, "batch")])
+    ({"batch": 1 << 23}, "batch")])
 def test_select_refusals(kw, message):
     from lbw_amd import _lib
     lib = _lib.load()
