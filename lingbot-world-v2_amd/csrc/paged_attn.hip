@@ -17,7 +17,7 @@
 #include <algorithm>
 
 #include "capi_util.h"
-#include "packed_tiles.h"
+#include "packed_loop.h"
 #include "paged.h"
 #include "sequence_tiles.h"
 
@@ -32,6 +32,9 @@ constexpr int RING_B = 2 * DT_B;            // per wave: K, V
 constexpr int NCOPY = DT_B / 1024;          // copies per lane for K or V of a tile
 constexpr int HEADS = 32;                   // query rows per workgroup
 enum Kind { DENSE, SPARSE, PREFIX };
+constexpr int P_LIST = 4096;                // table entries of a piece of the prefix (tile form)
+constexpr int PREFIX_LDS = FWD_LDS + 4 * P_LIST;
+typedef __attribute__((address_space(3))) int32_t lds_i32;
 
 // A sequence's keys: its length, limited to what its row of the table holds.
 __device__ __forceinline__ int keys_of(const PagedAttnArgs& a, int b) {
@@ -299,6 +302,125 @@ __global__ void __launch_bounds__(DW * 64, 2) paged_kernel(const PagedAttnArgs a
   } while (true);
 }
 
+// A piece of the prefix for 128 query rows of a key/value head: the packed attention's walk, 4 waves of 32 rows over
+// shared tiles of 64 keys, each wave copying the 16 tokens of a tile that lie in one page. A page outside the cache
+// becomes keys of NaN. `id`: piece, block of rows, head, the head fastest, so that a piece's blocks of rows run beside
+// each other on one XCD.
+__device__ __forceinline__ void prefix_tiles(const PagedAttnArgs& a, uint32_t id, unsigned char* lds) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hl = lane >> 5, l32 = lane & 31;
+  const int group = a.Hq / a.Hk;
+  const int64_t rows_all = (int64_t)a.B * group;
+  const uint32_t blocks = (uint32_t)((rows_all + PK_BLOCK - 1) / PK_BLOCK);
+  const int kv = id % (uint32_t)a.Hk;
+  id /= (uint32_t)a.Hk;
+  const int64_t r0 = (int64_t)(id % blocks) * PK_BLOCK + 32 * wave;  // this wave's first row
+  const int piece = id / blocks;
+  const int nr = (int)(rows_all - r0 < 32 ? rows_all - r0 : 32);      // and how many it has (0 or less: none)
+  const int len = (int)scalar64(prefix_keys(a)), shift = a.pt.shift, mask = (1 << shift) - 1;
+  const int n_tiles = (len + BN - 1) / BN;
+  const int t0 = (int)((int64_t)n_tiles * piece / a.p_splits);
+  const int T = (int)((int64_t)n_tiles * (piece + 1) / a.p_splits) - t0;
+
+  u32x4 qf[8];
+  {
+    const int64_t row = r0 + l32 < rows_all ? r0 + l32 : rows_all - 1;  // this lane's query row
+    const uint16_t* p = a.q.p + row / group * a.q.sl + (kv * group + row % group) * a.q.sh + 8 * hl;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const u32x4*>(p + 16 * s);
+  }
+  // the pages of the piece's table entries, behind the tiles in LDS (-1: outside the cache)
+  const int e0 = (int)(((int64_t)t0 * BN) >> shift), n_pages = T > 0 ? (int)(((int64_t)(t0 + T) * BN - 1) >> shift) - e0 + 1 : 0;
+  const int list = (int)lds_addr(lds) + FWD_LDS;
+  for (int i = threadIdx.x; i < n_pages; i += PK_WAVES * 64)
+    *(lds_i32*)(uintptr_t)(list + 4 * i) =
+        page_at(a.p_table, a.p_width, shift, a.pt.pages, (int64_t)(e0 + i) << shift);
+  __syncthreads();
+  // a wave's share of a tile: 16 tokens of one page; one without keys copies the prefix's last one
+  const int share = 16 * wave;
+  const int end = len > 0 ? len - 1 : 0;
+  const int crow = lane >> 4, ccol = ((lane & 15) ^ swz(lane >> 4)) * 16;
+  const uint32_t koff = (uint32_t)crow * (uint32_t)(a.k.sl * 2), voff = (uint32_t)crow * (uint32_t)(a.v.sl * 2);
+  const uint32_t dst = lds_addr(lds) + 1024 * PK_NDMA * wave;
+  auto page_of = [&](int u) {  // (read ahead of its use)
+    int pos = (t0 + u) * BN + share;
+    pos = pos < len ? pos : end;
+    return *(const lds_i32*)(uintptr_t)(list + 4 * ((pos >> shift) - e0));
+  };
+  auto issue = [&](const PageRows& src, uint32_t off, int page, int u, uint32_t to, bool is_k) {
+    const int pos = (t0 + u) * BN + share;
+    if (page < 0) {
+      if (is_k) {
+        // (opaque here and below: nothing of this is worth registers in the loop, which has none left)
+        const uint32_t nan = opaque(0x7fc07fc0);
+        const int at = opaque(16 * lane);
+#pragma unroll
+        for (int i = 0; i < PK_NDMA; ++i)
+          *(lds_u32x4*)(uintptr_t)(to + 1024 * i + at) = u32x4{nan, nan, nan, nan};
+        return;
+      }
+      page = 0;
+    }
+    const int64_t sl = src.sl * 2;
+    const int in = (pos < len ? pos : end) & mask, more = len - 1 - pos;  // tokens behind the share's first one
+    const unsigned char* b = reinterpret_cast<const unsigned char*>(src.p + kv * src.sh) + page * (src.sp * 2) + in * sl;
+    const int col = opaque(ccol);
+    if (more >= HT - 1) {
+#pragma unroll
+      for (int i = 0; i < PK_NDMA; ++i) dma16_guarded(b + 4 * i * sl, off + (col ^ (i << 4)), to + 1024 * i);
+    } else {
+      const int last = more > 0 ? more : 0, row = opaque(crow);
+#pragma unroll
+      for (int i = 0; i < PK_NDMA; ++i) {
+        const int x = row + 4 * i, r = x < last ? x : last;
+        dma16_guarded(b, (uint32_t)r * (uint32_t)sl + (col ^ (i << 4)), to + 1024 * i);
+      }
+    }
+  };
+  // K of tile u + 1 goes ahead of V of tile u: the page of the share before is kept
+  int ahead = T > 0 ? page_of(0) : 0, now = 0, prev = 0;
+  auto issue_k = [&](int u) {
+    prev = now;
+    now = __builtin_amdgcn_readfirstlane(ahead);
+    issue(a.k, koff, now, u, dst + (u & 1) * PK_TILE_B, true);
+    if (u + 1 < T) ahead = page_of(u + 1);
+  };
+  auto issue_v = [&](int u) {
+    issue(a.v, voff, u > 0 && u + 1 < T ? prev : now, u, dst + V_AT + (u & 1) * PK_TILE_B, false);
+  };
+  floatx16 o[4];
+  float m, l;
+  if (nr <= 0) {
+    copy_tiles(lds, wave, lane, T, issue_k, issue_v);
+    return;
+  }
+  // (every wave that gets here needs all tiles: a count of its own would cost 60 registers)
+  attend_tiles(lds, wave, lane, qf, sreg(a.scale_log2), t0, T, T, len, len, issue_k, issue_v, o, m, l);
+  l = wave_sum_xor32(l);
+  if (l32 >= nr) return;
+  // (the lane hidden: the row's place is worked out anew, not kept in registers all the way)
+  const int64_t row = r0 + opaque(l32), rows = all_rows(a);
+  const int64_t part = (kv * group + row % group) * rows + own_rows(a) + row / group * a.p_splits + piece;
+  float* const dst_o = a.part + part * D + 4 * hl;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<floatx4*>(dst_o + 32 * db + 8 * g) =
+          floatx4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+  if (hl == 0) {
+    float* st = a.part + a.Hq * rows * D;
+    st[part] = l == 0.0f ? -INFINITY : m;
+    st[a.Hq * rows + part] = l;
+  }
+}
+
+__global__ void __launch_bounds__(PK_WAVES * 64, 2) prefix_tiles_kernel(const PagedAttnArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  prefix_tiles(a, blockIdx.x, lds);
+}
+
 // A workgroup per (sequence, query head): the parts of its own keys, then the prefix's, joined, its waves taking
 // 64 / JW parts at a time in turn, then in the waves' order. No parts: zeros (or, end to end without a prefix, a
 // result that one piece has written already).
@@ -414,15 +536,30 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
   } else {
     a->pieces = decode_pieces(a->B, a->Hq, a->Hk, (int64_t)a->pt.width << a->pt.shift, num_splits, cus);
   }
-  if (a->p_max > 0)
-    a->p_splits = cut((a->p_max + DT - 1) / DT, a->Hk * ((a->B * group + HEADS - 1) / HEADS));
+  if (a->p_max > 0) {
+    const int64_t rows = a->B * group;
+    a->p_block = rows > HEADS ? PK_BLOCK : HEADS;
+    a->p_splits = cut((a->p_max + DT - 1) / DT, a->Hk * ((rows + a->p_block - 1) / a->p_block));
+    // (a piece's table entries fit their place: whole tiles of 64 keys, an entry more where a piece ends in a page)
+    const int64_t tiles = (a->p_max + BN - 1) / BN, most = ((int64_t)(P_LIST - 1) << a->pt.shift) / BN;
+    if (a->p_block == PK_BLOCK) a->p_splits = (int)std::max<int64_t>(a->p_splits, (tiles + most - 1) / most);
+  }
 }
 
 hipError_t launch_paged(const PagedAttnArgs& a, hipStream_t stream) {
   const int group = a.Hq / a.Hk, blocks = (group + HEADS - 1) / HEADS;
   hipError_t e;
   if (a.p_splits > 0) {
-    e = run<4, PREFIX>(a, a.p_splits * (((int64_t)a.B * group + HEADS - 1) / HEADS), stream);
+    const int64_t n = a.p_splits * (((int64_t)a.B * group + a.p_block - 1) / a.p_block);
+    if (a.p_block == HEADS) {
+      e = run<4, PREFIX>(a, n, stream);
+    } else {
+      static LdsAllowed allowed;
+      e = allow_lds((const void*)prefix_tiles_kernel, PREFIX_LDS, allowed);
+      if (e != hipSuccess) return e;
+      hipLaunchKernelGGL(prefix_tiles_kernel, dim3((uint32_t)(n * a.Hk)), dim3(PK_WAVES * 64), PREFIX_LDS, stream, a);
+      e = hipGetLastError();
+    }
     if (e != hipSuccess) return e;
   }
   const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B * a.splits) * blocks;
