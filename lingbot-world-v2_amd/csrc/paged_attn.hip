@@ -56,17 +56,16 @@ __device__ __forceinline__ int list_length(const int32_t* sel, int n, int lane) 
   return n;
 }
 
+// Workgroup `id` of those for one kind of keys: key/value head (fastest), block of query rows, piece.
 template <int DW, Kind KIND>  // waves per workgroup
-__global__ void __launch_bounds__(DW * 64, 2) paged_kernel(const PagedAttnArgs a) {
+__device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id, unsigned char* lds) {
   constexpr int DEC_LDS = DW * RING_B;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
   const int group = a.Hq / a.Hk;
   const int64_t rows_all = KIND == PREFIX ? (int64_t)a.B * group : group;  // query rows of a key/value head
   const uint32_t blocks = (uint32_t)((rows_all + HEADS - 1) / HEADS);
-  uint32_t id = blockIdx.x;
   const int kv = id % (uint32_t)a.Hk;
   id /= (uint32_t)a.Hk;
   const int64_t r0 = (int64_t)(id % blocks) * HEADS;
@@ -416,9 +415,25 @@ __device__ __forceinline__ void prefix_tiles(const PagedAttnArgs& a, uint32_t id
   }
 }
 
-__global__ void __launch_bounds__(PK_WAVES * 64, 2) prefix_tiles_kernel(const PagedAttnArgs a) {
+template <int DW, Kind KIND>
+__global__ void __launch_bounds__(DW * 64, 2) paged_kernel(const PagedAttnArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
-  prefix_tiles(a, blockIdx.x, lds);
+  attend_pages<DW, KIND>(a, blockIdx.x, lds);
+}
+
+// The prefix (TILES: 128 query rows at a time) and the sequences' own keys in one launch: their workgroups take turns,
+// in proportion, so that a CU has some of each. The prefix's matrix products then run while own keys are read.
+template <bool TILES, Kind KIND>
+__global__ void __launch_bounds__(4 * 64, 2) paged_both_kernel(const PagedAttnArgs a, uint32_t p_units, uint32_t units) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
+  const uint32_t unit = blockIdx.x / (uint32_t)a.Hk, kv = blockIdx.x % (uint32_t)a.Hk;
+  const uint32_t before = (uint32_t)((uint64_t)unit * p_units / units);  // units of the prefix among those before
+  if ((uint32_t)((uint64_t)(unit + 1) * p_units / units) > before) {
+    if constexpr (TILES) prefix_tiles(a, before * a.Hk + kv, lds);
+    else attend_pages<4, PREFIX>(a, before * a.Hk + kv, lds);
+  } else {
+    attend_pages<4, KIND>(a, (unit - before) * a.Hk + kv, lds);
+  }
 }
 
 // A workgroup per (sequence, query head): the parts of its own keys, then the prefix's, joined, its waves taking
@@ -507,13 +522,27 @@ __global__ void __launch_bounds__(JW * 64) paged_join_kernel(const PagedAttnArgs
       pack_bf16x2(x * inv, y * inv);
 }
 
+constexpr int lds_bytes(int waves) { return waves * RING_B + 2 * waves * HEADS * 4; }
+
 template <int DW, Kind KIND>
 hipError_t run(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
-  constexpr int bytes = DW * RING_B + 2 * DW * HEADS * 4;
+  constexpr int bytes = lds_bytes(DW);
   static LdsAllowed allowed;
   const hipError_t attr = allow_lds((const void*)paged_kernel<DW, KIND>, bytes, allowed);
   if (attr != hipSuccess) return attr;
   hipLaunchKernelGGL((paged_kernel<DW, KIND>), dim3((uint32_t)(units * a.Hk)), dim3(DW * 64), bytes, stream, a);
+  return hipGetLastError();
+}
+
+template <bool TILES, Kind KIND>
+hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
+  constexpr int bytes = TILES ? std::max(PREFIX_LDS, lds_bytes(4)) : lds_bytes(4);
+  static LdsAllowed allowed;
+  const hipError_t attr = allow_lds((const void*)paged_both_kernel<TILES, KIND>, bytes, allowed);
+  if (attr != hipSuccess) return attr;
+  const int64_t p_units = a.p_splits * (((int64_t)a.B * (a.Hq / a.Hk) + a.p_block - 1) / a.p_block);
+  hipLaunchKernelGGL((paged_both_kernel<TILES, KIND>), dim3((uint32_t)((p_units + units) * a.Hk)), dim3(4 * 64), bytes,
+                     stream, a, (uint32_t)p_units, (uint32_t)(p_units + units));
   return hipGetLastError();
 }
 
@@ -532,7 +561,9 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
   };
   if (a->B == 0) return;
   if (a->sel != nullptr) {
-    a->splits = cut((((int64_t)a->n_sel << a->pt.shift) + DT - 1) / DT, a->B * units);
+    // (as whole sequences: 1024 keys and fewer are not worth a second launch)
+    const int64_t keys = (int64_t)a->n_sel << a->pt.shift;
+    if (num_splits > 0 || keys > 1024) a->splits = cut((keys + DT - 1) / DT, a->B * units);
   } else {
     a->pieces = decode_pieces(a->B, a->Hq, a->Hk, (int64_t)a->pt.width << a->pt.shift, num_splits, cus);
   }
@@ -548,25 +579,18 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
 
 hipError_t launch_paged(const PagedAttnArgs& a, hipStream_t stream) {
   const int group = a.Hq / a.Hk, blocks = (group + HEADS - 1) / HEADS;
+  const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B * a.splits) * blocks;
   hipError_t e;
   if (a.p_splits > 0) {
-    const int64_t n = a.p_splits * (((int64_t)a.B * group + a.p_block - 1) / a.p_block);
-    if (a.p_block == HEADS) {
-      e = run<4, PREFIX>(a, n, stream);
-    } else {
-      static LdsAllowed allowed;
-      e = allow_lds((const void*)prefix_tiles_kernel, PREFIX_LDS, allowed);
-      if (e != hipSuccess) return e;
-      hipLaunchKernelGGL(prefix_tiles_kernel, dim3((uint32_t)(n * a.Hk)), dim3(PK_WAVES * 64), PREFIX_LDS, stream, a);
-      e = hipGetLastError();
-    }
-    if (e != hipSuccess) return e;
+    const bool tiles = a.p_block == PK_BLOCK;
+    if (a.sel != nullptr) e = tiles ? run_both<true, SPARSE>(a, n, stream) : run_both<false, SPARSE>(a, n, stream);
+    else e = tiles ? run_both<true, DENSE>(a, n, stream) : run_both<false, DENSE>(a, n, stream);
+  } else {
+    // whole sequences that leave every CU one workgroup at most: eight waves in it
+    const bool wide = a.pieces == 0 && n * a.Hk <= num_cus();
+    if (a.sel != nullptr) e = wide ? run<8, SPARSE>(a, n, stream) : run<4, SPARSE>(a, n, stream);
+    else e = wide ? run<8, DENSE>(a, n, stream) : run<4, DENSE>(a, n, stream);
   }
-  const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B * a.splits) * blocks;
-  // whole sequences that leave every CU one workgroup at most: eight waves in it
-  const bool wide = a.pieces == 0 && n * a.Hk <= num_cus();
-  if (a.sel != nullptr) e = wide ? run<8, SPARSE>(a, n, stream) : run<4, SPARSE>(a, n, stream);
-  else e = wide ? run<8, DENSE>(a, n, stream) : run<4, DENSE>(a, n, stream);
   if (e != hipSuccess || !has_parts(a)) return e;
   hipLaunchKernelGGL(paged_join_kernel, dim3((uint32_t)((int64_t)a.B * a.Hq)), dim3(JW * 64), 0, stream, a);
   return hipGetLastError();
