@@ -549,31 +549,45 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 }  // namespace
 
 // How the keys are cut: own ones as the single-token attention over whole caches cuts them (whole sequences where they
-// give work enough, else the batch's keys in equal pieces), selected and the prefix's in equal pieces for two
-// workgroups a CU, of 6 tiles or more.
+// give work enough, else the batch's keys in equal pieces), selected and the prefix's in equal pieces, of 6 tiles or
+// more, for as many workgroups as run at once.
+// Prefix, 32 / 128 query rows at a time: 14040 keys, 1500 own x 40/8 heads, 8 sequences (40 rows) 30.9 / 35.6 us, 20 (100)
+// 42.5 / 46.5, 40 (200) 65.6 / 54.4; 46800, 1000 own x 12/4, 24 rows 34.5 / 36.6, 60 rows 44.0 / 43.0, 78 rows 49.3 / 51.8,
+// 99 rows 58.5 / 54.8; 4680, 100 own x 12/12, 33 rows 27.5 / 24.4, 64 rows 31.9 / 30.1. Own keys whole / in pieces with
+// it: 16 of up to 1560 off 14040 x 12/12 42 / 38, 64 of up to 3600 off 46800 x 40/8 197 / 186.
 void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
   const int64_t group = a->Hq / a->Hk, units = a->Hk * ((group + HEADS - 1) / HEADS);
   a->splits = 1;
   a->pieces = a->p_splits = 0;
+  int64_t places = 2 * cus;  // workgroups that run at once
   auto cut = [&](int64_t tiles, int64_t busy) {
     if (num_splits > 0) return (int)num_splits;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * cus / busy, tiles / 6));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(places / busy, tiles / 6));
   };
   if (a->B == 0) return;
-  if (a->sel != nullptr) {
-    // (as whole sequences: 1024 keys and fewer are not worth a second launch)
-    const int64_t keys = (int64_t)a->n_sel << a->pt.shift;
-    if (num_splits > 0 || keys > 1024) a->splits = cut((keys + DT - 1) / DT, a->B * units);
-  } else {
-    a->pieces = decode_pieces(a->B, a->Hq, a->Hk, (int64_t)a->pt.width << a->pt.shift, num_splits, cus);
-  }
+  const int64_t cap = (int64_t)a->pt.width << a->pt.shift;
+  // own keys: whole sequences of 1024 keys and fewer, which are not worth a second launch; with a prefix, whose results
+  // are joined anyway, in pieces whatever the batch
+  const int64_t keys = a->sel != nullptr ? (int64_t)a->n_sel << a->pt.shift : cap;
+  const bool whole = num_splits == 1 || (num_splits == 0 && keys <= 1024);
   if (a->p_max > 0) {
     const int64_t rows = a->B * group;
-    a->p_block = rows > HEADS ? PK_BLOCK : HEADS;
+    a->p_block = rows > 3 * HEADS ? PK_BLOCK : HEADS;
+    // 32 rows at a time: the places that whole sequences leave, half of them at least (the other half for own keys in
+    // pieces); 128 rows: all, and own keys come on top, as such a workgroup alone on a CU waits most of the time
+    if (a->p_block == HEADS) places = std::max<int64_t>(cus, 2 * cus - (whole ? a->B * units : cus));
     a->p_splits = cut((a->p_max + DT - 1) / DT, a->Hk * ((rows + a->p_block - 1) / a->p_block));
     // (a piece's table entries fit their place: whole tiles of 64 keys, an entry more where a piece ends in a page)
     const int64_t tiles = (a->p_max + BN - 1) / BN, most = ((int64_t)(P_LIST - 1) << a->pt.shift) / BN;
     if (a->p_block == PK_BLOCK) a->p_splits = (int)std::max<int64_t>(a->p_splits, (tiles + most - 1) / most);
+    if (a->p_block == HEADS) places = cus;
+  }
+  if (a->sel != nullptr) {
+    if (!whole) a->splits = cut((keys + DT - 1) / DT, a->B * units);
+  } else if (a->p_max > 0 && num_splits == 0) {
+    if (!whole) a->pieces = cut(a->B * ((cap + DT - 1) / DT), units);
+  } else {
+    a->pieces = decode_pieces(a->B, a->Hq, a->Hk, cap, num_splits, cus);
   }
 }
 
