@@ -68,6 +68,7 @@ int fill_paged(const lbw_attention_paged_params* p, PagedAttnArgs* a) {
   a->out = {static_cast<uint16_t*>(p->out), p->out_stride_b, p->out_stride_h};
   LBW_TRY(check_scale(p->softmax_scale, p->head_dim, &a->scale));
   a->scale_log2 = (float)((double)a->scale * kLog2e);
+  a->group = a->Hq / a->Hk;
   if (p->selected != nullptr) {
     if (p->n_selected < 0 || ((int64_t)p->n_selected << a->pt.shift) > 0x7fffff00)
       return fail(LBW_ERR_INVALID, "n_selected %d pages of %d tokens", p->n_selected, p->cache.page_size);

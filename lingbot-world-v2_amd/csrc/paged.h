@@ -61,7 +61,7 @@ struct PagedAttnArgs {
   const int32_t* sel;         // [B][Hk][n_sel] entries of the table to attend to, up to the first negative one;
   int n_sel;                  // null: all
   RowsOut out;                // [B, Hq, D]
-  int B, Hq, Hk;
+  int B, Hq, Hk, group;       // group: Hq / Hk
   float scale, scale_log2;
   // own keys: the whole batch's in `pieces` equal pieces per key/value head, or (pieces 0) each sequence's in
   // `splits`

@@ -63,7 +63,7 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  const int group = a.Hq / a.Hk;
+  const int group = a.group;
   const int64_t rows_all = KIND == PREFIX ? (int64_t)a.B * group : group;  // query rows of a key/value head
   const uint32_t blocks = (uint32_t)((rows_all + HEADS - 1) / HEADS);
   const int kv = id % (uint32_t)a.Hk;
@@ -94,6 +94,7 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
   const int ka = row_address(ring, l32, hl), va = tr_address(ring + DT_B, lane, hl);
   // copy i of a tile: rows 4 i + lane / 16, chunk (lane % 16) ^ swz(row); rows i and i + 4 share the chunk
   const int crow = lane >> 4, ccol = ((lane & 15) ^ swz(lane >> 4)) * 16;
+  const uint32_t koff = (uint32_t)crow * (uint32_t)(a.k.sl * 2), voff = (uint32_t)crow * (uint32_t)(a.v.sl * 2);
   const float c = sreg(a.scale_log2);
   const int shift = a.pt.shift, mask = (1 << shift) - 1;
   const int64_t own = own_rows(a), rows = all_rows(a);
@@ -108,9 +109,14 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
                              : len;
     const int tiles = (int)((span + DT - 1) / DT);
     // this sequence's tiles of the piece
-    const int s0 = end_to_end ? (int)(at - before) : (int)((int64_t)tiles * split / splits);
-    const int s1 = end_to_end ? (int)(end - before < tiles ? end - before : tiles)
-                              : (int)((int64_t)tiles * (split + 1) / splits);
+    int s0 = 0, s1 = tiles;
+    if (end_to_end) {
+      s0 = (int)(at - before);
+      s1 = (int)(end - before < tiles ? end - before : tiles);
+    } else if (splits > 1) {
+      s0 = (int)((int64_t)tiles * split / splits);
+      s1 = (int)((int64_t)tiles * (split + 1) / splits);
+    }
 
     // query row x of the workgroup: its sequence and head
     auto seq_of = [&](int x) { return KIND == PREFIX ? (int)((r0 + x) / group) : b; };
@@ -143,7 +149,7 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
       h1.keys = __builtin_amdgcn_readlane(list.keys, i + 32);
       ++listed;
     };
-    auto issue = [&](const PageRows& src, int t, uint32_t to) {
+    auto issue = [&](const PageRows& src, uint32_t off, int t, uint32_t to) {
       const unsigned char* base = reinterpret_cast<const unsigned char*>(src.p + kv * src.sh);
       const int64_t sl = src.sl * 2, sp = src.sp * 2;
       const int in = (int)(((int64_t)t * DT) & mask), in1 = (in + HT) & mask;
@@ -151,18 +157,20 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
       const unsigned char* p0 = base + h0.page * sp + in * sl;
       const unsigned char* p1 = base + h1.page * sp + in1 * sl;
       // a half without keys copies the other's last one (a tile without any: anything, it is not used)
-      const unsigned char* b0 = (const unsigned char*)(uintptr_t)scalar64((int64_t)(uintptr_t)(n0 > 0 || n1 == 0 ? p0 : p1));
-      const unsigned char* b1 = (const unsigned char*)(uintptr_t)scalar64((int64_t)(uintptr_t)(n1 > 0 || n0 == 0 ? p1 : p0));
-      const int last0 = (n0 > 0 ? n0 : (n1 > 0 ? n1 : 1)) - 1, last1 = (n1 > 0 ? n1 : (n0 > 0 ? n0 : 1)) - 1;
+      // (scalar: the compiler does not see that an address is the same in every lane)
+      auto scalar = [](const unsigned char* p) { return (const unsigned char*)(uintptr_t)scalar64((int64_t)(uintptr_t)p); };
+      const unsigned char* b0 = scalar(n0 > 0 || n1 == 0 ? p0 : p1);
+      const unsigned char* b1 = scalar(n1 > 0 || n0 == 0 ? p1 : p0);
+      const uint32_t last0 = (uint32_t)((n0 > 0 ? n0 : (n1 > 0 ? n1 : 1)) - 1) * (uint32_t)sl;
+      const uint32_t last1 = (uint32_t)((n1 > 0 ? n1 : (n0 > 0 ? n0 : 1)) - 1) * (uint32_t)sl;
 #pragma unroll
-      for (int i = 0; i < NCOPY; ++i) {
-        const int x = crow + 4 * (i & 3), last = i < 4 ? last0 : last1;
-        const int r = x < last ? x : last;
-        dma16_guarded(i < 4 ? b0 : b1, (uint32_t)r * (uint32_t)sl + (ccol ^ ((i & 3) << 4)), to + 1024 * i);
+      for (int i = 0; i < NCOPY; ++i) {  // (rows past the last key copy it)
+        const uint32_t row = min(off + 4 * (i & 3) * (uint32_t)sl, i < 4 ? last0 : last1);
+        dma16_guarded(i < 4 ? b0 : b1, row + (ccol ^ ((i & 3) << 4)), to + 1024 * i);
       }
     };
-    auto issue_k = [&](int t) { issue(a.k, t, (uint32_t)ring); };
-    auto issue_v = [&](int t) { issue(a.v, t, (uint32_t)ring + DT_B); };
+    auto issue_k = [&](int t) { issue(a.k, koff, t, (uint32_t)ring); };
+    auto issue_v = [&](int t) { issue(a.v, voff, t, (uint32_t)ring + DT_B); };
     static_assert(NCOPY == 8, "the counts below are a tile's copies");
 
     floatx16 o[4];
@@ -309,7 +317,7 @@ __device__ __forceinline__ void prefix_tiles(const PagedAttnArgs& a, uint32_t id
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int hl = lane >> 5, l32 = lane & 31;
-  const int group = a.Hq / a.Hk;
+  const int group = a.group;
   const int64_t rows_all = (int64_t)a.B * group;
   const uint32_t blocks = (uint32_t)((rows_all + PK_BLOCK - 1) / PK_BLOCK);
   const int kv = id % (uint32_t)a.Hk;
@@ -364,18 +372,11 @@ __device__ __forceinline__ void prefix_tiles(const PagedAttnArgs& a, uint32_t id
     const int64_t sl = src.sl * 2;
     const int in = (pos < len ? pos : end) & mask, more = len - 1 - pos;  // tokens behind the share's first one
     const unsigned char* b = reinterpret_cast<const unsigned char*>(src.p + kv * src.sh) + page * (src.sp * 2) + in * sl;
+    const uint32_t last = (uint32_t)(more < HT - 1 ? (more > 0 ? more : 0) : HT - 1) * (uint32_t)sl;
     const int col = opaque(ccol);
-    if (more >= HT - 1) {
 #pragma unroll
-      for (int i = 0; i < PK_NDMA; ++i) dma16_guarded(b + 4 * i * sl, off + (col ^ (i << 4)), to + 1024 * i);
-    } else {
-      const int last = more > 0 ? more : 0, row = opaque(crow);
-#pragma unroll
-      for (int i = 0; i < PK_NDMA; ++i) {
-        const int x = row + 4 * i, r = x < last ? x : last;
-        dma16_guarded(b, (uint32_t)r * (uint32_t)sl + (col ^ (i << 4)), to + 1024 * i);
-      }
-    }
+    for (int i = 0; i < PK_NDMA; ++i)
+      dma16_guarded(b, min(off + 4 * i * (uint32_t)sl, last) + (col ^ (i << 4)), to + 1024 * i);
   };
   // K of tile u + 1 goes ahead of V of tile u: the page of the share before is kept
   int ahead = T > 0 ? page_of(0) : 0, now = 0, prev = 0;
@@ -540,7 +541,7 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
   static LdsAllowed allowed;
   const hipError_t attr = allow_lds((const void*)paged_both_kernel<TILES, KIND>, bytes, allowed);
   if (attr != hipSuccess) return attr;
-  const int64_t p_units = a.p_splits * (((int64_t)a.B * (a.Hq / a.Hk) + a.p_block - 1) / a.p_block);
+  const int64_t p_units = a.p_splits * (((int64_t)a.B * a.group + a.p_block - 1) / a.p_block);
   hipLaunchKernelGGL((paged_both_kernel<TILES, KIND>), dim3((uint32_t)((p_units + units) * a.Hk)), dim3(4 * 64), bytes,
                      stream, a, (uint32_t)p_units, (uint32_t)(p_units + units));
   return hipGetLastError();
@@ -592,7 +593,7 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
 }
 
 hipError_t launch_paged(const PagedAttnArgs& a, hipStream_t stream) {
-  const int group = a.Hq / a.Hk, blocks = (group + HEADS - 1) / HEADS;
+  const int blocks = (a.group + HEADS - 1) / HEADS;
   const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B * a.splits) * blocks;
   hipError_t e;
   if (a.p_splits > 0) {
