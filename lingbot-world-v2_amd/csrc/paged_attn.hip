@@ -471,8 +471,8 @@ __global__ void __launch_bounds__(JW * 64) paged_join_kernel(const PagedAttnArgs
   };
   const float* st = a.part + a.Hq * rows * D;
   float x = 0.0f, y = 0.0f, L = 0.0f, M = -INFINITY;
-  constexpr int N = 64 / JW;
-  for (int i0 = N * wave; i0 < n_all; i0 += 64) {  // N parts at a time, their weights one per lane
+  constexpr int N = 8;
+  for (int i0 = N * wave; i0 < n_all; i0 += N * JW) {  // N parts at a time, their weights one per lane
     const int n = min(N, n_all - i0);
     float2 v[N];
 #pragma unroll
