@@ -549,9 +549,13 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 
 }  // namespace
 
-// How the keys are cut: own ones as the single-token attention over whole caches cuts them (whole sequences where they
-// give work enough, else the batch's keys in equal pieces), selected and the prefix's in equal pieces, of 6 tiles or
-// more, for as many workgroups as run at once.
+// How the keys are cut. Own ones: whole sequences where they keep the chip busy or are short, else the batch's keys in
+// equal pieces, a workgroup a CU (two: 1 to 5 % slower); the longer for that the more sequences x key/value heads there
+// are. Whole / in pieces, x 40/8 heads, lengths from a third of the longest up to it: one sequence of 1100 keys 11.9 /
+// 13.8 us, of 1600 15.2 / 13.7; four of 1600 15.3 / 15.6, of 2400 20.2 / 17.6; eight of 2400 20.6 / 21.5, of 4000 30.4 /
+// 26.1; 16 of 4000 34.3 / 37.9, of 8000 86.6 / 63.1; 32 of 4000 64.9 / 69.1, of 8000 123 / 119; 48 of 2400 65.1 / 62.3, of 8000
+// 225 / 190; 64 of 2400 83.1 / 86.6, of 4000 131 / 133, of 8000 249 / 239; 128 of 2400 154 / 159, of 4000 246 / 242.
+// Selected pages and the prefix's: equal pieces of 6 tiles or more for as many workgroups as run at once.
 // Prefix, 32 / 128 query rows at a time: 14040 keys, 1500 own x 40/8 heads, 8 sequences (40 rows) 30.9 / 35.6 us, 20 (100)
 // 42.5 / 46.5, 40 (200) 65.6 / 54.4; 46800, 1000 own x 12/4, 24 rows 34.5 / 36.6, 60 rows 44.0 / 43.0, 78 rows 49.3 / 51.8,
 // 99 rows 58.5 / 54.8; 4680, 100 own x 12/12, 33 rows 27.5 / 24.4, 64 rows 31.9 / 30.1. Own keys whole / in pieces with
@@ -587,8 +591,11 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
     if (!whole) a->splits = cut((keys + DT - 1) / DT, a->B * units);
   } else if (a->p_max > 0 && num_splits == 0) {
     if (!whole) a->pieces = cut(a->B * ((cap + DT - 1) / DT), units);
-  } else {
-    a->pieces = decode_pieces(a->B, a->Hq, a->Hk, cap, num_splits, cus);
+  } else if (num_splits > 1) {
+    a->pieces = (int)std::min<int64_t>((int64_t)num_splits * a->B, 1 << 20);
+  } else if (num_splits == 0 && cap > (a->B * units <= cus ? 1024 + 20 * a->B * units : 3500)) {
+    places = cus;
+    a->pieces = cut(a->B * ((cap + DT - 1) / DT), units);
   }
 }
 
