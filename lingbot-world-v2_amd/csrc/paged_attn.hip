@@ -555,7 +555,9 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 // 13.8 us, of 1600 15.2 / 13.7; four of 1600 15.3 / 15.6, of 2400 20.2 / 17.6; eight of 2400 20.6 / 21.5, of 4000 30.4 /
 // 26.1; 16 of 4000 34.3 / 37.9, of 8000 86.6 / 63.1; 32 of 4000 64.9 / 69.1, of 8000 123 / 119; 48 of 2400 65.1 / 62.3, of 8000
 // 225 / 190; 64 of 2400 83.1 / 86.6, of 4000 131 / 133, of 8000 249 / 239; 128 of 2400 154 / 159, of 4000 246 / 242.
-// Selected pages and the prefix's: equal pieces of 6 tiles or more for as many workgroups as run at once.
+// Selected pages, by the same rule: equal pieces of 6 tiles or more for as many workgroups as run at once, as the
+// prefix's. 2560 keys for 32 sequences x 40/8 heads, whole / in pieces 48.5 / 52.6 us, 1536 for 8 x 12/12 16.7 / 19.2; 1600
+// for 2 x 40/8 15.7 / 10.6, 6400 for 4 x 40/8 45.1 / 23.7.
 // Prefix, 32 / 128 query rows at a time: 14040 keys, 1500 own x 40/8 heads, 8 sequences (40 rows) 30.9 / 35.6 us, 20 (100)
 // 42.5 / 46.5, 40 (200) 65.6 / 54.4; 46800, 1000 own x 12/4, 24 rows 34.5 / 36.6, 60 rows 44.0 / 43.0, 78 rows 49.3 / 51.8,
 // 99 rows 58.5 / 54.8; 4680, 100 own x 12/12, 33 rows 27.5 / 24.4, 64 rows 31.9 / 30.1. Own keys whole / in pieces with
@@ -571,10 +573,11 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
   };
   if (a->B == 0) return;
   const int64_t cap = (int64_t)a->pt.width << a->pt.shift;
-  // own keys: whole sequences of 1024 keys and fewer, which are not worth a second launch; with a prefix, whose results
-  // are joined anyway, in pieces whatever the batch
+  // (with a prefix, whose results are joined anyway, pieces cost less)
   const int64_t keys = a->sel != nullptr ? (int64_t)a->n_sel << a->pt.shift : cap;
-  const bool whole = num_splits == 1 || (num_splits == 0 && keys <= 1024);
+  const int64_t seqs = a->B * units;
+  const int64_t limit = a->p_max > 0 ? 1024 : seqs <= cus ? 1024 + 20 * seqs : 3500;
+  const bool whole = num_splits == 1 || (num_splits == 0 && keys <= limit);
   if (a->p_max > 0) {
     const int64_t rows = a->B * group;
     a->p_block = rows > 3 * HEADS ? PK_BLOCK : HEADS;
@@ -593,7 +596,7 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
     if (!whole) a->pieces = cut(a->B * ((cap + DT - 1) / DT), units);
   } else if (num_splits > 1) {
     a->pieces = (int)std::min<int64_t>((int64_t)num_splits * a->B, 1 << 20);
-  } else if (num_splits == 0 && cap > (a->B * units <= cus ? 1024 + 20 * a->B * units : 3500)) {
+  } else if (!whole) {
     places = cus;
     a->pieces = cut(a->B * ((cap + DT - 1) / DT), units);
   }
