@@ -49,7 +49,7 @@ struct AppendArgs {
   uint16_t* bounds;           // [pages][Hk][2][D] smallest and largest values, or null
   float q_scale, k_scale;
   int parts;                  // waves that share one token's heads
-  int run_block;              // tokens whose pages a workgroup of the bounds kernel looks after
+  int page_wgs, page_block;   // workgroups that look after pages' new keys, and the tokens of each
 };
 hipError_t launch_append(const AppendArgs& a, int D, hipStream_t stream);
 

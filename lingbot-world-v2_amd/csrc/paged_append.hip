@@ -6,8 +6,9 @@
 //   bounds[page] = (min, max) over the page's rows so far, of the rounded values: exact, so their order is free.
 //
 // Bound by memory: every value is read once and written once. As in the per-head norm a wave keeps a token, its
-// angles in registers, and walks its heads. 4680 + 3600 + 1561 tokens x 40/8 heads of 128, normed, 54 us (5.2 TB/s; a
-// large copy reaches 4.9), their pages' bounds 8 us; one token 4.3 us, most of it the launch.
+// angles in registers, and walks its heads. Several tokens for one page: the keys are turned by the workgroup that
+// makes the page's bounds, beside the tokens' q and v. 4680 + 3600 + 1561 tokens x 40/8 heads of 128, normed, pages of 64,
+// 58 us (4.9 TB/s; a large copy reaches 4.9); one token 4.3 us, most of it the launch.
 
 #include "head_rows.h"
 #include "paged.h"
@@ -16,7 +17,13 @@ namespace lbw {
 namespace {
 
 constexpr int AP_WAVES = 4;
+constexpr int KEY_HEADS = 2;   // heads of a workgroup that looks after a page's keys
 constexpr int EDGE_WAVES = 8;  // of the bounds kernel
+// Pages up to this size get their keys and bounds in the kernel of the tokens' q and v, larger ones, whose tokens would
+// follow one another too long, their bounds by a second kernel. Two kernels / one, x 40/8 heads: 100 tokens in pages of
+// 64 11.7 / 9.2 us, 500 14.0 / 14.2, 4680 + 3600 + 1561 64.5 / 58.7; in pages of 128 11.2 / 9.2, 14.8 / 20.6, 66.9 / 68.3, of 256
+// 11.4 / 11.2, 15.6 / 35.9, 67.8 / 79.0.
+constexpr int FUSED_PAGE = 64;
 
 // Where a token goes: its sequence (-1: none), row and page (-1: nowhere).
 struct Place {
@@ -169,11 +176,120 @@ __device__ __forceinline__ void load_rotation(const AppendArgs& a, int t, int64_
   }
 }
 
+// The tokens of block `block` whose pages this workgroup looks after: those that are the first new ones of their page.
+// The page's new keys are turned and put there, heads KH chunk .., and its bounds made of them and, where the page was
+// begun before, the old ones: every page has one owner, no atomics. A wave takes 64 / LPH tokens at a time, a head
+// after the other, so that a token's angles are read once; the tokens' smallest and largest values meet by shuffles,
+// the waves' in LDS.
 template <int LPH, bool INTER>
+__device__ __forceinline__ void append_pages(const AppendArgs& a, int64_t block, int chunk, int lane, int wave) {
+  constexpr int TPW = 64 / LPH, D = 8 * LPH, KH = KEY_HEADS;
+  __shared__ u32x4 red[AP_WAVES][KH][2][LPH];  // (bf16: what was rounded once stays)
+  const int e0 = 8 * (lane % LPH), sub = lane / LPH, h0 = chunk * KH;
+  const int64_t t0 = block * a.page_block;
+  const int t1 = (int)(t0 + a.page_block < a.T ? t0 + a.page_block : a.T);
+  const int mask = (1 << a.pt.shift) - 1;
+  float wt[8];
+  load_weights(a.wk, a.w32, e0, wt);
+  for (int t = (int)t0; t < t1;) {
+    const Place w = place_of(a, t, lane);
+    if (w.b < 0) {
+      ++t;
+      continue;
+    }
+    const int in = (int)(w.row & mask);
+    const int n = w.end - t < mask + 1 - in ? w.end - t : mask + 1 - in;  // this page's tokens from t on
+    if (w.page < 0 || (in != 0 && t != w.start)) {  // nowhere, or not its first new token
+      t += n;
+      continue;
+    }
+    const int turns = (n + TPW - 1) / TPW;
+    for (int g = wave; g < turns; g += AP_WAVES) {
+      const int mine = g * TPW + sub, tok = mine < n ? mine : n - 1;  // (past the end: the last one once more)
+      u32x4 x[KH];
+      const uint16_t* const src = a.k.p + (int64_t)(t + tok) * a.k.sl + e0;
+#pragma unroll
+      for (int i = 0; i < KH; ++i) x[i] = load16(src + (h0 + i < a.Hk ? h0 + i : a.Hk - 1) * a.k.sh);
+      Turn rot;
+      load_rotation<INTER>(a, t + tok, w.row + tok, e0, lane, rot);
+      uint16_t* const dst = a.kp.p + w.page * a.kp.sp + (in + tok) * a.kp.sl + e0;
+#pragma unroll
+      for (int i = 0; i < KH; ++i) {
+        if (h0 + i >= a.Hk) break;
+        const u32x4 out = turn_chunk<LPH, INTER>(a, x[i], wt, a.k_scale, rot);
+        if (mine < n) *reinterpret_cast<u32x4*>(dst + (h0 + i) * a.kp.sh) = out;
+        float lo[8], hi[8], y[8];
+        unpack8(out, lo);
+        unpack8(out, hi);
+        u32x4 pl = out, ph = out;
+#pragma unroll
+        for (int o = LPH; o < 64; o <<= 1) {
+          u32x4 ql, qh;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ql[e] = __shfl_xor(pl[e], o);
+          qh = ql;
+          if (o > LPH) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qh[e] = __shfl_xor(ph[e], o);
+          }
+          unpack8(ql, y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], y[j]);
+          unpack8(qh, y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) hi[j] = max_nan(hi[j], y[j]);
+          pl = pack8(lo);
+          ph = pack8(hi);
+        }
+        if (lane < LPH) {
+          if (g != wave) {
+            unpack8(red[wave][i][0][lane], y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], y[j]);
+            unpack8(red[wave][i][1][lane], y);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) hi[j] = max_nan(hi[j], y[j]);
+          }
+          red[wave][i][0][lane] = pack8(lo);
+          red[wave][i][1][lane] = pack8(hi);
+        }
+      }
+    }
+    __syncthreads();
+    const int used = turns < AP_WAVES ? turns : AP_WAVES;
+    for (int x = threadIdx.x; x < KH * 2 * LPH; x += AP_WAVES * 64) {
+      const int c = x % LPH, edge = x / LPH % 2, i = x / (2 * LPH);
+      if (h0 + i >= a.Hk) break;
+      uint16_t* const p = a.bounds + (((int64_t)w.page * a.Hk + h0 + i) * 2 + edge) * D + 8 * c;
+      float m[8], y[8];
+      unpack8(in != 0 ? load16(p) : red[0][i][edge][c], m);
+      for (int v = 0; v < used; ++v) {
+        unpack8(red[v][i][edge][c], y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m[j] = edge == 0 ? min_nan(m[j], y[j]) : max_nan(m[j], y[j]);
+      }
+      *reinterpret_cast<u32x4*>(p) = pack8(m);
+    }
+    __syncthreads();  // the waves' results are read
+    t += n;
+  }
+}
+
+// PAGES: the first a.page_wgs workgroups look after the new keys of whole pages, the others after the tokens' q and v.
+template <int LPH, bool INTER, bool PAGES>
 __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs a) {
   constexpr int HPW = 64 / LPH, D = 8 * LPH;
-  const int lane = threadIdx.x & 63;
-  const int64_t id = (int64_t)blockIdx.x * AP_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t wg = blockIdx.x;
+  if constexpr (PAGES) {
+    if (wg < (uint32_t)a.page_wgs) {
+      const uint32_t chunks = (uint32_t)((a.Hk + KEY_HEADS - 1) / KEY_HEADS);
+      append_pages<LPH, INTER>(a, wg / chunks, wg % chunks, lane, wave);
+      return;
+    }
+    wg -= a.page_wgs;
+  }
+  const int64_t id = (int64_t)wg * AP_WAVES + wave;
   const int64_t tt = id / a.parts;
   if (tt >= a.T) return;
   const int t = (int)tt, part = (int)(id % a.parts);
@@ -192,21 +308,21 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs 
                         a.wq, a.q_scale, rot, nullptr, false);
   if (w.page < 0) return;
   const int64_t in = w.row & ((1 << a.pt.shift) - 1);
-  // one new token per sequence: its page's bounds are this wave's
-  uint16_t* const bounds =
-      a.bounds != nullptr && a.starts == nullptr ? a.bounds + (int64_t)w.page * a.Hk * 2 * D : nullptr;
-  turn_rows<LPH, INTER>(a, a.k.p + t * a.k.sl, a.k.sh, a.kp.p + w.page * a.kp.sp + in * a.kp.sl, a.kp.sh, a.Hk,
-                        first(cq), a.parts, e0, hsub, a.wk, a.k_scale, rot, bounds, in == 0);
+  if constexpr (!PAGES) {
+    // one new token per sequence: its page's bounds are this wave's
+    uint16_t* const bounds =
+        a.bounds != nullptr && a.starts == nullptr ? a.bounds + (int64_t)w.page * a.Hk * 2 * D : nullptr;
+    turn_rows<LPH, INTER>(a, a.k.p + t * a.k.sl, a.k.sh, a.kp.p + w.page * a.kp.sp + in * a.kp.sl, a.kp.sh, a.Hk,
+                          first(cq), a.parts, e0, hsub, a.wk, a.k_scale, rot, bounds, in == 0);
+  }
   copy_rows<LPH>(a.v.p + t * a.v.sl, a.v.sh, a.vp.p + w.page * a.vp.sp + in * a.vp.sl, a.vp.sh, a.Hk,
-                 first(cq + ck), a.parts, e0, hsub);
+                 first(PAGES ? cq : cq + ck), a.parts, e0, hsub);
 }
 
-// Bounds of the pages that several tokens were put into: blockIdx.x counts blocks of a.run_block tokens, blockIdx.y
+// Bounds of the pages that several tokens were put into: blockIdx.x counts blocks of a.page_block tokens, blockIdx.y
 // chunks of heads. The workgroup whose block holds a page's first new token reads the page's new keys back (from
 // cache: they were written just before), its waves in turn, and joins them with the old bounds where the page was
-// begun before: every page has one owner, no atomics. (One kernel, in which the workgroup that makes a page's bounds
-// turns its keys: 4680 + 3600 + 1561 tokens x 40/8 heads 69 to 90 us against 54 + 8, as a page's tokens follow one
-// another.)
+// begun before.
 template <int LPH>
 __global__ void __launch_bounds__(EDGE_WAVES * 64) append_bounds_kernel(const AppendArgs a) {
   constexpr int HPW = 64 / LPH, D = 8 * LPH, U = 8;
@@ -214,8 +330,8 @@ __global__ void __launch_bounds__(EDGE_WAVES * 64) append_bounds_kernel(const Ap
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int e0 = 8 * (lane % LPH), head = (int)blockIdx.y * HPW + lane / LPH;
   const int hh = head < a.Hk ? head : a.Hk - 1;  // (lanes past the last head do its work again and write nothing)
-  const int64_t t0 = (int64_t)blockIdx.x * a.run_block;
-  const int t1 = (int)(t0 + a.run_block < a.T ? t0 + a.run_block : a.T);
+  const int64_t t0 = (int64_t)blockIdx.x * a.page_block;
+  const int t1 = (int)(t0 + a.page_block < a.T ? t0 + a.page_block : a.T);
   const int mask = (1 << a.pt.shift) - 1;
   for (int t = (int)t0; t < t1;) {
     const Place w = place_of(a, t, lane);
@@ -275,22 +391,38 @@ __global__ void __launch_bounds__(EDGE_WAVES * 64) append_bounds_kernel(const Ap
   }
 }
 
+template <int LPH, bool PAGES>
+hipError_t launch(const AppendArgs& a, hipStream_t stream) {
+  const int64_t waves = (int64_t)a.T * a.parts;
+  const dim3 grid((uint32_t)(a.page_wgs + (waves + AP_WAVES - 1) / AP_WAVES)), block(AP_WAVES * 64);
+  if (a.inter) hipLaunchKernelGGL((append_kernel<LPH, true, PAGES>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((append_kernel<LPH, false, PAGES>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
 template <int LPH>
 hipError_t run(AppendArgs a, hipStream_t stream) {
   constexpr int HPW = 64 / LPH;
-  const int64_t waves = (int64_t)a.T * a.parts;
-  const dim3 grid((uint32_t)((waves + AP_WAVES - 1) / AP_WAVES)), block(AP_WAVES * 64);
-  if (a.inter) hipLaunchKernelGGL((append_kernel<LPH, true>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((append_kernel<LPH, false>), grid, block, 0, stream, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.bounds == nullptr || a.starts == nullptr) return e;
-  // as many tokens as a page has, so that a workgroup finds one page to look after, or fewer where sequences are
-  // shorter or workgroups few (a page takes its workgroup some microseconds, most of them waiting)
-  a.run_block = 1;
-  while (a.run_block < (1 << a.pt.shift) && (int64_t)2 * a.run_block * a.B <= a.T && a.T / a.run_block > 512)
-    a.run_block *= 2;
-  const dim3 runs((a.T + a.run_block - 1) / a.run_block, (a.Hk + HPW - 1) / HPW);
-  hipLaunchKernelGGL(append_bounds_kernel<LPH>, runs, dim3(EDGE_WAVES * 64), 0, stream, a);
+  a.page_wgs = 0;
+  if (a.bounds == nullptr || a.starts == nullptr) return launch<LPH, false>(a, stream);
+  const int page = 1 << a.pt.shift;
+  // tokens that a workgroup looks for pages in: as many as a page has, so that it finds one, or fewer where sequences
+  // are shorter or workgroups few
+  auto block_for = [&](int wgs) {
+    int n = 1;
+    while (n < page && (int64_t)2 * n * a.B <= a.T && a.T / n > wgs) n *= 2;
+    return n;
+  };
+  if (page <= FUSED_PAGE) {
+    a.page_block = block_for(256);
+    a.page_wgs = (a.T + a.page_block - 1) / a.page_block * ((a.Hk + KEY_HEADS - 1) / KEY_HEADS);
+    return launch<LPH, true>(a, stream);
+  }
+  const hipError_t e = launch<LPH, false>(a, stream);
+  if (e != hipSuccess) return e;
+  a.page_block = block_for(512);
+  const dim3 blocks((a.T + a.page_block - 1) / a.page_block, (a.Hk + HPW - 1) / HPW);
+  hipLaunchKernelGGL(append_bounds_kernel<LPH>, blocks, dim3(EDGE_WAVES * 64), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -298,10 +430,12 @@ hipError_t run(AppendArgs a, hipStream_t stream) {
 
 hipError_t launch_append(const AppendArgs& args, int D, hipStream_t stream) {
   AppendArgs a = args;
-  // a token's heads are shared by several waves while the tokens alone do not fill the chip
+  // a token's heads are shared by several waves while the tokens alone do not fill the chip (each of them reads the
+  // token's place and angles: up to 16384 waves / up to 4096, 2000 tokens x 40/8 heads 36.2 / 24.1 us, 3000 31.8 / 23.0, 5000
+  // x 12/12 27.8 / 21.2, 16000 83 / 70; fewer tokens and more the same)
   const int nch = (a.Hq + 2 * a.Hk + 512 / D - 1) / (512 / D);
   a.parts = 1;
-  while (a.parts < nch && (int64_t)a.T * a.parts < 16384) a.parts *= 2;
+  while (a.parts < nch && (int64_t)a.T * a.parts < 4096) a.parts *= 2;
   switch (D) {
     case 32: return run<4>(a, stream);
     case 64: return run<8>(a, stream);
