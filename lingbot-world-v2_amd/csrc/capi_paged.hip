@@ -145,8 +145,8 @@ int lbw_paged_append(const lbw_paged_append_params* p, void* stream) {
   if (p->batch > 0 && p->lens == nullptr) return fail(LBW_ERR_INVALID, "lens missing");
   if (p->cache.bounds != nullptr && !aligned16(p->cache.bounds))
     return fail(LBW_ERR_INVALID, "bounds must be a 16-byte aligned device pointer");
-  // (a workgroup of 512 for one token and 2 heads, at most)
-  if (p->cache.bounds != nullptr && p->tokens * (int64_t)p->k_heads > kMaxWorkgroups)
+  // (a workgroup of 256 for one token and 2 heads beside those of the tokens, or one of 512 for 2 to 16 heads, at most)
+  if (p->cache.bounds != nullptr && p->tokens * (int64_t)p->k_heads > kMaxWorkgroups / 2)
     return fail(LBW_ERR_UNSUPPORTED, "tokens %d x %d heads", p->tokens, p->k_heads);
   a.B = p->batch;
   a.norm = p->norm != 0;

@@ -558,47 +558,63 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 // Selected pages, by the same rule: equal pieces of 6 tiles or more for as many workgroups as run at once, as the
 // prefix's. 2560 keys for 32 sequences x 40/8 heads, whole / in pieces 48.5 / 52.6 us, 1536 for 8 x 12/12 16.7 / 19.2; 1600
 // for 2 x 40/8 15.7 / 10.6, 6400 for 4 x 40/8 45.1 / 23.7.
-// Prefix, 32 / 128 query rows at a time: 14040 keys, 1500 own x 40/8 heads, 8 sequences (40 rows) 30.9 / 35.6 us, 20 (100)
-// 42.5 / 46.5, 40 (200) 65.6 / 54.4; 46800, 1000 own x 12/4, 24 rows 34.5 / 36.6, 60 rows 44.0 / 43.0, 78 rows 49.3 / 51.8,
-// 99 rows 58.5 / 54.8; 4680, 100 own x 12/12, 33 rows 27.5 / 24.4, 64 rows 31.9 / 30.1. Own keys whole / in pieces with
-// it: 16 of up to 1560 off 14040 x 12/12 42 / 38, 64 of up to 3600 off 46800 x 40/8 197 / 186.
+// With a prefix, places shared out by tiles: 4 of up to 1600 off 14040 keys x 40/8 heads, 20 pieces of the prefix and 12
+// of own keys 22.2 us, 32 and 32 25.8; 8 of 3600 off 6000 x 12/4, 9 and 55 21.2, 64 and 64 28.2; 64 of 3600 off 46800 x 40/8
+// (128 rows at a time), 10 and 34 163, 21 and 64 185, 5 and 17 205; 26 of 1500 off 14040 x 40/8 16 and 32 40.4, 8 and 16 45.8;
+// 30 of 1500 off 10000 x 16/2, 32 and 64 23.5, 64 and 128 27.6. Whole sequences: 16 of 200 off 6000 x 12/4, 24 pieces (one
+// workgroup a CU) 14.4, 48 16.6; off 46800 20 35.9, 48 39.6; 16 of 200 off 14040 x 40/8 (128 sequences x heads), 4 pieces 47.1,
+// 16 (two a CU) 26.6. Pieces of 4 tiles or more, of 6: 4 of 40 off 1560 x 12/4 12.3 / 13.3, one of 3000 x 40/8 11.7 / 13.0.
+// 32 / 128 query rows at a time: 8 of 1500 off 14040 x 40/8 (40 rows) 30.9 / 35.6, 20 (100) 42.5 / 46.5, 40 (200) 65.6 /
+// 54.4; 46800, 1000 own x 12/4, 24 rows 34.5 / 36.6, 60 rows 44.0 / 43.0, 78 rows 49.3 / 51.8, 99 rows 58.5 / 54.8.
 void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
-  const int64_t group = a->Hq / a->Hk, units = a->Hk * ((group + HEADS - 1) / HEADS);
+  const int64_t group = a->Hq / a->Hk, units = a->Hk * ((group + HEADS - 1) / HEADS), seqs = a->B * units;
   a->splits = 1;
   a->pieces = a->p_splits = 0;
-  int64_t places = 2 * cus;  // workgroups that run at once
-  auto cut = [&](int64_t tiles, int64_t busy) {
-    if (num_splits > 0) return (int)num_splits;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(places / busy, tiles / 6));
-  };
   if (a->B == 0) return;
+  // pieces of `tiles` tiles for `places` workgroups, `each` of them a piece, of `least` tiles or more
+  auto cut = [&](int64_t tiles, int64_t places, int64_t each, int64_t least) {
+    return (int)std::max<int64_t>(1, std::min<int64_t>(places / each, tiles / least));
+  };
   const int64_t cap = (int64_t)a->pt.width << a->pt.shift;
-  // (with a prefix, whose results are joined anyway, pieces cost less)
   const int64_t keys = a->sel != nullptr ? (int64_t)a->n_sel << a->pt.shift : cap;
-  const int64_t seqs = a->B * units;
+  const int64_t own_tiles = (keys + DT - 1) / DT;  // of a sequence
+  // (with a prefix, whose results are joined anyway, pieces cost less)
   const int64_t limit = a->p_max > 0 ? 1024 : seqs <= cus ? 1024 + 20 * seqs : 3500;
   const bool whole = num_splits == 1 || (num_splits == 0 && keys <= limit);
+  int64_t own_places = a->sel != nullptr ? 2 * cus : cus;
   if (a->p_max > 0) {
-    const int64_t rows = a->B * group;
+    const int64_t rows = a->B * group, p_tiles = (a->p_max + DT - 1) / DT;
     a->p_block = rows > 3 * HEADS ? PK_BLOCK : HEADS;
-    // 32 rows at a time: the places that whole sequences leave, half of them at least (the other half for own keys in
-    // pieces); 128 rows: all, and own keys come on top, as such a workgroup alone on a CU waits most of the time
-    if (a->p_block == HEADS) places = std::max<int64_t>(cus, 2 * cus - (whole ? a->B * units : cus));
-    a->p_splits = cut((a->p_max + DT - 1) / DT, a->Hk * ((rows + a->p_block - 1) / a->p_block));
+    const int64_t each = a->Hk * ((rows + a->p_block - 1) / a->p_block);
+    const bool wide = a->p_block == PK_BLOCK;
+    // tiles of all workgroups; own ones are counted to the longest sequence's end, 0.7 of that beside 128 rows at a
+    // time, whose few pieces are the last to end (64 of 3600 off 46800, 40/8 heads: 163 us, 7 pieces at 1.0 215)
+    const int64_t of_prefix = p_tiles * each, of_own = own_tiles * seqs * (wide ? 7 : 10) / 10;
+    int64_t places;
+    if (whole) {
+      // a workgroup a CU, whole sequences included; two where those would leave the prefix less than 0.7 of the CUs
+      const int64_t one = std::max<int64_t>(0, cus - seqs) / each * each;
+      places = !wide && 10 * one >= 7 * cus ? one : std::max<int64_t>(2 * cus - seqs, wide ? 3 * cus / 2 : 0);
+    } else {
+      // a workgroup a CU, shared out by their tiles; two where each still gets 16 tiles (of 128 rows, which alone on
+      // a CU wait most of the time) or 32
+      const int64_t all = of_prefix + of_own >= (wide ? 32 : 64) * cus ? 2 * cus : cus;
+      places = all * of_prefix / (of_prefix + of_own) + (wide ? each / 2 : 0);
+      own_places = all - std::max<int64_t>(1, places / each) * each;
+    }
+    a->p_splits = cut(p_tiles, places, each, 4);
+    if (num_splits > 0) a->p_splits = num_splits;
     // (a piece's table entries fit their place: whole tiles of 64 keys, an entry more where a piece ends in a page)
     const int64_t tiles = (a->p_max + BN - 1) / BN, most = ((int64_t)(P_LIST - 1) << a->pt.shift) / BN;
     if (a->p_block == PK_BLOCK) a->p_splits = (int)std::max<int64_t>(a->p_splits, (tiles + most - 1) / most);
-    if (a->p_block == HEADS) places = cus;
   }
   if (a->sel != nullptr) {
-    if (!whole) a->splits = cut((keys + DT - 1) / DT, a->B * units);
-  } else if (a->p_max > 0 && num_splits == 0) {
-    if (!whole) a->pieces = cut(a->B * ((cap + DT - 1) / DT), units);
+    if (num_splits > 0) a->splits = num_splits;
+    else if (!whole) a->splits = cut(own_tiles, own_places, seqs, 4);
   } else if (num_splits > 1) {
     a->pieces = (int)std::min<int64_t>((int64_t)num_splits * a->B, 1 << 20);
   } else if (!whole) {
-    places = cus;
-    a->pieces = cut(a->B * ((cap + DT - 1) / DT), units);
+    a->pieces = cut(a->B * own_tiles, own_places, units, 4);
   }
 }
 
