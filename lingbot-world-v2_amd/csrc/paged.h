@@ -84,6 +84,14 @@ __host__ __device__ inline int64_t all_rows(const PagedAttnArgs& a) { return own
 __host__ __device__ inline bool has_parts(const PagedAttnArgs& a) {
   return a.pieces > 0 || a.splits > 1 || a.p_splits > 0;
 }
+// Workgroups per key/value head: of the prefix, and of own keys (32 query rows each).
+inline int64_t prefix_units(const PagedAttnArgs& a) {
+  return a.p_splits > 0 ? a.p_splits * (((int64_t)a.B * a.group + a.p_block - 1) / a.p_block) : 0;
+}
+inline int64_t own_units(const PagedAttnArgs& a) {
+  return (a.pieces > 0 ? (int64_t)a.pieces : (int64_t)a.B * a.splits) * ((a.group + 31) / 32);
+}
+inline int64_t workgroups(const PagedAttnArgs& a) { return (prefix_units(a) + own_units(a)) * a.Hk; }
 hipError_t launch_paged(const PagedAttnArgs& a, hipStream_t stream);
 void plan_paged(PagedAttnArgs* a, int num_splits, int cus);
 

@@ -9,7 +9,12 @@
 // tokens, each inside one page (pages are 16 tokens or more). The pages of a wave's next 32 tiles are looked
 // up at once, one half a lane, and handed to the scalar side a tile ahead.
 //
-// The prefix's keys are the same for the whole batch: its query rows are those of all sequences, 32 at a time.
+// The prefix's keys are the same for the whole batch: its query rows are those of all sequences, 32 at a time, or 128
+// where there are more (four waves over shared tiles of 64 keys), in one launch with the sequences' own keys.
+//
+// Measured, x 40/8 heads: eight sequences of up to 46800 keys 187 us, K and V at 5.6 TB/s (a kernel that only reads
+// reaches 5.7); 64 of up to 3600 behind a prefix of 46800 172 us, 16 of 200 (12/4 heads) behind 46800 37; one
+// sequence of 500 keys 8.8 us, 3 us of it the launch and 1.5 a tile of each wave.
 //
 // A half's rows past its last key copy that key (or the other half's), so the products never meet what lies
 // behind a sequence. A page outside the cache makes its keys' scores NaN.
@@ -30,7 +35,7 @@ static_assert(HT == HALF_KEYS, "half_at looks up half a tile");
 constexpr int DT_B = DT * PK_ROWB;          // 8 KB
 constexpr int RING_B = 2 * DT_B;            // per wave: K, V
 constexpr int NCOPY = DT_B / 1024;          // copies per lane for K or V of a tile
-constexpr int HEADS = 32;                   // query rows per workgroup
+constexpr int HEADS = 32;                   // query rows per workgroup (as own_units counts them)
 enum Kind { DENSE, SPARSE, PREFIX };
 constexpr int P_LIST = 4096;                // table entries of a piece of the prefix (tile form)
 constexpr int PREFIX_LDS = FWD_LDS + 4 * P_LIST;
@@ -541,7 +546,7 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
   static LdsAllowed allowed;
   const hipError_t attr = allow_lds((const void*)paged_both_kernel<TILES, KIND>, bytes, allowed);
   if (attr != hipSuccess) return attr;
-  const int64_t p_units = a.p_splits * (((int64_t)a.B * a.group + a.p_block - 1) / a.p_block);
+  const int64_t p_units = prefix_units(a);
   hipLaunchKernelGGL((paged_both_kernel<TILES, KIND>), dim3((uint32_t)((p_units + units) * a.Hk)), dim3(4 * 64), bytes,
                      stream, a, (uint32_t)p_units, (uint32_t)(p_units + units));
   return hipGetLastError();
@@ -619,8 +624,7 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
 }
 
 hipError_t launch_paged(const PagedAttnArgs& a, hipStream_t stream) {
-  const int blocks = (a.group + HEADS - 1) / HEADS;
-  const int64_t n = (int64_t)(a.pieces > 0 ? a.pieces : a.B * a.splits) * blocks;
+  const int64_t n = own_units(a);
   hipError_t e;
   if (a.p_splits > 0) {
     const bool tiles = a.p_block == PK_BLOCK;

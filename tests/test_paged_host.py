@@ -142,6 +142,19 @@ def test_select_refusals(kw, message):
     assert message in lib.lbw_last_error().decode()
 
 
+def test_prefixes_of_more_pieces_than_a_launch_has():
+    """A piece lists 4095 pages at most, so 2^27 pages of 16 tokens make 32801 pieces, here for 16000 query rows."""
+    from lbw_amd import _lib
+    lib = _lib.load()
+    long = {"prefix_table": ADDR, "prefix_width": 1 << 27, "prefix_keys": 0x7fffff00, "cache.page_size": 16,
+            "q_heads": 8, "k_heads": 8}
+    p = _attention(batch=16000, **long)
+    assert lib.lbw_attention_paged_workspace_size(ctypes.byref(p)) == 0
+    assert lib.lbw_attention_paged(ctypes.byref(p), None, 0, None) == 2
+    assert "prefix of 2147483392 keys in pages of 16" in lib.lbw_last_error().decode()
+    assert lib.lbw_attention_paged_workspace_size(ctypes.byref(_attention(batch=100, **long))) > 100 * 8 * 32800 * 520
+
+
 def test_null_params_and_empty_calls():
     from lbw_amd import _lib
     lib = _lib.load()
