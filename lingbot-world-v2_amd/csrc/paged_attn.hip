@@ -54,9 +54,16 @@ __device__ __forceinline__ int64_t prefix_keys(const PagedAttnArgs& a) {
 }
 // Entries of a list of selected pages: those before the first negative one.
 __device__ __forceinline__ int list_length(const int32_t* sel, int n, int lane) {
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const uint64_t stop = __ballot(i0 + lane < n && sel[i0 + lane] < 0);
-    if (stop != 0) return i0 + __ffsll((unsigned long long)stop) - 1;
+  constexpr int U = 4;  // (loads under way at once)
+  for (int i0 = 0; i0 < n; i0 += 64 * U) {
+    int32_t x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = i0 + 64 * u + lane < n ? sel[i0 + 64 * u + lane] : 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t stop = __ballot(x[u] < 0);
+      if (stop != 0) return i0 + 64 * u + __ffsll((unsigned long long)stop) - 1;
+    }
   }
   return n;
 }
@@ -105,6 +112,16 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
   const int64_t own = own_rows(a), rows = all_rows(a);
 
   do {
+    // query row x of the workgroup: its sequence and head
+    auto seq_of = [&](int x) { return KIND == PREFIX ? (int)((r0 + x) / group) : b; };
+    auto head_of = [&](int x) { return kv * group + (int)(KIND == PREFIX ? (r0 + x) % group : r0 + x); };
+    u32x4 qf[8];
+    {
+      const int x = l32 < nr ? l32 : nr - 1;
+      const uint16_t* p = a.q.p + seq_of(x) * a.q.sl + head_of(x) * a.q.sh + 8 * hl;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const u32x4*>(p + 16 * s);
+    }
     // the list of this sequence's pages: `count` entries of 2^shift tokens, `len` keys in all
     const int64_t len = KIND == PREFIX ? scalar64(prefix_keys(a)) : __builtin_amdgcn_readfirstlane(keys_of(a, b));
     const int32_t* const table = KIND == PREFIX ? a.p_table : a.pt.p + b * a.pt.sb;
@@ -123,16 +140,6 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
       s1 = (int)((int64_t)tiles * (split + 1) / splits);
     }
 
-    // query row x of the workgroup: its sequence and head
-    auto seq_of = [&](int x) { return KIND == PREFIX ? (int)((r0 + x) / group) : b; };
-    auto head_of = [&](int x) { return kv * group + (int)(KIND == PREFIX ? (r0 + x) % group : r0 + x); };
-    u32x4 qf[8];
-    {
-      const int x = l32 < nr ? l32 : nr - 1;
-      const uint16_t* p = a.q.p + seq_of(x) * a.q.sl + head_of(x) * a.q.sh + 8 * hl;
-#pragma unroll
-      for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const u32x4*>(p + 16 * s);
-    }
     // halves of tiles base, base + DW, ..: tile i's first half in lane i, its second in lane 32 + i
     auto look_up = [&](int base) {
       return half_at(sel, span, table, KIND == PREFIX ? a.p_width : a.pt.width, shift, a.pt.pages, len,
