@@ -114,10 +114,11 @@ int fill_select(const lbw_paged_select_params* p, SelectArgs* a) {
   a->bounds = static_cast<const uint16_t*>(p->cache.bounds);
   a->count = p->count; a->first = p->first; a->last = p->last;
   a->sel = p->selected;
+  plan_select(a, num_cus());
   return LBW_OK;
 }
 size_t select_bytes(const SelectArgs& a) {
-  return a.pt.width > a.count ? (size_t)a.B * a.Hk * a.pt.width * sizeof(uint64_t) : 0;
+  return a.pt.width > a.count && a.chunk > 0 ? (size_t)a.B * a.Hk * a.pt.width * sizeof(uint64_t) : 0;
 }
 
 }  // namespace

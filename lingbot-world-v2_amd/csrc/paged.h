@@ -101,10 +101,11 @@ struct SelectArgs {
   PageTable pt;
   const int32_t* lens;
   int B, Hq, Hk, count, first, last;
-  int chunk;                  // pages that a workgroup of the score kernel takes
+  int chunk;                  // pages that a workgroup of the score kernel takes; 0: one kernel does all
   uint64_t* score;            // [B][Hk][width] order-preserving images of the scores
   int32_t* sel;               // [B][Hk][count]
 };
+void plan_select(SelectArgs* a, int cus);
 hipError_t launch_select(const SelectArgs& a, hipStream_t stream);
 
 }  // namespace lbw

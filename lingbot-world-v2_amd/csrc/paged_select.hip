@@ -11,9 +11,10 @@
 // bytes per page and head against 16 KB and more of the page's keys; the choice by its rounds of counting.
 //
 // A wave scores four pages at a time: 16 lanes a page, 8 components each, with q's positive and negative parts in
-// registers. The second kernel has a workgroup per sequence and key/value head: it narrows the range of scores that
+// registers. A second kernel has a workgroup per sequence and key/value head: it narrows the range of scores that
 // holds the last chosen one, 1024 equal bins at a time, until no more than 256 are left (one round mostly), whose ranks
-// are counted one against another.
+// are counted one against another. Few pages: one kernel for both. Eight sequences of up to 1463 pages x 40/8 heads 16 +
+// 8 us (their bounds take 10 at the rate of a large copy, the 64-bit sums 9), one of 732 pages 4.5 + 6.3.
 
 #include "capi_util.h"
 #include "head_rows.h"
@@ -25,8 +26,8 @@ namespace {
 constexpr int SEL_D = 128;
 constexpr int SC_G = 5;           // query heads at a time, at most (64 registers of q each two)
 constexpr int TOP_T = 256;        // threads of the choice
-constexpr int TOP_U = 16;         // scores per thread in registers
-constexpr int TOP_W = TOP_T / 64;
+constexpr int ONE_T = 512;        // threads of the kernel that scores and chooses
+constexpr int ONE_PAGES = 256;    // scores that it keeps
 constexpr int BINS = 1024;
 constexpr uint64_t INF_IMAGE = 0xfff0000000000000ull;
 
@@ -59,17 +60,13 @@ __device__ __forceinline__ int pages_of(const SelectArgs& a, int b) {
   return __builtin_amdgcn_readfirstlane((int)((n + (1 << a.pt.shift) - 1) >> a.pt.shift));
 }
 
-template <int G>
-__global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t chunks = (uint32_t)((a.pt.width + a.chunk - 1) / a.chunk);
-  const int chunk = blockIdx.x % chunks, kv = (blockIdx.x / chunks) % (uint32_t)a.Hk,
-            b = blockIdx.x / chunks / (uint32_t)a.Hk;
+// Scores of pages from .. end - 1 of a sequence and key/value head, four a wave at a time; `put(page, score, first)`:
+// the higher of it and what is there, unless it is the first.
+template <int G, typename Put>
+__device__ __forceinline__ void score_pages(const SelectArgs& a, int b, int kv, int from, int end, int lane, int wave,
+                                            int waves, Put put) {
   const int group = a.Hq / a.Hk, e0 = 8 * (lane & 15), sub = lane >> 4;
   const int32_t* const table = a.pt.p + b * a.pt.sb;
-  uint64_t* const score = a.score + ((int64_t)b * a.Hk + kv) * a.pt.width;
-  const int n = pages_of(a, b);
-  if (n <= a.count || chunk * a.chunk >= n) return;  // (all pages are chosen, or none is here)
   for (int h0 = 0; h0 < group; h0 += G) {
     double up[G][8], down[G][8];
 #pragma unroll
@@ -84,8 +81,7 @@ __global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
       }
     }
     // the next pages' bounds are fetched while these are summed
-    int page = chunk * a.chunk + 4 * wave + sub;
-    const int end = min(n, (chunk + 1) * a.chunk);
+    int page = from + 4 * wave + sub;
     u32x4 lw, hw;
     bool bad = false;
     auto fetch = [&](int i) {
@@ -98,12 +94,12 @@ __global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
       hw = load16(p + SEL_D);
     };
     fetch(page);
-    for (; __any(page < end); page += 16) {
+    for (; __any(page < end); page += 4 * waves) {
       float lo[8], hi[8];
       unpack8(lw, lo);
       unpack8(hw, hi);
       const bool is_bad = bad;
-      fetch(page + 16);
+      fetch(page + 4 * waves);
       double x[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) x[g] = 0.0;
@@ -121,47 +117,57 @@ __global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
         nan |= y != y;
         most = fmax(most, y);
       }
-      uint64_t best = nan ? INF_IMAGE : image(most);
-      if (page < end && (lane & 15) == 0) {
-        if (h0 > 0 && score[page] > best) best = score[page];
-        score[page] = best;
-      }
+      const uint64_t best = nan ? INF_IMAGE : image(most);
+      if (page < end && (lane & 15) == 0) put(page, best, h0 == 0);
     }
   }
 }
 
-__global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
+template <int G>
+__global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t chunks = (uint32_t)((a.pt.width + a.chunk - 1) / a.chunk), unit = blockIdx.x / (uint32_t)a.Hk;
+  // (another chunk first in each sequence: the last ones, of few pages or none, would often meet on one XCD; 64 sequences
+  // of up to 98 pages x 40/8 heads 22.4 to 18.5 us, 16 of 1463 x 64/8 48.1 to 43.8)
+  const int kv = blockIdx.x % (uint32_t)a.Hk, b = unit / chunks, chunk = (unit % chunks + (uint32_t)b) % chunks;
+  uint64_t* const score = a.score + ((int64_t)b * a.Hk + kv) * a.pt.width;
+  const int n = pages_of(a, b);
+  if (n <= a.count || chunk * a.chunk >= n) return;  // (all pages are chosen, or none is here)
+  score_pages<G>(a, b, kv, chunk * a.chunk, min(n, (chunk + 1) * a.chunk), lane, wave, 4,
+                 [&](int page, uint64_t best, bool first) {
+                   if (!first && score[page] > best) best = score[page];
+                   score[page] = best;
+                 });
+}
+
+// The choice among n > count pages by their scores, by T threads.
+template <int T>
+__device__ __forceinline__ void choose(const SelectArgs& a, int n, const uint64_t* score, int32_t* sel) {
+  constexpr int TOP_W = T / 64;
+  constexpr int TOP_U = 64 / TOP_W;  // scores per thread in registers
   __shared__ uint32_t hist[BINS], sums[TOP_W], counts[TOP_U * TOP_W][2];
-  __shared__ uint64_t range[TOP_W][2], cand[TOP_T], border;
-  __shared__ int32_t place[TOP_T];
+  __shared__ uint64_t range[TOP_W][2], cand[T], border;
+  __shared__ int32_t place[T];
   __shared__ uint32_t found[3], collected;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kv = blockIdx.x % (uint32_t)a.Hk, b = blockIdx.x / (uint32_t)a.Hk;
-  const int n = pages_of(a, b);
-  int32_t* const sel = a.sel + ((int64_t)b * a.Hk + kv) * a.count;
-  if (n <= a.count) {
-    for (int i = tid; i < a.count; i += TOP_T) sel[i] = i < n ? i : -1;
-    return;
-  }
-  const uint64_t* const score = a.score + ((int64_t)b * a.Hk + kv) * a.pt.width;
   auto kept = [&](int i) { return i < a.first || i >= n - a.last; };
   // 0 for a page that is kept anyway, or is none
   auto score_of = [&](int i) { return i < n && !kept(i) ? score[i] : 0; };
-  // page j * TOP_T + tid in mine[j]; those past TOP_U * TOP_T are read anew each time
+  // page j * T + tid in mine[j]; those past TOP_U * T are read anew each time
   uint64_t mine[TOP_U];
 #pragma unroll
-  for (int j = 0; j < TOP_U; ++j) mine[j] = j * TOP_T < n ? score_of(j * TOP_T + tid) : 0;
+  for (int j = 0; j < TOP_U; ++j) mine[j] = j * T < n ? score_of(j * T + tid) : 0;
   auto each = [&](auto f) {
 #pragma unroll
     for (int j = 0; j < TOP_U; ++j) {
-      if (j * TOP_T >= n) break;
-      f(mine[j], j * TOP_T + tid);
+      if (j * T >= n) break;
+      f(mine[j], j * T + tid);
     }
-    for (int i = TOP_U * TOP_T + tid; i < n; i += TOP_T) f(score_of(i), i);
+    for (int i = TOP_U * T + tid; i < n; i += T) f(score_of(i), i);
   };
   auto clear = [&] {
 #pragma unroll
-    for (int i = 0; i < BINS / TOP_T; ++i) hist[i * TOP_T + tid] = 0;
+    for (int i = 0; i < BINS / T; ++i) hist[i * T + tid] = 0;
   };
   uint32_t need = (uint32_t)(a.count - a.first - a.last);  // (n > count: first and last do not meet)
   uint64_t over = ~0ull;  // chosen: scores above this, and the first `need` of those that equal it
@@ -203,7 +209,7 @@ __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
       });
       __syncthreads();
       // four bins a thread, from the top: how many scores are in them and in those above
-      constexpr int BPT = BINS / TOP_T;
+      constexpr int BPT = BINS / T;
       uint32_t own[BPT], sum = 0;
 #pragma unroll
       for (int i = 0; i < BPT; ++i) sum += own[i] = hist[BINS - 1 - (tid * BPT + i)];
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
         need = 0;
         break;
       }
-      if (in_bin <= TOP_T) {
+      if (in_bin <= T) {
         each([&](uint64_t u, int i) {
           if (u >= lo && u <= hi) {
             const uint32_t at = atomicAdd(&collected, 1u);
@@ -272,15 +278,15 @@ __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
   // in ascending order: kept pages and scores above, of equal ones the first `need`
   const uint64_t before = ((uint64_t)1 << lane) - 1;
   uint32_t above0 = 0, equal0 = 0;
-  for (int base = 0; base < n; base += TOP_U * TOP_T) {
+  for (int base = 0; base < n; base += TOP_U * T) {
     // a page's: bit 16 above, bit 17 equal, and how many above (bits 0 ..) and equal ones (bits 8 ..) the wave's lower
     // lanes hold
     uint32_t turn[TOP_U];
 #pragma unroll
     for (int j = 0; j < TOP_U; ++j) {
       turn[j] = 0;
-      if (base + j * TOP_T >= n) continue;
-      const int i = base + j * TOP_T + tid;
+      if (base + j * T >= n) continue;
+      const int i = base + j * T + tid;
       const uint64_t u = base == 0 ? mine[j] : score_of(i);
       const bool above = (i < n && kept(i)) || u > over, equal = u == over;
       const uint64_t ma = __ballot(above), me = __ballot(equal);
@@ -294,7 +300,7 @@ __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
     __syncthreads();
     // lane x: how many are in the first x + 1 of the waves' turns
     static_assert(TOP_U * TOP_W == 64, "a lane for each turn of each wave");
-    const bool there = base + (lane / TOP_W) * TOP_T < n;
+    const bool there = base + (lane / TOP_W) * T < n;
     const uint32_t na = there ? counts[lane][0] : 0, ne = there ? counts[lane][1] : 0;
     uint32_t sa = na, se = ne;
 #pragma unroll
@@ -307,12 +313,12 @@ __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < TOP_U; ++j) {
-      if (base + j * TOP_T >= n) continue;
+      if (base + j * T >= n) continue;
       const int x = j * TOP_W + wave;
       const uint32_t pa = above0 + __builtin_amdgcn_readlane(sa - na, x) + (turn[j] & 255);
       const uint32_t pe = equal0 + __builtin_amdgcn_readlane(se - ne, x) + (turn[j] >> 8 & 255);
       if ((turn[j] >> 16 & 1) || ((turn[j] >> 17) && pe < need))
-        sel[pa + (pe < need ? pe : need)] = base + j * TOP_T + tid;
+        sel[pa + (pe < need ? pe : need)] = base + j * T + tid;
     }
     above0 += __shfl(sa, 63);
     equal0 += __shfl(se, 63);
@@ -320,20 +326,65 @@ __global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
   }
 }
 
+// All of a sequence's pages, where there are no more than `count`.
+template <int T>
+__device__ __forceinline__ bool chose_all(const SelectArgs& a, int n, int32_t* sel) {
+  if (n > a.count) return false;
+  for (int i = threadIdx.x; i < a.count; i += T) sel[i] = i < n ? i : -1;
+  return true;
+}
+
+__global__ void __launch_bounds__(TOP_T) select_top_kernel(const SelectArgs a) {
+  const int kv = blockIdx.x % (uint32_t)a.Hk, b = blockIdx.x / (uint32_t)a.Hk;
+  const int n = pages_of(a, b);
+  int32_t* const sel = a.sel + ((int64_t)b * a.Hk + kv) * a.count;
+  if (!chose_all<TOP_T>(a, n, sel)) choose<TOP_T>(a, n, a.score + ((int64_t)b * a.Hk + kv) * a.pt.width, sel);
+}
+
+// Both for a sequence and key/value head of few pages, whose scores stay in LDS.
+template <int G>
+__global__ void __launch_bounds__(ONE_T) select_one_kernel(const SelectArgs a) {
+  __shared__ uint64_t score[ONE_PAGES];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kv = blockIdx.x % (uint32_t)a.Hk, b = blockIdx.x / (uint32_t)a.Hk;
+  const int n = pages_of(a, b);
+  int32_t* const sel = a.sel + ((int64_t)b * a.Hk + kv) * a.count;
+  if (chose_all<ONE_T>(a, n, sel)) return;
+  score_pages<G>(a, b, kv, 0, n, lane, wave, ONE_T / 64, [&](int page, uint64_t best, bool first) {
+    score[page] = first || best > score[page] ? best : score[page];
+  });
+  __syncthreads();
+  choose<ONE_T>(a, n, score, sel);
+}
+
 template <int G>
 void score(const SelectArgs& a, hipStream_t stream) {
+  if (a.chunk == 0) {
+    hipLaunchKernelGGL(select_one_kernel<G>, dim3((uint32_t)((int64_t)a.B * a.Hk)), dim3(ONE_T), 0, stream, a);
+    return;
+  }
   const int64_t chunks = (a.pt.width + a.chunk - 1) / a.chunk;
   hipLaunchKernelGGL(select_score_kernel<G>, dim3((uint32_t)(chunks * a.Hk * a.B)), dim3(256), 0, stream, a);
 }
 
 }  // namespace
 
-hipError_t launch_select(const SelectArgs& args, hipStream_t stream) {
-  SelectArgs a = args;
+// One kernel while a workgroup for each sequence and key/value head has little to score and a CU of its own. Two kernels
+// / one, tables of 20, 64, 128 and 192 pages, us: eight sequences x 40/8 heads 9.7 / 7.7, 9.7 / 8.7, 9.9 / 10.6, 10.9 / 12.3; x
+// 12/4 9.6 / 7.1, 9.6 / 8.0, 9.7 / 9.3, 9.6 / 10.5; x 12/12 9.7 / 6.9, 9.7 / 7.4, 9.6 / 8.4, 9.7 / 9.2 (256: 9.8 / 10.4); x 64/8
+// 10.8 / 9.2, 11.4 / 10.8, 11.4 / 14.0, 13.2 / 17.0; 64 sequences x 12/4 9.5 / 7.4, 9.8 / 8.2, 11.7 / 9.5, 13.4 / 10.8, x 40/8
+// (512 workgroups) 10.8 / 14.0, 14.5 / 15.6, 17.4 / 19.0, 21.4 / 22.8.
+void plan_select(SelectArgs* a, int cus) {
+  const int64_t rows = (int64_t)a->B * a->Hk, width = a->pt.width;
+  a->chunk = 0;
+  if (width <= ONE_PAGES && rows <= cus && (a->Hq / a->Hk + 2) * width <= 700) return;
+  // pages of a workgroup: 32, more once that gives eight workgroups a CU (each turns its q into 64 bits first)
+  a->chunk = 32;
+  while (a->chunk < 256 && rows * width > (int64_t)8 * cus * a->chunk) a->chunk *= 2;
+}
+
+hipError_t launch_select(const SelectArgs& a, hipStream_t stream) {
   if (a.pt.width > a.count) {  // (else every page is chosen)
-    // pages of a workgroup: 32, more once that gives eight workgroups a CU (each turns its q into 64 bits first)
-    a.chunk = 32;
-    while (a.chunk < 256 && (int64_t)a.B * a.Hk * a.pt.width > (int64_t)8 * num_cus() * a.chunk) a.chunk *= 2;
     // a group's heads in equal turns of five at most
     const int group = a.Hq / a.Hk, turns = (group + SC_G - 1) / SC_G;
     switch ((group + turns - 1) / turns) {
@@ -344,7 +395,7 @@ hipError_t launch_select(const SelectArgs& args, hipStream_t stream) {
       default: score<5>(a, stream); break;
     }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    if (e != hipSuccess || a.chunk == 0) return e;
   }
   hipLaunchKernelGGL(select_top_kernel, dim3((uint32_t)((int64_t)a.B * a.Hk)), dim3(TOP_T), 0, stream, a);
   return hipGetLastError();

@@ -171,10 +171,12 @@ def test_null_params_and_empty_calls():
 def test_workspaces():
     from lbw_amd import _lib
     lib = _lib.load()
-    # scores only where a table is wider than the choice: 8 bytes a page
-    assert lib.lbw_paged_select_workspace_size(ctypes.byref(_select(count=3, first=0, last=0))) == 0
-    p = _select()
-    assert lib.lbw_paged_select_workspace_size(ctypes.byref(p)) == 3 * 2 * 3 * 8
+    # scores only where a table is wider than the choice and not short: 8 bytes a page
+    wide = {"cache.table_width": 1000, "cache.table_stride": 1000}
+    assert lib.lbw_paged_select_workspace_size(ctypes.byref(_select(count=1000, **wide))) == 0
+    assert lib.lbw_paged_select_workspace_size(ctypes.byref(_select())) == 0
+    p = _select(**wide)
+    assert lib.lbw_paged_select_workspace_size(ctypes.byref(p)) == 3 * 2 * 1000 * 8
     assert lib.lbw_paged_select(ctypes.byref(p), None, 0, None) == 4
     assert lib.lbw_paged_select(ctypes.byref(p), ctypes.c_void_p(ADDR + 8), 1 << 20, None) == 4
     # partial results of 130 floats a row: (pieces + batch) or batch * splits rows a head
