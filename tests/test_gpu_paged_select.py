@@ -148,3 +148,28 @@ def test_bounds_hold_every_key_and_scores_every_product():
     assert torch.all(score >= best)
     sel = lbw_amd.paged_select(q, lbw_amd.PagedKV(k, v, edge), table, _i32([128]), 3, first=0, last=0)
     assert torch.equal(sel[0].cpu(), torch.sort(score.topk(3).indices, -1).values.int().cpu())
+
+
+@pytest.mark.parametrize("hq,hk", [(1, 1), (2, 1), (3, 1), (4, 2), (5, 1), (7, 1), (12, 4), (64, 8)])
+def test_short_tables_and_the_same_ones_widened(hq, hk):
+    """A short table is scored and chosen from by one kernel, a wide one by two: the same choice, with ties, infinities, NaN
+    and pages outside the cache among the scores."""
+    import lbw_amd
+    grp = hq // hk
+    n = min(256, 700 // (grp + 2))           # the longest table that one kernel takes
+    lens = [16 * n, 16 * n - 9, 16 * (n - 1), 16 * (n // 2) + 1, 16, 0]
+    for width in (n, n + 1, 4 * n):
+        q, cache, table = _case(lens, hq, hk, 16, seed=hq, width=4 * n)
+        e = cache.bounds
+        e[table[0, 3].long(), :, 0, 7] = float("-inf")
+        e[table[0, 9].long(), :, 1, 5] = float("nan")
+        e[table[1, 4:30].long()] = e[table[1, 4].long()].clone()
+        table[2, 5] = e.shape[0]
+        table[2, n - 3] = -7
+        t = table[:, :width].contiguous()
+        for count in (1, 8, n // 2, n - 1):
+            _check(q, cache, t, lens, count, 0, 0)
+            _check(q, cache, t, lens, count, count // 4, count // 3)
+    # more sequences and heads than CUs: two kernels for short tables too
+    many = [16 * 6 - i % 90 for i in range(300)]
+    _check(*_case(many, grp, 1, 16, seed=3), many, 3, 1, 1)

@@ -343,3 +343,74 @@ def test_large_batches():
     out = lbw_amd.attention_paged(m.q, m.cache, m.table, m.lens, selected=sel)
     want, allow = P.attention(m.q, m.cache.k, m.cache.v, m.table, m.host, SCALE, selected=sel)
     R.assert_within("selected", out, want, allow)
+
+
+def test_several_tokens_of_one_sequence_are_as_many_rows():
+    """A draft is appended at once; each of its tokens looks at what is before it, itself included."""
+    import lbw_amd
+    m = Model(3, 12, 40, seed=70)
+    m.append([40, 0, 90])
+    before, new = list(m.host), [5, 3, 0]
+    m.q, q, pos = m.append(new)
+    row = [b for b, n in enumerate(new) for _ in range(n)]
+    lens = [before[b] + 1 + i for b, n in enumerate(new) for i in range(n)]
+    table = m.table[row].contiguous()
+    out = lbw_amd.attention_paged(m.q, m.cache, table, _i32(lens))
+    want, allow = P.attention(m.q, m.cache.k, m.cache.v, table, lens, SCALE)
+    R.assert_within("out", out, want, allow)
+    sel = lbw_amd.paged_select(m.q, m.cache, table, _i32(lens), 2, first=1, last=1)
+    assert torch.equal(sel.cpu(), P.select(m.q, m.cache.bounds, table, lens, PAGE, 2, 1, 1))
+    # taken back and written anew: bounds that hold what is there, and may be wider
+    m.lens -= _i32(new)
+    q2, k2, v2 = torch.randn(8, HQ + 2 * HK, D, generator=m.g).to(BF).cuda().split([HQ, HK, HK], 1)
+    lbw_amd.paged_append_(m.cache, q2, k2, v2, m.table, m.lens, m.rope, pos, starts=_i32([0, 5, 8, 8]), wq=m.w[0],
+                          wk=m.w[1], eps=1e-6)
+    for b in range(3):
+        n = before[b] + new[b]
+        k = P.rows(m.cache.k, m.table[b, :P.pages_of(n, PAGE)], n)
+        for j in range(P.pages_of(n, PAGE)):
+            lo, hi = m.cache.bounds[m.table[b, j].long()].unbind(1)
+            rows = k[j * PAGE:(j + 1) * PAGE]
+            assert (lo <= rows.amin(0)).all() and (hi >= rows.amax(0)).all()
+
+
+def test_a_prompt_beside_packed_attention():
+    """The last token of a prompt over its pages is the last row of attention over the prompt packed."""
+    import lbw_amd
+    m = Model(2, 12, 40, seed=71)
+    qkv, pos = m.tokens(150)
+    q, k, v = qkv.split([HQ, HK, HK], 1)
+    m.grow(0, 100), m.grow(1, 50)
+    starts = _i32([0, 100, 150])
+    qt = lbw_amd.paged_append_(m.cache, q, k, v, m.table, m.lens, m.rope, pos, starts=starts, wq=m.w[0], wk=m.w[1],
+                               eps=1e-6)
+    m.lens += starts.diff()
+    qn, kn = lbw_amd.qk_head_norm_rope(q, k, m.w[0], m.w[1], m.rope, pos, eps=1e-6)
+    assert torch.equal(qn, qt)
+    for b, (s, e) in enumerate(((0, 100), (100, 150))):
+        assert torch.equal(P.rows(m.cache.k, m.table[b, :P.pages_of(e - s, PAGE)], e - s), kn[s:e])
+    packed = lbw_amd.attention_packed(qn, kn, v, lbw_amd.packed_plan([100, 50]))
+    out = lbw_amd.attention_paged(qt[[99, 149]].contiguous(), m.cache, m.table, m.lens)
+    want, allow = P.attention(qt[[99, 149]], m.cache.k, m.cache.v, m.table, m.host, SCALE)
+    R.assert_within("paged", out, want, allow)
+    R.assert_within("packed", packed[[99, 149]], want, allow)
+
+
+def test_tensors_on_two_devices_are_refused():
+    import lbw_amd
+    s = _step_state(72)
+    c, q = s["cache"], s["qkv"][:, :HQ].contiguous()
+    cpu = lbw_amd.PagedKV(c.k.cpu(), c.v.cpu(), c.bounds.cpu())
+    for kw in ({"q": q.cpu()}, {"cache": cpu}, {"table": s["table"].cpu()}, {"lens": s["lens"].cpu()}):
+        a = {"q": q, "cache": c, "table": s["table"], "lens": s["lens"], **kw}
+        with pytest.raises((RuntimeError, ValueError)):
+            lbw_amd.attention_paged(**a)
+        with pytest.raises((RuntimeError, ValueError)):
+            lbw_amd.paged_select(**a, count=3)
+        k = s["qkv"][:, HQ:HQ + HK]
+        with pytest.raises((RuntimeError, ValueError)):
+            lbw_amd.paged_append_(a["cache"], a["q"], k, k, a["table"], a["lens"], s["rope"])
+    for kw in ({"prefix_table": s["prefix"].cpu()}, {"prefix_table": s["prefix"], "prefix_len": s["prefix_len"].cpu()},
+               {"selected": torch.zeros(3, HK, 2, dtype=torch.int32)}, {"out": q.cpu()}):
+        with pytest.raises((RuntimeError, ValueError)):
+            lbw_amd.attention_paged(q, c, s["table"], s["lens"], **kw)

@@ -209,6 +209,37 @@ def test_shapes_for_tracing():
                       True, None, False, 0.0, 1.0, 1.0, table, lens, None, q, pool, pool, None)
 
 
+def test_no_gradients_and_no_tangents():
+    import torch.autograd.forward_ad as fwd
+    from lbw_amd import _lib
+    ops = _lib.ops()
+    q, pool, edge = _meta(3, 4, 128), _meta(9, 16, 2, 128), _meta(9, 2, 2, 128)
+    table, lens = _meta(3, 5, dtype=torch.int32), _meta(3, dtype=torch.int32)
+
+    def calls(q):
+        return [lambda: ops.attention_paged(q, pool, pool, table, lens),
+                lambda: ops.paged_select(q, edge, table, lens, 16, 7, 1, 1),
+                lambda: ops.attention_paged_out(q, pool, pool, table, lens, None, None, None, -1, 0.0, 0, _meta(3, 4, 128)),
+                lambda: ops.paged_append_(q, _meta(3, 2, 128), _meta(3, 2, 128), None, None,
+                                          _meta(8, 64, 2, dtype=torch.float32), [64], True, None, False, 0.0, 1.0, 1.0,
+                                          table, lens, None, _meta(3, 4, 128), pool, pool, None)]
+
+    wanted = calls(_meta(3, 4, 128).requires_grad_())
+    out = wanted[0]()
+    with pytest.raises(RuntimeError, match="not implemented"):
+        out.backward(torch.empty_like(out))
+    assert not wanted[1]().requires_grad
+    for call in wanted[2:]:
+        with pytest.raises(NotImplementedError, match="not differentiable"):
+            call()
+        with torch.no_grad():
+            call()
+    with fwd.dual_level():
+        for call in calls(fwd.make_dual(q, _meta(3, 4, 128))):
+            with pytest.raises(NotImplementedError):
+                call()
+
+
 def test_wrapper_errors():
     """Wrong arguments are named, whatever device they are on."""
     import lbw_amd as L
