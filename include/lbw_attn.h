@@ -375,7 +375,7 @@ int lbw_attention_decode(const lbw_decode_params* p, void* workspace, size_t wor
  * table int32 [batch][table_width] on the device: entry j of a row is the page of the sequence's tokens
  * j * page_size ... Sequences may share pages that none of them writes to any more. bounds, optional: bf16
  * [pages][k_heads][2][head_dim], contiguous, the smallest and the largest value of each key component of a page.
- * Entries behind a sequence's length are not read. A page outside the cache is never followed: what would go there is
+ * Entries behind a sequence's length may hold anything. A page outside the cache is never followed: what would go there is
  * not written, keys that would come from there make the result NaN, and it counts as the highest when pages are
  * selected. */
 typedef struct lbw_paged_kv {
@@ -392,7 +392,8 @@ typedef struct lbw_paged_kv {
  * the bounds kept up. Token t of sequence b (starts[b] <= t < starts[b + 1], int32 [batch + 1] on the device; NULL:
  * token t is sequence t's, batch == tokens) goes to row lens[b] + t - starts[b]; a row outside the table is not
  * written. Tokens outside every sequence are left alone, their q_out too. q_out may be q itself. A page that gets its
- * row 0 starts its bounds anew. No two sequences may be given tokens for one page. */
+ * row 0 starts its bounds anew. No two sequences, nor two entries of one's row of the table, may be given tokens for one
+ * page. */
 typedef struct lbw_paged_append_params {
   lbw_paged_kv cache;
   int32_t tokens, batch, q_heads, k_heads, head_dim;

@@ -87,12 +87,14 @@ def paged_append_(cache: PagedKV, q, k, v, table, lens, rope: AxisRope, pos=None
     token per sequence, token b goes to row ``lens[b]``. Otherwise int32 ``[batch + 1]`` on the device, rising: tokens
     ``starts[b] .. starts[b + 1] - 1`` are sequence b's next ones; tokens outside all of them are left alone, their
     ``q_out`` rows too. A row outside the table is not written. ``pos`` int32 ``[tokens, axes]`` (``[tokens]`` for one
-    axis); None: a token's row in its sequence, for a rotation of one axis. A position outside the rotation's table turns
+    axis); None: a token's row in its sequence's table, for a rotation of one axis (behind a prefix that is not the
+    position: give it). A position outside the rotation's table turns
     its pairs into NaN. ``eps`` not None: RMSNorm of every q and k head first, as in :func:`qk_head_norm_rope`, with
     weights ``wq``, ``wk`` or none.
 
-    A page that gets its row 0 starts its bounds anew. No two sequences of a call may put tokens into one page (copy a
-    shared page that is not full before a branch goes on in it). Returns the turned q, in ``q_out`` when given (q
+    A page that gets its row 0 starts its bounds anew; rows written over later only widen them. No two sequences of a call,
+    nor two entries of a sequence's row of the table, may put tokens into one page (copy a shared page that is not full,
+    with its bounds, before a branch goes on in it). Returns the turned q, in ``q_out`` when given (q
     itself, or apart from every other tensor of the call). Not differentiable: raises while gradients are recorded and
     one of the tensors, weights included, requires one (``torch.no_grad`` takes it)."""
     if q_out is None:
@@ -146,7 +148,7 @@ def attention_paged(q, cache: PagedKV, table, lens, *, selected=None, prefix_tab
 
     ``prefix_table`` int32 ``[pages]``: keys that come before every sequence's own, ``prefix_len`` of them (an int, or
     one int32 on the device, limited to the pages; None: all). They are read once for the whole batch; table and lens
-    then describe what each sequence has behind them.
+    then describe what each sequence has behind them. Several tokens of one sequence are as many rows of q, table and lens.
 
     ``selected`` int32 ``[batch, kv_heads, n]`` (from :func:`paged_select`): a key/value head attends to the table entries
     that its list names, up to the first negative one; entries at or past the length name no keys, one that is named twice
