@@ -76,6 +76,17 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int t, int lane) 
 __device__ __forceinline__ float min_nan(float x, float y) { return __builtin_elementwise_minimum(x, y); }
 __device__ __forceinline__ float max_nan(float x, float y) { return __builtin_elementwise_maximum(x, y); }
 
+// A chunk of a row. PAST: past the caches, for prompts' rows in their pages, which the next call mostly does not read in
+// full; q, and a decoded token's row, are read next. Prompts x 40/8 heads, inputs from memory, into the caches / past: 1000
+// tokens 23.6 / 22.6 us, 2000 32.1 / 31.9, 4680 37.8 / 37.4, 9841 61.5 / 60.4 (inputs in the last cache 54.6 / 45); with q read
+// by a copy behind it 28.3 / 27.5, 39.5 / 39.1, 51.3 / 50.7, 97.0 / 95.8 (q past the caches too: 26.9, 39.4, 52.4, 96.1). No
+// bounds: 3500 tokens 29.4 / 24.4, 9841 61.7 / 59.7.
+template <bool PAST>
+__device__ __forceinline__ void put16(uint16_t* p, const u32x4& x) {
+  if constexpr (PAST) __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
+  else *reinterpret_cast<u32x4*>(p) = x;
+}
+
 // Eight values of a head: normed (or not), turned, scaled, rounded.
 template <int LPH, bool INTER>
 __device__ __forceinline__ u32x4 turn_chunk(const AppendArgs& a, const u32x4& x, const float (&wt)[8], float scale,
@@ -97,7 +108,7 @@ __device__ __forceinline__ u32x4 turn_chunk(const AppendArgs& a, const u32x4& x,
 
 // Chunks first, first + step, .. of a token's heads; `bounds` (of the token's page, or null): the page's, started anew
 // if `fresh`.
-template <int LPH, bool INTER>
+template <int LPH, bool INTER, bool PAST>
 __device__ __forceinline__ void turn_rows(const AppendArgs& a, const uint16_t* src, int64_t ssh, uint16_t* dst,
                                           int64_t dsh, int heads, int first, int step, int e0, int hsub,
                                           const void* w, float scale, const Turn& rot, uint16_t* bounds, bool fresh) {
@@ -121,7 +132,7 @@ __device__ __forceinline__ void turn_rows(const AppendArgs& a, const uint16_t* s
       if (ch >= nch) break;
       const u32x4 out = turn_chunk<LPH, INTER>(a, x[u], wt, scale, rot);
       if (ch * HPW + hsub >= heads) continue;
-      *reinterpret_cast<u32x4*>(dst + (int64_t)ch * HPW * dsh + dof) = out;
+      put16<PAST>(dst + (int64_t)ch * HPW * dsh + dof, out);
       if (bounds == nullptr) continue;
       uint16_t* const lo = bounds + (int64_t)(ch * HPW + hsub) * 2 * D + e0;
       u32x4 l = out, h = out;
@@ -143,7 +154,7 @@ __device__ __forceinline__ void turn_rows(const AppendArgs& a, const uint16_t* s
   }
 }
 
-template <int LPH>
+template <int LPH, bool PAST>
 __device__ __forceinline__ void copy_rows(const uint16_t* src, int64_t ssh, uint16_t* dst, int64_t dsh, int heads,
                                           int first, int step, int e0, int hsub) {
   constexpr int HPW = 64 / LPH, U = 4;
@@ -159,7 +170,7 @@ __device__ __forceinline__ void copy_rows(const uint16_t* src, int64_t ssh, uint
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int ch = it + u * step;
-      if (ch * HPW + hsub < heads) *reinterpret_cast<u32x4*>(dst + (int64_t)ch * HPW * dsh + dof) = x[u];
+      if (ch * HPW + hsub < heads) put16<PAST>(dst + (int64_t)ch * HPW * dsh + dof, x[u]);
     }
   }
 }
@@ -217,7 +228,7 @@ __device__ __forceinline__ void append_pages(const AppendArgs& a, int64_t block,
       for (int i = 0; i < KH; ++i) {
         if (h0 + i >= a.Hk) break;
         const u32x4 out = turn_chunk<LPH, INTER>(a, x[i], wt, a.k_scale, rot);
-        if (mine < n) *reinterpret_cast<u32x4*>(dst + (h0 + i) * a.kp.sh) = out;
+        if (mine < n) put16<true>(dst + (h0 + i) * a.kp.sh, out);
         float lo[8], hi[8], y[8];
         unpack8(out, lo);
         unpack8(out, hi);
@@ -275,13 +286,15 @@ __device__ __forceinline__ void append_pages(const AppendArgs& a, int64_t block,
   }
 }
 
-// PAGES: the first a.page_wgs workgroups look after the new keys of whole pages, the others after the tokens' q and v.
-template <int LPH, bool INTER, bool PAGES>
+// One token of each sequence, prompts' rows, or (PAGES) the first a.page_wgs workgroups look after the new keys of whole
+// pages, the others after the tokens' q and v.
+enum Keys { TOKEN, ROWS, PAGES };
+template <int LPH, bool INTER, Keys KEYS>
 __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs a) {
   constexpr int HPW = 64 / LPH, D = 8 * LPH;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t wg = blockIdx.x;
-  if constexpr (PAGES) {
+  if constexpr (KEYS == PAGES) {
     if (wg < (uint32_t)a.page_wgs) {
       const uint32_t chunks = (uint32_t)((a.Hk + KEY_HEADS - 1) / KEY_HEADS);
       append_pages<LPH, INTER>(a, wg / chunks, wg % chunks, lane, wave);
@@ -304,19 +317,27 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs 
     const int x = (part - before) % a.parts;
     return x < 0 ? x + a.parts : x;
   };
-  turn_rows<LPH, INTER>(a, a.q.p + t * a.q.sl, a.q.sh, a.qo.p + t * a.qo.sl, a.qo.sh, a.Hq, part, a.parts, e0, hsub,
-                        a.wq, a.q_scale, rot, nullptr, false);
+  turn_rows<LPH, INTER, false>(a, a.q.p + t * a.q.sl, a.q.sh, a.qo.p + t * a.qo.sl, a.qo.sh, a.Hq, part, a.parts, e0,
+                               hsub, a.wq, a.q_scale, rot, nullptr, false);
   if (w.page < 0) return;
   const int64_t in = w.row & ((1 << a.pt.shift) - 1);
-  if constexpr (!PAGES) {
+  const uint16_t *const k = a.k.p + t * a.k.sl, *const v = a.v.p + t * a.v.sl;
+  uint16_t *const kp = a.kp.p + w.page * a.kp.sp + in * a.kp.sl, *const vp = a.vp.p + w.page * a.vp.sp + in * a.vp.sl;
+  if constexpr (KEYS == TOKEN) {
     // one new token per sequence: its page's bounds are this wave's
-    uint16_t* const bounds =
-        a.bounds != nullptr && a.starts == nullptr ? a.bounds + (int64_t)w.page * a.Hk * 2 * D : nullptr;
-    turn_rows<LPH, INTER>(a, a.k.p + t * a.k.sl, a.k.sh, a.kp.p + w.page * a.kp.sp + in * a.kp.sl, a.kp.sh, a.Hk,
-                          first(cq), a.parts, e0, hsub, a.wk, a.k_scale, rot, bounds, in == 0);
+    uint16_t* const bounds = a.bounds != nullptr ? a.bounds + (int64_t)w.page * a.Hk * 2 * D : nullptr;
+    turn_rows<LPH, INTER, false>(a, k, a.k.sh, kp, a.kp.sh, a.Hk, first(cq), a.parts, e0, hsub, a.wk, a.k_scale, rot,
+                                 bounds, in == 0);
+  } else if constexpr (KEYS == ROWS) {
+    if (a.bounds == nullptr) {
+      turn_rows<LPH, INTER, true>(a, k, a.k.sh, kp, a.kp.sh, a.Hk, first(cq), a.parts, e0, hsub, a.wk, a.k_scale, rot,
+                                  nullptr, false);
+    } else {  // (the bounds kernel reads them)
+      turn_rows<LPH, INTER, false>(a, k, a.k.sh, kp, a.kp.sh, a.Hk, first(cq), a.parts, e0, hsub, a.wk, a.k_scale, rot,
+                                   nullptr, false);
+    }
   }
-  copy_rows<LPH>(a.v.p + t * a.v.sl, a.v.sh, a.vp.p + w.page * a.vp.sp + in * a.vp.sl, a.vp.sh, a.Hk,
-                 first(PAGES ? cq : cq + ck), a.parts, e0, hsub);
+  copy_rows<LPH, KEYS != TOKEN>(v, a.v.sh, vp, a.vp.sh, a.Hk, first(KEYS == PAGES ? cq : cq + ck), a.parts, e0, hsub);
 }
 
 // Bounds of the pages that several tokens were put into: blockIdx.x counts blocks of a.page_block tokens, blockIdx.y
@@ -391,12 +412,12 @@ __global__ void __launch_bounds__(EDGE_WAVES * 64) append_bounds_kernel(const Ap
   }
 }
 
-template <int LPH, bool PAGES>
+template <int LPH, Keys KEYS>
 hipError_t launch(const AppendArgs& a, hipStream_t stream) {
   const int64_t waves = (int64_t)a.T * a.parts;
   const dim3 grid((uint32_t)(a.page_wgs + (waves + AP_WAVES - 1) / AP_WAVES)), block(AP_WAVES * 64);
-  if (a.inter) hipLaunchKernelGGL((append_kernel<LPH, true, PAGES>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((append_kernel<LPH, false, PAGES>), grid, block, 0, stream, a);
+  if (a.inter) hipLaunchKernelGGL((append_kernel<LPH, true, KEYS>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((append_kernel<LPH, false, KEYS>), grid, block, 0, stream, a);
   return hipGetLastError();
 }
 
@@ -404,7 +425,8 @@ template <int LPH>
 hipError_t run(AppendArgs a, hipStream_t stream) {
   constexpr int HPW = 64 / LPH;
   a.page_wgs = 0;
-  if (a.bounds == nullptr || a.starts == nullptr) return launch<LPH, false>(a, stream);
+  if (a.starts == nullptr) return launch<LPH, TOKEN>(a, stream);
+  if (a.bounds == nullptr) return launch<LPH, ROWS>(a, stream);
   const int page = 1 << a.pt.shift;
   // tokens that a workgroup looks for pages in: as many as a page has, so that it finds one, or fewer where sequences
   // are shorter or workgroups few
@@ -416,9 +438,9 @@ hipError_t run(AppendArgs a, hipStream_t stream) {
   if (page <= FUSED_PAGE) {
     a.page_block = block_for(256);
     a.page_wgs = (a.T + a.page_block - 1) / a.page_block * ((a.Hk + KEY_HEADS - 1) / KEY_HEADS);
-    return launch<LPH, true>(a, stream);
+    return launch<LPH, PAGES>(a, stream);
   }
-  const hipError_t e = launch<LPH, false>(a, stream);
+  const hipError_t e = launch<LPH, ROWS>(a, stream);
   if (e != hipSuccess) return e;
   a.page_block = block_for(512);
   const dim3 blocks((a.T + a.page_block - 1) / a.page_block, (a.Hk + HPW - 1) / HPW);
