@@ -8,8 +8,9 @@
 // Bound by memory: every value is read once and written once. As in the per-head norm a wave keeps a token, its
 // angles in registers, and walks its heads. Several tokens for one page: the keys are turned by the workgroup that
 // makes the page's bounds, beside the tokens' q and v. 4680 + 3600 + 1561 tokens x 40/8 heads of 128, normed, pages of 64,
-// 58 us (4.9 TB/s; a large copy reaches 4.9); one token 4.3 us, most of it the launch.
+// from memory 60 us (4.7 TB/s; a large copy reaches 4.9), inputs in the last cache 46; one token 4.3 us, most of it the launch.
 
+#include "capi_util.h"
 #include "head_rows.h"
 #include "paged.h"
 
@@ -17,12 +18,12 @@ namespace lbw {
 namespace {
 
 constexpr int AP_WAVES = 4;
-constexpr int KEY_HEADS = 2;   // heads of a workgroup that looks after a page's keys
+constexpr int KEY_HEADS = 2;   // heads of a workgroup that looks after a page's keys, at most
 constexpr int EDGE_WAVES = 8;  // of the bounds kernel
 // Pages up to this size get their keys and bounds in the kernel of the tokens' q and v, larger ones, whose tokens would
-// follow one another too long, their bounds by a second kernel. Two kernels / one, x 40/8 heads: 100 tokens in pages of
-// 64 11.7 / 9.2 us, 500 14.0 / 14.2, 4680 + 3600 + 1561 64.5 / 58.7; in pages of 128 11.2 / 9.2, 14.8 / 20.6, 66.9 / 68.3, of 256
-// 11.4 / 11.2, 15.6 / 35.9, 67.8 / 79.0.
+// follow one another too long, their bounds by a second kernel. Two kernels / one, x 40/8 heads: pages of 64, 100 tokens
+// 13.4 / 10.3 us, 500 14.8 / 16.4, 1000 16.9 / 16.7, 4680 38.5 / 37.1, 9841 69.1 / 60.4; of 128 13.4 / 13.5, 15.9 / 23.4, 18.1 / 27.1,
+// 41.1 / 46.6, 73.4 / 71.6; of 256 13.0 / 13.2, 18.0 / 33.7, 20.2 / 39.7, 41.9 / 66.3, 72.8 / 88.5.
 constexpr int FUSED_PAGE = 64;
 
 // Where a token goes: its sequence (-1: none), row and page (-1: nowhere).
@@ -188,7 +189,7 @@ __device__ __forceinline__ void load_rotation(const AppendArgs& a, int t, int64_
 }
 
 // The tokens of block `block` whose pages this workgroup looks after: those that are the first new ones of their page.
-// The page's new keys are turned and put there, heads KH chunk .., and its bounds made of them and, where the page was
+// The page's new keys are turned and put there, heads h0 .., and its bounds made of them and, where the page was
 // begun before, the old ones: every page has one owner, no atomics. A wave takes 64 / LPH tokens at a time, a head
 // after the other, so that a token's angles are read once; the tokens' smallest and largest values meet by shuffles,
 // the waves' in LDS.
@@ -196,7 +197,8 @@ template <int LPH, bool INTER>
 __device__ __forceinline__ void append_pages(const AppendArgs& a, int64_t block, int chunk, int lane, int wave) {
   constexpr int TPW = 64 / LPH, D = 8 * LPH, KH = KEY_HEADS;
   __shared__ u32x4 red[AP_WAVES][KH][2][LPH];  // (bf16: what was rounded once stays)
-  const int e0 = 8 * (lane % LPH), sub = lane / LPH, h0 = chunk * KH;
+  const int e0 = 8 * (lane % LPH), sub = lane / LPH, h0 = chunk * a.page_heads;
+  const int h1 = h0 + a.page_heads < a.Hk ? h0 + a.page_heads : a.Hk;  // heads h0 .. h1 - 1
   const int64_t t0 = block * a.page_block;
   const int t1 = (int)(t0 + a.page_block < a.T ? t0 + a.page_block : a.T);
   const int mask = (1 << a.pt.shift) - 1;
@@ -220,13 +222,13 @@ __device__ __forceinline__ void append_pages(const AppendArgs& a, int64_t block,
       u32x4 x[KH];
       const uint16_t* const src = a.k.p + (int64_t)(t + tok) * a.k.sl + e0;
 #pragma unroll
-      for (int i = 0; i < KH; ++i) x[i] = load16(src + (h0 + i < a.Hk ? h0 + i : a.Hk - 1) * a.k.sh);
+      for (int i = 0; i < KH; ++i) x[i] = load16(src + (h0 + i < h1 ? h0 + i : h0) * a.k.sh);
       Turn rot;
       load_rotation<INTER>(a, t + tok, w.row + tok, e0, lane, rot);
       uint16_t* const dst = a.kp.p + w.page * a.kp.sp + (in + tok) * a.kp.sl + e0;
 #pragma unroll
       for (int i = 0; i < KH; ++i) {
-        if (h0 + i >= a.Hk) break;
+        if (h0 + i >= h1) break;
         const u32x4 out = turn_chunk<LPH, INTER>(a, x[i], wt, a.k_scale, rot);
         if (mine < n) put16<true>(dst + (h0 + i) * a.kp.sh, out);
         float lo[8], hi[8], y[8];
@@ -270,7 +272,7 @@ __device__ __forceinline__ void append_pages(const AppendArgs& a, int64_t block,
     const int used = turns < AP_WAVES ? turns : AP_WAVES;
     for (int x = threadIdx.x; x < KH * 2 * LPH; x += AP_WAVES * 64) {
       const int c = x % LPH, edge = x / LPH % 2, i = x / (2 * LPH);
-      if (h0 + i >= a.Hk) break;
+      if (h0 + i >= h1) break;
       uint16_t* const p = a.bounds + (((int64_t)w.page * a.Hk + h0 + i) * 2 + edge) * D + 8 * c;
       float m[8], y[8];
       unpack8(in != 0 ? load16(p) : red[0][i][edge][c], m);
@@ -296,7 +298,7 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs 
   uint32_t wg = blockIdx.x;
   if constexpr (KEYS == PAGES) {
     if (wg < (uint32_t)a.page_wgs) {
-      const uint32_t chunks = (uint32_t)((a.Hk + KEY_HEADS - 1) / KEY_HEADS);
+      const uint32_t chunks = (uint32_t)((a.Hk + a.page_heads - 1) / a.page_heads);
       append_pages<LPH, INTER>(a, wg / chunks, wg % chunks, lane, wave);
       return;
     }
@@ -437,7 +439,12 @@ hipError_t run(AppendArgs a, hipStream_t stream) {
   };
   if (page <= FUSED_PAGE) {
     a.page_block = block_for(256);
-    a.page_wgs = (a.T + a.page_block - 1) / a.page_block * ((a.Hk + KEY_HEADS - 1) / KEY_HEADS);
+    const int blocks = (a.T + a.page_block - 1) / a.page_block, chunks = (a.Hk + KEY_HEADS - 1) / KEY_HEADS;
+    // a head a workgroup, not two, while pages are few: 120 tokens x 40/8 heads in pages of 64 13.6 to 10.7 us, 500 19.5 to
+    // 16.3, 2000 (132 workgroups of two) 30.7 to 27.9, but 2500 25.9 to 31.0
+    const int64_t pages = (a.T >> a.pt.shift) + a.B;
+    a.page_heads = pages * chunks <= num_cus() / 2 ? 1 : KEY_HEADS;
+    a.page_wgs = blocks * ((a.Hk + a.page_heads - 1) / a.page_heads);
     return launch<LPH, PAGES>(a, stream);
   }
   const hipError_t e = launch<LPH, ROWS>(a, stream);
@@ -452,12 +459,13 @@ hipError_t run(AppendArgs a, hipStream_t stream) {
 
 hipError_t launch_append(const AppendArgs& args, int D, hipStream_t stream) {
   AppendArgs a = args;
-  // a token's heads are shared by several waves while the tokens alone do not fill the chip (each of them reads the
-  // token's place and angles: up to 16384 waves / up to 4096, 2000 tokens x 40/8 heads 36.2 / 24.1 us, 3000 31.8 / 23.0, 5000
-  // x 12/12 27.8 / 21.2, 16000 83 / 70; fewer tokens and more the same)
+  // a token's heads are shared by several waves while the tokens alone do not fill the chip, up to 7000 waves: each of them
+  // reads the token's place and angles (up to 16384 waves / up to 4096, 3000 tokens x 40/8 heads 31.8 / 23.0 us, 5000 x 12/12
+  // 27.8 / 21.2, 16000 83 / 70; up to 8191 / 7000 / 5200, 1000 x 40/8 without bounds 11.4 / 9.5 / 9.4, 1500, from memory, 13.3 / 13.2
+  // / 14.8, 2000 18.6 / 16.8 / 16.8, 3500 24.5 / 24.3 / 25.2)
   const int nch = (a.Hq + 2 * a.Hk + 512 / D - 1) / (512 / D);
   a.parts = 1;
-  while (a.parts < nch && (int64_t)a.T * a.parts < 4096) a.parts *= 2;
+  while (a.parts < nch && (int64_t)a.T * a.parts * 2 <= 7000) a.parts *= 2;
   switch (D) {
     case 32: return run<4>(a, stream);
     case 64: return run<8>(a, stream);
