@@ -9,7 +9,7 @@ import paged_ref as P
 
 pytestmark = pytest.mark.gpu
 BF = torch.bfloat16
-POSITIONS = 4096   # rows of the rotation table: more than any test has tokens in a sequence
+POSITIONS = 4096   # rows of the rotation table, at least
 
 
 def _rope(dim, rot, axes, inter, positions, device="cuda"):
@@ -28,7 +28,9 @@ class Case:
         g = torch.Generator().manual_seed(seed)
         self.new, self.old, self.page, self.eps, self.scales = new, old, page, eps, scales
         T = sum(new) + spare_tokens
-        self.rope, self.ang, self.split = _rope(dim, dim if rot is None else rot, axes, inter, POSITIONS)
+        # (a row for every token of a sequence: the definition looks its angles up there)
+        self.rope, self.ang, self.split = _rope(dim, dim if rot is None else rot, axes, inter,
+                                                max(POSITIONS, *(o + n for o, n in zip(old, new))))
         self.inter = inter
         qkv = (torch.randn(T, hq + 2 * hk, dim, generator=g) * 1.7).to(BF).cuda()
         self.q, self.k, self.v = qkv.split([hq, hk, hk], 1)
@@ -58,6 +60,7 @@ class Case:
     def want(self):
         n = len(self.rows)
         pos = torch.tensor(self.rows, device="cuda")[:, None] if self.pos is None else self.pos[:n]
+        assert self.pos is not None or max(self.rows, default=0) < len(self.ang)
         ang = R.token_angles(self.ang, self.split, pos)
         wq, wk = self.w if self.w else (None, None)
         return (P.turned(self.q[:n], wq, ang, self.inter, self.eps, self.scales[0]),
@@ -304,3 +307,11 @@ def test_no_tokens_and_refusals():
     n = x._version
     lbw_amd.paged_append_(*args, starts=c.starts)
     assert c.cache.k._version > n and c.cache.bounds._version > 0
+
+
+@pytest.mark.parametrize("hq,hk,dim,inter", [(3, 3, 128, True), (10, 5, 64, False), (7, 7, 32, True), (6, 3, 256, False)])
+@pytest.mark.parametrize("page,new", [(16, [1500, 0, 1100]), (32, [2600, 900]), (64, [7000, 33]), (128, [300, 90]), (16, [9, 40])])
+def test_many_pages_and_few_with_odd_heads(hq, hk, dim, inter, page, new):
+    """Pages whose keys are looked after one head and two at a time, an odd one last, or by a kernel of its own."""
+    Case(new, [5 + 30 * i for i in range(len(new))], hq=hq, hk=hk, dim=dim, inter=inter, page=page, eps=1e-6, weights=BF,
+         seed=dim + page).go()
