@@ -64,6 +64,10 @@ __device__ __forceinline__ void dma16_guarded(const unsigned char* sbase, uint32
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(lds_dst)
                : "memory");
 }
+// dma16_guarded past the caches, for what one workgroup reads once
+__device__ __forceinline__ void dma16_past(const unsigned char* sbase, uint32_t voff, uint32_t lds_dst) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(sbase), "{m0}"(lds_dst) : "memory");
+}
 // 4 bytes per lane from a per-lane 64-bit address (global_load_lds_dword): lane l's dword lands
 // at LDS byte address lds_dst + 4 l.
 __device__ __forceinline__ void dma4(uint64_t addr, uint32_t lds_dst) {

@@ -178,7 +178,10 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
 #pragma unroll
       for (int i = 0; i < NCOPY; ++i) {  // (rows past the last key copy it)
         const uint32_t row = min(off + 4 * (i & 3) * (uint32_t)sl, i < 4 ? last0 : last1);
-        dma16_guarded(i < 4 ? b0 : b1, row + (ccol ^ ((i & 3) << 4)), to + 1024 * i);
+        // (own keys past the caches: eight of up to 46800 x 40/8 heads 186 to 165 us, 12/12 of 14040 95 to 84, selected pages too;
+        // the prefix's, which other rows' workgroups read, not: 16 of 3000 off 46800 67 to 97)
+        if constexpr (KIND == PREFIX) dma16_guarded(i < 4 ? b0 : b1, row + (ccol ^ ((i & 3) << 4)), to + 1024 * i);
+        else dma16_past(i < 4 ? b0 : b1, row + (ccol ^ ((i & 3) << 4)), to + 1024 * i);
       }
     };
     auto issue_k = [&](int t) { issue(a.k, koff, t, (uint32_t)ring); };
