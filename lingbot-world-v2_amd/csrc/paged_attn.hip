@@ -12,9 +12,9 @@
 // The prefix's keys are the same for the whole batch: its query rows are those of all sequences, 32 at a time, or 128
 // where there are more (four waves over shared tiles of 64 keys), in one launch with the sequences' own keys.
 //
-// Measured, x 40/8 heads: eight sequences of up to 46800 keys 187 us, K and V at 5.6 TB/s (a kernel that only reads
-// reaches 5.7); 64 of up to 3600 behind a prefix of 46800 172 us, 16 of 200 (12/4 heads) behind 46800 37; one
-// sequence of 500 keys 8.8 us, 3 us of it the launch and 1.5 a tile of each wave.
+// Measured, x 40/8 heads: eight sequences of up to 46800 keys 165 us, K and V at 6.4 TB/s (a plain kernel that only reads
+// reaches 5.7); 64 of up to 3600 behind a prefix of 46800 155 us, 16 of 200 (12/4 heads) behind 46800 37; one
+// sequence of 500 keys 8.7 us, 3 us of it the launch and 1.5 a tile of each wave.
 //
 // A half's rows past its last key copy that key (or the other half's), so the products never meet what lies
 // behind a sequence. A page outside the cache makes its keys' scores NaN.
@@ -565,11 +565,13 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 }  // namespace
 
 // How the keys are cut. Own ones: whole sequences where they keep the chip busy or are short, else the batch's keys in
-// equal pieces, a workgroup a CU (two: 1 to 5 % slower); the longer for that the more sequences x key/value heads there
-// are. Whole / in pieces, x 40/8 heads, lengths from a third of the longest up to it: one sequence of 1100 keys 11.9 /
-// 13.8 us, of 1600 15.2 / 13.7; four of 1600 15.3 / 15.6, of 2400 20.2 / 17.6; eight of 2400 20.6 / 21.5, of 4000 30.4 /
-// 26.1; 16 of 4000 34.3 / 37.9, of 8000 86.6 / 63.1; 32 of 4000 64.9 / 69.1, of 8000 123 / 119; 48 of 2400 65.1 / 62.3, of 8000
-// 225 / 190; 64 of 2400 83.1 / 86.6, of 4000 131 / 133, of 8000 249 / 239; 128 of 2400 154 / 159, of 4000 246 / 242.
+// equal pieces, a workgroup a CU (two: 0 to 5 % slower); the longer for that the more sequences x key/value heads there
+// are, up to one a CU, and shorter again where those behind the first one of each CU are few. Whole / in pieces, x 40/8
+// heads, lengths from a third of the longest up to it, from memory: one sequence of 1100 keys 11.6 / 14.4 us, of 1300 16.2 /
+// 13.9; four of 1000 14.7 / 16.0, of 1300 17.0 / 15.9; eight of 1000 14.7 / 16.3, of 1500 19.4 / 18.4; 16 of 1600 20.6 / 21.6, of
+// 2000 25.2 / 23.5, of 4000 45.7 / 38.9; 20 of 2400 30.4 / 31.7, of 3200 38.0 / 35.9; 24 of 3200 40.2 / 41.3, of 4000 49.6 / 48.6; 32 of
+// 4000 60.6 / 63.6, of 5000 74.7 / 73.9; 40 of 1600 41.9 / 40.8, of 3200 74.1 / 63.1; 64 of 2400 72.5 / 76.6, of 4000 115 / 116, of 8000
+// 221 / 211; 128 of 2400 135 / 140, of 4000 218 / 214.
 // Selected pages, by the same rule: equal pieces of 6 tiles or more for as many workgroups as run at once, as the
 // prefix's. 2560 keys for 32 sequences x 40/8 heads, whole / in pieces 48.5 / 52.6 us, 1536 for 8 x 12/12 16.7 / 19.2; 1600
 // for 2 x 40/8 15.7 / 10.6, 6400 for 4 x 40/8 45.1 / 23.7.
@@ -594,7 +596,10 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
   const int64_t keys = a->sel != nullptr ? (int64_t)a->n_sel << a->pt.shift : cap;
   const int64_t own_tiles = (keys + DT - 1) / DT;  // of a sequence
   // (with a prefix, whose results are joined anyway, pieces cost less)
-  const int64_t limit = a->p_max > 0 ? 1024 : seqs <= cus ? 1024 + 20 * seqs : 3500;
+  const int64_t limit = a->p_max > 0                                ? 1024
+                        : seqs <= cus                               ? 1150 + 3200 * seqs * seqs / ((int64_t)cus * cus)
+                        : 8 * seqs > 9 * cus && 2 * seqs <= 3 * cus ? 1800
+                                                                    : 3500;
   const bool whole = num_splits == 1 || (num_splits == 0 && keys <= limit);
   int64_t own_places = a->sel != nullptr ? 2 * cus : cus;
   if (a->p_max > 0) {
