@@ -575,7 +575,8 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 // Selected pages, by the same rule: equal pieces of 6 tiles or more for as many workgroups as run at once, as the
 // prefix's. 2560 keys for 32 sequences x 40/8 heads, whole / in pieces 48.5 / 52.6 us, 1536 for 8 x 12/12 16.7 / 19.2; 1600
 // for 2 x 40/8 15.7 / 10.6, 6400 for 4 x 40/8 45.1 / 23.7.
-// With a prefix, places shared out by tiles: 4 of up to 1600 off 14040 keys x 40/8 heads, 20 pieces of the prefix and 12
+// With a prefix (measured before own keys went past the caches, which changes both sides alike; 0.5 to 0.8 instead of 0.7
+// below then gave 167, 166, 160 and 177 us), places shared out by tiles: 4 of up to 1600 off 14040 keys x 40/8 heads, 20 pieces of the prefix and 12
 // of own keys 22.2 us, 32 and 32 25.8; 8 of 3600 off 6000 x 12/4, 9 and 55 21.2, 64 and 64 28.2; 64 of 3600 off 46800 x 40/8
 // (128 rows at a time), 10 and 34 163, 21 and 64 185, 5 and 17 205; 26 of 1500 off 14040 x 40/8 16 and 32 40.4, 8 and 16 45.8;
 // 30 of 1500 off 10000 x 16/2, 32 and 64 23.5, 64 and 128 27.6. Whole sequences: 16 of 200 off 6000 x 12/4, 24 pieces (one
