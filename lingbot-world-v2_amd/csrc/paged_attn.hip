@@ -572,9 +572,9 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 // 2000 25.2 / 23.5, of 4000 45.7 / 38.9; 20 of 2400 30.4 / 31.7, of 3200 38.0 / 35.9; 24 of 3200 40.2 / 41.3, of 4000 49.6 / 48.6; 32 of
 // 4000 60.6 / 63.6, of 5000 74.7 / 73.9; 40 of 1600 41.9 / 40.8, of 3200 74.1 / 63.1; 64 of 2400 72.5 / 76.6, of 4000 115 / 116, of 8000
 // 221 / 211; 128 of 2400 135 / 140, of 4000 218 / 214.
-// Selected pages, by the same rule: equal pieces of 6 tiles or more for as many workgroups as run at once, as the
-// prefix's. 2560 keys for 32 sequences x 40/8 heads, whole / in pieces 48.5 / 52.6 us, 1536 for 8 x 12/12 16.7 / 19.2; 1600
-// for 2 x 40/8 15.7 / 10.6, 6400 for 4 x 40/8 45.1 / 23.7.
+// Selected pages, by the same rule: a list in equal pieces of 4 tiles or more. Whole / in pieces: 2560 keys for 32
+// sequences x 40/8 heads 50.6 / 50.5 us, 1536 for 8 x 12/12 21.3 / 18.6, 4096 for 16 x 40/8 48.7 / 41.1, 2560 for 2 x 40/8 28.1 /
+// 11.8; a workgroup a CU / two: 5760 for 8 x 40/8 35.4 / 35.5, 6400 for 4 x 40/8 23.1 / 23.7, for 24 x 40/8 88.5 / 100.6.
 // With a prefix (measured before own keys went past the caches, which changes both sides alike; 0.5 to 0.8 instead of 0.7
 // below then gave 167, 166, 160 and 177 us), places shared out by tiles: 4 of up to 1600 off 14040 keys x 40/8 heads, 20 pieces of the prefix and 12
 // of own keys 22.2 us, 32 and 32 25.8; 8 of 3600 off 6000 x 12/4, 9 and 55 21.2, 64 and 64 28.2; 64 of 3600 off 46800 x 40/8
@@ -602,7 +602,7 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
                         : 8 * seqs > 9 * cus && 2 * seqs <= 3 * cus ? 1800
                                                                     : 3500;
   const bool whole = num_splits == 1 || (num_splits == 0 && keys <= limit);
-  int64_t own_places = a->sel != nullptr ? 2 * cus : cus;
+  int64_t own_places = cus;
   if (a->p_max > 0) {
     const int64_t rows = a->B * group, p_tiles = (a->p_max + DT - 1) / DT;
     a->p_block = rows > 3 * HEADS ? PK_BLOCK : HEADS;
