@@ -572,9 +572,10 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 // 2000 25.2 / 23.5, of 4000 45.7 / 38.9; 20 of 2400 30.4 / 31.7, of 3200 38.0 / 35.9; 24 of 3200 40.2 / 41.3, of 4000 49.6 / 48.6; 32 of
 // 4000 60.6 / 63.6, of 5000 74.7 / 73.9; 40 of 1600 41.9 / 40.8, of 3200 74.1 / 63.1; 64 of 2400 72.5 / 76.6, of 4000 115 / 116, of 8000
 // 221 / 211; 128 of 2400 135 / 140, of 4000 218 / 214.
-// Selected pages, by the same rule: a list in equal pieces of 4 tiles or more. Whole / in pieces: 2560 keys for 32
-// sequences x 40/8 heads 50.6 / 50.5 us, 1536 for 8 x 12/12 21.3 / 18.6, 4096 for 16 x 40/8 48.7 / 41.1, 2560 for 2 x 40/8 28.1 /
-// 11.8; a workgroup a CU / two: 5760 for 8 x 40/8 35.4 / 35.5, 6400 for 4 x 40/8 23.1 / 23.7, for 24 x 40/8 88.5 / 100.6.
+// Selected pages: equal lengths, so pieces pay sooner, of 4 tiles or more (and a whole list each where there are more
+// lists than half the CUs). Whole / in pieces, x 40/8 heads: 512 keys for one sequence 9.3 / 11.0 us, for 8 11.0 / 11.1, for 16
+// 11.6 / 12.5; 768 12.3 / 11.2, 13.4 / 12.7, 14.0 / 14.5; 1024 14.7 / 11.3, 15.8 / 13.4, 16.7 / 16.6; 2560 28.0 / 10.9, 30.8 / 20.6,
+// 33.1 / 29.3; a workgroup a CU / two: 5760 for 8 35.4 / 35.5, 6400 for 4 23.1 / 23.7, for 24 88.5 / 100.6.
 // With a prefix (measured before own keys went past the caches, which changes both sides alike; 0.5 to 0.8 instead of 0.7
 // below then gave 167, 166, 160 and 177 us), places shared out by tiles: 4 of up to 1600 off 14040 keys x 40/8 heads, 20 pieces of the prefix and 12
 // of own keys 22.2 us, 32 and 32 25.8; 8 of 3600 off 6000 x 12/4, 9 and 55 21.2, 64 and 64 28.2; 64 of 3600 off 46800 x 40/8
@@ -598,6 +599,7 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
   const int64_t own_tiles = (keys + DT - 1) / DT;  // of a sequence
   // (with a prefix, whose results are joined anyway, pieces cost less)
   const int64_t limit = a->p_max > 0                                ? 1024
+                        : a->sel != nullptr                         ? 512 + 3 * seqs
                         : seqs <= cus                               ? 1150 + 3200 * seqs * seqs / ((int64_t)cus * cus)
                         : 8 * seqs > 9 * cus && 2 * seqs <= 3 * cus ? 1800
                                                                     : 3500;
