@@ -98,7 +98,7 @@ def check_func(f, path):
             continue
         reads = set()
         for o in e[2][1:]:
-            reads |= sgprs(o)
+            reads |= sgprs(o.split()[0])  # (cache modifiers follow the last operand)
         if not reads:
             continue
         hit = walk(i, WAIT, reads, set())

@@ -90,3 +90,14 @@ def test_every_source_with_inline_asm_copies_is_checked_by_the_build():
                 users.add(f[:-4])
     assert users, "no source issues the copies: the pattern is stale"
     assert users <= checked, f"not checked by the build: {sorted(users - checked)}"
+
+
+def test_a_copy_with_cache_modifiers_is_looked_at_too(tmp_path):
+    body = """\
+\tv_readlane_b32 s27, v214, 6
+{nop}\tglobal_load_lds_dwordx4 v2, s[26:27] nt
+\tglobal_load_lds_dwordx4 v2, s[26:27] offset:16 sc0 nt
+\ts_endpgm
+"""
+    assert _run(tmp_path, body.format(nop="")) == 1
+    assert _run(tmp_path, body.format(nop="\ts_nop 4\n")) == 0
