@@ -12,12 +12,14 @@
 
 namespace lbw {
 
+// The page that a table's entry names; -1: outside the cache of `pages`.
+LBW_LOOKUP int page_of_entry(int32_t page, int pages) { return page >= 0 && page < pages ? page : -1; }
+
 // The page of a sequence's token `row`, by its `width` table entries of 2^shift tokens each; -1: the table does not
 // reach that far, or names a page outside the cache of `pages`.
 LBW_LOOKUP int page_at(const int32_t* entries, int width, int shift, int pages, int64_t row) {
   if (row < 0 || (row >> shift) >= width) return -1;
-  const int32_t page = entries[row >> shift];
-  return page >= 0 && page < pages ? page : -1;
+  return page_of_entry(entries[row >> shift], pages);
 }
 
 // Half a tile of keys: 16 consecutive tokens of one page. `keys` of them are the sequence's; with BAD_PAGE added, their

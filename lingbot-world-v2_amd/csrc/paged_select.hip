@@ -60,46 +60,60 @@ __device__ __forceinline__ int pages_of(const SelectArgs& a, int b) {
   return __builtin_amdgcn_readfirstlane((int)((n + (1 << a.pt.shift) - 1) >> a.pt.shift));
 }
 
-// Scores of pages from .. end - 1 of a sequence and key/value head, four a wave at a time; `put(page, score, first)`:
-// the higher of it and what is there, unless it is the first.
+// Scores of a sequence's pages from .. from + most - 1 for one key/value head, four a wave at a time, unless all of its n
+// pages are chosen (returns n either way); `put(page, score, first)`: the higher of it and what is there, unless it is
+// the first.
 template <int G, typename Put>
-__device__ __forceinline__ void score_pages(const SelectArgs& a, int b, int kv, int from, int end, int lane, int wave,
-                                            int waves, Put put) {
-  const int group = a.Hq / a.Hk, e0 = 8 * (lane & 15), sub = lane >> 4;
+__device__ __forceinline__ int score_pages(const SelectArgs& a, int b, int kv, int from, int most, int lane, int wave,
+                                           int waves, Put put) {
+  const int group = a.Hq / a.Hk, e0 = 8 * (lane & 15), step = 4 * waves, first = from + 4 * wave + (lane >> 4);
   const int32_t* const table = a.pt.p + b * a.pt.sb;
+  int n = 0, end = 0;
   for (int h0 = 0; h0 < group; h0 += G) {
+    // the queries and the first page's entry are on their way together with the length
+    u32x4 raw[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const int h = h0 + g < group ? h0 + g : group - 1;  // (past the last head: it once more)
+      raw[g] = load16(a.q.p + b * a.q.sl + (int64_t)(kv * group + h) * a.q.sh + e0);
+    }
+    int page = first;
+    int32_t entry = page < a.pt.width ? table[page] : 0;
+    if (h0 == 0) {
+      n = pages_of(a, b);
+      if (n <= a.count || from >= n) return n;
+      end = n < from + most ? n : from + most;
+    }
+    // a page's bounds are fetched while the one before is summed, its entry while the one before that is
+    u32x4 lw, hw;
+    bool bad = false;
+    auto fetch = [&](int next) {
+      int at = page_of_entry(entry, a.pt.pages);
+      bad = at < 0;
+      at = bad ? 0 : at;  // (pages past the last are scored too, as page 0 or any, and not written)
+      const uint16_t* p = a.bounds + ((int64_t)at * a.Hk + kv) * 2 * SEL_D + e0;
+      lw = load16(p);
+      hw = load16(p + SEL_D);
+      entry = next < end ? table[next] : 0;
+    };
+    fetch(page + step);
     double up[G][8], down[G][8];
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       float f[8];
-      const int h = h0 + g < group ? h0 + g : group - 1;  // (past the last head: it once more)
-      unpack8(load16(a.q.p + b * a.q.sl + (int64_t)(kv * group + h) * a.q.sh + e0), f);
+      unpack8(raw[g], f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {  // (a NaN stays in one of the two)
         up[g][j] = f[j] < 0.0f ? 0.0 : (double)f[j];
         down[g][j] = f[j] < 0.0f ? (double)f[j] : 0.0;
       }
     }
-    // the next pages' bounds are fetched while these are summed
-    int page = from + 4 * wave + sub;
-    u32x4 lw, hw;
-    bool bad = false;
-    auto fetch = [&](int i) {
-      // (pages past the last are scored too, as page 0, and not written)
-      int at = i < end ? page_at(table, a.pt.width, a.pt.shift, a.pt.pages, (int64_t)i << a.pt.shift) : 0;
-      bad = at < 0;
-      at = bad ? 0 : at;
-      const uint16_t* p = a.bounds + ((int64_t)at * a.Hk + kv) * 2 * SEL_D + e0;
-      lw = load16(p);
-      hw = load16(p + SEL_D);
-    };
-    fetch(page);
-    for (; __any(page < end); page += 4 * waves) {
+    for (; __any(page < end); page += step) {
       float lo[8], hi[8];
       unpack8(lw, lo);
       unpack8(hw, hi);
       const bool is_bad = bad;
-      fetch(page + 4 * waves);
+      fetch(page + 2 * step);
       double x[G];
 #pragma unroll
       for (int g = 0; g < G; ++g) x[g] = 0.0;
@@ -109,18 +123,19 @@ __device__ __forceinline__ void score_pages(const SelectArgs& a, int b, int kv, 
 #pragma unroll
         for (int g = 0; g < G; ++g) x[g] = __builtin_fma(down[g][j], l, __builtin_fma(up[g][j], h, x[g]));
       }
-      double most = -INFINITY;
+      double best = -INFINITY;
       bool nan = is_bad;
 #pragma unroll
       for (int g = 0; g < G; ++g) {
         const double y = row_sum(x[g]);
         nan |= y != y;
-        most = fmax(most, y);
+        best = fmax(best, y);
       }
-      const uint64_t best = nan ? INF_IMAGE : image(most);
-      if (page < end && (lane & 15) == 0) put(page, best, h0 == 0);
+      const uint64_t s = nan ? INF_IMAGE : image(best);
+      if (page < end && (lane & 15) == 0) put(page, s, h0 == 0);
     }
   }
+  return n;
 }
 
 template <int G>
@@ -131,13 +146,10 @@ __global__ void __launch_bounds__(256) select_score_kernel(const SelectArgs a) {
   // of up to 98 pages x 40/8 heads 22.4 to 18.5 us, 16 of 1463 x 64/8 48.1 to 43.8)
   const int kv = blockIdx.x % (uint32_t)a.Hk, b = unit / chunks, chunk = (unit % chunks + (uint32_t)b) % chunks;
   uint64_t* const score = a.score + ((int64_t)b * a.Hk + kv) * a.pt.width;
-  const int n = pages_of(a, b);
-  if (n <= a.count || chunk * a.chunk >= n) return;  // (all pages are chosen, or none is here)
-  score_pages<G>(a, b, kv, chunk * a.chunk, min(n, (chunk + 1) * a.chunk), lane, wave, 4,
-                 [&](int page, uint64_t best, bool first) {
-                   if (!first && score[page] > best) best = score[page];
-                   score[page] = best;
-                 });
+  score_pages<G>(a, b, kv, chunk * a.chunk, a.chunk, lane, wave, 4, [&](int page, uint64_t best, bool first) {
+    if (!first && score[page] > best) best = score[page];
+    score[page] = best;
+  });
 }
 
 // The choice among n > count pages by their scores, by T threads.
@@ -347,12 +359,11 @@ __global__ void __launch_bounds__(ONE_T) select_one_kernel(const SelectArgs a) {
   __shared__ uint64_t score[ONE_PAGES];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kv = blockIdx.x % (uint32_t)a.Hk, b = blockIdx.x / (uint32_t)a.Hk;
-  const int n = pages_of(a, b);
   int32_t* const sel = a.sel + ((int64_t)b * a.Hk + kv) * a.count;
-  if (chose_all<ONE_T>(a, n, sel)) return;
-  score_pages<G>(a, b, kv, 0, n, lane, wave, ONE_T / 64, [&](int page, uint64_t best, bool first) {
+  const int n = score_pages<G>(a, b, kv, 0, ONE_PAGES, lane, wave, ONE_T / 64, [&](int page, uint64_t best, bool first) {
     score[page] = first || best > score[page] ? best : score[page];
   });
+  if (chose_all<ONE_T>(a, n, sel)) return;
   __syncthreads();
   choose<ONE_T>(a, n, score, sel);
 }
