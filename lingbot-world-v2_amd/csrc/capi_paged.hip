@@ -86,14 +86,14 @@ int fill_paged(const lbw_attention_paged_params* p, PagedAttnArgs* a) {
     a->p_len = p->prefix_len;
     a->p_max = p->prefix_keys;
   }
-  // (128 pieces a sequence at most)
-  if ((int64_t)p->batch * p->q_heads * 128 > kMaxWorkgroups)
+  // (a workgroup each in the join)
+  if ((int64_t)p->batch * p->q_heads > kMaxWorkgroups)
     return fail(LBW_ERR_UNSUPPORTED, "batch %d x %d heads", p->batch, p->q_heads);
   plan_paged(a, p->num_splits, num_cus());
-  // (a prefix of many small pages has more: its pieces' page lists fit a workgroup's memory)
+  // (many for a prefix of many small pages: its pieces' page lists fit a workgroup's memory)
   if (workgroups(*a) > kMaxWorkgroups)
-    return fail(LBW_ERR_UNSUPPORTED, "batch %d x %d heads off a prefix of %lld keys in pages of %d", p->batch, p->q_heads,
-                (long long)p->prefix_keys, p->cache.page_size);
+    return fail(LBW_ERR_UNSUPPORTED, "batch %d x %d heads, num_splits %d, off a prefix of %lld keys in pages of %d", p->batch,
+                p->q_heads, p->num_splits, (long long)p->prefix_keys, p->cache.page_size);
   return LBW_OK;
 }
 size_t paged_bytes(const PagedAttnArgs& a) {

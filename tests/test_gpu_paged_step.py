@@ -414,3 +414,27 @@ def test_tensors_on_two_devices_are_refused():
                {"selected": torch.zeros(3, HK, 2, dtype=torch.int32)}, {"out": q.cpu()}):
         with pytest.raises((RuntimeError, ValueError)):
             lbw_amd.attention_paged(q, c, s["table"], s["lens"], **kw)
+
+
+def test_thousands_of_sequences_are_as_a_few_of_them():
+    import lbw_amd
+    B, hq, hk, width = 4500, 40, 8, 3
+    g = torch.Generator(device="cuda").manual_seed(80)
+    k, v = (torch.randn(700, PAGE, hk, D, generator=g, device="cuda").to(BF) for _ in range(2))
+    cache = lbw_amd.PagedKV(k, v, torch.stack((k.amin(1), k.amax(1)), 2).contiguous())
+    table = torch.randint(0, 700, (B, width), generator=g, device="cuda", dtype=torch.int32)
+    lens = torch.randint(0, width * PAGE + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+    q = torch.randn(B, hq, D, generator=g, device="cuda").to(BF)
+    prefix = table[0]
+    sel = lbw_amd.paged_select(q, cache, table, lens, 2)
+    some = torch.randint(0, B, (60,), generator=g, device="cuda").tolist() + [0, B - 1]
+    few = (q[some].contiguous(), cache, table[some].contiguous(), lens[some].contiguous())
+    assert torch.equal(lbw_amd.paged_select(few[0], cache, few[2], few[3], 2), sel[some])
+    for kw, kw_few in (({}, {}), ({"selected": sel}, {"selected": sel[some].contiguous()}),
+                       ({"prefix_table": prefix, "prefix_len": 40},) * 2):
+        got = lbw_amd.attention_paged(q, cache, table, lens, num_splits=1, **kw)
+        want, allow = P.attention(few[0], k, v, few[2], few[3].tolist(), SCALE, kw.get("prefix_table"), kw.get("prefix_len", 0),
+                                  kw_few.get("selected"))
+        R.assert_within(str(list(kw)), got[some], want, allow)
+        again = lbw_amd.attention_paged(q, cache, table, lens, **kw)
+        R.assert_within(str(list(kw)), again[some], want, allow)

@@ -153,6 +153,12 @@ def test_prefixes_of_more_pieces_than_a_launch_has():
     assert lib.lbw_attention_paged(ctypes.byref(p), None, 0, None) == 2
     assert "prefix of 2147483392 keys in pages of 16" in lib.lbw_last_error().decode()
     assert lib.lbw_attention_paged_workspace_size(ctypes.byref(_attention(batch=100, **long))) > 100 * 8 * 32800 * 520
+    # as many as a launch has, and more
+    big = {"q_heads": 40, "k_heads": 8, "batch": 400000}
+    assert lib.lbw_attention_paged_workspace_size(ctypes.byref(_attention(num_splits=1, **big))) == 0
+    assert lib.lbw_attention_paged(ctypes.byref(_attention(num_splits=128, selected=ADDR, n_selected=1, **big)), None, 0,
+                                   None) == 2
+    assert "num_splits 128" in lib.lbw_last_error().decode()
 
 
 def test_null_params_and_empty_calls():
