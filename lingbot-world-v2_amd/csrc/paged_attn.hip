@@ -582,7 +582,11 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 // (128 rows at a time), 10 and 34 163, 21 and 64 185, 5 and 17 205; 26 of 1500 off 14040 x 40/8 16 and 32 40.4, 8 and 16 45.8;
 // 30 of 1500 off 10000 x 16/2, 32 and 64 23.5, 64 and 128 27.6. Whole sequences: 16 of 200 off 6000 x 12/4, 24 pieces (one
 // workgroup a CU) 14.4, 48 16.6; off 46800 20 35.9, 48 39.6; 16 of 200 off 14040 x 40/8 (128 sequences x heads), 4 pieces 47.1,
-// 16 (two a CU) 26.6. Pieces of 4 tiles or more, of 6: 4 of 40 off 1560 x 12/4 12.3 / 13.3, one of 3000 x 40/8 11.7 / 13.0.
+// 16 (two a CU) 26.6. Ten of
+// 472 off 4254 x 40/40 (400), 2 pieces 49.1, 6 36.5; 60 of 300 off 10000 x 12/12 (720), one 122.7, 21 44.8; 128 rows at a time: 29 of
+// 102 off 9496 x 40/8 (232), 17 pieces 30.5, 24 38.6; 64 of 200 off 14040 (512), 10 58.3, 16 53.6. Pieces of 4 tiles or more, of
+// 6: 4 of 40 off 1560 x 12/4 12.3 / 13.3, one of 3000 x 40/8 11.7 / 13.0; of 128 rows, of 4 or 8: 41 of 800 off 3366 x 12/4 25.3 /
+// 20.3, 64 of 500 off 6000 30.8 / 25.9.
 // 32 / 128 query rows at a time: 8 of 1500 off 14040 x 40/8 (40 rows) 30.9 / 35.6, 20 (100) 42.5 / 46.5, 40 (200) 65.6 /
 // 54.4; 46800, 1000 own x 12/4, 24 rows 34.5 / 36.6, 60 rows 44.0 / 43.0, 78 rows 49.3 / 51.8, 99 rows 58.5 / 54.8.
 void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
@@ -615,9 +619,10 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
     const int64_t of_prefix = p_tiles * each, of_own = own_tiles * seqs * (wide ? 7 : 10) / 10;
     int64_t places;
     if (whole) {
-      // a workgroup a CU, whole sequences included; two where those would leave the prefix less than 0.7 of the CUs
+      // a workgroup a CU, whole sequences included; two where those would leave the prefix less than 0.7 of the CUs; one a
+      // CU (or three for two) for the prefix alone where they fill the chip by themselves
       const int64_t one = std::max<int64_t>(0, cus - seqs) / each * each;
-      places = !wide && 10 * one >= 7 * cus ? one : std::max<int64_t>(2 * cus - seqs, wide ? 3 * cus / 2 : 0);
+      places = !wide && 10 * one >= 7 * cus ? one : std::max<int64_t>(2 * cus - seqs, wide && seqs > cus ? 3 * cus / 2 : cus);
     } else {
       // a workgroup a CU, shared out by their tiles; two where each still gets 16 tiles (of 128 rows, which alone on
       // a CU wait most of the time) or 32
@@ -625,7 +630,7 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
       places = all * of_prefix / (of_prefix + of_own) + (wide ? each / 2 : 0);
       own_places = all - std::max<int64_t>(1, places / each) * each;
     }
-    a->p_splits = cut(p_tiles, places, each, 4);
+    a->p_splits = cut(p_tiles, places, each, wide ? 8 : 4);
     if (num_splits > 0) a->p_splits = num_splits;
     // (a piece's table entries fit their place: whole tiles of 64 keys, an entry more where a piece ends in a page)
     const int64_t tiles = (a->p_max + BN - 1) / BN, most = ((int64_t)(P_LIST - 1) << a->pt.shift) / BN;
