@@ -21,9 +21,9 @@ constexpr int AP_WAVES = 4;
 constexpr int KEY_HEADS = 2;   // heads of a workgroup that looks after a page's keys, at most
 constexpr int EDGE_WAVES = 8;  // of the bounds kernel
 // Pages up to this size get their keys and bounds in the kernel of the tokens' q and v, larger ones, whose tokens would
-// follow one another too long, their bounds by a second kernel. Two kernels / one, x 40/8 heads: pages of 64, 100 tokens
-// 13.4 / 10.3 us, 500 14.8 / 16.4, 1000 16.9 / 16.7, 4680 38.5 / 37.1, 9841 69.1 / 60.4; of 128 13.4 / 13.5, 15.9 / 23.4, 18.1 / 27.1,
-// 41.1 / 46.6, 73.4 / 71.6; of 256 13.0 / 13.2, 18.0 / 33.7, 20.2 / 39.7, 41.9 / 66.3, 72.8 / 88.5.
+// follow one another too long, their bounds by a second kernel. Two kernels / one, x 40/8 heads, pages of 64: 100 tokens
+// 12.5 / 10.1 us, 500 12.5 / 11.4, 2000 17.7 / 14.8, 4680 35.6 / 35.0, 9841 67.5 / 60.1; of 128 11.9 / 13.2, 12.9 / 17.3, 18.9 / 20.1,
+// 36.6 / 38.7, 67.0 / 62.3; of 256 11.8 / 13.2, 14.4 / 29.4, 20.5 / 31.8, 37.6 / 48.7, 67.6 / 73.2.
 constexpr int FUSED_PAGE = 64;
 
 // Where a token goes: its sequence (-1: none), row and page (-1: nowhere).
@@ -431,26 +431,30 @@ hipError_t run(AppendArgs a, hipStream_t stream) {
   if (a.bounds == nullptr) return launch<LPH, ROWS>(a, stream);
   const int page = 1 << a.pt.shift;
   // tokens that a workgroup looks for pages in: as many as a page has, so that it finds one, or fewer where sequences
-  // are shorter or workgroups few
-  auto block_for = [&](int wgs) {
+  // are shorter or workgroups few (half the CUs; those that find none cost more than they gain: four a CU / two / one / a
+  // half, 250 tokens x 40/8 heads in pages of 64 13.0 / 13.4 / 10.7 / 9.9 us, 1000 16.7 / 15.4 / 12.9 / 12.3, x 40/40 17.5 / 17.6 /
+  // 17.6 / 17.6, 2000 x 40/40 in pages of 128, two kernels, 35.4 / 36.8 / 34.1 / 34.5, five thousand blocks 61.0)
+  auto block_for = [&](int chunks) {
     int n = 1;
-    while (n < page && (int64_t)2 * n * a.B <= a.T && a.T / n > wgs) n *= 2;
+    while (n < page && (int64_t)2 * n * a.B <= a.T && (int64_t)a.T / n * chunks > num_cus() / 2) n *= 2;
     return n;
   };
   if (page <= FUSED_PAGE) {
-    a.page_block = block_for(256);
-    const int blocks = (a.T + a.page_block - 1) / a.page_block, chunks = (a.Hk + KEY_HEADS - 1) / KEY_HEADS;
-    // a head a workgroup, not two, while pages are few: 120 tokens x 40/8 heads in pages of 64 13.6 to 10.7 us, 500 19.5 to
-    // 16.3, 2000 (132 workgroups of two) 30.7 to 27.9, but 2500 25.9 to 31.0
+    const int chunks = (a.Hk + KEY_HEADS - 1) / KEY_HEADS;
+    a.page_block = block_for(chunks);
+    const int blocks = (a.T + a.page_block - 1) / a.page_block;
+    // a head a workgroup, not two, while pages are few: two / one, in pages of 64, 500 tokens x 40/8 heads (32 workgroups of
+    // two) 13.5 / 11.4 us, 2000 (128) 16.2 / 14.8, 2500 (160) 16.6 / 16.9, 3500 (220) 21.2 / 22.2, 2000 x 12/12 (192) 14.4 / 12.9
     const int64_t pages = (a.T >> a.pt.shift) + a.B;
-    a.page_heads = pages * chunks <= num_cus() / 2 ? 1 : KEY_HEADS;
+    a.page_heads = pages * chunks <= 3 * num_cus() / 4 ? 1 : KEY_HEADS;
     a.page_wgs = blocks * ((a.Hk + a.page_heads - 1) / a.page_heads);
     return launch<LPH, PAGES>(a, stream);
   }
   const hipError_t e = launch<LPH, ROWS>(a, stream);
   if (e != hipSuccess) return e;
-  a.page_block = block_for(512);
-  const dim3 blocks((a.T + a.page_block - 1) / a.page_block, (a.Hk + HPW - 1) / HPW);
+  const int chunks = (a.Hk + HPW - 1) / HPW;
+  a.page_block = block_for(chunks);
+  const dim3 blocks((a.T + a.page_block - 1) / a.page_block, chunks);
   hipLaunchKernelGGL(append_bounds_kernel<LPH>, blocks, dim3(EDGE_WAVES * 64), 0, stream, a);
   return hipGetLastError();
 }
