@@ -49,8 +49,8 @@ struct AppendArgs {
   uint16_t* bounds;           // [pages][Hk][2][D] smallest and largest values, or null
   float q_scale, k_scale;
   int parts;                  // waves that share one token's heads
-  int page_wgs, page_block;   // workgroups that look after pages' new keys, the tokens of each
-  int page_heads;             // and the heads
+  int page_wgs, page_heads;   // workgroups that look after pages' new keys, and the heads of each
+  int page_slots;             // they are told apart by pages (else by tokens)
 };
 hipError_t launch_append(const AppendArgs& a, int D, hipStream_t stream);
 

@@ -10,6 +10,8 @@
 // makes the page's bounds, beside the tokens' q and v. 4680 + 3600 + 1561 tokens x 40/8 heads of 128, normed, pages of 64,
 // from memory 60 us (4.7 TB/s; a large copy reaches 4.9), inputs in the last cache 46; one token 4.3 us, most of it the launch.
 
+#include <algorithm>
+
 #include "capi_util.h"
 #include "head_rows.h"
 #include "paged.h"
@@ -71,6 +73,61 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int t, int lane) 
   w.page = __builtin_amdgcn_readfirstlane(
       page_at(a.pt.p + (int64_t)w.b * a.pt.sb, a.pt.width, a.pt.shift, a.pt.pages, w.row));
   return w;
+}
+
+// A page's new tokens: t .. t + n - 1, rows row .. of their sequence, from row `in` of page `page` on. Its owner is a
+// workgroup: number `slot` of those that a.page_slots tells from one another --
+//   tokens: that of the page's first new token;
+//   pages: sequence b has those from starts[b] / P + 2 b on, P tokens a page, as many as its tokens can touch pages, so
+//   that no sequence's lengths are wanted to find another's.
+// False: no page is here (or the sequence's table does not hold it).
+struct Fresh {
+  int t, n, in, page;
+  int64_t row;
+};
+__device__ __forceinline__ bool fresh_page(const AppendArgs& a, int64_t slot, int lane, Fresh& f) {
+  const int shift = a.pt.shift, mask = (1 << shift) - 1;
+  if (a.page_slots == 0) {
+    const Place w = place_of(a, (int)slot, lane);
+    if (w.b < 0 || w.page < 0) return false;
+    f = {(int)slot, 0, (int)(w.row & mask), w.page, w.row};
+    if (f.in != 0 && f.t != w.start) return false;
+    f.n = w.end - f.t < mask + 1 - f.in ? w.end - f.t : mask + 1 - f.in;
+    return true;
+  }
+  // the last sequence whose first slot is this one or before
+  auto at = [&](int b) { return (int64_t)(a.starts[b] >> shift) + 2 * (int64_t)b; };
+  int base = 0, left = a.B;
+  while (left > 64) {
+    const int step = (left + 63) >> 6, off = lane * step;
+    const uint64_t past = __ballot(off < left && at(base + off) <= slot);
+    if (past == 0) return false;
+    const int c = (63 - __clzll((unsigned long long)past)) * step;
+    base += c;
+    left = left - c < step ? left - c : step;
+  }
+  int s = 0, e = 0, l = 0;
+  const bool mine = lane < left;
+  if (mine) {
+    s = a.starts[base + lane];
+    e = a.starts[base + lane + 1];
+    l = a.lens[base + lane];
+  }
+  const uint64_t past = __ballot(mine && (int64_t)(s >> shift) + 2 * (int64_t)(base + lane) <= slot);
+  if (past == 0) return false;
+  const int c = 63 - __clzll((unsigned long long)past), b = base + c;
+  const int start = __builtin_amdgcn_readlane(s, c), stop = __builtin_amdgcn_readlane(e, c);
+  const int first = start > 0 ? start : 0, end = stop < a.T ? stop : a.T;  // (the tokens that there are)
+  if (first >= end) return false;
+  const int64_t row0 = (int64_t)__builtin_amdgcn_readlane(l, c) + ((int64_t)first - start);
+  const int64_t j = slot - ((int64_t)(start >> shift) + 2 * (int64_t)b);
+  const int64_t row = j == 0 ? row0 : ((row0 >> shift) + j) * (mask + 1), t = first + (row - row0);
+  if (t >= end) return false;
+  f = {(int)t, 0, (int)(row & mask), -1, row};
+  f.n = end - f.t < mask + 1 - f.in ? end - f.t : mask + 1 - f.in;
+  f.page = __builtin_amdgcn_readfirstlane(
+      page_at(a.pt.p + (int64_t)b * a.pt.sb, a.pt.width, shift, a.pt.pages, row));
+  return f.page >= 0;
 }
 
 // The smaller and the larger of two values, NaN if one of them is.
@@ -188,103 +245,84 @@ __device__ __forceinline__ void load_rotation(const AppendArgs& a, int t, int64_
   }
 }
 
-// The tokens of block `block` whose pages this workgroup looks after: those that are the first new ones of their page.
-// The page's new keys are turned and put there, heads h0 .., and its bounds made of them and, where the page was
-// begun before, the old ones: every page has one owner, no atomics. A wave takes 64 / LPH tokens at a time, a head
-// after the other, so that a token's angles are read once; the tokens' smallest and largest values meet by shuffles,
-// the waves' in LDS.
+// The page's new keys, turned and put there, heads h0 .., and its bounds, made of them and, where the page was begun
+// before, the old ones: every page has one owner, no atomics. A wave takes 64 / LPH tokens at a time, a head after the
+// other, so that a token's angles are read once; the tokens' smallest and largest values meet by shuffles, the waves'
+// in LDS.
 template <int LPH, bool INTER>
-__device__ __forceinline__ void append_pages(const AppendArgs& a, int64_t block, int chunk, int lane, int wave) {
+__device__ __forceinline__ void append_page(const AppendArgs& a, const Fresh& f, int chunk, int lane, int wave) {
   constexpr int TPW = 64 / LPH, D = 8 * LPH, KH = KEY_HEADS;
   __shared__ u32x4 red[AP_WAVES][KH][2][LPH];  // (bf16: what was rounded once stays)
   const int e0 = 8 * (lane % LPH), sub = lane / LPH, h0 = chunk * a.page_heads;
   const int h1 = h0 + a.page_heads < a.Hk ? h0 + a.page_heads : a.Hk;  // heads h0 .. h1 - 1
-  const int64_t t0 = block * a.page_block;
-  const int t1 = (int)(t0 + a.page_block < a.T ? t0 + a.page_block : a.T);
-  const int mask = (1 << a.pt.shift) - 1;
   float wt[8];
   load_weights(a.wk, a.w32, e0, wt);
-  for (int t = (int)t0; t < t1;) {
-    const Place w = place_of(a, t, lane);
-    if (w.b < 0) {
-      ++t;
-      continue;
-    }
-    const int in = (int)(w.row & mask);
-    const int n = w.end - t < mask + 1 - in ? w.end - t : mask + 1 - in;  // this page's tokens from t on
-    if (w.page < 0 || (in != 0 && t != w.start)) {  // nowhere, or not its first new token
-      t += n;
-      continue;
-    }
-    const int turns = (n + TPW - 1) / TPW;
-    for (int g = wave; g < turns; g += AP_WAVES) {
-      const int mine = g * TPW + sub, tok = mine < n ? mine : n - 1;  // (past the end: the last one once more)
-      u32x4 x[KH];
-      const uint16_t* const src = a.k.p + (int64_t)(t + tok) * a.k.sl + e0;
+  const int turns = (f.n + TPW - 1) / TPW;
+  for (int g = wave; g < turns; g += AP_WAVES) {
+    const int mine = g * TPW + sub, tok = mine < f.n ? mine : f.n - 1;  // (past the end: the last one once more)
+    u32x4 x[KH];
+    const uint16_t* const src = a.k.p + (int64_t)(f.t + tok) * a.k.sl + e0;
 #pragma unroll
-      for (int i = 0; i < KH; ++i) x[i] = load16(src + (h0 + i < h1 ? h0 + i : h0) * a.k.sh);
-      Turn rot;
-      load_rotation<INTER>(a, t + tok, w.row + tok, e0, lane, rot);
-      uint16_t* const dst = a.kp.p + w.page * a.kp.sp + (in + tok) * a.kp.sl + e0;
+    for (int i = 0; i < KH; ++i) x[i] = load16(src + (h0 + i < h1 ? h0 + i : h0) * a.k.sh);
+    Turn rot;
+    load_rotation<INTER>(a, f.t + tok, f.row + tok, e0, lane, rot);
+    uint16_t* const dst = a.kp.p + f.page * a.kp.sp + (f.in + tok) * a.kp.sl + e0;
 #pragma unroll
-      for (int i = 0; i < KH; ++i) {
-        if (h0 + i >= h1) break;
-        const u32x4 out = turn_chunk<LPH, INTER>(a, x[i], wt, a.k_scale, rot);
-        if (mine < n) put16<true>(dst + (h0 + i) * a.kp.sh, out);
-        float lo[8], hi[8], y[8];
-        unpack8(out, lo);
-        unpack8(out, hi);
-        u32x4 pl = out, ph = out;
+    for (int i = 0; i < KH; ++i) {
+      if (h0 + i >= h1) break;
+      const u32x4 out = turn_chunk<LPH, INTER>(a, x[i], wt, a.k_scale, rot);
+      if (mine < f.n) put16<true>(dst + (h0 + i) * a.kp.sh, out);
+      float lo[8], hi[8], y[8];
+      unpack8(out, lo);
+      unpack8(out, hi);
+      u32x4 pl = out, ph = out;
 #pragma unroll
-        for (int o = LPH; o < 64; o <<= 1) {
-          u32x4 ql, qh;
+      for (int o = LPH; o < 64; o <<= 1) {
+        u32x4 ql, qh;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) ql[e] = __shfl_xor(pl[e], o);
-          qh = ql;
-          if (o > LPH) {
+        for (int e = 0; e < 4; ++e) ql[e] = __shfl_xor(pl[e], o);
+        qh = ql;
+        if (o > LPH) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) qh[e] = __shfl_xor(ph[e], o);
-          }
-          unpack8(ql, y);
+          for (int e = 0; e < 4; ++e) qh[e] = __shfl_xor(ph[e], o);
+        }
+        unpack8(ql, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], y[j]);
+        unpack8(qh, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) hi[j] = max_nan(hi[j], y[j]);
+        pl = pack8(lo);
+        ph = pack8(hi);
+      }
+      if (lane < LPH) {
+        if (g != wave) {
+          unpack8(red[wave][i][0][lane], y);
 #pragma unroll
           for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], y[j]);
-          unpack8(qh, y);
+          unpack8(red[wave][i][1][lane], y);
 #pragma unroll
           for (int j = 0; j < 8; ++j) hi[j] = max_nan(hi[j], y[j]);
-          pl = pack8(lo);
-          ph = pack8(hi);
         }
-        if (lane < LPH) {
-          if (g != wave) {
-            unpack8(red[wave][i][0][lane], y);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) lo[j] = min_nan(lo[j], y[j]);
-            unpack8(red[wave][i][1][lane], y);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) hi[j] = max_nan(hi[j], y[j]);
-          }
-          red[wave][i][0][lane] = pack8(lo);
-          red[wave][i][1][lane] = pack8(hi);
-        }
+        red[wave][i][0][lane] = pack8(lo);
+        red[wave][i][1][lane] = pack8(hi);
       }
     }
-    __syncthreads();
-    const int used = turns < AP_WAVES ? turns : AP_WAVES;
-    for (int x = threadIdx.x; x < KH * 2 * LPH; x += AP_WAVES * 64) {
-      const int c = x % LPH, edge = x / LPH % 2, i = x / (2 * LPH);
-      if (h0 + i >= h1) break;
-      uint16_t* const p = a.bounds + (((int64_t)w.page * a.Hk + h0 + i) * 2 + edge) * D + 8 * c;
-      float m[8], y[8];
-      unpack8(in != 0 ? load16(p) : red[0][i][edge][c], m);
-      for (int v = 0; v < used; ++v) {
-        unpack8(red[v][i][edge][c], y);
+  }
+  __syncthreads();
+  const int used = turns < AP_WAVES ? turns : AP_WAVES;
+  for (int x = threadIdx.x; x < KH * 2 * LPH; x += AP_WAVES * 64) {
+    const int c = x % LPH, edge = x / LPH % 2, i = x / (2 * LPH);
+    if (h0 + i >= h1) break;
+    uint16_t* const p = a.bounds + (((int64_t)f.page * a.Hk + h0 + i) * 2 + edge) * D + 8 * c;
+    float m[8], y[8];
+    unpack8(f.in != 0 ? load16(p) : red[0][i][edge][c], m);
+    for (int v = 0; v < used; ++v) {
+      unpack8(red[v][i][edge][c], y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m[j] = edge == 0 ? min_nan(m[j], y[j]) : max_nan(m[j], y[j]);
-      }
-      *reinterpret_cast<u32x4*>(p) = pack8(m);
+      for (int j = 0; j < 8; ++j) m[j] = edge == 0 ? min_nan(m[j], y[j]) : max_nan(m[j], y[j]);
     }
-    __syncthreads();  // the waves' results are read
-    t += n;
+    *reinterpret_cast<u32x4*>(p) = pack8(m);
   }
 }
 
@@ -299,7 +337,8 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs 
   if constexpr (KEYS == PAGES) {
     if (wg < (uint32_t)a.page_wgs) {
       const uint32_t chunks = (uint32_t)((a.Hk + a.page_heads - 1) / a.page_heads);
-      append_pages<LPH, INTER>(a, wg / chunks, wg % chunks, lane, wave);
+      Fresh f;
+      if (fresh_page(a, wg / chunks, lane, f)) append_page<LPH, INTER>(a, f, wg % chunks, lane, wave);
       return;
     }
     wg -= a.page_wgs;
@@ -342,10 +381,9 @@ __global__ void __launch_bounds__(AP_WAVES * 64) append_kernel(const AppendArgs 
   copy_rows<LPH, KEYS != TOKEN>(v, a.v.sh, vp, a.vp.sh, a.Hk, first(KEYS == PAGES ? cq : cq + ck), a.parts, e0, hsub);
 }
 
-// Bounds of the pages that several tokens were put into: blockIdx.x counts blocks of a.page_block tokens, blockIdx.y
-// chunks of heads. The workgroup whose block holds a page's first new token reads the page's new keys back (from
-// cache: they were written just before), its waves in turn, and joins them with the old bounds where the page was
-// begun before.
+// Bounds of the pages that several tokens were put into: a workgroup a page (blockIdx.x: fresh_page's slot) and chunk of
+// heads (blockIdx.y) reads the page's new keys back (from cache: they were written just before), its waves in turn, and
+// joins them with the old bounds where the page was begun before.
 template <int LPH>
 __global__ void __launch_bounds__(EDGE_WAVES * 64) append_bounds_kernel(const AppendArgs a) {
   constexpr int HPW = 64 / LPH, D = 8 * LPH, U = 8;
@@ -353,64 +391,48 @@ __global__ void __launch_bounds__(EDGE_WAVES * 64) append_bounds_kernel(const Ap
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int e0 = 8 * (lane % LPH), head = (int)blockIdx.y * HPW + lane / LPH;
   const int hh = head < a.Hk ? head : a.Hk - 1;  // (lanes past the last head do its work again and write nothing)
-  const int64_t t0 = (int64_t)blockIdx.x * a.page_block;
-  const int t1 = (int)(t0 + a.page_block < a.T ? t0 + a.page_block : a.T);
-  const int mask = (1 << a.pt.shift) - 1;
-  for (int t = (int)t0; t < t1;) {
-    const Place w = place_of(a, t, lane);
-    if (w.b < 0) {
-      ++t;
-      continue;
+  Fresh w;
+  if (!fresh_page(a, blockIdx.x, lane, w)) return;
+  const uint16_t* const rows = a.kp.p + w.page * a.kp.sp + w.in * a.kp.sl + hh * a.kp.sh + e0;
+  uint16_t* const edge = a.bounds + ((int64_t)w.page * a.Hk + hh) * 2 * D + (wave & 1) * D + e0;
+  const u32x4 before = load16(edge);
+  float lo[8], hi[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    lo[j] = INFINITY;
+    hi[j] = -INFINITY;
+  }
+  for (int r = wave; r < w.n; r += EDGE_WAVES * U) {
+    u32x4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {  // (past the end: the last row once more)
+      const int rr = r + u * EDGE_WAVES < w.n ? r + u * EDGE_WAVES : w.n - 1;
+      x[u] = load16(rows + (int64_t)rr * a.kp.sl);
     }
-    const int in = (int)(w.row & mask);
-    const int n = w.end - t < mask + 1 - in ? w.end - t : mask + 1 - in;  // this page's tokens from t on
-    if (w.page < 0 || (in != 0 && t != w.start)) {  // nowhere, or not its first new token
-      t += n;
-      continue;
-    }
-    const uint16_t* const rows = a.kp.p + w.page * a.kp.sp + in * a.kp.sl + hh * a.kp.sh + e0;
-    uint16_t* const edge = a.bounds + ((int64_t)w.page * a.Hk + hh) * 2 * D + (wave & 1) * D + e0;
-    const u32x4 before = load16(edge);
-    float lo[8], hi[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      lo[j] = INFINITY;
-      hi[j] = -INFINITY;
-    }
-    for (int r = wave; r < n; r += EDGE_WAVES * U) {
-      u32x4 x[U];
+    for (int u = 0; u < U; ++u) {
+      float f[8];
+      unpack8(x[u], f);
 #pragma unroll
-      for (int u = 0; u < U; ++u) {  // (past the end: the last row once more)
-        const int rr = r + u * EDGE_WAVES < n ? r + u * EDGE_WAVES : n - 1;
-        x[u] = load16(rows + (int64_t)rr * a.kp.sl);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float f[8];
-        unpack8(x[u], f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          lo[j] = min_nan(lo[j], f[j]);
-          hi[j] = max_nan(hi[j], f[j]);
-        }
+      for (int j = 0; j < 8; ++j) {
+        lo[j] = min_nan(lo[j], f[j]);
+        hi[j] = max_nan(hi[j], f[j]);
       }
     }
-    __syncthreads();  // the last page's results are read
-    red[0][wave][lane] = pack8(lo);
-    red[1][wave][lane] = pack8(hi);
-    __syncthreads();
-    if (wave < 2 && head < a.Hk) {  // one wave for the smallest values, one for the largest
-      float m[8], y[8];
-      unpack8(in != 0 ? before : red[wave][0][lane], m);
+  }
+  red[0][wave][lane] = pack8(lo);
+  red[1][wave][lane] = pack8(hi);
+  __syncthreads();
+  if (wave < 2 && head < a.Hk) {  // one wave for the smallest values, one for the largest
+    float m[8], y[8];
+    unpack8(w.in != 0 ? before : red[wave][0][lane], m);
 #pragma unroll
-      for (int x = 0; x < EDGE_WAVES; ++x) {
-        unpack8(red[wave][x][lane], y);
+    for (int x = 0; x < EDGE_WAVES; ++x) {
+      unpack8(red[wave][x][lane], y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m[j] = wave == 0 ? min_nan(m[j], y[j]) : max_nan(m[j], y[j]);
-      }
-      *reinterpret_cast<u32x4*>(edge) = pack8(m);
+      for (int j = 0; j < 8; ++j) m[j] = wave == 0 ? min_nan(m[j], y[j]) : max_nan(m[j], y[j]);
     }
-    t += n;
+    *reinterpret_cast<u32x4*>(edge) = pack8(m);
   }
 }
 
@@ -430,32 +452,24 @@ hipError_t run(AppendArgs a, hipStream_t stream) {
   if (a.starts == nullptr) return launch<LPH, TOKEN>(a, stream);
   if (a.bounds == nullptr) return launch<LPH, ROWS>(a, stream);
   const int page = 1 << a.pt.shift;
-  // tokens that a workgroup looks for pages in: as many as a page has, so that it finds one, or fewer where sequences
-  // are shorter or workgroups few (half the CUs; those that find none cost more than they gain: four a CU / two / one / a
-  // half, 250 tokens x 40/8 heads in pages of 64 13.0 / 13.4 / 10.7 / 9.9 us, 1000 16.7 / 15.4 / 12.9 / 12.3, x 40/40 17.5 / 17.6 /
-  // 17.6 / 17.6, 2000 x 40/40 in pages of 128, two kernels, 35.4 / 36.8 / 34.1 / 34.5, five thousand blocks 61.0)
-  auto block_for = [&](int chunks) {
-    int n = 1;
-    while (n < page && (int64_t)2 * n * a.B <= a.T && (int64_t)a.T / n * chunks > num_cus() / 2) n *= 2;
-    return n;
-  };
+  // a workgroup for every page that the sequences can touch, or every token where that is less (blocks of tokens searched
+  // for pages, four times as many workgroups / half as many as CUs / a workgroup a page: 1000 tokens x 40/8 heads in pages of
+  // 64 16.8 / 12.5 / 12.7 us, x 40/40 25.1 / 17.7 / 17.1, eight times 400 23.4 / 33.8 / 25.1, 400 + 4 x 40 + 3 x 4 x 12/12 in pages of 32
+  // 12.4 / 18.7 / 10.8; 2000 x 40/40 in pages of 128, two kernels, 61.3 / 34.7 / 34.5)
+  const int64_t slots = (a.T >> a.pt.shift) + 2 * (int64_t)a.B;
+  a.page_slots = slots < a.T;
+  const int owners = (int)std::min<int64_t>(slots, a.T);
   if (page <= FUSED_PAGE) {
-    const int chunks = (a.Hk + KEY_HEADS - 1) / KEY_HEADS;
-    a.page_block = block_for(chunks);
-    const int blocks = (a.T + a.page_block - 1) / a.page_block;
     // a head a workgroup, not two, while pages are few: two / one, in pages of 64, 500 tokens x 40/8 heads (32 workgroups of
     // two) 13.5 / 11.4 us, 2000 (128) 16.2 / 14.8, 2500 (160) 16.6 / 16.9, 3500 (220) 21.2 / 22.2, 2000 x 12/12 (192) 14.4 / 12.9
     const int64_t pages = (a.T >> a.pt.shift) + a.B;
-    a.page_heads = pages * chunks <= 3 * num_cus() / 4 ? 1 : KEY_HEADS;
-    a.page_wgs = blocks * ((a.Hk + a.page_heads - 1) / a.page_heads);
+    a.page_heads = pages * ((a.Hk + KEY_HEADS - 1) / KEY_HEADS) <= 3 * num_cus() / 4 ? 1 : KEY_HEADS;
+    a.page_wgs = owners * ((a.Hk + a.page_heads - 1) / a.page_heads);
     return launch<LPH, PAGES>(a, stream);
   }
   const hipError_t e = launch<LPH, ROWS>(a, stream);
   if (e != hipSuccess) return e;
-  const int chunks = (a.Hk + HPW - 1) / HPW;
-  a.page_block = block_for(chunks);
-  const dim3 blocks((a.T + a.page_block - 1) / a.page_block, chunks);
-  hipLaunchKernelGGL(append_bounds_kernel<LPH>, blocks, dim3(EDGE_WAVES * 64), 0, stream, a);
+  hipLaunchKernelGGL(append_bounds_kernel<LPH>, dim3(owners, (a.Hk + HPW - 1) / HPW), dim3(EDGE_WAVES * 64), 0, stream, a);
   return hipGetLastError();
 }
 

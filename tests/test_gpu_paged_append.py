@@ -315,3 +315,33 @@ def test_many_pages_and_few_with_odd_heads(hq, hk, dim, inter, page, new):
     """Pages whose keys are looked after one head and two at a time, an odd one last, or by a kernel of its own."""
     Case(new, [5 + 30 * i for i in range(len(new))], hq=hq, hk=hk, dim=dim, inter=inter, page=page, eps=1e-6, weights=BF,
          seed=dim + page).go()
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("new,old", [
+    ([20, 0, 40, 1], [3, 9, 0, 16]), ([150, 300], [70, 0]), ([0] * 70 + [5] + [0] * 130 + [3, 0], [1] * 203),
+    ([16, 0, 64, 128, 127], [0, 0, 64, 128, 1]), ([33] * 80, list(range(80))), ([0, 0, 0], [5, 0, 1])])
+def test_tokens_before_the_first_sequence_are_left_alone(page, new, old):
+    """The same tokens behind others that belong to nobody, to the bit; among empty sequences too."""
+    import lbw_amd
+    lead = 9
+    c = Case(new, old, page=page, spare_tokens=lead + 4, axes=2, eps=1e-6, weights=BF, seed=page)
+    args = (c.table, c.lens, c.rope)
+    outs, caches = [], []
+    for shift in (0, lead):
+        cache = lbw_amd.PagedKV(c.cache.k.clone(), c.cache.v.clone(), c.cache.bounds.clone())
+        part = slice(lead - shift, None)
+        q = c.q[part]
+        out = torch.full(q.shape, 3.0, dtype=BF, device="cuda")
+        lbw_amd.paged_append_(cache, q, c.k[part], c.v[part], *args, c.pos[part], starts=c.starts + shift, q_out=out,
+                              wq=c.w[0], wk=c.w[1], eps=1e-6)
+        assert (out[:shift] == 3).all() and (out[shift + sum(new):] == 3).all()
+        outs.append(out[shift:])
+        caches.append(cache)
+    assert torch.equal(*outs)
+    for n in ("k", "v", "bounds"):
+        assert torch.equal(getattr(caches[0], n), getattr(caches[1], n))
+    # and as the definition has it
+    c.q, c.k, c.v, c.pos = (x[lead:] for x in (c.q, c.k, c.v, c.pos))
+    if sum(new):
+        c.go()
