@@ -22,8 +22,8 @@ namespace {
 constexpr int AP_WAVES = 4;
 constexpr int KEY_HEADS = 2;   // heads of a workgroup that looks after a page's keys, at most
 constexpr int EDGE_WAVES = 8;  // of the bounds kernel
-// Pages up to this size get their keys and bounds in the kernel of the tokens' q and v, larger ones, whose tokens would
-// follow one another too long, their bounds by a second kernel. Two kernels / one, x 40/8 heads, pages of 64: 100 tokens
+// Pages that can get up to so many new tokens get their keys and bounds in the kernel of the tokens' q and v, others, whose
+// tokens would follow one another too long, their bounds by a second kernel. Two kernels / one, x 40/8 heads, pages of 64: 100 tokens
 // 12.5 / 10.1 us, 500 12.5 / 11.4, 2000 17.7 / 14.8, 4680 35.6 / 35.0, 9841 67.5 / 60.1; of 128 11.9 / 13.2, 12.9 / 17.3, 18.9 / 20.1,
 // 36.6 / 38.7, 67.0 / 62.3; of 256 11.8 / 13.2, 14.4 / 29.4, 20.5 / 31.8, 37.6 / 48.7, 67.6 / 73.2.
 constexpr int FUSED_PAGE = 64;
@@ -459,7 +459,7 @@ hipError_t run(AppendArgs a, hipStream_t stream) {
   const int64_t slots = (a.T >> a.pt.shift) + 2 * (int64_t)a.B;
   a.page_slots = slots < a.T;
   const int owners = (int)std::min<int64_t>(slots, a.T);
-  if (page <= FUSED_PAGE) {
+  if (std::min(page, a.T) <= FUSED_PAGE) {
     // a head a workgroup, not two, while pages are few: two / one, in pages of 64, 500 tokens x 40/8 heads (32 workgroups of
     // two) 13.5 / 11.4 us, 2000 (128) 16.2 / 14.8, 2500 (160) 16.6 / 16.9, 3500 (220) 21.2 / 22.2, 2000 x 12/12 (192) 14.4 / 12.9
     const int64_t pages = (a.T >> a.pt.shift) + a.B;
