@@ -73,6 +73,7 @@ struct PagedAttnArgs {
   const int32_t* p_len;       // [1] or null
   int64_t p_max;              // at most so many keys
   int p_splits, p_block;      // p_block: query rows of a workgroup
+  int p_inline;               // every sequence walks the prefix itself, before its own keys (p_splits 0)
   // partial results: own parts then the prefix's, [Hq][rows][D] each, then m and l of all of them
   float* part;
 };

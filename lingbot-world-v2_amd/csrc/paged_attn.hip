@@ -10,7 +10,8 @@
 // up at once, one half a lane, and handed to the scalar side a tile ahead.
 //
 // The prefix's keys are the same for the whole batch: its query rows are those of all sequences, 32 at a time, or 128
-// where there are more (four waves over shared tiles of 64 keys), in one launch with the sequences' own keys.
+// where there are more (four waves over shared tiles of 64 keys), in one launch with the sequences' own keys. A short prefix
+// is walked by every sequence before its own keys.
 //
 // Measured, x 40/8 heads: eight sequences of up to 46800 keys 165 us, K and V at 6.4 TB/s (a plain kernel that only reads
 // reaches 5.7); 64 of up to 3600 behind a prefix of 46800 155 us, 16 of 200 (12/4 heads) behind 46800 37; one
@@ -126,9 +127,13 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
     const int64_t len = KIND == PREFIX ? scalar64(prefix_keys(a)) : __builtin_amdgcn_readfirstlane(keys_of(a, b));
     const int32_t* const table = KIND == PREFIX ? a.p_table : a.pt.p + b * a.pt.sb;
     const int32_t* const sel = KIND == SPARSE ? a.sel + ((int64_t)b * a.Hk + kv) * a.n_sel : nullptr;
-    const int64_t span = KIND == SPARSE
-                             ? (len > 0 ? (int64_t)__builtin_amdgcn_readfirstlane(list_length(sel, a.n_sel, lane)) << shift : 0)
-                             : len;
+    const int64_t own_span =
+        KIND == SPARSE
+            ? (len > 0 ? (int64_t)__builtin_amdgcn_readfirstlane(list_length(sel, a.n_sel, lane)) << shift : 0)
+            : len;
+    // a short prefix's keys, in halves of their own, come before the sequence's
+    const int64_t p_keys = KIND != PREFIX && a.p_inline != 0 ? scalar64(prefix_keys(a)) : 0;
+    const int64_t pre = (p_keys + HT - 1) / HT * HT, span = pre + own_span;
     const int tiles = (int)((span + DT - 1) / DT);
     // this sequence's tiles of the piece
     int s0 = 0, s1 = tiles;
@@ -142,8 +147,9 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
 
     // halves of tiles base, base + DW, ..: tile i's first half in lane i, its second in lane 32 + i
     auto look_up = [&](int base) {
-      return half_at(sel, span, table, KIND == PREFIX ? a.p_width : a.pt.width, shift, a.pt.pages, len,
-                     ((int64_t)base + (int64_t)l32 * DW) * DT + HT * hl);
+      const int64_t pos = ((int64_t)base + (int64_t)l32 * DW) * DT + HT * hl;
+      if (pos < pre) return half_at(nullptr, p_keys, a.p_table, a.p_width, shift, a.pt.pages, p_keys, pos);
+      return half_at(sel, own_span, table, KIND == PREFIX ? a.p_width : a.pt.width, shift, a.pt.pages, len, pos - pre);
     };
     Half list = {0, 0}, h0, h1;  // h0, h1: the halves of the tile that is fetched next, scalar
     int listed = 0;              // tiles of the list that are used up
@@ -164,7 +170,9 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
     auto issue = [&](const PageRows& src, uint32_t off, int t, uint32_t to) {
       const unsigned char* base = reinterpret_cast<const unsigned char*>(src.p + kv * src.sh);
       const int64_t sl = src.sl * 2, sp = src.sp * 2;
-      const int in = (int)(((int64_t)t * DT) & mask), in1 = (in + HT) & mask;
+      // (places behind a prefix count from its end)
+      const int64_t at0 = (int64_t)t * DT, at1 = at0 + HT;
+      const int in = (int)((at0 < pre ? at0 : at0 - pre) & mask), in1 = (int)((at1 < pre ? at1 : at1 - pre) & mask);
       const int n0 = h0.keys & (BAD_PAGE - 1), n1 = h1.keys & (BAD_PAGE - 1);
       const unsigned char* p0 = base + h0.page * sp + in * sl;
       const unsigned char* p1 = base + h1.page * sp + in1 * sl;
@@ -609,6 +617,11 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
                                                                     : 3500;
   const bool whole = num_splits == 1 || (num_splits == 0 && keys <= limit);
   int64_t own_places = cus;
+  // A short prefix: every sequence walks it itself, one launch without a join. Apart / so: 16 sequences x 40/8 heads, 400 keys
+  // and 20 own 14.8 / 9.9 us, 500 and 500 16.1 / 13.6, 1200 and 40 18.5 / 14.4; 4 x 12/12 14.2 / 9.8, 15.0 / 14.3, 13.9 / 15.0; more
+  // than one a CU, 32 x 12/12 14.7 / 13.7, 21.5 / 23.7, 18.0 / 24.0, 64 x 12/12 21.5 / 21.4, 32.2 / 41.6, 24.5 / 39.3.
+  a->p_inline = a->p_max > 0 && num_splits == 0 && a->p_max + keys <= (seqs <= cus ? 1100 : 450);
+  if (a->p_inline) return;
   if (a->p_max > 0) {
     const int64_t rows = a->B * group, p_tiles = (a->p_max + DT - 1) / DT;
     a->p_block = rows > 3 * HEADS ? PK_BLOCK : HEADS;

@@ -304,3 +304,36 @@ def test_no_sequences_and_refusals():
         out.float().sum().backward()
     with pytest.raises(NotImplementedError, match="not differentiable"):
         lbw_amd.attention_paged(x, c.cache, c.table, _i32([3, 3]), out=torch.empty_like(c.q))
+
+
+@pytest.mark.parametrize("prefix", [1, 15, 16, 17, 31, 32, 33, 47, 100, 449, 1000])
+@pytest.mark.parametrize("lens,hq,hk,page", [
+    ([0, 1, 15, 16, 17, 33, 90], 12, 4, 16), ([64, 70, 0], 66, 1, 64), ([5, 60], 6, 3, 1024), ([40, 1] * 70, 4, 2, 32)])
+def test_short_prefixes_walked_by_each_sequence_and_apart(prefix, lens, hq, hk, page):
+    c = Case(lens, hq, hk, page, prefix=prefix, seed=prefix)
+    for splits in (0, 1, 2):
+        c.check(num_splits=splits)
+    n = P.pages_of(max(lens), page)
+    sel = torch.full((len(lens), hk, n + 1), -1, dtype=torch.int32)
+    sel[..., :n] = torch.arange(n, dtype=torch.int32).flip(0)
+    sel[0] = -1
+    for splits in (0, 1):
+        c.check(num_splits=splits, selected=sel.cuda())
+    # lengths of it that the device holds
+    for m in (0, 1, 18, prefix, prefix + 1, 2 ** 31 - 1, -5):
+        kw = {"prefix_table": c.prefix_table, "prefix_len": _i32([m])}
+        got = c.run(**kw)
+        want, allow = P.attention(c.q, c.cache.k, c.cache.v, c.table, lens, SCALE, c.prefix_table,
+                                  max(0, min(m, len(c.prefix_table) * page)))
+        R.assert_within("out", got, want, allow)
+
+
+def test_a_bad_page_of_a_short_prefix_reaches_all_and_of_a_sequence_only_it():
+    for splits in (0, 1):
+        c = Case([20, 0, 50], 4, 2, 16, prefix=60, seed=90)
+        want = c.run(num_splits=splits)
+        c.table[2, 1] = -9
+        got = c.run(num_splits=splits)
+        assert torch.isnan(got[2]).all() and torch.equal(got[:2], want[:2])
+        c.prefix_table[3] = c.cache.k.shape[0]
+        assert torch.isnan(c.run(num_splits=splits)).all()
