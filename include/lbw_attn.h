@@ -419,7 +419,7 @@ int lbw_paged_append(const lbw_paged_append_params* p, void* stream);
  * [batch][k_heads][n_selected], device, contiguous) a key/value head attends to the table entries it names, up to the
  * first negative one (an entry named twice counts twice). With a prefix (int32 [prefix_width] pages, min(*prefix_len,
  * prefix_keys) keys; prefix_len NULL: prefix_keys) those keys come before every sequence's own and are read once for
- * the batch. */
+ * the batch (unless they are few). */
 typedef struct lbw_attention_paged_params {
   lbw_paged_kv cache;
   int32_t batch, q_heads, k_heads, head_dim;

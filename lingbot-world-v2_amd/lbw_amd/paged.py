@@ -147,8 +147,8 @@ def attention_paged(q, cache: PagedKV, table, lens, *, selected=None, prefix_tab
     ``out`` when given). A sequence of no keys gives 0. Rows behind a length may hold anything.
 
     ``prefix_table`` int32 ``[pages]``: keys that come before every sequence's own, ``prefix_len`` of them (an int, or
-    one int32 on the device, limited to the pages; None: all). They are read once for the whole batch; table and lens
-    then describe what each sequence has behind them. Several tokens of one sequence are as many rows of q, table and lens.
+    one int32 on the device, limited to the pages; None: all). They are read once for the whole batch (unless they are
+    few); table and lens then describe what each sequence has behind them. Several tokens of one sequence are as many rows of q, table and lens.
 
     ``selected`` int32 ``[batch, kv_heads, n]`` (from :func:`paged_select`): a key/value head attends to the table entries
     that its list names, up to the first negative one; entries at or past the length name no keys, one that is named twice
