@@ -584,17 +584,18 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 // lists than half the CUs). Whole / in pieces, x 40/8 heads: 512 keys for one sequence 9.3 / 11.0 us, for 8 11.0 / 11.1, for 16
 // 11.6 / 12.5; 768 12.3 / 11.2, 13.4 / 12.7, 14.0 / 14.5; 1024 14.7 / 11.3, 15.8 / 13.4, 16.7 / 16.6; 2560 28.0 / 10.9, 30.8 / 20.6,
 // 33.1 / 29.3; a workgroup a CU / two: 5760 for 8 35.4 / 35.5, 6400 for 4 23.1 / 23.7, for 24 88.5 / 100.6.
-// With a prefix (measured before own keys went past the caches, which changes both sides alike; 0.5 to 0.8 instead of 0.7
-// below then gave 167, 166, 160 and 177 us), places shared out by tiles: 4 of up to 1600 off 14040 keys x 40/8 heads, 20 pieces of the prefix and 12
-// of own keys 22.2 us, 32 and 32 25.8; 8 of 3600 off 6000 x 12/4, 9 and 55 21.2, 64 and 64 28.2; 64 of 3600 off 46800 x 40/8
-// (128 rows at a time), 10 and 34 163, 21 and 64 185, 5 and 17 205; 26 of 1500 off 14040 x 40/8 16 and 32 40.4, 8 and 16 45.8;
-// 30 of 1500 off 10000 x 16/2, 32 and 64 23.5, 64 and 128 27.6. Whole sequences: 16 of 200 off 6000 x 12/4, 24 pieces (one
-// workgroup a CU) 14.4, 48 16.6; off 46800 20 35.9, 48 39.6; 16 of 200 off 14040 x 40/8 (128 sequences x heads), 4 pieces 47.1,
-// 16 (two a CU) 26.6. Ten of
-// 472 off 4254 x 40/40 (400), 2 pieces 49.1, 6 36.5; 60 of 300 off 10000 x 12/12 (720), one 122.7, 21 44.8; 128 rows at a time: 29 of
-// 102 off 9496 x 40/8 (232), 17 pieces 30.5, 24 38.6; 64 of 200 off 14040 (512), 10 58.3, 16 53.6. Pieces of 4 tiles or more, of
-// 6: 4 of 40 off 1560 x 12/4 12.3 / 13.3, one of 3000 x 40/8 11.7 / 13.0; of 128 rows, of 4 or 8: 41 of 800 off 3366 x 12/4 25.3 /
-// 20.3, 64 of 500 off 6000 30.8 / 25.9.
+// With a prefix (measured before own keys went past the caches, which changes both sides alike; shares by 0.5, 0.6,
+// 0.7 and 0.8 of own keys then gave 167, 166, 160 and 177 us for 64 of 3600 off 46800), places shared out by tiles:
+// 4 of up to 1600 off 14040 keys x 40/8 heads, 20 pieces of the prefix and 12 of own keys 22.2 us, 32 and 32 25.8; 8
+// of 3600 off 6000 x 12/4, 9 and 55 21.2, 64 and 64 28.2; 64 of 3600 off 46800 x 40/8 (128 rows at a time), 10 and
+// 34 163, 21 and 64 185, 5 and 17 205; 26 of 1500 off 14040 x 40/8 16 and 32 40.4, 8 and 16 45.8; 30 of 1500 off
+// 10000 x 16/2, 32 and 64 23.5, 64 and 128 27.6. Whole sequences: 16 of 200 off 6000 x 12/4, 24 pieces (one
+// workgroup a CU) 14.4, 48 16.6; off 46800 20 35.9, 48 39.6; 16 of 200 off 14040 x 40/8 (128 sequences x heads), 4
+// pieces 47.1, 16 (two a CU) 26.6. Ten of 472 off 4254 x 40/40 (400), 2 pieces 49.1, 6 36.5; 60 of 300 off 10000 x
+// 12/12 (720), one 122.7, 21 44.8; 128 rows at a time: 29 of 102 off 9496 x 40/8 (232), 17 pieces 30.5, 24 38.6; 64
+// of 200 off 14040 (512), 10 58.3, 16 53.6. Pieces of 4 tiles or more, of 6: 4 of 40 off 1560 x 12/4 12.3 / 13.3,
+// one of 3000 x 40/8 11.7 / 13.0; of 128 rows, of 4 or 8: 41 of 800 off 3366 x 12/4 25.3 / 20.3, 64 of 500 off 6000
+// 30.8 / 25.9.
 // 32 / 128 query rows at a time: 8 of 1500 off 14040 x 40/8 (40 rows) 30.9 / 35.6, 20 (100) 42.5 / 46.5, 40 (200) 65.6 /
 // 54.4; 46800, 1000 own x 12/4, 24 rows 34.5 / 36.6, 60 rows 44.0 / 43.0, 78 rows 49.3 / 51.8, 99 rows 58.5 / 54.8.
 void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
