@@ -19,6 +19,7 @@
 #include "capi_util.h"
 #include "head_rows.h"
 #include "paged.h"
+#include "score_range.h"
 
 namespace lbw {
 namespace {
@@ -28,7 +29,7 @@ constexpr int SC_G = 5;           // query heads at a time, at most (64 register
 constexpr int TOP_T = 256;        // threads of the choice
 constexpr int ONE_T = 512;        // threads of the kernel that scores and chooses
 constexpr int ONE_PAGES = 256;    // scores that it keeps
-constexpr int BINS = 1024;
+constexpr int BINS = SCORE_BINS;
 constexpr uint64_t INF_IMAGE = 0xfff0000000000000ull;
 
 // Order-preserving image of a score that is not NaN, -0 as 0; never 0. (NaN counts as infinity.)
@@ -208,16 +209,16 @@ __device__ __forceinline__ void choose(const SelectArgs& a, int n, const uint64_
       lo = range[w][0] < lo ? range[w][0] : lo;
       hi = range[w][1] > hi ? range[w][1] : hi;
     }
-    ++lo;
-    // the last chosen score is in [lo, hi], the need-th highest of those there
+    ScoreRange r = {lo + 1, hi};
+    // the last chosen score is in the range, the need-th highest of those there
     while (true) {
-      if (lo == hi) {
-        over = lo;
+      if (r.lo == r.hi) {
+        over = r.lo;
         break;
       }
-      const int bits = 64 - __clzll((unsigned long long)(hi - lo)), shift = bits > 10 ? bits - 10 : 0;
+      const int shift = bin_shift(r);
       each([&](uint64_t u, int) {
-        if (u >= lo && u <= hi) atomicAdd(&hist[(u - lo) >> shift], 1u);
+        if (in_range(r, u)) atomicAdd(&hist[bin_of(r, shift, u)], 1u);
       });
       __syncthreads();
       // four bins a thread, from the top: how many scores are in them and in those above
@@ -247,19 +248,17 @@ __device__ __forceinline__ void choose(const SelectArgs& a, int n, const uint64_
       }
       clear();
       __syncthreads();
-      lo += (uint64_t)found[0] << shift;
-      const uint64_t h = lo + ((1ull << shift) - 1);
-      hi = h < hi ? h : hi;
+      r = bin_range(r, shift, (int)found[0]);
       need = found[2];
       const uint32_t in_bin = found[1];
       if (need == in_bin) {  // every score of the bin
-        over = lo - 1;
+        over = r.lo - 1;
         need = 0;
         break;
       }
       if (in_bin <= T) {
         each([&](uint64_t u, int i) {
-          if (u >= lo && u <= hi) {
+          if (in_range(r, u)) {
             const uint32_t at = atomicAdd(&collected, 1u);
             cand[at] = u;
             place[at] = i;
@@ -329,8 +328,9 @@ __device__ __forceinline__ void choose(const SelectArgs& a, int n, const uint64_
       const int x = j * TOP_W + wave;
       const uint32_t pa = above0 + __builtin_amdgcn_readlane(sa - na, x) + (turn[j] & 255);
       const uint32_t pe = equal0 + __builtin_amdgcn_readlane(se - ne, x) + (turn[j] >> 8 & 255);
-      if ((turn[j] >> 16 & 1) || ((turn[j] >> 17) && pe < need))
-        sel[pa + (pe < need ? pe : need)] = base + j * T + tid;
+      const uint32_t at = pa + (pe < need ? pe : need);
+      // (the list's end is asked for all the same: what is behind it is another list)
+      if (((turn[j] >> 16 & 1) || ((turn[j] >> 17) && pe < need)) && at < (uint32_t)a.count) sel[at] = base + j * T + tid;
     }
     above0 += __shfl(sa, 63);
     equal0 += __shfl(se, 63);
