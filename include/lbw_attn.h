@@ -390,8 +390,8 @@ typedef struct lbw_paged_kv {
 /* New tokens: q and k normalised per head (norm != 0, as lbw_head_norm_rope) or not, their pairs turned by the tokens'
  * positions (pos; NULL: a token's row in its sequence, one axis), q into q_out, k and v into their rows of the cache,
  * the bounds kept up. Token t of sequence b (starts[b] <= t < starts[b + 1], int32 [batch + 1] on the device; NULL:
- * token t is sequence t's, batch == tokens) goes to row lens[b] + t - starts[b]; a row outside the table is not
- * written. Tokens outside every sequence are left alone, their q_out too. q_out may be q itself. A page that gets its
+ * token t is sequence t's, batch == tokens) goes to row lens[b] + t - starts[b]; starts rise, and may lie below 0 or
+ * past the tokens; a row outside the table is not written. Tokens outside every sequence are left alone, their q_out too. q_out may be q itself. A page that gets its
  * row 0 starts its bounds anew. No two sequences, nor two entries of one's row of the table, may be given tokens for one
  * page. */
 typedef struct lbw_paged_append_params {

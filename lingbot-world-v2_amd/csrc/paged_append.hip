@@ -75,32 +75,24 @@ __device__ __forceinline__ Place place_of(const AppendArgs& a, int t, int lane) 
   return w;
 }
 
-// A page's new tokens: t .. t + n - 1, rows row .. of their sequence, from row `in` of page `page` on. Its owner is a
-// workgroup: number `slot` of those that a.page_slots tells from one another --
-//   tokens: that of the page's first new token;
-//   pages: sequence b has those from starts[b] / P + 2 b on, P tokens a page, as many as its tokens can touch pages, so
-//   that no sequence's lengths are wanted to find another's.
-// False: no page is here (or the sequence's table does not hold it).
-struct Fresh {
-  int t, n, in, page;
-  int64_t row;
+// A page's new tokens, of page `page`. Its owner is a workgroup: number `slot` of those that a.page_slots tells from one
+// another by pages (first_owner), else by tokens. False: no page is here (or the sequence's table does not hold it).
+struct Fresh : PageRun {
+  int page;
 };
 __device__ __forceinline__ bool fresh_page(const AppendArgs& a, int64_t slot, int lane, Fresh& f) {
-  const int shift = a.pt.shift, mask = (1 << shift) - 1;
+  const int shift = a.pt.shift;
   if (a.page_slots == 0) {
     const Place w = place_of(a, (int)slot, lane);
     if (w.b < 0 || w.page < 0) return false;
-    f = {(int)slot, 0, (int)(w.row & mask), w.page, w.row};
-    if (f.in != 0 && f.t != w.start) return false;
-    f.n = w.end - f.t < mask + 1 - f.in ? w.end - f.t : mask + 1 - f.in;
-    return true;
+    f.page = w.page;
+    return opened_run((int)slot, w.row, w.start, w.end, a.T, shift, f);
   }
   // the last sequence whose first slot is this one or before
-  auto at = [&](int b) { return (int64_t)(a.starts[b] >> shift) + 2 * (int64_t)b; };
   int base = 0, left = a.B;
   while (left > 64) {
     const int step = (left + 63) >> 6, off = lane * step;
-    const uint64_t past = __ballot(off < left && at(base + off) <= slot);
+    const uint64_t past = __ballot(off < left && first_owner(base + off, a.starts[base + off], shift) <= slot);
     if (past == 0) return false;
     const int c = (63 - __clzll((unsigned long long)past)) * step;
     base += c;
@@ -113,20 +105,13 @@ __device__ __forceinline__ bool fresh_page(const AppendArgs& a, int64_t slot, in
     e = a.starts[base + lane + 1];
     l = a.lens[base + lane];
   }
-  const uint64_t past = __ballot(mine && (int64_t)(s >> shift) + 2 * (int64_t)(base + lane) <= slot);
+  const uint64_t past = __ballot(mine && first_owner(base + lane, s, shift) <= slot);
   if (past == 0) return false;
   const int c = 63 - __clzll((unsigned long long)past), b = base + c;
   const int start = __builtin_amdgcn_readlane(s, c), stop = __builtin_amdgcn_readlane(e, c);
-  const int first = start > 0 ? start : 0, end = stop < a.T ? stop : a.T;  // (the tokens that there are)
-  if (first >= end) return false;
-  const int64_t row0 = (int64_t)__builtin_amdgcn_readlane(l, c) + ((int64_t)first - start);
-  const int64_t j = slot - ((int64_t)(start >> shift) + 2 * (int64_t)b);
-  const int64_t row = j == 0 ? row0 : ((row0 >> shift) + j) * (mask + 1), t = first + (row - row0);
-  if (t >= end) return false;
-  f = {(int)t, 0, (int)(row & mask), -1, row};
-  f.n = end - f.t < mask + 1 - f.in ? end - f.t : mask + 1 - f.in;
+  if (!owned_run(start, stop, a.T, __builtin_amdgcn_readlane(l, c), shift, slot - first_owner(b, start, shift), f)) return false;
   f.page = __builtin_amdgcn_readfirstlane(
-      page_at(a.pt.p + (int64_t)b * a.pt.sb, a.pt.width, shift, a.pt.pages, row));
+      page_at(a.pt.p + (int64_t)b * a.pt.sb, a.pt.width, shift, a.pt.pages, f.row));
   return f.page >= 0;
 }
 
@@ -456,7 +441,7 @@ hipError_t run(AppendArgs a, hipStream_t stream) {
   // for pages, four times as many workgroups / half as many as CUs / a workgroup a page: 1000 tokens x 40/8 heads in pages of
   // 64 16.8 / 12.5 / 12.7 us, x 40/40 25.1 / 17.7 / 17.1, eight times 400 23.4 / 33.8 / 25.1, 400 + 4 x 40 + 3 x 4 x 12/12 in pages of 32
   // 12.4 / 18.7 / 10.8; 2000 x 40/40 in pages of 128, two kernels, 61.3 / 34.7 / 34.5)
-  const int64_t slots = (a.T >> a.pt.shift) + 2 * (int64_t)a.B;
+  const int64_t slots = page_owners(a.T, a.B, a.pt.shift);
   a.page_slots = slots < a.T;
   const int owners = (int)std::min<int64_t>(slots, a.T);
   if (std::min(page, a.T) <= FUSED_PAGE) {

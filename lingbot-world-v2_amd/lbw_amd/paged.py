@@ -85,8 +85,8 @@ def paged_append_(cache: PagedKV, q, k, v, table, lens, rope: AxisRope, pos=None
 
     ``lens`` int32 ``[batch]``: the rows that each sequence has so far; the call does not change it. ``starts`` None: one
     token per sequence, token b goes to row ``lens[b]``. Otherwise int32 ``[batch + 1]`` on the device, rising: tokens
-    ``starts[b] .. starts[b + 1] - 1`` are sequence b's next ones; tokens outside all of them are left alone, their
-    ``q_out`` rows too. A row outside the table is not written. ``pos`` int32 ``[tokens, axes]`` (``[tokens]`` for one
+    ``starts[b] .. starts[b + 1] - 1`` are sequence b's next ones, as far as there are such tokens (a slice of a longer
+    batch may have starts below 0 and past its end); tokens outside all of them are left alone, their ``q_out`` rows too. A row outside the table is not written. ``pos`` int32 ``[tokens, axes]`` (``[tokens]`` for one
     axis); None: a token's row in its sequence's table, for a rotation of one axis (behind a prefix that is not the
     position: give it). A position outside the rotation's table turns
     its pairs into NaN. ``eps`` not None: RMSNorm of every q and k head first, as in :func:`qk_head_norm_rope`, with
