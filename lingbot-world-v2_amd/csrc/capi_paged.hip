@@ -160,7 +160,7 @@ int lbw_paged_append(const lbw_paged_append_params* p, void* stream) {
   a.starts = p->starts;
   a.lens = p->lens;
   a.bounds = static_cast<uint16_t*>(p->cache.bounds);
-  if (p->tokens == 0) return LBW_OK;
+  if (p->tokens == 0 || p->batch == 0) return LBW_OK;  // (tokens of no sequence are left alone)
   const hipError_t e = launch_append(a, p->head_dim, static_cast<hipStream_t>(stream));
   return e == hipSuccess ? LBW_OK : hip_fail(e, "paged append launch");
 }

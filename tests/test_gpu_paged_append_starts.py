@@ -87,3 +87,17 @@ def test_a_batch_in_slices_is_the_batch():
     for c in caches[1:]:
         for a, b in zip(c, caches[0]):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128, 256])
+@pytest.mark.parametrize("tokens", [1, 65, 100, 1000])
+@pytest.mark.parametrize("bounds", [True, False])
+def test_tokens_without_sequences_are_left_alone(page, tokens, bounds):
+    import lbw_amd
+    cache = lbw_amd.paged_kv(3, page, 2, bounds=bounds)
+    q, k, v = torch.ones(tokens, 8, 128, dtype=BF, device="cuda").split([4, 2, 2], 1)
+    rope = lbw_amd.axis_rope(lbw_amd.wan_rope_freqs(128, 2048).cuda())
+    out = torch.full((tokens, 4, 128), 7.0, dtype=BF, device="cuda")
+    table, none = torch.zeros(0, 2, dtype=torch.int32, device="cuda"), _i32([])
+    assert lbw_amd.paged_append_(cache, q, k, v, table, none, rope, starts=_i32([0]), q_out=out) is out
+    assert torch.all(out == 7) and not cache.k.any() and not cache.v.any() and (not bounds or not cache.bounds.any())

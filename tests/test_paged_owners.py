@@ -3,6 +3,8 @@ tokens, every token of a sequence is in one owner's run, at its row and inside o
 import os
 import subprocess
 
+import pytest
+
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "lingbot-world-v2_amd", "csrc")
 
@@ -89,3 +91,16 @@ def test_every_token_has_one_owner(tmp_path):
                     str(src), "-o", str(exe)], check=True)
     out = subprocess.run([str(exe)], capture_output=True, text=True)
     assert out.returncode == 0 and out.stdout == "ok\n", out.stdout + out.stderr[-2000:]
+
+
+@pytest.mark.parametrize("page", [16, 64, 128, 256, 1024])
+@pytest.mark.parametrize("tokens", [1, 64, 65, 100, 255, 1000])
+def test_tokens_of_no_sequence_are_no_launch(page, tokens):
+    """A batch of none: every token belongs to nobody, so there is nothing to do (and no device is wanted)."""
+    import ctypes
+
+    from lbw_amd import _lib
+    from test_paged_host import ADDR, _append
+    for bounds in (ADDR, None):
+        p = _append(tokens=tokens, batch=0, starts=ADDR, lens=None, **{"cache.page_size": page, "cache.bounds": bounds})
+        assert _lib.load().lbw_paged_append(ctypes.byref(p), None) == 0
