@@ -18,7 +18,8 @@
 // sequence of 500 keys 8.7 us, 3 us of it the launch and 1.5 a tile of each wave.
 //
 // A half's rows past its last key copy that key (or the other half's), so the products never meet what lies
-// behind a sequence. A page outside the cache makes its keys' scores NaN.
+// behind a sequence; V's of them are zeros before the product, as their weight of 0 would make NaN of a copy of an infinite
+// value. A page outside the cache makes its keys' scores NaN. Scores that are all -infinity give NaN (0 / 0), no keys 0.
 
 #include <algorithm>
 
@@ -52,6 +53,10 @@ __device__ __forceinline__ int tiles_of(const PagedAttnArgs& a, int b) { return 
 __device__ __forceinline__ int64_t prefix_keys(const PagedAttnArgs& a) {
   int64_t n = a.p_len != nullptr ? a.p_len[0] : a.p_max;
   return n < 0 ? 0 : (n > a.p_max ? a.p_max : n);
+}
+// 1 / L of a row with reference M: 0 without keys (M = -inf), NaN where they give no sum (scores of -infinity alone).
+__device__ __forceinline__ float inverse_sum(float M, float L) {
+  return L > 0.0f ? 1.0f / L : (M == -INFINITY ? 0.0f : __uint_as_float(0x7fc00000u));
 }
 // Entries of a list of selected pages: those before the first negative one.
 __device__ __forceinline__ int list_length(const int32_t* sel, int n, int lane) {
@@ -202,6 +207,7 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
     float m = M_INIT, l = 0.0f;
     __builtin_amdgcn_s_waitcnt(0x0070);  // the query is there: only tile copies are counted below
     int t = s0 + wave, k0 = 0, k1 = 0;   // keys of the current tile's halves
+    int any = 0;                         // whether the wave had keys
     if (t < s1) {
       next_halves(t);
       issue_k(t);
@@ -212,6 +218,7 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
       const bool more = t + DW < s1;
       k0 = h0.keys;
       k1 = h1.keys;
+      any |= k0 | k1;
       if (more) next_halves(t + DW);
       asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // K is there (V may be on its way)
       floatx16 s;
@@ -253,6 +260,14 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
       if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V is there (the next K may not be)
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (((k0 | k1) & (2 * BAD_PAGE - 1)) != 0) {  // (a tile without keys holds anything)
+        if (k0 != HT || k1 != HT) {  // two lanes a row
+          const int row = lane >> 1;
+          if ((row & (HT - 1)) >= ((row < HT ? k0 : k1) & (BAD_PAGE - 1))) {
+            const int at = ring + DT_B + row * PK_ROWB + (lane & 1) * (PK_ROWB / 2);
+#pragma unroll
+            for (int i = 0; i < PK_ROWB / 32; ++i) *(lds_u32x4*)(uintptr_t)(at + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+          }
+        }
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -265,8 +280,8 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
     // O^T as rows [row][128] fp32 into the wave's LDS, m and l behind the rings
     float* const sm = reinterpret_cast<float*>(lds + DEC_LDS);
     float* const sl = sm + DW * HEADS;
-    if (hl == 0) {  // (no keys: a reference of -inf, weight 0; a sum that is NaN keeps its own and stays)
-      sm[wave * HEADS + l32] = l == 0.0f ? -INFINITY : m;
+    if (hl == 0) {  // (no keys: a reference of -inf, weight 0; scores of -inf alone: the first reference, a sum of 0)
+      sm[wave * HEADS + l32] = any != 0 ? m : -INFINITY;
       sl[wave * HEADS + l32] = l;
     }
     float* mine = reinterpret_cast<float*>(lds + RING_B * wave);
@@ -300,7 +315,7 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
       }
       const int sq = seq_of(hh), head = head_of(hh);
       if (whole) {
-        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+        const float inv = inverse_sum(M, L);
         u32x2 w;
         w[0] = pack_bf16x2(acc[0] * inv, acc[1] * inv);
         w[1] = pack_bf16x2(acc[2] * inv, acc[3] * inv);
@@ -397,6 +412,17 @@ __device__ __forceinline__ void prefix_tiles(const PagedAttnArgs& a, uint32_t id
     const unsigned char* b = reinterpret_cast<const unsigned char*>(src.p + kv * src.sh) + page * (src.sp * 2) + in * sl;
     const uint32_t last = (uint32_t)(more < HT - 1 ? (more > 0 ? more : 0) : HT - 1) * (uint32_t)sl;
     const int col = opaque(ccol);
+    if (!is_k && more < HT - 1) {  // (the last tile: zeros behind the last key)
+      const int at = opaque(16 * lane);
+#pragma unroll
+      for (int i = 0; i < PK_NDMA; ++i) {
+        const int row = (at >> 8) + 4 * i;
+        u32x4 x = {0u, 0u, 0u, 0u};
+        if (row <= more) x = *reinterpret_cast<const u32x4*>(b + row * sl + (col ^ (i << 4)));
+        *(lds_u32x4*)(uintptr_t)(to + 1024 * i + at) = x;
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < PK_NDMA; ++i)
       dma16_guarded(b, min(off + 4 * i * (uint32_t)sl, last) + (col ^ (i << 4)), to + 1024 * i);
@@ -434,7 +460,7 @@ __device__ __forceinline__ void prefix_tiles(const PagedAttnArgs& a, uint32_t id
           floatx4{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
   if (hl == 0) {
     float* st = a.part + a.Hq * rows * D;
-    st[part] = l == 0.0f ? -INFINITY : m;
+    st[part] = T > 0 ? m : -INFINITY;
     st[a.Hq * rows + part] = l;
   }
 }
@@ -541,7 +567,7 @@ __global__ void __launch_bounds__(JW * 64) paged_join_kernel(const PagedAttnArgs
     x += f * wx[w][lane].x;
     y += f * wx[w][lane].y;
   }
-  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  const float inv = inverse_sum(M, L);
   *reinterpret_cast<uint32_t*>(a.out.p + b * a.out.sl + h * a.out.sh + 2 * lane) =
       pack_bf16x2(x * inv, y * inv);
 }
