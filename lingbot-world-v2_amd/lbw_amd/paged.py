@@ -133,7 +133,7 @@ def _check_append(cache, q, k, v, table, lens, rope, pos, starts, q_out, wq, wk,
         p = pos[:, None] if pos.dim() == 1 else pos
         if p.dtype != torch.int32 or tuple(p.shape) != (T, len(rope.axes)):
             raise ValueError(f"pos must be int32 [{T}, {len(rope.axes)}], got {tuple(pos.shape)} {pos.dtype}")
-    batch = T if starts is None else lens.shape[0]
+    batch = T if starts is None else lens.numel()
     _check_table(table, lens, batch)
     if starts is not None and (starts.dtype != torch.int32 or tuple(starts.shape) != (batch + 1,)):
         raise ValueError(f"starts must be int32 [{batch + 1}], got {tuple(starts.shape)} {starts.dtype}")
@@ -215,10 +215,10 @@ def paged_select(q, cache: PagedKV, table, lens, count: int, *, first: int = 1, 
     than ``count`` pages get all of theirs. q ``[batch, heads, 128]``, the cache with its bounds."""
     if cache.bounds is None:
         raise ValueError("the cache has no bounds: paged_kv(..., bounds=True)")
+    page_size, heads = cache.k.shape[1:3] if cache.k.dim() == 4 else (0, 0)
     try:
-        return _lib.ops().paged_select.default(q, cache.bounds, table, lens, cache.k.shape[1], count, first, last)
+        return _lib.ops().paged_select.default(q, cache.bounds, table, lens, page_size, count, first, last)
     except (RuntimeError, NotImplementedError):
-        heads = cache.k.shape[2] if cache.k.dim() == 4 else 0
         _check_query(q, heads)
         _check_cache(cache, heads, HEAD_DIM)
         _check_table(table, lens, q.shape[0])
