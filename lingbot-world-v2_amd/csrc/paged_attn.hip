@@ -600,12 +600,15 @@ hipError_t run_both(const PagedAttnArgs& a, int64_t units, hipStream_t stream) {
 
 // How the keys are cut. Own ones: whole sequences where they keep the chip busy or are short, else the batch's keys in
 // equal pieces, a workgroup a CU (two: 0 to 5 % slower); the longer for that the more sequences x key/value heads there
-// are, up to one a CU, and shorter again where those behind the first one of each CU are few. Whole / in pieces, x 40/8
-// heads, lengths from a third of the longest up to it, from memory: one sequence of 1100 keys 11.6 / 14.4 us, of 1300 16.2 /
-// 13.9; four of 1000 14.7 / 16.0, of 1300 17.0 / 15.9; eight of 1000 14.7 / 16.3, of 1500 19.4 / 18.4; 16 of 1600 20.6 / 21.6, of
-// 2000 25.2 / 23.5, of 4000 45.7 / 38.9; 20 of 2400 30.4 / 31.7, of 3200 38.0 / 35.9; 24 of 3200 40.2 / 41.3, of 4000 49.6 / 48.6; 32 of
-// 4000 60.6 / 63.6, of 5000 74.7 / 73.9; 40 of 1600 41.9 / 40.8, of 3200 74.1 / 63.1; 64 of 2400 72.5 / 76.6, of 4000 115 / 116, of 8000
-// 221 / 211; 128 of 2400 135 / 140, of 4000 218 / 214.
+// are, up to one a CU, and shorter again up to half as many more, which would leave most of the CUs idle while they end.
+// Whole / in pieces, x 40/8 heads, lengths from a third of the longest up to it, from memory: one sequence of 1100 keys
+// 11.6 / 14.4 us, of 1300 16.2 / 13.9; four of 1000 14.7 / 16.0, of 1300 17.0 / 15.9; eight of 1000 14.7 / 16.3, of 1500
+// 19.4 / 18.4; 16 of 1600 20.6 / 21.6, of 2000 25.2 / 23.5, of 4000 45.7 / 38.9; 20 of 2400 30.4 / 31.7, of 3200 38.0 /
+// 35.9; 24 of 3200 40.2 / 41.3, of 4000 49.6 / 48.6; 32 of 4000 60.6 / 63.6, of 5000 74.7 / 73.9; 33 of 1200 28.7 / 30.4,
+// of 1700 41.7 / 36.6, of 3200 65.6 / 57.0; 36 of 1200 31.8 / 32.2, of 1700 42.7 / 38.9, of 3200 70.0 / 61.3; 40 of 1200
+// 32.5 / 33.6, of 1700 44.8 / 42.1, of 3200 77.8 / 67.7; 48 of 1700 47.2 / 49.3, of 2400 61.6 / 61.4, of 3200 83.7 / 79.1;
+// 50 of 2400 62.5 / 62.6, of 3200 84.6 / 81.6; 56 of 2400 67.6 / 70.7, of 3500 98.6 / 96.7; 64 of 2400 72.5 / 76.6, of 4000
+// 115 / 116, of 8000 221 / 211; 128 of 2400 135 / 140, of 4000 218 / 214.
 // Selected pages: equal lengths, so pieces pay sooner, of 4 tiles or more (and a whole list each where there are more
 // lists than half the CUs). Whole / in pieces, x 40/8 heads: 512 keys for one sequence 9.3 / 11.0 us, for 8 11.0 / 11.1, for 16
 // 11.6 / 12.5; 768 12.3 / 11.2, 13.4 / 12.7, 14.0 / 14.5; 1024 14.7 / 11.3, 15.8 / 13.4, 16.7 / 16.6; 2560 28.0 / 10.9, 30.8 / 20.6,
@@ -640,7 +643,7 @@ void plan_paged(PagedAttnArgs* a, int num_splits, int cus) {
   const int64_t limit = a->p_max > 0                                ? 1024
                         : a->sel != nullptr                         ? 512 + 3 * seqs
                         : seqs <= cus                               ? 1150 + 3200 * seqs * seqs / ((int64_t)cus * cus)
-                        : 8 * seqs > 9 * cus && 2 * seqs <= 3 * cus ? 1800
+                        : 2 * seqs <= 3 * cus                       ? 1500
                                                                     : 3500;
   const bool whole = num_splits == 1 || (num_splits == 0 && keys <= limit);
   int64_t own_places = cus;
