@@ -260,13 +260,11 @@ __device__ __forceinline__ void attend_pages(const PagedAttnArgs& a, uint32_t id
       if (more) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");  // V is there (the next K may not be)
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (((k0 | k1) & (2 * BAD_PAGE - 1)) != 0) {  // (a tile without keys holds anything)
-        if (k0 != HT || k1 != HT) {  // two lanes a row
-          const int row = lane >> 1;
-          if ((row & (HT - 1)) >= ((row < HT ? k0 : k1) & (BAD_PAGE - 1))) {
-            const int at = ring + DT_B + row * PK_ROWB + (lane & 1) * (PK_ROWB / 2);
+        if (k0 != HT || k1 != HT) {  // (16 lanes a row, so the writes meet no bank conflict)
 #pragma unroll
-            for (int i = 0; i < PK_ROWB / 32; ++i) *(lds_u32x4*)(uintptr_t)(at + 16 * i) = u32x4{0u, 0u, 0u, 0u};
-          }
+          for (int i = 0; i < NCOPY; ++i)
+            if (4 * (i & 3) + crow >= ((i < 4 ? k0 : k1) & (BAD_PAGE - 1)))
+              *(lds_u32x4*)(uintptr_t)(ring + DT_B + 1024 * i + 16 * lane) = u32x4{0u, 0u, 0u, 0u};
         }
 #pragma unroll
         for (int db = 0; db < 4; ++db)
