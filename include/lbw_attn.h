@@ -371,7 +371,8 @@ int lbw_attention_decode(const lbw_decode_params* p, void* workspace, size_t wor
 /* ---- A paged key/value cache: serving beside the per-sequence caches above.
  *
  * A page holds page_size consecutive tokens (a power of two, 16 to 1024) of one sequence, k and v bf16
- * [pages][page_size][k_heads][head_dim] with any strides that are multiples of 8 elements (token strides below 2^24);
+ * [pages][page_size][k_heads][head_dim] with any strides that are multiples of 8 elements (token strides below 2^24; for
+ * lbw_paged_append head strides below 2^26);
  * table int32 [batch][table_width] on the device: entry j of a row is the page of the sequence's tokens
  * j * page_size ... Sequences may share pages that none of them writes to any more. bounds, optional: bf16
  * [pages][k_heads][2][head_dim], contiguous, the smallest and the largest value of each key component of a page.
@@ -391,9 +392,9 @@ typedef struct lbw_paged_kv {
  * positions (pos; NULL: a token's row in its sequence, one axis), q into q_out, k and v into their rows of the cache,
  * the bounds kept up. Token t of sequence b (starts[b] <= t < starts[b + 1], int32 [batch + 1] on the device; NULL:
  * token t is sequence t's, batch == tokens) goes to row lens[b] + t - starts[b]; starts rise, and may lie below 0 or
- * past the tokens; a row outside the table is not written. Tokens outside every sequence are left alone, their q_out too. q_out may be q itself. A page that gets its
- * row 0 starts its bounds anew. No two sequences, nor two entries of one's row of the table, may be given tokens for one
- * page. */
+ * past the tokens; a row outside the table is not written. Tokens outside every sequence are left alone, their q_out
+ * too. q_out may be q itself. A page that gets its row 0 starts its bounds anew. No two sequences, nor two entries of
+ * one's row of the table, may be given tokens for one page. */
 typedef struct lbw_paged_append_params {
   lbw_paged_kv cache;
   int32_t tokens, batch, q_heads, k_heads, head_dim;
@@ -419,7 +420,8 @@ int lbw_paged_append(const lbw_paged_append_params* p, void* stream);
  * [batch][k_heads][n_selected], device, contiguous) a key/value head attends to the table entries it names, up to the
  * first negative one (an entry named twice counts twice). With a prefix (int32 [prefix_width] pages, min(*prefix_len,
  * prefix_keys) keys; prefix_len NULL: prefix_keys) those keys come before every sequence's own and are read once for
- * the batch (unless they are few). */
+ * the batch (unless they are few). Scores that are all -infinity give NaN, no keys 0. The work is cut by table_width,
+ * n_selected and prefix_keys, as the lengths are on the device: the nearer they are to the lengths, the better. */
 typedef struct lbw_attention_paged_params {
   lbw_paged_kv cache;
   int32_t batch, q_heads, k_heads, head_dim;

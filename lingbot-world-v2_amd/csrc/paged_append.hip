@@ -8,7 +8,7 @@
 // Bound by memory: every value is read once and written once. As in the per-head norm a wave keeps a token, its
 // angles in registers, and walks its heads. Several tokens for one page: the keys are turned by the workgroup that
 // makes the page's bounds, beside the tokens' q and v. 4680 + 3600 + 1561 tokens x 40/8 heads of 128, normed, pages of 64,
-// from memory 60 us (4.7 TB/s; a large copy reaches 4.9), inputs in the last cache 46; one token 4.3 us, most of it the launch.
+// from memory 62 us (4.6 TB/s; a large copy reaches 4.9), inputs in the last cache 46; one token 4.4 us, most of it the launch.
 
 #include <algorithm>
 

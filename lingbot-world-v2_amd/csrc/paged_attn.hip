@@ -13,9 +13,14 @@
 // where there are more (four waves over shared tiles of 64 keys), in one launch with the sequences' own keys. A short prefix
 // is walked by every sequence before its own keys.
 //
-// Measured, x 40/8 heads: eight sequences of up to 46800 keys 165 us, K and V at 6.4 TB/s (a plain kernel that only reads
-// reaches 5.7); 64 of up to 3600 behind a prefix of 46800 155 us, 16 of 200 (12/4 heads) behind 46800 37; one
-// sequence of 500 keys 8.7 us, 3 us of it the launch and 1.5 a tile of each wave.
+// Measured, x 40/8 heads: eight sequences of up to 46800 keys 166 us, K and V at 6.4 TB/s (a plain kernel that only reads
+// reaches 5.7); 64 of up to 3600 behind a prefix of 46800 160 us, 16 of 200 (12/4 heads) behind 46800 37; one
+// sequence of 500 keys 9.1 us, 3 us of it the launch and 1.5 a tile of each wave.
+//
+// The softmax weights are rounded to bf16 for the product with V, as the matrix instruction takes them (their sum is not):
+// over many keys of like weight that is an error of the size of the result's own rounding. Distance from the 64-bit result,
+// relative to its norm, where rounding that result once gives 0.0016 to 0.0017: 0.0018 for 16 branches, 0.0020 for eight
+// sequences of up to 46800 keys, 0.0023 for 64 branches off 46800.
 //
 // A half's rows past its last key copy that key (or the other half's), so the products never meet what lies
 // behind a sequence; V's of them are zeros before the product, as their weight of 0 would make NaN of a copy of an infinite

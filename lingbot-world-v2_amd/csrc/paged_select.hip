@@ -14,7 +14,7 @@
 // registers. A second kernel has a workgroup per sequence and key/value head: it narrows the range of scores that
 // holds the last chosen one, 1024 equal bins at a time, until no more than 256 are left (one round mostly), whose ranks
 // are counted one against another. Few pages: one kernel for both. Eight sequences of up to 1463 pages x 40/8 heads 16 +
-// 8 us (their bounds take 10 at the rate of a large copy, the 64-bit sums 9), one of 732 pages 4.5 + 6.3.
+// 8 us (their bounds take 7 at the rate of a large copy, the 64-bit sums 8), one of 732 pages 4.7 + 6.7.
 
 #include "capi_util.h"
 #include "head_rows.h"

@@ -35,8 +35,9 @@ class PagedKV:
 
 def paged_kv(pages: int, page_size: int, kv_heads: int, head_dim: int = HEAD_DIM, *, bounds: bool = False,
              device=None) -> PagedKV:
-    """A cache of zeros. ``page_size``: a power of two from 16 to 1024. A page holds each head's tokens together, so a
-    head's part of it is one block of memory."""
+    """A cache of zeros. ``page_size``: a power of two from 16 to 1024. ``head_dim``: 128 (:func:`paged_append_` also fills
+    pages of 32, 64 and 256, for readers of one's own). A page holds each head's tokens together, so a head's part of it
+    is one block of memory."""
     if pages < 1 or kv_heads < 1 or head_dim < 1:
         raise ValueError(f"a cache of {pages} pages, {kv_heads} heads of {head_dim}")
     if not 16 <= page_size <= 1024 or page_size & (page_size - 1):
@@ -153,6 +154,11 @@ def attention_paged(q, cache: PagedKV, table, lens, *, selected=None, prefix_tab
     ``selected`` int32 ``[batch, kv_heads, n]`` (from :func:`paged_select`): a key/value head attends to the table entries
     that its list names, up to the first negative one; entries at or past the length name no keys, one that is named twice
     counts twice. It applies to the sequences' own keys, not to a prefix.
+
+    Scores that are all -infinity give NaN.
+
+    The lengths are on the device, so the work is cut by what the table and the prefix can hold: where lengths stay far
+    below that, give the columns that they can reach (``table[:, :n]`` is taken as it is).
 
     Not differentiable; with ``out`` it raises while gradients are recorded and one of the tensors requires one.
     ``num_splits`` as in :func:`attention_decode`; the keys of a list or prefix are cut into so many pieces."""
